@@ -16,18 +16,25 @@ from . import hxmi, weights
 from .hxmi import (
     HxmiError,
     HxmiNotBuiltError,
+    KVCache,
+    KVPlan,
     attention,
     bgemm,
     fold_rms_weight,
     gemm,
     gemv,
     hexkl_matmul,
+    kv_append,
+    kv_attention,
+    kv_plan,
+    kv_read,
     linear,
     load_library,
     pack_gate_up,
     quantize_int8,
     rms_norm,
     rms_norm_linear,
+    sample,
     set_tuning,
     softmax,
     tuning,
@@ -39,18 +46,25 @@ __all__ = [
     "weights",
     "HxmiError",
     "HxmiNotBuiltError",
+    "KVCache",
+    "KVPlan",
     "attention",
     "bgemm",
     "fold_rms_weight",
     "gemm",
     "gemv",
     "hexkl_matmul",
+    "kv_append",
+    "kv_attention",
+    "kv_plan",
+    "kv_read",
     "linear",
     "load_library",
     "pack_gate_up",
     "quantize_int8",
     "rms_norm",
     "rms_norm_linear",
+    "sample",
     "set_tuning",
     "softmax",
     "tuning",

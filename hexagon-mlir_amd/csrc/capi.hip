@@ -673,6 +673,231 @@ int hxmi_decode_status(void* workspace, int clear, int* status, void* stream) {
   return from_hip(e, "hxmi_decode_status");
 }
 
+// log2 of a cache's block size, -1 for one that it cannot have.
+static int log2_block(int64_t block) {
+  return block >= 16 && block <= 256 && (block & (block - 1)) == 0 ? __builtin_ctzll((unsigned long long)block) : -1;
+}
+
+int hxmi_kv_plan(const int32_t* lens, const int32_t* added, int32_t* block_table, int32_t* free_blocks,
+                 const int32_t* free_count, int64_t* slots, int32_t* positions, int32_t* cu, int32_t* lens_out,
+                 int32_t* free_count_out, int64_t requests, int64_t width, int64_t ld_table, int64_t capacity,
+                 int64_t tokens, int64_t block_size, void* stream) {
+  const char* name = "hxmi_kv_plan";
+  REQUIRE(requests >= 0 && width >= 0 && capacity >= 0 && tokens >= 0, "%s: negative size", name);
+  const int lb = log2_block(block_size);
+  REQUIRE(lb >= 0, "%s: block_size must be a power of two from 16 to 256, got %lld", name, (long long)block_size);
+  REQUIRE(requests <= hxmi::kPlanRequests, "%s: at most %lld requests a call, got %lld", name,
+          (long long)hxmi::kPlanRequests, (long long)requests);
+  REQUIRE(tokens < (1ll << 31) && capacity < (1ll << 31) && width <= (1ll << 30) / block_size &&
+              requests * width < (1ll << 31),
+          "%s: tokens, capacity and table entries must be below 2^31, a table row at most 2^30 tokens", name);
+  REQUIRE(ld_table >= width, "%s: ld_table below the table's width", name);
+  REQUIRE(free_count && cu && free_count_out && (lens || !requests) && (added || !requests) &&
+              (lens_out || !requests) && (block_table || !requests || !width) && (free_blocks || !capacity) &&
+              ((slots && positions) || !tokens),
+          "%s: null pointer", name);
+  hxmi::KvPlanProblem p{};
+  p.lens = lens;
+  p.added = added;
+  p.table = block_table;
+  p.stack = free_blocks;
+  p.count = free_count;
+  p.slots = slots;
+  p.positions = positions;
+  p.cu = cu;
+  p.lens_out = lens_out;
+  p.count_out = free_count_out;
+  p.requests = requests;
+  p.width = width;
+  p.ldt = ld_table;
+  p.capacity = capacity;
+  p.tokens = tokens;
+  p.log2_block = lb;
+  return from_hip(hxmi::launch_kv_plan(p, (hipStream_t)stream), name);
+}
+
+// The cache's own arguments, which every call on it takes.
+static int cache_check(const char* name, const void* k_codes, const void* v_codes, const void* k_scale,
+                       const void* v_scale, int64_t blocks, int64_t kv_heads, int64_t head_dim, int64_t block_size) {
+  REQUIRE(kv_heads > 0 && head_dim > 0 && blocks >= 0, "%s: sizes must be positive", name);
+  REQUIRE(log2_block(block_size) >= 0, "%s: block_size must be a power of two from 16 to 256, got %lld", name,
+          (long long)block_size);
+  REQUIRE(head_dim % 8 == 0 && head_dim <= 128, "%s: head_dim must be a multiple of 8 up to 128, got %lld", name,
+          (long long)head_dim);
+  REQUIRE(kv_heads < (1 << 20) && blocks < (1ll << 31), "%s: too many heads or blocks", name);
+  REQUIRE(blocks == 0 || (k_codes && v_codes && k_scale && v_scale), "%s: null cache pointer", name);
+  REQUIRE((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0, "%s: codes must be 16-byte aligned", name);
+  return HXMI_OK;
+}
+
+int hxmi_kv_append(int is_bf16, const void* k, const void* v, const int64_t* slots, int8_t* k_codes, int8_t* v_codes,
+                   float* k_scale, float* v_scale, int64_t tokens, int64_t blocks, int64_t kv_heads, int64_t head_dim,
+                   int64_t block_size, int64_t ldk, int64_t head_stride_k, int64_t ldv, int64_t head_stride_v,
+                   void* stream) {
+  const char* name = "hxmi_kv_append";
+  REQUIRE(is_bf16 == 0 || is_bf16 == 1, "%s: is_bf16 must be 0 or 1", name);
+  REQUIRE(tokens >= 0 && tokens < (1ll << 31), "%s: bad number of tokens %lld", name, (long long)tokens);
+  if (const int rc = cache_check(name, k_codes, v_codes, k_scale, v_scale, blocks, kv_heads, head_dim, block_size))
+    return rc;
+  if (tokens == 0 || blocks == 0) return ok();
+  REQUIRE(k && v && slots, "%s: null pointer", name);
+  REQUIRE(ldk >= 0 && head_stride_k >= 0 && ldv >= 0 && head_stride_v >= 0, "%s: negative stride", name);
+  hxmi::KvCacheProblem p{};
+  p.k_codes = k_codes;
+  p.v_codes = v_codes;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.slots = slots;
+  p.k = k;
+  p.v = v;
+  p.tokens = tokens;
+  p.blocks = blocks;
+  p.kv_heads = kv_heads;
+  p.d = head_dim;
+  p.ldk = ldk;
+  p.hsk = head_stride_k;
+  p.ldv = ldv;
+  p.hsv = head_stride_v;
+  p.log2_block = log2_block(block_size);
+  p.dtype = is_bf16 ? hxmi::DT_BF16 : hxmi::DT_F16;
+  return from_hip(hxmi::launch_kv_append(p, (hipStream_t)stream), name);
+}
+
+int hxmi_kv_read(int is_bf16, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                 const int64_t* slots, void* k, void* v, int64_t tokens, int64_t blocks, int64_t kv_heads,
+                 int64_t head_dim, int64_t block_size, void* stream) {
+  const char* name = "hxmi_kv_read";
+  REQUIRE(is_bf16 == 0 || is_bf16 == 1, "%s: is_bf16 must be 0 or 1", name);
+  REQUIRE(tokens >= 0 && tokens < (1ll << 31), "%s: bad number of tokens %lld", name, (long long)tokens);
+  if (const int rc = cache_check(name, k_codes, v_codes, k_scale, v_scale, blocks, kv_heads, head_dim, block_size))
+    return rc;
+  if (tokens == 0) return ok();
+  REQUIRE(k && v && slots, "%s: null pointer", name);
+  hxmi::KvCacheProblem p{};
+  p.k_codes = const_cast<int8_t*>(k_codes);
+  p.v_codes = const_cast<int8_t*>(v_codes);
+  p.k_scale = const_cast<float*>(k_scale);
+  p.v_scale = const_cast<float*>(v_scale);
+  p.slots = slots;
+  p.k_out = k;
+  p.v_out = v;
+  p.tokens = tokens;
+  p.blocks = blocks;
+  p.kv_heads = kv_heads;
+  p.d = head_dim;
+  p.log2_block = log2_block(block_size);
+  p.dtype = is_bf16 ? hxmi::DT_BF16 : hxmi::DT_F16;
+  return from_hip(hxmi::launch_kv_read(p, (hipStream_t)stream), name);
+}
+
+int64_t hxmi_kv_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
+                                          int64_t head_dim, int64_t block_size, int64_t width, int ragged) {
+  if (tokens <= 0 || requests <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 ||
+      head_dim > 128 || log2_block(block_size) < 0 || width < 0)
+    return 0;
+  static const int one = 0;
+  hxmi::KvAttnProblem p{};
+  p.tokens = tokens;
+  p.requests = requests;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.d = head_dim;
+  p.block = block_size;
+  p.width = width;
+  p.cu = ragged ? &one : nullptr;
+  return hxmi::kv_attention_workspace_bytes(p);
+}
+
+int hxmi_kv_attention(int is_bf16, const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
+                      const float* v_scale, const int32_t* block_table, const int32_t* lens, const int32_t* cu,
+                      void* o, int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                      int64_t block_size, int64_t blocks, int64_t width, int64_t ld_table, int64_t ldq,
+                      int64_t head_stride_q, int64_t ldo, int64_t head_stride_o, float scale, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  const char* name = "hxmi_kv_attention";
+  REQUIRE(is_bf16 == 0 || is_bf16 == 1, "%s: is_bf16 must be 0 or 1", name);
+  REQUIRE(tokens >= 0 && requests >= 0 && heads >= 0 && width >= 0, "%s: negative size", name);
+  if (const int rc = cache_check(name, k_codes, v_codes, k_scale, v_scale, blocks, kv_heads, head_dim, block_size))
+    return rc;
+  REQUIRE(heads % kv_heads == 0, "%s: heads must be a multiple of kv_heads (%lld, %lld)", name, (long long)heads,
+          (long long)kv_heads);
+  REQUIRE(cu || tokens == requests, "%s: without cu there is one row a request (%lld rows, %lld requests)", name,
+          (long long)tokens, (long long)requests);
+  REQUIRE(scale > 0.f && scale < __builtin_inff(), "%s: scale must be positive and finite", name);
+  REQUIRE(tokens < (1ll << 31) && requests < (1ll << 31) && heads < (1ll << 31) &&
+              (tokens + requests) * (heads > 128 ? heads : 128) < (1ll << 31) && width <= (1ll << 30) / block_size,
+          "%s: (tokens + requests) * heads must be below 2^31, a table row at most 2^30 tokens", name);
+  if (tokens == 0 || requests == 0 || heads == 0) return ok();
+  REQUIRE(blocks > 0, "%s: a cache without blocks", name);
+  REQUIRE(q && o && lens && (block_table || !width), "%s: null pointer", name);
+  REQUIRE(ld_table >= width, "%s: ld_table below the table's width", name);
+  REQUIRE(ldq >= 0 && head_stride_q >= 0 && ldo >= 0 && head_stride_o >= 0, "%s: negative stride", name);
+  REQUIRE(!workspace || al(workspace, 256), "%s: workspace must be 256-byte aligned", name);
+  hxmi::KvAttnProblem p{};
+  p.q = q;
+  p.k_codes = k_codes;
+  p.v_codes = v_codes;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.table = block_table;
+  p.lens = lens;
+  p.cu = cu;
+  p.o = o;
+  p.ws = workspace;
+  p.ws_bytes = workspace_bytes;
+  p.tokens = tokens;
+  p.requests = requests;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.d = head_dim;
+  p.block = block_size;
+  p.blocks = blocks;
+  p.width = width;
+  p.ldt = ld_table;
+  p.ldq = ldq;
+  p.hsq = head_stride_q;
+  p.ldo = ldo;
+  p.hso = head_stride_o;
+  p.scale = scale;
+  p.dtype = is_bf16 ? hxmi::DT_BF16 : hxmi::DT_F16;
+  return from_hip(hxmi::launch_kv_attention(p, (hipStream_t)stream), name);
+}
+
+int hxmi_sample(int dtype, const void* logits, const float* u, const float* temperature, const int32_t* top_k,
+                const float* top_p, const float* min_p, float all_temperature, int32_t all_top_k, float all_top_p,
+                float all_min_p, int64_t* tokens, int64_t rows, int64_t vocab, int64_t ldx, void* stream) {
+  const char* name = "hxmi_sample";
+  REQUIRE(dtype >= HXMI_SAMPLE_F16 && dtype <= HXMI_SAMPLE_F32, "%s: unknown dtype %d", name, dtype);
+  REQUIRE(rows >= 0 && rows < (1ll << 31), "%s: bad number of rows %lld", name, (long long)rows);
+  if (rows == 0) return ok();
+  REQUIRE(vocab > 0 && vocab <= hxmi::kSampleMaxVocab, "%s: vocab must be 1 to %lld, got %lld", name,
+          (long long)hxmi::kSampleMaxVocab, (long long)vocab);
+  REQUIRE(ldx >= vocab || rows == 1, "%s: leading dimension below vocab", name);
+  REQUIRE(logits && u && tokens, "%s: null pointer", name);
+  REQUIRE((uintptr_t)logits % (dtype == HXMI_SAMPLE_F32 ? 4 : 2) == 0, "%s: logits must be aligned to their type", name);
+  REQUIRE(temperature || (all_temperature >= 0.f && all_temperature < __builtin_inff()),
+          "%s: temperature must be finite and >= 0", name);
+  REQUIRE(top_p || all_top_p == all_top_p, "%s: top_p must be a number", name);
+  REQUIRE(min_p || all_min_p == all_min_p, "%s: min_p must be a number", name);
+  hxmi::SampleProblem p{};
+  p.logits = logits;
+  p.u = u;
+  p.temperature = temperature;
+  p.top_k = top_k;
+  p.top_p = top_p;
+  p.min_p = min_p;
+  p.tokens = tokens;
+  p.rows = rows;
+  p.vocab = vocab;
+  p.ldx = ldx;
+  p.t = all_temperature;
+  p.k = all_top_k;
+  p.p = all_top_p;
+  p.m = all_min_p;
+  p.dtype = dtype;
+  return from_hip(hxmi::launch_sample(p, (hipStream_t)stream), name);
+}
+
 int hxmi_lwp_record(uint32_t* records, int64_t slot, uint32_t id, void* stream) {
   const char* name = "hxmi_lwp_record";
   REQUIRE(records, "%s: null record buffer", name);

@@ -196,6 +196,67 @@ struct AttnProblem {
 
 hipError_t launch_attention(const AttnProblem& p, hipStream_t stream);
 
+// Block tables and slot maps of one serving step (kvcache.hip).
+constexpr int64_t kPlanRequests = 4096;  // a call's requests (three 32-bit words of LDS each)
+struct KvPlanProblem {
+  const int *lens, *added;
+  int *table, *stack;
+  const int* count;
+  int64_t* slots;
+  int *positions, *cu, *lens_out, *count_out;
+  int64_t requests, width, ldt, capacity, tokens;
+  int log2_block;
+};
+hipError_t launch_kv_plan(const KvPlanProblem& p, hipStream_t stream);
+
+// Rows of keys and values into the 8-bit cache (k, v) or out of it (k_out, v_out).
+struct KvCacheProblem {
+  int8_t *k_codes, *v_codes;
+  float *k_scale, *v_scale;
+  const int64_t* slots;
+  const void *k, *v;
+  void *k_out, *v_out;
+  int64_t tokens, blocks, kv_heads, d;
+  int64_t ldk, hsk, ldv, hsv;  // row and head strides of k and v
+  int log2_block, dtype;
+};
+hipError_t launch_kv_append(const KvCacheProblem& p, hipStream_t stream);
+hipError_t launch_kv_read(const KvCacheProblem& p, hipStream_t stream);
+
+// Attention over the 8-bit cache (kv_attention.hip).
+struct KvAttnProblem {
+  const void* q;
+  const int8_t *k_codes, *v_codes;
+  const float *k_scale, *v_scale;
+  const int *table, *lens;
+  const int* cu;  // null: one row a request
+  void* o;
+  void* ws;
+  int64_t ws_bytes;
+  int64_t tokens, requests, heads, kv_heads, d, block, blocks, width, ldt;
+  int64_t ldq, hsq, ldo, hso;
+  float scale;
+  int dtype;
+};
+int64_t kv_attention_workspace_bytes(const KvAttnProblem& p);
+hipError_t launch_kv_attention(const KvAttnProblem& p, hipStream_t stream);
+
+// A token a row from logits (sample.hip).
+constexpr int64_t kSampleMaxVocab = 1 << 20;
+struct SampleProblem {
+  const void* logits;
+  const float *u, *temperature;  // per-row parameters, or null: t, k, p, m
+  const int* top_k;
+  const float *top_p, *min_p;
+  int64_t* tokens;
+  int64_t rows, vocab, ldx;
+  float t, p, m;
+  int k;
+  int dtype;  // DT_F16, DT_BF16 or SAMPLE_F32
+};
+constexpr int SAMPLE_F32 = 2;
+hipError_t launch_sample(const SampleProblem& p, hipStream_t stream);
+
 // One-token decoder step of a Llama / Qwen2 stack (persistent kernel).
 struct DecodeProblem {
   const void* x;        // [H] fp16: the token's embedding row

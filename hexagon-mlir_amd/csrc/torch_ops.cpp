@@ -489,9 +489,197 @@ PyObject* op_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The tensors of a cache: (k, v, k_scale, v_scale, head_dim) from args[0] on.
+struct Cache {
+  const Tensor *k, *v, *ks, *vs;
+  long d = 0;
+  int64_t blocks = 0, heads = 0, block = 0;
+  bool ok = false;
+
+  Cache(Operands& in, PyObject* const* args)
+      : k(in.get(args[0])), v(in.get(args[1])), ks(in.get(args[2])), vs(in.get(args[3])) {
+    if (!in.ok || !number(args[4], d) || k->dim() != 4 || k->scalar_type() != at::kChar ||
+        v->scalar_type() != at::kChar || ks->scalar_type() != at::kFloat || vs->scalar_type() != at::kFloat)
+      return;
+    blocks = k->size(0);
+    heads = k->size(1);
+    block = k->size(2);
+    const int64_t dp = (d + 15) / 16 * 16;
+    ok = heads > 0 && k->size(3) == dp && v->sizes() == at::IntArrayRef({blocks, heads, block / 16, dp, 16}) &&
+         ks->sizes() == at::IntArrayRef({blocks, heads}) && vs->sizes() == ks->sizes() && k->is_contiguous() &&
+         v->is_contiguous() && ks->is_contiguous() && vs->is_contiguous();
+  }
+};
+
+// Rows [tokens, heads, d] with unit last stride.
+bool head_rows(const Tensor& t, int64_t heads, int64_t d) {
+  return t.dim() == 3 && t.size(1) == heads && t.size(2) == d && t.stride(2) == 1;
+}
+
+bool table(const Tensor& t, int64_t requests, int64_t& ld) {
+  return t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == requests && rows(t, ld);
+}
+
+Tensor fresh(const Tensor& like, at::IntArrayRef shape, at::ScalarType type) {
+  return at::empty(shape, like.options().dtype(type));
+}
+
+// kv_plan(lens, new, table, free, free_count, block_size, tokens)
+PyObject* op_kv_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NOT_PLAIN_UNLESS(n == 7);
+  Operands in;
+  const Tensor *lens = in.get(args[0]), *added = in.get(args[1]), *tab = in.get(args[2]), *stack = in.get(args[3]),
+               *count = in.get(args[4]);
+  long block, tokens;
+  NOT_PLAIN_UNLESS(in.ok && number(args[5], block) && number(args[6], tokens) && tokens >= 0 && lens->dim() == 1);
+  const int64_t R = lens->size(0);
+  int64_t ldt;
+  NOT_PLAIN_UNLESS(vec(lens, R, at::kInt) && vec(added, R, at::kInt) && vec(count, 1, at::kInt) &&
+                   stack->dim() == 1 && vec(stack, stack->size(0), at::kInt) && table(*tab, R, ldt));
+  const c10::DeviceGuard guard(lens->device());
+  const Tensor slots = fresh(*lens, {tokens}, at::kLong), positions = fresh(*lens, {tokens}, at::kInt),
+               cu = fresh(*lens, {R + 1}, at::kInt), after = fresh(*lens, {R}, at::kInt),
+               left = fresh(*lens, {1}, at::kInt);
+  void* s = in.stream();
+  const int rc = unlocked([&] {
+    return hxmi_kv_plan((const int32_t*)ptr(lens), (const int32_t*)ptr(added), (int32_t*)ptr(tab), (int32_t*)ptr(stack),
+                        (const int32_t*)ptr(count), (int64_t*)ptr(&slots), (int32_t*)ptr(&positions), (int32_t*)ptr(&cu),
+                        (int32_t*)ptr(&after), (int32_t*)ptr(&left), R, tab->size(1), ldt, stack->size(0), tokens, block,
+                        s);
+  });
+  if (rc != HXMI_OK) Py_RETURN_NONE;
+  return Py_BuildValue("(NNNNN)", THPVariable_Wrap(slots), THPVariable_Wrap(positions), THPVariable_Wrap(cu),
+                       THPVariable_Wrap(after), THPVariable_Wrap(left));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_append(*cache, k, v, slots): True once done
+PyObject* op_kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NOT_PLAIN_UNLESS(n == 8);
+  Operands in;
+  const Cache c(in, args);
+  const Tensor *k = in.get(args[5]), *v = in.get(args[6]), *slots = in.get(args[7]);
+  NOT_PLAIN_UNLESS(in.ok && c.ok && half_type(*k) && v->scalar_type() == k->scalar_type() &&
+                   head_rows(*k, c.heads, c.d) && head_rows(*v, c.heads, c.d) && v->size(0) == k->size(0) &&
+                   vec(slots, k->size(0), at::kLong));
+  const c10::DeviceGuard guard(k->device());
+  void* s = in.stream();
+  const int rc = unlocked([&] {
+    return hxmi_kv_append(bf16(*k), ptr(k), ptr(v), (const int64_t*)ptr(slots), (int8_t*)ptr(c.k), (int8_t*)ptr(c.v),
+                          (float*)ptr(c.ks), (float*)ptr(c.vs), k->size(0), c.blocks, c.heads, c.d, c.block,
+                          k->stride(0), k->stride(1), v->stride(0), v->stride(1), s);
+  });
+  if (rc != HXMI_OK) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_read(*cache, slots, bf16)
+PyObject* op_kv_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NOT_PLAIN_UNLESS(n == 7);
+  Operands in;
+  const Cache c(in, args);
+  const Tensor* slots = in.get(args[5]);
+  NOT_PLAIN_UNLESS(in.ok && c.ok && slots->dim() == 1 && vec(slots, slots->size(0), at::kLong));
+  const bool b16 = PyObject_IsTrue(args[6]);
+  const int64_t T = slots->size(0);
+  const c10::DeviceGuard guard(slots->device());
+  const Tensor k = fresh(*slots, {T, c.heads, c.d}, b16 ? at::kBFloat16 : at::kHalf), v = at::empty_like(k);
+  void* s = in.stream();
+  const int rc = unlocked([&] {
+    return hxmi_kv_read(b16, (const int8_t*)ptr(c.k), (const int8_t*)ptr(c.v), (const float*)ptr(c.ks),
+                        (const float*)ptr(c.vs), (const int64_t*)ptr(slots), ptr(&k), ptr(&v), T, c.blocks, c.heads, c.d,
+                        c.block, s);
+  });
+  if (rc != HXMI_OK) Py_RETURN_NONE;
+  return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_attention(q, *cache, table, lens, cu or None, scale or None, out or None): an out apart from every operand
+PyObject* op_kv_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NOT_PLAIN_UNLESS(n == 11);
+  Operands in;
+  const Tensor* q = in.get(args[0]);
+  const Cache c(in, args + 1);
+  const Tensor *tab = in.get(args[6]), *lens = in.get(args[7]), *cu = in.get(args[8], true), *o = in.get(args[10], true);
+  NOT_PLAIN_UNLESS(in.ok && c.ok && half_type(*q) && q->dim() == 3 && q->size(1) % c.heads == 0 &&
+                   head_rows(*q, q->size(1), c.d) && lens->dim() == 1);
+  const int64_t T = q->size(0), H = q->size(1), R = lens->size(0);
+  double scale = 1.0 / std::sqrt((double)c.d);
+  int64_t ldt;
+  NOT_PLAIN_UNLESS((args[9] == Py_None || number(args[9], scale)) && vec(lens, R, at::kInt) &&
+                   vec(cu, R + 1, at::kInt) && (cu || T == R) && table(*tab, R, ldt) && q->numel() > 0);
+  NOT_PLAIN_UNLESS(!o || (o->sizes() == q->sizes() && o->scalar_type() == q->scalar_type() && o->is_contiguous() &&
+                          !overlap(*o, *q) && !overlap(*o, *c.k) && !overlap(*o, *c.v) && !overlap(*o, *c.ks) &&
+                          !overlap(*o, *c.vs) && !overlap(*o, *lens) && !(tab->numel() && overlap(*o, *tab)) &&
+                          !(cu && overlap(*o, *cu))));
+  const c10::DeviceGuard guard(q->device());
+  const Tensor out = o ? *o : like(*q, q->sizes());
+  const Workspace ws(hxmi_kv_attention_workspace_bytes(T, R, H, c.heads, c.d, c.block, tab->size(1), cu != nullptr), *q);
+  if (!ws.ok) return nullptr;
+  void* s = in.stream();
+  return result(unlocked([&] {
+                  return hxmi_kv_attention(bf16(*q), ptr(q), (const int8_t*)ptr(c.k), (const int8_t*)ptr(c.v),
+                                           (const float*)ptr(c.ks), (const float*)ptr(c.vs), (const int32_t*)ptr(tab),
+                                           (const int32_t*)ptr(lens), (const int32_t*)ptr(cu), ptr(&out), T, R, H,
+                                           c.heads, c.d, c.block, c.blocks, tab->size(1), ldt, q->stride(0),
+                                           q->stride(1), out.stride(0), out.stride(1), (float)scale, ws.data, ws.bytes,
+                                           s);
+                }),
+                out);
+  END_HANDLE_TH_ERRORS
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p)
+PyObject* op_sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NOT_PLAIN_UNLESS(n == 6);
+  Operands in;
+  const Tensor *x = in.get(args[0]), *u = in.get(args[1]);
+  NOT_PLAIN_UNLESS(in.ok && x->dim() >= 1 && x->numel() > 0);
+  int64_t M, V, ld;
+  const int dtype = x->scalar_type() == at::kHalf       ? HXMI_SAMPLE_F16
+                    : x->scalar_type() == at::kBFloat16 ? HXMI_SAMPLE_BF16
+                    : x->scalar_type() == at::kFloat    ? HXMI_SAMPLE_F32
+                                                        : -1;
+  const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
+  NOT_PLAIN_UNLESS(dtype >= 0 && as_rows(*x, M, V, ld) && u->sizes() == lead && u->is_contiguous() &&
+                   u->scalar_type() == at::kFloat);
+  const Tensor* own[4] = {};
+  double all[4] = {1, 0, 1, 0};
+  for (int i = 0; i < 4; ++i) {
+    if (THPVariable_Check(args[2 + i])) {
+      own[i] = in.get(args[2 + i]);
+      NOT_PLAIN_UNLESS(in.ok && own[i]->sizes() == lead && own[i]->is_contiguous() &&
+                       own[i]->scalar_type() == (i == 1 ? at::kInt : at::kFloat));
+    } else {
+      long k;
+      NOT_PLAIN_UNLESS(i == 1 ? number(args[3], k) && k >= 0 && k < (1l << 31) : number(args[2 + i], all[i]));
+      if (i == 1) all[1] = (double)k;
+    }
+  }
+  const c10::DeviceGuard guard(x->device());
+  const Tensor out = fresh(*x, lead, at::kLong);
+  void* s = in.stream();
+  return result(unlocked([&] {
+                  return hxmi_sample(dtype, ptr(x), (const float*)ptr(u), (const float*)ptr(own[0]),
+                                     (const int32_t*)ptr(own[1]), (const float*)ptr(own[2]), (const float*)ptr(own[3]),
+                                     (float)all[0], (int32_t)all[1], (float)all[2], (float)all[3], (int64_t*)ptr(&out),
+                                     M, V, ld, s);
+                }),
+                out);
+  END_HANDLE_TH_ERRORS
+}
+
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))op_##name, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {ENTRY(gemm),         ENTRY(bgemm),    ENTRY(linear),  ENTRY(rms_norm_linear), ENTRY(gemv),
                           ENTRY(w8a16_linear), ENTRY(rms_norm), ENTRY(softmax), ENTRY(attention),
+                          ENTRY(kv_plan),      ENTRY(kv_append), ENTRY(kv_read), ENTRY(kv_attention),  ENTRY(sample),
                           {"set_workspace", set_workspace, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "hxmi_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -13,9 +13,10 @@ import contextlib
 import ctypes
 import importlib.machinery
 import importlib.util
+import math
 import pathlib
 import warnings
-from typing import Optional
+from typing import NamedTuple, Optional, Union
 
 import torch
 
@@ -69,6 +70,12 @@ SIGNATURES = {
     "hxmi_decode_step_ov_f16": ([_P] * 15 + [_I64] * 7 + [_F, _I64, _P, _I64, _P], _I),
     "hxmi_decode_workspace_bytes": ([_I64, _I64, _I64], _I64),
     "hxmi_decode_status": ([_P, _I, ctypes.POINTER(_I), _P], _I),
+    "hxmi_kv_plan": ([_P] * 10 + [_I64] * 6 + [_P], _I),
+    "hxmi_kv_append": ([_I] + [_P] * 7 + [_I64] * 9 + [_P], _I),
+    "hxmi_kv_read": ([_I] + [_P] * 7 + [_I64] * 5 + [_P], _I),
+    "hxmi_kv_attention": ([_I] + [_P] * 9 + [_I64] * 13 + [_F, _P, _I64, _P], _I),
+    "hxmi_kv_attention_workspace_bytes": ([_I64] * 7 + [_I], _I64),
+    "hxmi_sample": ([_I] + [_P] * 6 + [_F, ctypes.c_int32, _F, _F, _P] + [_I64] * 3 + [_P], _I),
     "hxmi_lwp_record": ([_P, _I64, ctypes.c_uint32, _P], _I),
     "hxmi_lwp_clock_hz": ([], _I64),
     "hexkl_matmul_f16f16_f32": ([_I64, _I64, _I64, _P, _P, _P], _I),
@@ -959,6 +966,299 @@ def decode_status(device: Optional[torch.device] = None, clear: bool = True) -> 
             _check(load_library().hxmi_decode_status(ws.data_ptr(), int(clear), ctypes.byref(st), stream))
             status |= st.value
     return status
+
+
+# ---- serving: an 8-bit key/value cache, attention over it, sampling ---------------------
+
+@dataclasses.dataclass
+class KVCache:
+    """The keys and values of a serving loop in 8 bits, in blocks of tokens
+    with one scale for each block and head (include/hxmi.h):
+
+    k int8 [blocks, kv_heads, block_size, Dp], v int8 [blocks, kv_heads,
+    block_size / 16, Dp, 16] (Dp = head_dim rounded up to 16), k_scale and
+    v_scale fp32 [blocks, kv_heads]; a held value is code * scale.  block_size
+    is a power of two from 16 to 256, head_dim a multiple of 8 up to 128.
+    Token t of block b is slot b * block_size + t."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    head_dim: int
+
+    @classmethod
+    def empty(cls, blocks: int, kv_heads: int, head_dim: int, block_size: int = 64, device="cuda") -> "KVCache":
+        """A cache that holds nothing yet."""
+        if block_size not in (16, 32, 64, 128, 256):
+            raise HxmiError(f"block_size must be a power of two from 16 to 256, got {block_size}")
+        if head_dim % 8 or not 8 <= head_dim <= 128:
+            raise HxmiError(f"head_dim must be a multiple of 8 up to 128, got {head_dim}")
+        dp = (head_dim + 15) // 16 * 16
+        zeros = lambda *shape, dtype=torch.int8: torch.zeros(shape, dtype=dtype, device=device)  # noqa: E731
+        return cls(zeros(blocks, kv_heads, block_size, dp), zeros(blocks, kv_heads, block_size // 16, dp, 16),
+                   zeros(blocks, kv_heads, dtype=torch.float32), zeros(blocks, kv_heads, dtype=torch.float32), head_dim)
+
+    @property
+    def blocks(self) -> int:
+        return self.k.shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.k.shape[1]
+
+    @property
+    def block_size(self) -> int:
+        return self.k.shape[2]
+
+
+class KVPlan(NamedTuple):
+    """What kv_plan gives one step: slots [tokens] (int64, -1: none) and
+    positions [tokens] (int32) of the step's rows, their requests' bounds cu
+    [requests + 1], the requests' lengths afterwards and the number of blocks
+    left free [1] (int32)."""
+    slots: torch.Tensor
+    positions: torch.Tensor
+    cu: torch.Tensor
+    lens: torch.Tensor
+    free_count: torch.Tensor
+
+
+def _on(t: torch.Tensor):
+    """t's device as the current one (a launch goes to the current device)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _ints(t: torch.Tensor, n: Optional[int], name: str, dtype: torch.dtype = torch.int32) -> torch.Tensor:
+    if t.dim() != 1 or t.dtype != dtype or (n is not None and t.numel() != n):
+        raise HxmiError(f"{name} must be a 1-D {dtype} tensor" + ("" if n is None else f" of {n} elements"))
+    return t.contiguous()
+
+
+def _table(t: torch.Tensor, requests: int) -> int:
+    """Row stride of a block table."""
+    if t.dim() != 2 or t.dtype != torch.int32 or t.shape[0] != requests:
+        raise HxmiError(f"block_table must be a 2-D torch.int32 tensor of {requests} rows")
+    return _rowmajor(t, "block_table")
+
+
+def _cache_args(c: KVCache) -> tuple:
+    """(pointers, (blocks, kv_heads, head_dim, block_size)) of a cache."""
+    if not isinstance(c, KVCache):
+        raise HxmiError(f"cache must be a KVCache, got {type(c).__name__}")
+    _require_gpu(c.k, c.v, c.k_scale, c.v_scale)
+    d = c.head_dim
+    if c.k.dim() != 4:
+        raise HxmiError(f"cache.k must be [blocks, kv_heads, block_size, Dp], got shape {tuple(c.k.shape)}")
+    n, h, b, dp = c.k.shape
+    if b not in (16, 32, 64, 128, 256):
+        raise HxmiError(f"the cache's block_size must be a power of two from 16 to 256, got {b}")
+    if d % 8 or not 8 <= d <= 128:
+        raise HxmiError(f"the cache's head_dim must be a multiple of 8 up to 128, got {d}")
+    if dp != (d + 15) // 16 * 16 or c.v.shape != (n, h, b // 16, dp, 16) or c.k_scale.shape != (n, h) \
+            or c.v_scale.shape != (n, h) or h < 1:
+        raise HxmiError(f"the cache's tensors do not belong together: k {tuple(c.k.shape)}, v {tuple(c.v.shape)}, "
+                        f"scales {tuple(c.k_scale.shape)} and {tuple(c.v_scale.shape)}, head_dim {d}")
+    if c.k.dtype != torch.int8 or c.v.dtype != torch.int8 or c.k_scale.dtype != torch.float32 \
+            or c.v_scale.dtype != torch.float32:
+        raise HxmiError("a cache holds int8 codes and fp32 scales")
+    if not all(t.is_contiguous() for t in (c.k, c.v, c.k_scale, c.v_scale)):
+        raise HxmiError("the cache's tensors must be contiguous")
+    return (c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr()), (n, h, d, b)
+
+
+def kv_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
+            free_count: torch.Tensor, *, block_size: int, tokens: int) -> KVPlan:
+    """Blocks and slots of one serving step, on the GPU in one launch.
+
+    lens [requests] tokens each request holds, new [requests] tokens it adds
+    (0: idle, negative: it has ended), block_table [requests, width] and the
+    stack free_blocks [capacity] whose first free_count [1] entries are free
+    (all int32).  Ended requests' blocks go onto the stack, then requests take
+    what they need from its top, both in request order; table and stack are
+    updated in place.  tokens: rows of the step (rows past the last request's
+    get slot -1, so a captured step can be padded).  A request whose rows do
+    not fit, whose blocks the table has no room for, or for which the free
+    blocks do not last is left as it was, with slot -1 for its rows: its
+    length in the result has not grown.  Copy the result's lens and free_count
+    over the inputs before the next step.  At most 4096 requests."""
+    y = _ops.kv_plan(lens, new, block_table, free_blocks, free_count, block_size, tokens)
+    if y is not None:
+        return KVPlan(*y)
+    _require_gpu(lens, new, block_table, free_blocks, free_count)
+    lens = _ints(lens, None, "lens")
+    n = lens.numel()
+    new = _ints(new, n, "new")
+    free_count = _ints(free_count, 1, "free_count")
+    ldt = _table(block_table, n)
+    if free_blocks.dim() != 1 or free_blocks.dtype != torch.int32 or not free_blocks.is_contiguous():
+        raise HxmiError("free_blocks must be a contiguous 1-D torch.int32 tensor")
+    if tokens < 0:
+        raise HxmiError(f"tokens must be >= 0, got {tokens}")
+    empty = lambda k, dtype=torch.int32: torch.empty(k, dtype=dtype, device=lens.device)  # noqa: E731
+    out = KVPlan(empty(tokens, torch.int64), empty(tokens), empty(n + 1), empty(n), empty(1))
+    with _on(lens):
+        _check(load_library().hxmi_kv_plan(
+            lens.data_ptr(), new.data_ptr(), block_table.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(),
+            *(t.data_ptr() for t in out), n, block_table.shape[1], ldt, free_blocks.numel(), int(tokens),
+            int(block_size), _stream(lens)))
+    return out
+
+
+def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Write k and v rows [tokens, kv_heads, head_dim] (fp16 or bf16) to the
+    given slots [tokens] (int64; those outside the cache are skipped).  Rows of
+    one block are consecutive rows with consecutive slots, as kv_plan gives
+    them.  A block and head's scale is what its largest value needs: it grows
+    with later rows (earlier codes are rounded again) and starts anew when the
+    block's first token is written."""
+    if isinstance(cache, KVCache) and _ops.kv_append(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim,
+                                                     k, v, slots):
+        return
+    ptrs, (n, h, d, b) = _cache_args(cache)
+    _require_gpu(cache.k, k, v, slots)
+    if k.dtype not in (torch.float16, torch.bfloat16) or v.dtype != k.dtype:
+        raise HxmiError(f"kv_append takes fp16 or bf16 k and v of one dtype, got {k.dtype} and {v.dtype}")
+    if k.dim() != 3 or k.shape[1:] != (h, d) or v.shape != k.shape:
+        raise HxmiError(f"k and v must be [tokens, {h}, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    slots = _ints(slots, k.shape[0], "slots", torch.int64)
+    k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (k, v))
+    with _on(k):
+        _check(load_library().hxmi_kv_append(
+            int(k.dtype == torch.bfloat16), k.data_ptr(), v.data_ptr(), slots.data_ptr(), *ptrs, k.shape[0], n, h, d, b,
+            k.stride(0), k.stride(1), v.stride(0), v.stride(1), _stream(k)))
+
+
+def kv_read(cache: KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values held at slots [tokens] (int64), rounded to fp16 or
+    bf16: two tensors [tokens, kv_heads, head_dim], zeros for slots outside the
+    cache."""
+    if isinstance(cache, KVCache) and dtype in (torch.float16, torch.bfloat16):
+        y = _ops.kv_read(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim, slots, dtype == torch.bfloat16)
+        if y is not None:
+            return y
+    ptrs, (n, h, d, b) = _cache_args(cache)
+    _require_gpu(cache.k, slots)
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise HxmiError(f"kv_read gives fp16 or bf16, got {dtype}")
+    slots = _ints(slots, None, "slots", torch.int64)
+    k, v = (torch.empty((slots.numel(), h, d), dtype=dtype, device=slots.device) for _ in range(2))
+    with _on(slots):
+        _check(load_library().hxmi_kv_read(int(dtype == torch.bfloat16), *ptrs, slots.data_ptr(), k.data_ptr(),
+                                           v.data_ptr(), slots.numel(), n, h, d, b, _stream(slots)))
+    return k, v
+
+
+def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, *,
+                 cu: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of q [tokens, heads, head_dim] (fp16 or bf16) over the
+    cache.  Request r's rows cu[r] to cu[r+1] (without cu: one row each) are
+    the last of its lens[r] tokens, all of them in the cache by now: row i of n
+    sees keys j <= lens[r] - n + i of the pages block_table[r] (int32).
+    heads may be a multiple of the cache's kv_heads.  A row that sees no key
+    gets zeros; pages outside the cache are left out; rows that belong to no
+    request are not written (in a new result they hold nothing)."""
+    if isinstance(cache, KVCache):
+        y = _ops.kv_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim, block_table, lens, cu,
+                              scale, out)
+        if y is not None:
+            return out if out is not None else y
+    ptrs, (n, h, d, b) = _cache_args(cache)
+    _require_gpu(cache.k, q, block_table, lens, cu, out)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise HxmiError(f"kv_attention takes fp16 or bf16 q, got {q.dtype}")
+    if q.dim() != 3 or q.shape[2] != d or q.shape[1] % h:
+        raise HxmiError(f"q must be [tokens, a multiple of {h} heads, {d}], got {tuple(q.shape)}")
+    T, H, _ = q.shape
+    lens = _ints(lens, None, "lens")
+    R = lens.numel()
+    ldt = _table(block_table, R)
+    if cu is not None:
+        cu = _ints(cu, R + 1, "cu")
+    elif T != R:
+        raise HxmiError(f"without cu there is one row a request: q has {T} rows, lens {R} requests")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0 < ctypes.c_float(scale).value < float("inf"):
+        raise HxmiError(f"scale must be positive and finite, got {scale}")
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    o = out
+    if out is None:
+        o = torch.empty((T, H, d), dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise HxmiError(f"out must be {q.dtype} {tuple(q.shape)}")
+        s0, s1, s2 = out.stride()
+        apart = (T == 1 or s0 >= (H - 1) * s1 + d or (s0 >= d and (H == 1 or s1 >= (T - 1) * s0 + d))) \
+            and (H == 1 or s1 >= d)
+        same = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()  # (a tile has read its rows by then)
+        others = [t for t in (block_table, lens, cu, cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+        if not apart:
+            raise HxmiError(f"the rows of out must not share elements (strides {out.stride()})")
+        if s2 != 1 or (_overlap(q, out) and not same) or any(_overlap(t, out) for t in others):
+            return out.copy_(kv_attention(q, cache, block_table, lens, cu=cu, scale=scale))
+    lib = load_library()
+    with _on(q):
+        ws = _workspace(lib.hxmi_kv_attention_workspace_bytes(T, R, H, h, d, b, block_table.shape[1],
+                                                              int(cu is not None)), q.device)
+        _check(lib.hxmi_kv_attention(
+            int(q.dtype == torch.bfloat16), q.data_ptr(), *ptrs, block_table.data_ptr(), lens.data_ptr(), _ptr(cu),
+            o.data_ptr(), T, R, H, h, d, b, n, block_table.shape[1], ldt, q.stride(0), q.stride(1), o.stride(0),
+            o.stride(1), scale, _ptr(ws), 0 if ws is None else ws.numel() * 4, _stream(q)))
+    return o
+
+
+_SAMPLE_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[float, torch.Tensor] = 1.0,
+           top_k: Union[int, torch.Tensor] = 0, top_p: Union[float, torch.Tensor] = 1.0,
+           min_p: Union[float, torch.Tensor] = 0.0) -> torch.Tensor:
+    """A token (int64) for every row of logits [..., vocab] (fp16, bf16 or
+    fp32) at the row's random number u [...] (fp32, in [0, 1)).  The weights
+    exp((x - max) / temperature) of the tokens that top_k (0: all), top_p (1:
+    all) and min_p (0: all; relative to the largest) keep are summed in index
+    order; the first token whose running sum exceeds u times the whole is
+    taken.  Of equal logits the lowest index comes first.  temperature 0 takes
+    the largest logit.  Each parameter is a number or a tensor of the rows'
+    own (fp32, top_k int32).  A row with a NaN or no logit above -inf gives
+    -1."""
+    y = _ops.sample(logits, u, temperature, top_k, top_p, min_p)
+    if y is not None:
+        return y
+    given = [temperature, top_k, top_p, min_p]
+    _require_gpu(logits, u, *(p for p in given if isinstance(p, torch.Tensor)))
+    if logits.dtype not in _SAMPLE_TYPES or logits.dim() < 1:
+        raise HxmiError(f"sample takes fp16, bf16 or fp32 logits [..., vocab], got {logits.dtype}")
+    lead = logits.shape[:-1]
+    rows, vocab = math.prod(lead), logits.shape[-1]
+    if u.shape != lead or u.dtype != torch.float32:
+        raise HxmiError(f"u must be torch.float32 {tuple(lead)}, got {u.dtype} {tuple(u.shape)}")
+    ptrs, alls, keep = [], [], []
+    for name, p, dtype, neutral in zip(("temperature", "top_k", "top_p", "min_p"), given,
+                                       (torch.float32, torch.int32, torch.float32, torch.float32), (1.0, 0, 1.0, 0.0)):
+        if isinstance(p, torch.Tensor):
+            if p.shape != lead or p.dtype != dtype:
+                raise HxmiError(f"{name} must be a number or a {dtype} tensor {tuple(lead)}")
+            keep.append(p.contiguous())
+            ptrs.append(keep[-1].data_ptr())
+            alls.append(neutral)
+        else:
+            ptrs.append(None)
+            alls.append(max(-1, min(int(p), 2**31 - 1)) if dtype == torch.int32 else float(p))
+    out = torch.empty(lead, dtype=torch.int64, device=logits.device)
+    if rows == 0:
+        return out
+    x, u = logits.reshape(rows, vocab), u.contiguous()
+    if x.stride(1) != 1 and vocab > 1:
+        x = x.contiguous()
+    x = _own_rows(x)
+    with _on(x):
+        _check(load_library().hxmi_sample(_SAMPLE_TYPES[x.dtype], x.data_ptr(), u.data_ptr(), *ptrs, *alls,
+                                          out.data_ptr(), rows, vocab, _lead(x, "logits"), _stream(x)))
+    return out
 
 
 def release_workspaces() -> None:

@@ -445,6 +445,130 @@ int64_t hxmi_decode_workspace_bytes(int64_t hidden, int64_t kv_dim, int64_t inte
 int hxmi_decode_status(void* workspace, int clear, int* status, void* stream);
 
 /*
+ * The 8-bit key/value cache of a serving loop.  `blocks` blocks of block_size
+ * tokens (a power of two from 16 to 256), kv_heads heads of head_dim (a
+ * multiple of 8 up to 128; Dp = head_dim rounded up to 16):
+ *   k_codes int8 [blocks, kv_heads, block_size, Dp]
+ *   v_codes int8 [blocks, kv_heads, block_size / 16, Dp, 16]  (token 16 c + i
+ *           of a block, dimension d at [c, d, i])
+ *   k_scale, v_scale fp32 [blocks, kv_heads]
+ * A held value is code * scale.  Codes past head_dim must be zero (zero the
+ * cache once after allocating it).  Token t of a block b is slot
+ * b * block_size + t.  No counterpart in the reference, whose one-token run
+ * keeps no cache (benchmark_models/run_qwen2.5-0.5b.py:171-173, 224-233).
+ */
+
+/*
+ * Block table and slot map of one step, from the requests' lengths, on the
+ * GPU in one launch.  lens [requests]: tokens each holds; added: tokens it
+ * adds (0: idle, negative: it has ended and its blocks go back).  block_table
+ * [requests, width] (row stride ld_table) and the stack of free blocks
+ * free_blocks [capacity], whose first *free_count entries are free, are
+ * updated in place: ended requests' blocks go onto the stack in request order,
+ * then requests take what they need from its top in request order.  A request
+ * gets its blocks if its rows lie within `tokens`, its blocks within the
+ * table, and it needs none or what it and the requests before it need (those
+ * that meet the first two) is there; otherwise it stays as it was and has no
+ * slots, so that a caller sees it by its length.
+ * Outputs: cu [requests + 1], prefix sums of the tokens added (rows cu[r] to
+ * cu[r+1] are request r's); slots [tokens] and positions [tokens] of those
+ * rows, -1 and 0 for rows without a place and rows past cu[requests];
+ * lens_out; free_count_out.  Entries of the stack past the new count hold
+ * nothing.  The outputs must not be the inputs (copy them over afterwards).
+ * At most 4096 requests a call.
+ */
+int hxmi_kv_plan(const int32_t* lens, const int32_t* added, int32_t* block_table, int32_t* free_blocks,
+                 const int32_t* free_count, int64_t* slots, int32_t* positions, int32_t* cu, int32_t* lens_out,
+                 int32_t* free_count_out, int64_t requests, int64_t width, int64_t ld_table, int64_t capacity,
+                 int64_t tokens, int64_t block_size, void* stream);
+
+/*
+ * Writes k and v rows [tokens, kv_heads, head_dim] (fp16, or bf16 with
+ * is_bf16 = 1; row strides ldk / ldv, head strides head_stride_*, elements,
+ * any alignment of the type) to the given slots.  Slots outside the cache are
+ * skipped.  Rows of one block must be consecutive rows of the call with
+ * consecutive slots, as hxmi_kv_plan lays them out (otherwise what that block
+ * holds is unspecified).  Per block and head of K and of V:
+ *   amax  = largest magnitude among the rows written
+ *   old   = 0 if the block's first token is among them (the block starts
+ *           anew), else its scale
+ *   scale = old if amax <= 127 * old, else the smallest number of 11
+ *           significant bits that is at least amax / 127 (and 2^-100); codes
+ *           already in the block become rint(code * old / scale)
+ *   code  = rint(value / scale), half to even
+ * so a value is off by at most half a step of the scale of its write, plus
+ * half a step of each scale it has moved to since.  A row that is not finite
+ * makes the scale NaN until the block starts anew.
+ */
+int hxmi_kv_append(int is_bf16, const void* k, const void* v, const int64_t* slots, int8_t* k_codes, int8_t* v_codes,
+                   float* k_scale, float* v_scale, int64_t tokens, int64_t blocks, int64_t kv_heads, int64_t head_dim,
+                   int64_t block_size, int64_t ldk, int64_t head_stride_k, int64_t ldv, int64_t head_stride_v,
+                   void* stream);
+
+/* The values held at the given slots, rounded once to fp16 / bf16 (at most
+ * the type's largest finite number), into contiguous k and v [tokens,
+ * kv_heads, head_dim]; zeros for slots outside the cache. */
+int hxmi_kv_read(int is_bf16, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                 const int64_t* slots, void* k, void* v, int64_t tokens, int64_t blocks, int64_t kv_heads,
+                 int64_t head_dim, int64_t block_size, void* stream);
+
+/*
+ * Causal attention over the cache.  q / o [tokens, heads, head_dim] (fp16 or
+ * bf16, any row and head strides), query head h reads key/value head
+ * h / (heads / kv_heads).  Request r has rows cu[r] to cu[r+1] (cu NULL: one
+ * row each, tokens == requests), its last ones, and lens[r] tokens in the
+ * cache, these rows' own among them: row i of n sees keys j <= lens[r] - n + i,
+ *   o = softmax_j(scale * q . K_j) . V_j,
+ * K_j and V_j the held values of page block_table[r][j / block_size], fp32
+ * scores, softmax and accumulation.  Keys of a page outside the cache are
+ * left out; a row that sees no key gives zeros; rows of no request are not
+ * written.  scale > 0 and finite.
+ * workspace: as for hxmi_gemm_f16 (zeroed once after allocation, left zeroed,
+ * one call at a time), hxmi_kv_attention_workspace_bytes() bytes; with few
+ * rows the keys are shared out over workgroups that join their parts there.
+ * NULL runs unshared.
+ */
+int hxmi_kv_attention(int is_bf16, const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
+                      const float* v_scale, const int32_t* block_table, const int32_t* lens, const int32_t* cu,
+                      void* o, int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                      int64_t block_size, int64_t blocks, int64_t width, int64_t ld_table, int64_t ldq,
+                      int64_t head_stride_q, int64_t ldo, int64_t head_stride_o, float scale, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of hxmi_kv_attention for these sizes (ragged: a cu is
+ * given); 0: the keys are not shared out. */
+int64_t hxmi_kv_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
+                                          int64_t head_dim, int64_t block_size, int64_t width, int ragged);
+
+/* Types of hxmi_sample's logits. */
+#define HXMI_SAMPLE_F16 0
+#define HXMI_SAMPLE_BF16 1
+#define HXMI_SAMPLE_F32 2
+
+/*
+ * tokens[r] sampled from row r of logits [rows, vocab] (row stride ldx) at
+ * the given u[r] in [0, 1):
+ *   w_i = exp((x_i - max x) / temperature)
+ *   top_k  keeps the k largest (k <= 0 or >= vocab: all)
+ *   top_p  keeps, in descending order, the tokens before which the weight is
+ *          below p * (weight of the top_k) (p >= 1: all; the first always)
+ *   min_p  keeps w_i >= min_p (min_p <= 0: all)
+ *   tokens[r] = the lowest kept index whose running weight, in index order,
+ *          exceeds u * (kept weight)
+ * Of equal logits the lowest index comes first.  temperature 0 (or below, in
+ * a row's own) takes the largest logit.  A row with a NaN or with no logit
+ * above -inf gives -1.  Parameters are per row (pointers of `rows` entries)
+ * or, where NULL, the all_* value.  Weights are held as integers of 44 or
+ * more fraction bits (vocab <= 2^18), so the token does not depend on an
+ * order of summation.  vocab <= 2^20.
+ * No counterpart in the reference, which takes the argmax of its logits on
+ * the host (benchmark_models/run_qwen2.5-0.5b.py:224-233).
+ */
+int hxmi_sample(int dtype, const void* logits, const float* u, const float* temperature, const int32_t* top_k,
+                const float* top_p, const float* min_p, float all_temperature, int32_t all_top_k, float all_top_p,
+                float all_min_p, int64_t* tokens, int64_t rows, int64_t vocab, int64_t ldx, void* stream);
+
+/*
  * Region profiling hook: enqueues on `stream` a one-wave marker that, when it
  * runs (after every kernel enqueued before it on that stream has finished),
  * writes record `slot` of `records` -- three uint32 words {id, t low word,

@@ -9,21 +9,27 @@
 //   token   the lowest kept i whose running weight exceeds u * (kept weight)
 //
 // Weights are integers, round(w * 2^shift) with room for the whole row's sum
-// in 62 bits (44 fraction bits at a vocabulary of 2^18): integer sums do not
-// depend on their order, so neither does the token, and every comparison above
-// is exact in them (p * sum and u * sum as 128-bit products).  w comes from a
-// 64-bit evaluation good to 2^-48, a few 2^-45 of the largest weight in all.
-// fp32 sums would put about one row in a hundred of a flat distribution on
-// another token.
+// in 62 bits (44 fraction bits at a vocabulary of 2^18, 50 at most): integer
+// sums do not depend on their order, so neither does the token, and every
+// comparison above is exact in them (p * sum and u * sum as 128-bit products).
+// w comes from a 64-bit evaluation good to 2^-48.  fp32 sums would put about
+// one row in a hundred of a flat distribution on another token.
 //
-// One workgroup a row.  top-k and top-p are thresholds on the logits: a radix
-// descent over order-preserving integer keys (8 bits a pass; 16-bit logits
-// have 16-bit keys, fp32 ones 32) gives the key of the last token kept and
-// how many of its equals stay.  The pass's histogram has a column for each
-// lane: no two lanes of a wave meet in one counter however the logits
-// cluster.  The last passes sum the kept weights by pieces of 512 tokens,
-// then look inside one piece.  Bound by the passes over a row in L2 (2-3 us
-// each at 151936 16-bit logits) and the 64-bit weights.
+// One workgroup a row.  top-k and top-p are thresholds on the logits, kept as
+// the key (an integer that orders as the logits do) of the last token kept and
+// the number of its equals that stay:
+//   * tokens so far below the largest that their weight is 0 take no part;
+//   * the others are counted by the upper 16 bits of their keys in LDS (65536
+//     counts of 16 bits, 128 KB).  For 16-bit logits that is every value, and
+//     both thresholds follow from counts and one weight a value;
+//   * fp32 logits: the tokens of the top k's bins go on a list in LDS, on which
+//     both thresholds are found bit by bit; without top-k the weights are summed
+//     by the upper 14 bits and the list is the threshold's bin;
+//   * where a count passes 16 bits (more than 65535 equal values) or a list
+//     its room, a radix descent over the row, 8 bits a pass with a column of
+//     the histogram for each lane, takes their place.
+// Then the kept weights are summed by pieces of 512 tokens, the piece that
+// reaches u * sum is found and the token in it.
 #include "hxmi_common.h"
 #include "hxmi_internal.h"
 
@@ -49,112 +55,207 @@ struct SArgs {
 
 constexpr int NT = 1024, NW = NT / 64, PIECE = 512;
 constexpr int kMaxPieces = kSampleMaxVocab / PIECE;
+constexpr int kList = 8192;
 
-// Keys that order as the logits do, equal for -0 and 0.
+// A logit's key: an unsigned integer that orders as the logits do, equal for
+// -0 and 0 (its magnitude's bits under its sign, moved up by half the range).
 template <typename T>
-struct Key;
-template <>
-struct Key<_Float16> {
+struct Key {
   static constexpr int bits = 16;
-  static __device__ __forceinline__ uint32_t of(_Float16 v) {
-    const uint32_t b = __builtin_bit_cast(unsigned short, (_Float16)(v + (_Float16)0.f));
-    return b & 0x8000u ? 0xffffu & ~b : b | 0x8000u;
-  }
-};
-template <>
-struct Key<__bf16> {
-  static constexpr int bits = 16;
-  static __device__ __forceinline__ uint32_t of(__bf16 v) {
-    uint32_t b = __builtin_bit_cast(unsigned short, v);
-    b = b == 0x8000u ? 0 : b;
-    return b & 0x8000u ? 0xffffu & ~b : b | 0x8000u;
+  static constexpr uint32_t zero = 0x8000, magnitude = 0x7fff;
+  static constexpr uint32_t inf = std::is_same_v<T, _Float16> ? 0x7c00 : 0x7f80;
+  static __device__ __forceinline__ uint32_t of(T v) {
+    const short b = __builtin_bit_cast(short, v), s = b >> 15;
+    return (uint32_t)(uint16_t)(short)((b ^ (s & 0x7fff)) - s) ^ zero;
   }
 };
 template <>
 struct Key<float> {
   static constexpr int bits = 32;
+  static constexpr uint32_t zero = 0x80000000u, magnitude = 0x7fffffffu, inf = 0x7f800000u;
   static __device__ __forceinline__ uint32_t of(float v) {
-    const uint32_t b = __float_as_uint(v + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const int b = (int)__float_as_uint(v), s = b >> 31;
+    return (uint32_t)((b ^ (s & 0x7fffffff)) - s) ^ zero;
   }
 };
+template <typename T>
+__device__ __forceinline__ float value_of(uint32_t key) {
+  const bool neg = key < Key<T>::zero;
+  const uint32_t mag = neg ? Key<T>::zero - key : key - Key<T>::zero, b = neg ? mag | Key<T>::zero : mag;
+  if constexpr (Key<T>::bits == 32) return __uint_as_float(b);
+  else return (float)__builtin_bit_cast(T, (unsigned short)b);
+}
 
-// 2^(j / 32)
-struct Exp2Table {
-  double v[32];
+// The weights of a row: round(2^shift * 2^y), y = (v - max) * log2(e) / T.
+struct Weights {
+  double rate32;  // 32 log2(e) / T
+  double xmax;
+  int shift;
+  const double* table;  // 2^(j / 32)
+  int infinite;         // the largest logit is (in a scalar register)
+
+  __device__ __forceinline__ uint64_t one() const { return 1ull << shift; }
+  __device__ __forceinline__ uint64_t of(float v) const {
+    if (infinite) return (double)v == xmax ? one() : 0;
+    // k = round(32 y), from the low bits of y + 1.5 * 2^52; 2^(r / 32) by its
+    // Taylor series, |r ln 2 / 32| <= 0.0109: the first term left out is below 2^-48
+    const double y = fmax(((double)v - xmax) * rate32, -32.0 * 120);
+    const double t = y + 0x1.8p52, r = y - (t - 0x1.8p52);
+    const int k = (int)__double2loint(t);
+    constexpr double z = 0.69314718055994530942 / 32;
+    double p = z * z * z * z * z / 120;
+    p = __builtin_fma(p, r, z * z * z * z / 24);
+    p = __builtin_fma(p, r, z * z * z / 6);
+    p = __builtin_fma(p, r, z * z / 2);
+    p = __builtin_fma(p, r, z);
+    p = __builtin_fma(p, r, 1.0);
+    const double w = __builtin_ldexp(table[k & 31] * p, (k >> 5) + shift) + 0x1p52;  // (rounds; below 2^51)
+    return (uint64_t)__double_as_longlong(w) & 0xfffffffffffffull;
+  }
 };
-__device__ __forceinline__ double exp2_poly(double r) {
-  // 2^r = e^(r ln 2) for |r| <= 1/64, Taylor to degree 6: the next term is below 2^-58
-  const double z = r * 0.69314718055994530942;
-  double p = 1.0 / 720;
-  p = __builtin_fma(p, z, 1.0 / 120);
-  p = __builtin_fma(p, z, 1.0 / 24);
-  p = __builtin_fma(p, z, 1.0 / 6);
-  p = __builtin_fma(p, z, 0.5);
-  p = __builtin_fma(p, z, 1.0);
-  return __builtin_fma(p, z, 1.0);
-}
-// w * 2^shift for y = log2 w <= 0 (0 far below).
-__device__ __forceinline__ double weight(double y, int shift, const double* table) {
-  y = y > -1000.0 ? y : -1000.0;
-  const double k = __builtin_rint(y * 32.0);
-  const int j = (int)k;
-  return __builtin_ldexp(table[j & 31] * exp2_poly(__builtin_fma(k, -1.0 / 32, y)), (j >> 5) + shift);
-}
-__device__ __forceinline__ uint64_t to_fixed(double w) { return (uint64_t)__builtin_rint(w); }
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) {
   return ((uint64_t)(uint32_t)__shfl((int)(v >> 32), lane, 64) << 32) | (uint32_t)__shfl((int)v, lane, 64);
 }
-__device__ __forceinline__ uint64_t scan64(uint64_t v) {  // inclusive, over the wave
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t t = __shfl_up((unsigned long long)v, o, 64);
-    if (lane >= o) v += t;
-  }
-  return v;
+// Inclusive sum over the wave in lane order, by DPP: within rows of 16 lanes,
+// then each row's last lane to the next row, then lane 31 to the upper half.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_add64(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ uint64_t scan64(uint64_t v) {
+  v = dpp_add64<0x111, 0xf>(v);  // row_shr:1
+  v = dpp_add64<0x112, 0xf>(v);
+  v = dpp_add64<0x114, 0xf>(v);
+  v = dpp_add64<0x118, 0xf>(v);
+  v = dpp_add64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  return dpp_add64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
 }
 // floor(f * 2^64) of f in [0, 1)
 __device__ __forceinline__ uint64_t fraction64(float f) {
-  return (uint64_t)((double)f * 0x1p32) << 32 |
-         (uint64_t)(((double)f * 0x1p32 - __builtin_floor((double)f * 0x1p32)) * 0x1p32);
+  const double g = (double)f * 0x1p32, hi = __builtin_floor(g);
+  return (uint64_t)(uint32_t)hi << 32 | (uint32_t)((g - hi) * 0x1p32);
 }
 
 struct Shared {
   union {
-    unsigned long long mass[256][64];
+    uint32_t count2[32768];         // 16-bit counts of the upper 16 bits of a key, two a word
+    unsigned long long bin[16384];  // weights by the upper 14 bits
+    unsigned long long mass[256][64];  // radix descent: a column a lane
     uint32_t count[256][64];
+    struct {
+      uint32_t key[kList];
+      unsigned long long weight[kList];
+    } list;
     struct {
       unsigned long long sum[kMaxPieces];  // kept weight of a piece, less its equals of the last key
       uint32_t ties[kMaxPieces];
+      uint32_t kept[NW][PIECE];
     } piece;
   };
+  unsigned long long group[NT];  // of 64 bins each: their weight,
+  uint32_t group_count[NT];      // their count
   double table[32];
   unsigned long long part[NW];
   uint32_t upart[NW];
-  uint32_t key;
+  uint32_t key, listed;
   unsigned long long above;
 };
 
-// The eight logits of piece-lane i (8 i .. 8 i + 7); `n` of them exist.
+// Eight logits as they lie, and their keys.
 template <typename T>
-__device__ __forceinline__ int load8(const T* x, int i, int vocab, T (&v)[8]) {
-  const int at = i * 8, n = vocab - at;
-  if (n >= 8) {
+struct Eight {
+  int4v r[sizeof(T) / 2];
+
+  __device__ __forceinline__ void load(const T* x) {
     if constexpr (sizeof(T) == 2) {
-      const int4v r = *(const int4u2*)(x + at);
-      __builtin_memcpy(v, &r, 16);
+      r[0] = *(const int4u2*)x;
     } else {
-      const int4v r0 = *(const int4u4*)(x + at), r1 = *(const int4u4*)(x + at + 4);
-      __builtin_memcpy(v, &r0, 16);
-      __builtin_memcpy(v + 4, &r1, 16);
+      r[0] = *(const int4u4*)x;
+      r[1] = *(const int4u4*)(x + 4);
     }
-    return 8;
   }
+  __device__ __forceinline__ void keys(uint32_t (&key)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+      typedef short short2v __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = e < n ? x[at + e] : (T)0.f;
-  return n < 0 ? 0 : n;
+      for (int e = 0; e < 4; ++e) {  // two at a time
+        const int bits = r[0][e];
+        const short2v b = __builtin_bit_cast(short2v, bits), s = b >> 15;
+        const uint32_t k2 = __builtin_bit_cast(uint32_t, (short2v)((b ^ (s & (short)0x7fff)) - s)) ^ 0x80008000u;
+        key[2 * e] = k2 & 0xffffu;
+        key[2 * e + 1] = k2 >> 16;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) key[e] = Key<T>::of(__uint_as_float((uint32_t)r[e >> 2][e & 3]));
+    }
+  }
+};
+// The keys of logits 8 i .. 8 i + 7, 0 (no logit's key, below them all) past the row.
+template <typename T>
+__device__ __forceinline__ void load_keys(const T* x, int i, int vocab, uint32_t (&key)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) key[e] = i * 8 + e < vocab ? Key<T>::of(x[i * 8 + e]) : 0;
+}
+
+// f(keys of logits 8 i .. 8 i + 7, j) for i = i0 + step * j, j < U: the loads
+// all ahead of the first use where the whole wave's are inside the row.
+template <int U, typename T, typename F>
+__device__ __forceinline__ void load_groups(const T* x, int i0, int step, int vocab, F&& f) {
+  if (__all((i0 + step * (U - 1)) * 8 + 8 <= vocab)) {
+    Eight<T> raw[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) raw[j].load(x + (i0 + step * j) * 8);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      uint32_t key[8];
+      raw[j].keys(key);
+      f(key, j);
+    }
+  } else {
+    for (int j = 0; j < U; ++j) {
+      uint32_t key[8];
+      load_keys(x, i0 + step * j, vocab, key);
+      f(key, j);
+    }
+  }
+}
+
+// f(key) for the logits of a row (and for a few keys 0, which none has).
+template <int U, typename T, typename F>
+__device__ __forceinline__ void each_key(const T* x, int vocab, F&& f) {
+  const int lanes = (vocab + 7) >> 3, wave0 = threadIdx.x & ~63;
+  for (int i0 = wave0; i0 < lanes; i0 += NT * U)  // (a wave stays together)
+    load_groups<U>(x, i0 + (threadIdx.x & 63), NT, vocab, [&](const uint32_t (&key)[8], int) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f(key[e]);
+    });
+}
+
+// Inclusive sum over the workgroup's threads and (in `total`) the whole.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, Shared& sh, uint64_t& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  v = scan64(v);
+  __syncthreads();
+  if (lane == 63) sh.part[w] = v;
+  __syncthreads();
+  uint64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const uint64_t t = sh.part[i];
+    before += i < w ? t : 0;
+    total += t;
+  }
+  return before + v;
+}
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, Shared& sh) {
+  uint64_t total;
+  block_scan(v, sh, total);
+  return total;
 }
 
 template <typename T>
@@ -163,62 +264,66 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t row = blockIdx.x;
   const T* const x = (const T*)a.x + row * a.ldx;
-  const int lanes = (a.vocab + 7) >> 3;  // groups of eight logits
+  const int vocab = a.vocab;
   constexpr int KB = Key<T>::bits;
 
   if (threadIdx.x < 32) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 32);
 
-  // the largest logit and its first index
-  uint32_t top = 0, first = 0;
-  bool bad = false;
-  for (int i = threadIdx.x; i < lanes; i += NT) {
-    T v[8];
-    const int n = load8(x, i, a.vocab, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (e >= n) continue;
-      const uint32_t key = Key<T>::of(v[e]);
-      bad |= v[e] != v[e];
-      if (key > top) {  // (a lane's indices grow)
-        top = key;
-        first = i * 8 + e;
-      }
-    }
-  }
+  // the largest logit; NaNs have keys over inf's or under -inf's
+  uint32_t top = 0, low = 0xffffffffu;
+  each_key<4>(x, vocab, [&](uint32_t key) {
+    top = max(top, key);
+    low = min(low, key - 1);  // (0, no key, goes past every other)
+  });
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
-    const uint32_t k2 = __shfl_xor((int)top, o, 64), f2 = __shfl_xor((int)first, o, 64);
-    if (k2 > top || (k2 == top && f2 < first)) {
-      top = k2;
-      first = f2;
-    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    low = min(low, (uint32_t)__shfl_xor((int)low, o, 64));
   }
-  bad = __any(bad);
-  if (lane == 0) {
-    sh.part[w] = ((unsigned long long)top << 32) | first;
-    sh.upart[w] = bad;
-  }
+  if (lane == 0) sh.part[w] = ((unsigned long long)top << 32) | low;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
-    const uint32_t k2 = (uint32_t)(sh.part[i] >> 32), f2 = (uint32_t)sh.part[i];
-    bad |= sh.upart[i] != 0;
-    if (k2 > top || (k2 == top && f2 < first)) {
-      top = k2;
-      first = f2;
-    }
+    top = max(top, (uint32_t)(sh.part[i] >> 32));
+    low = min(low, (uint32_t)sh.part[i]);
   }
-  const float xmax = (float)x[first];
+  constexpr uint32_t kInf = Key<T>::zero + Key<T>::inf, kMinusInf = Key<T>::zero - Key<T>::inf;
+  if (top > kInf || low + 1 < kMinusInf || top == kMinusInf) {
+    if (threadIdx.x == 0) a.token[row] = -1;
+    return;
+  }
+  const float xmax = value_of<T>(top);
   const float t = a.temperature ? a.temperature[row] : a.t;
-  if (bad || xmax == -INFINITY || !(t > 0.f)) {
-    if (threadIdx.x == 0) a.token[row] = bad || xmax == -INFINITY ? -1 : (int64_t)first;
+  if (!(t > 0.f)) {  // the first of the largest
+    if (threadIdx.x == 0) sh.key = 0xffffffffu;
+    __syncthreads();
+    for (int i = threadIdx.x; i < (vocab + 7) >> 3; i += NT) {
+      uint32_t key[8];
+      load_keys(x, i, vocab, key);
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (key[e] == top) atomicMin(&sh.key, (uint32_t)(i * 8 + e));
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) a.token[row] = (int64_t)sh.key;
     return;
   }
   const double rate = 1.44269504088896340736 / (double)t;
-  // (the largest logit's weight is 1 also where it is infinite)
-  auto weight_of = [&](float v) {
-    return v == xmax ? __builtin_ldexp(1.0, a.shift) : weight(((double)v - (double)xmax) * rate, a.shift, sh.table);
+  const Weights weights{rate * 32, (double)xmax, a.shift, sh.table,
+                        __builtin_amdgcn_readfirstlane(xmax == INFINITY)};
+  // Logits with keys below `cut` have a weight that rounds to 0: they change no
+  // sum, and whether the top k holds some of them changes nothing.  (Any value
+  // under the rounding of a bound is under the bound.)
+  auto key_from = [&](double v) {  // the key from which logits are at least v (of a NaN: all)
+    const float f = (float)v;
+    if constexpr (KB == 32) return f != f ? 1u : max(1u, Key<float>::of(f));
+    else {
+      // (rounded to 16 bits: down to a value, or up to one that v's side of it is all below)
+      const T h = (T)f;
+      return f != f ? 1u : max(1u, Key<T>::of(h));
+    }
   };
+  const uint32_t cut = min(top, key_from((double)xmax - (a.shift + 3) / rate * 1.000001));
 
   // Descends to the key at which the counts (or weights) from the largest key
   // down first reach `goal`; `above`: what lies over that key.
@@ -233,18 +338,11 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
         else ((unsigned long long*)sh.mass)[i] = 0;
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < lanes; i += NT) {
-        T v[8];
-        const int n = load8(x, i, a.vocab, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t key = Key<T>::of(v[e]);
-          if (e < n && (b + 8 >= KB || key >> (b + 8) == prefix)) {
-            if constexpr (COUNT) atomicAdd(&sh.count[(key >> b) & 255][lane], 1u);
-            else atomicAdd(&sh.mass[(key >> b) & 255][lane], (unsigned long long)to_fixed(weight_of((float)v[e])));
-          }
-        }
-      }
+      each_key<1>(x, vocab, [&](uint32_t key) {
+        if (key < cut || (b + 8 < KB && key >> (b + 8) != prefix)) return;
+        if constexpr (COUNT) atomicAdd(&sh.count[(key >> b) & 255][lane], 1u);
+        else atomicAdd(&sh.mass[(key >> b) & 255][lane], (unsigned long long)weights.of(value_of<T>(key)));
+      });
       __syncthreads();
       // Each wave sums 16 digits' columns; then wave 0 looks for the digit.
       for (int d = w * 16; d < w * 16 + 16; ++d) {
@@ -284,135 +382,300 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     return prefix;
   };
 
+  // ---- counts by the upper 16 bits ------------------------------------------------
+  // Thread t owns the 64 bins from 64 * (1023 - t) on: threads in order go
+  // from the largest keys down.
+  const uint32_t bin0 = 64u * (NT - 1 - threadIdx.x);
+  auto count_of = [&](uint32_t bin) -> uint32_t { return sh.count2[bin >> 1] >> (16 * (bin & 1)) & 0xffffu; };
+  // Counts the tokens with a weight (`counted` in all); false if a count passed 16 bits.
+  uint64_t counted = 0, count_incl = 0, count_own = 0;
+  auto count_keys = [&]() {
+    int4v* const z = (int4v*)sh.count2;
+    for (int i = threadIdx.x; i < 32768 / 4; i += NT) z[i] = int4v{};
+    __syncthreads();
+    uint32_t mine = 0;
+    each_key<4>(x, vocab, [&](uint32_t key) {
+      if (key < cut) return;
+      const uint32_t bin = key >> (KB - 16);
+      atomicAdd(&sh.count2[bin >> 1], 1u + (bin & 1) * 0xffffu);
+      ++mine;
+    });
+    counted = block_sum(mine, sh);
+    count_own = 0;
+    for (int j = 0; j < 32; ++j) {
+      const uint32_t two = sh.count2[(bin0 >> 1) + ((j + threadIdx.x) & 31)];  // (banks apart)
+      count_own += (two & 0xffffu) + (two >> 16);
+    }
+    uint64_t held;
+    count_incl = block_scan(count_own, sh, held);
+    return held == counted;  // (a carry loses 65535 of 65536)
+  };
+  // The bin, from the largest down, at which per-thread sums (`incl`
+  // inclusive, `own`, of weight_of_bin over a thread's bins) reach the goal;
+  // `above`: what lies over it.
+  auto find_bin = [&](uint64_t incl, uint64_t own, uint64_t goal, uint64_t& above, auto&& weight_of_bin) {
+    __syncthreads();
+    if (incl >= goal && incl - own < goal) {  // (one thread)
+      sh.key = bin0;
+      sh.above = incl - own;
+    }
+    __syncthreads();
+    const uint32_t base = sh.key;
+    const uint64_t over = sh.above;
+    const uint32_t bin = base + 63 - lane;
+    const uint64_t mine = weight_of_bin(bin), s = over + scan64(mine);  // (every wave the same)
+    const int at = __ffsll((unsigned long long)__ballot(s >= goal)) - 1;
+    above = shfl64(s - mine, at);
+    return base + 63 - (uint32_t)at;
+  };
+
   // Kept: keys over `tau`, and the first `equal` tokens whose key is tau.
-  uint32_t tau = 0;
-  uint32_t equal = 0xffffffffu;
+  uint32_t tau = 0, equal = 0;
   const int k = a.top_k ? a.top_k[row] : a.k;
-  if (k > 0 && k < a.vocab) {
+  const float p = a.top_p ? a.top_p[row] : a.p;
+  bool need_k = k > 0 && k < vocab, need_p = !(p >= 1.f);
+  const uint64_t pf = fraction64(p > 0.f ? fminf(p, 0x1.fffffep-1f) : 0.f);
+  auto goal_of = [&](uint64_t whole) {  // ceil(p * whole), at least 1
+    const uint64_t g = __umul64hi(pf, whole) + (pf * whole != 0);
+    return g > 1 ? g : 1;
+  };
+  // How many equals of tau make up what `above` leaves to the goal (which
+  // tau's weight reaches, so it is not 0).
+  auto equals_of = [&](uint64_t goal, uint64_t above) {
+    const uint64_t wt = weights.of(value_of<T>(tau));
+    return (uint32_t)min((goal - above + wt - 1) / wt, (uint64_t)0xffffffffu);
+  };
+
+  // List in LDS of the keys that `in` takes: their number (over kList: not all are there).
+  auto make_list = [&](auto&& in) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    each_key<4>(x, vocab, [&](uint32_t key) {
+      if (key >= cut && in(key)) {
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kList) sh.list.key[at] = key;
+      }
+    });
+    __syncthreads();
+    const uint32_t n = sh.listed;
+    if (n <= kList)
+      for (uint32_t i = threadIdx.x; i < n; i += NT) sh.list.weight[i] = weights.of(value_of<T>(sh.list.key[i]));
+    __syncthreads();
+    return n;
+  };
+  auto list_count = [&](uint32_t n, uint32_t from) {  // listed keys >= from
+    uint32_t c = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += NT) c += sh.list.key[i] >= from;
+    return block_sum(c, sh);
+  };
+  auto list_weight = [&](uint32_t n, uint32_t over) {  // weight of the listed keys > over
+    uint64_t c = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += NT) c += sh.list.key[i] > over ? sh.list.weight[i] : 0;
+    return block_sum(c, sh);
+  };
+  // The largest key from lo to hi down to which the list's weight, with
+  // `base`, reaches the goal (at lo it does).
+  auto list_key = [&](uint32_t n, uint32_t lo, uint32_t hi, uint64_t base, uint64_t goal) {
+    while (lo < hi) {
+      const uint32_t mid = lo + ((hi - lo + 1) >> 1);
+      if (base + list_weight(n, mid - 1) >= goal) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  };
+
+  if constexpr (KB == 16) {
+    if ((need_k || need_p) && count_keys()) {
+      if (need_k && (uint64_t)k < counted) {
+        uint64_t above;
+        tau = find_bin(count_incl, count_own, (uint64_t)k, above, [&](uint32_t bin) -> uint64_t { return count_of(bin); });
+        equal = (uint32_t)(k - above);
+      }
+      if (need_p) {
+        auto masses = [&](uint32_t bin) -> uint64_t {
+          const uint32_t c = bin > tau ? count_of(bin) : bin == tau ? min(count_of(bin), equal) : 0;
+          return c ? c * weights.of(value_of<T>(bin)) : 0;
+        };
+        // each wave takes every 16th group of 64 bins, those that hold something
+        sh.group_count[threadIdx.x] = (uint32_t)count_own;
+        __syncthreads();
+        const uint32_t some = sh.group_count[lane * NW + w];
+        if (some == 0) sh.group[lane * NW + w] = 0;
+        for (uint64_t left = __ballot(some != 0); left; left &= left - 1) {
+          const int g = (__ffsll((unsigned long long)left) - 1) * NW + w;
+          const uint64_t sum = scan64(masses(64u * (NT - 1 - g) + lane));
+          if (lane == 63) sh.group[g] = sum;
+        }
+        __syncthreads();
+        const uint64_t own = sh.group[threadIdx.x];
+        uint64_t whole, above;
+        const uint64_t incl = block_scan(own, sh, whole), goal = goal_of(whole);
+        tau = find_bin(incl, own, goal, above, masses);
+        equal = equals_of(goal, above);
+      }
+      need_k = need_p = false;
+    } else if (need_k && (uint64_t)k >= counted) {
+      need_k = false;
+    }
+  } else {
+    if (need_k) {
+      const bool ok = count_keys();
+      if ((uint64_t)k >= counted) {
+        need_k = false;
+      } else if (ok) {
+        uint64_t above;
+        const uint32_t bin =
+            find_bin(count_incl, count_own, (uint64_t)k, above, [&](uint32_t b) -> uint64_t { return count_of(b); });
+        if (above + count_of(bin) <= kList) {
+          const uint32_t n = make_list([&](uint32_t key) { return key >> 16 >= bin; });
+          tau = bin << 16;
+          for (int b = 15; b >= 0; --b)
+            if (list_count(n, tau | 1u << b) >= (uint64_t)k) tau |= 1u << b;
+          equal = (uint32_t)(k - list_count(n, tau + 1));  // (tau is no key past +inf's)
+          if (need_p) {
+            const uint64_t goal = goal_of(list_weight(n, tau) + equal * weights.of(value_of<T>(tau)));
+            tau = list_key(n, tau, top, 0, goal);
+            equal = equals_of(goal, list_weight(n, tau));
+          }
+          need_k = need_p = false;
+        }
+      }
+    }
+    if (!need_k && need_p) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < 16384; i += NT) sh.bin[i] = 0;
+      __syncthreads();
+      each_key<1>(x, vocab, [&](uint32_t key) {
+        if (key >= cut) atomicAdd(&sh.bin[key >> 18], (unsigned long long)weights.of(value_of<T>(key)));
+      });
+      __syncthreads();
+      uint64_t own = 0, whole;
+      const uint32_t b0 = 16u * (NT - 1 - threadIdx.x);  // (threads from the largest keys down)
+      for (int j = 0; j < 16; ++j) own += sh.bin[b0 + ((j + threadIdx.x) & 15)];
+      const uint64_t incl = block_scan(own, sh, whole), goal = goal_of(whole);
+      __syncthreads();
+      if (incl >= goal && incl - own < goal) {  // (one thread)
+        uint64_t over = incl - own;
+        int j = 15;
+        for (; j > 0 && over + sh.bin[b0 + j] < goal; --j) over += sh.bin[b0 + j];
+        sh.key = b0 + j;
+        sh.above = over;
+      }
+      __syncthreads();
+      const uint32_t bin = sh.key;
+      const uint64_t above = sh.above;
+      const uint32_t n = make_list([&](uint32_t key) { return key >> 18 == bin; });
+      if (n <= kList) {
+        tau = list_key(n, bin << 18, min(bin << 18 | 0x3ffffu, top), above, goal);
+        equal = equals_of(goal, above + list_weight(n, tau));
+        need_p = false;
+      }
+    }
+  }
+  if (need_k) {
     uint64_t above;
     tau = descend(std::true_type{}, (uint64_t)k, above);
     equal = (uint32_t)((uint64_t)k - above);
   }
-  auto value_of = [&](uint32_t key) -> float {
-    if constexpr (KB == 32) return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-    else return (float)__builtin_bit_cast(T, (unsigned short)(key & 0x8000u ? key & 0x7fffu : ~key));
-  };
 
-  // Sum over the workgroup of what each piece keeps; fills the pieces' sums
-  // and equals of tau.
-  const int pieces = (lanes + 63) >> 6;
-  const float mp = a.min_p ? a.min_p[row] : a.m;
-  auto pieces_of = [&](double least) {
+  // What each piece keeps: the weights (of at least `least`) of its keys over
+  // tau and from `from` on, and the number of its equals of tau.  The wave
+  // first gathers those keys: 64 at a time then take one evaluation.
+  const int pieces = (vocab + PIECE - 1) / PIECE;
+  auto sum_pieces = [&](uint64_t least, uint32_t from) {
     __syncthreads();
-    for (int c = w; c < pieces; c += NW) {
-      T v[8];
-      const int n = load8(x, c * 64 + lane, a.vocab, v);
-      uint64_t sum = 0;
-      uint32_t ties = 0;
-      bool over = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t key = Key<T>::of(v[e]);
-        over |= e < n && key > tau;
-        ties += e < n && key == tau;
-      }
-      if (__any(over)) {
+    constexpr int U = 4;
+    uint32_t* const kept = sh.piece.kept[w];
+    const uint32_t over = max(tau, from - 1);
+    for (int c0 = w; c0 < pieces; c0 += NW * U)
+      load_groups<U>(x, c0 * 64 + lane, NW * 64, vocab, [&](const uint32_t (&key)[8], int j) {
+        const int c = c0 + j * NW;
+        if (c >= pieces) return;
+        int some = 0, ties = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (e < n && Key<T>::of(v[e]) > tau) {
-            const double wd = weight_of((float)v[e]);
-            sum += wd >= least ? to_fixed(wd) : 0;
-          }
+          const uint64_t m = __ballot(key[e] > over);
+          if (key[e] > over)
+            kept[some + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = key[e];
+          some += __popcll(m);
+          ties += __popcll(__ballot(key[e] == tau));
         }
-        sum = scan64(sum);
-      }
-      if (__any(ties != 0)) ties = (uint32_t)scan64(ties);
-      if (lane == 63) {
-        sh.piece.sum[c] = sum;
-        sh.piece.ties[c] = ties;
-      }
-    }
+        uint64_t sum = 0;
+        for (int i = lane; i < some; i += 64) {
+          const uint64_t wf = weights.of(value_of<T>(kept[i]));
+          sum += wf >= least ? wf : 0;
+        }
+        if (some) sum = scan64(sum);
+        if (lane == 63) {
+          sh.piece.sum[c] = sum;
+          sh.piece.ties[c] = (uint32_t)ties;
+        }
+      });
     __syncthreads();
   };
-  // Wave 0: sums of the pieces with the first `equal` ties of weight wt.
-  auto total_of = [&](uint64_t wt) {
-    uint64_t sum = 0, seen = 0;
-    for (int c0 = 0; c0 < pieces; c0 += 64) {
-      const int c = c0 + lane;
-      const uint64_t ties = c < pieces ? sh.piece.ties[c] : 0;
-      const uint64_t incl = scan64(ties), before = seen + incl - ties;
-      const uint64_t kept = before >= equal ? 0 : min(ties, (uint64_t)equal - before);
-      seen = shfl64(seen + incl, 63);
-      const uint64_t s = scan64((c < pieces ? sh.piece.sum[c] : 0) + kept * wt);
-      sum += shfl64(s, 63);
+  // A wave over the pieces, each lane a run of `per`: its pieces' kept weight
+  // `own` (equals of tau at wt each), the equals before its run.
+  const int per = (pieces + 63) >> 6;
+  auto lane_pieces = [&](uint64_t wt, uint64_t& before) {
+    uint64_t ties = 0, own = 0;
+    for (int c = lane * per; c < min(lane * per + per, pieces); ++c) {
+      ties += sh.piece.ties[c];
+      own += sh.piece.sum[c];
     }
-    return sum;
+    before = scan64(ties) - ties;
+    return own + (before >= equal ? 0 : min(ties, (uint64_t)equal - before)) * wt;
   };
 
-  const float p = a.top_p ? a.top_p[row] : a.p;
-  if (!(p >= 1.f)) {
-    pieces_of(0.0);
-    if (w == 0) {
-      const uint64_t sum = total_of(to_fixed(weight_of(value_of(tau))));
-      if (lane == 0) sh.above = sum;
-    }
-    __syncthreads();
-    const uint64_t whole = sh.above;
-    const uint64_t f = fraction64(p > 0.f ? p : 0.f);
-    uint64_t goal = __umul64hi(f, whole) + (f * whole != 0);  // ceil(p * whole)
-    goal = goal > 1 ? goal : 1;
-    uint64_t above;
+  if (need_p) {
+    sum_pieces(0, cut);
+    uint64_t before, above;
+    const uint64_t whole = shfl64(scan64(lane_pieces(weights.of(value_of<T>(tau)), before)), 63);  // (every wave the same)
+    const uint64_t goal = goal_of(whole);
     tau = descend(std::false_type{}, goal, above);
-    const uint64_t wt = to_fixed(weight_of(value_of(tau)));
-    equal = (uint32_t)min((goal - above + wt - 1) / wt, (uint64_t)0xffffffffu);
-    __syncthreads();
+    equal = equals_of(goal, above);
   }
 
-  const double one = __builtin_ldexp(1.0, a.shift);
-  const double least = mp > 0.f ? (double)fminf(mp, 1.f) * one : 0.0;
-  pieces_of(least);
+  const float mp = a.min_p ? a.min_p[row] : a.m;
+  const double m = mp > 0.f ? (double)fminf(mp, 1.f) : 0.0;
+  const uint64_t least = (uint64_t)__builtin_rint(__builtin_ldexp(m, a.shift));
+  // (logits below `from` are below min_p or have weight 0)
+  const uint32_t from = m > 0.0 ? max(cut, min(top, key_from((double)xmax + (log2(m) * 1.000001 - 1e-5) / rate))) : cut;
+  sum_pieces(least, from);
   if (w != 0) return;
-  const double wtd = weight_of(value_of(tau));
-  const uint64_t wt = wtd >= least ? to_fixed(wtd) : 0;
-  const uint64_t whole = total_of(wt);
+  const uint64_t wt_all = weights.of(value_of<T>(tau)), wt = wt_all >= least ? wt_all : 0;
+  uint64_t before;
+  const uint64_t run = lane_pieces(wt, before), incl = scan64(run), whole = shfl64(incl, 63);
   float u = a.u[row];
   u = u > 0.f ? (u < 1.f ? u : 0x1.fffffep-1f) : 0.f;
   const uint64_t goal = __umul64hi(fraction64(u), whole);  // floor(u * whole) < whole
 
-  // the piece, then the token in it, whose running weight first exceeds the goal
-  uint64_t sum = 0, seen = 0;
-  int at = 0;
-  for (int c0 = 0; c0 < pieces; c0 += 64) {
-    const int c = c0 + lane;
-    const uint64_t ties = c < pieces ? sh.piece.ties[c] : 0;
-    const uint64_t incl = scan64(ties), before = seen + incl - ties;
-    const uint64_t kept = before >= equal ? 0 : min(ties, (uint64_t)equal - before);
-    const uint64_t own = (c < pieces ? sh.piece.sum[c] : 0) + kept * wt, s = sum + scan64(own);
-    const uint64_t reach = __ballot(s > goal);
-    if (reach) {
-      const int l = __ffsll((unsigned long long)reach) - 1;
-      at = c0 + l;
-      sum = shfl64(s - own, l);
-      seen = shfl64(before, l);
-      break;
-    }
-    sum = shfl64(s, 63);
-    seen = shfl64(seen + incl, 63);
+  // the lane's run, the piece, then the token whose running weight first exceeds the goal
+  const int l = __ffsll((unsigned long long)__ballot(incl > goal)) - 1;
+  uint64_t sum = shfl64(incl - run, l);
+  before = shfl64(before, l);
+  int at = l * per;
+  for (;; ++at) {  // (every lane the same)
+    const uint64_t ties = sh.piece.ties[at];
+    const uint64_t own = sh.piece.sum[at] + (before >= equal ? 0 : min(ties, (uint64_t)equal - before)) * wt;
+    if (sum + own > goal || at + 1 >= min((l + 1) * per, pieces)) break;
+    sum += own;
+    before += ties;
   }
-  T v[8];
-  const int n = load8(x, at * 64 + lane, a.vocab, v);
+  uint32_t key[8];
+  load_keys(x, at * 64 + lane, vocab, key);
   uint32_t ties = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) ties += e < n && Key<T>::of(v[e]) == tau;
-  uint64_t before = seen + scan64(ties) - ties, own[8], mine = 0;
+  for (int e = 0; e < 8; ++e) ties += key[e] == tau;
+  before += scan64(ties) - ties;
+  uint64_t own[8], mine = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const uint32_t key = Key<T>::of(v[e]);
     own[e] = 0;
-    if (e < n && key > tau) {
-      const double wd = weight_of((float)v[e]);
-      own[e] = wd >= least ? to_fixed(wd) : 0;
-    } else if (e < n && key == tau) {
+    if (key[e] > tau && key[e] >= from) {
+      const uint64_t wf = weights.of(value_of<T>(key[e]));
+      own[e] = wf >= least ? wf : 0;
+    } else if (key[e] == tau) {
       own[e] = before < equal ? wt : 0;
       ++before;
     }
@@ -421,11 +684,11 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   const uint64_t s = sum + scan64(mine);
   const uint64_t reach = __ballot(s > goal);
   if (lane == __ffsll((unsigned long long)reach) - 1) {
-    uint64_t run = s - mine;
+    uint64_t so_far = s - mine;
     int e = 0;
     for (; e < 7; ++e) {
-      run += own[e];
-      if (run > goal) break;
+      so_far += own[e];
+      if (so_far > goal) break;
     }
     a.token[row] = (int64_t)(at * 64 + lane) * 8 + e;
   }
@@ -446,6 +709,7 @@ hipError_t launch_sample(const SampleProblem& p, hipStream_t stream) {
   a.vocab = (int)p.vocab;
   a.shift = 62;
   while ((1ll << (62 - a.shift)) < p.vocab) --a.shift;
+  a.shift = a.shift < 50 ? a.shift : 50;
   a.t = p.t;
   a.k = p.k;
   a.p = p.p;

@@ -9,26 +9,31 @@
 //   token   the lowest kept i whose running weight exceeds u * (kept weight)
 //
 // Weights are integers, round(w * 2^shift) with room for the whole row's sum
-// in 62 bits (44 fraction bits at a vocabulary of 2^18, 50 at most): integer
-// sums do not depend on their order, so neither does the token, and every
-// comparison above is exact in them (p * sum and u * sum as 128-bit products).
-// w comes from a 64-bit evaluation good to 2^-48.  fp32 sums would put about
-// one row in a hundred of a flat distribution on another token.
+// in 62 bits (44 fraction bits up to a vocabulary of 2^18): integer sums do not
+// depend on their order, so neither does the token, and every comparison above
+// is exact in them (p * sum and u * sum as 128-bit products).  w comes from a
+// 64-bit evaluation good to 2^-46.  fp32 sums would put about one row in a
+// hundred of a flat distribution on another token.
 //
 // One workgroup a row.  top-k and top-p are thresholds on the logits, kept as
 // the key (an integer that orders as the logits do) of the last token kept and
 // the number of its equals that stay:
-//   * tokens so far below the largest that their weight is 0 take no part;
-//   * the others are counted by the upper 16 bits of their keys in LDS (65536
-//     counts of 16 bits, 128 KB).  For 16-bit logits that is every value, and
-//     both thresholds follow from counts and one weight a value;
-//   * fp32 logits: the tokens of the top k's bins go on a list in LDS, on which
-//     both thresholds are found bit by bit; without top-k the weights are summed
-//     by the upper 14 bits and the list is the threshold's bin;
+//   * top-k of up to 512: the k-th largest of the threads' own largest logits
+//     over the row's first quarter is a bound below the k-th largest of all; one
+//     pass puts the tokens from it on (a few thousand) on a list in LDS, and
+//     everything else happens there;
+//   * 16-bit logits otherwise: the tokens are counted by value in LDS (65536
+//     counts of 16 bits, 128 KB); both thresholds follow from counts and one
+//     weight a value.  Tokens so far below the largest that their weight is 0
+//     take no part;
+//   * fp32 logits otherwise: counted by the upper 16 bits, those of the top k's
+//     bins on the list; without top-k the weights are summed by the upper 14
+//     bits and the list is the threshold's bin;
 //   * where a count passes 16 bits (more than 65535 equal values) or a list
 //     its room, a radix descent over the row, 8 bits a pass with a column of
 //     the histogram for each lane, takes their place.
-// Then the kept weights are summed by pieces of 512 tokens, the piece that
+// Then the kept weights are summed by pieces of 512 tokens (from the list, from
+// a table of the weight of every kept value, or evaluated), the piece that
 // reaches u * sum is found and the token in it.
 #include "hxmi_common.h"
 #include "hxmi_internal.h"
@@ -55,7 +60,8 @@ struct SArgs {
 
 constexpr int NT = 1024, NW = NT / 64, PIECE = 512;
 constexpr int kMaxPieces = kSampleMaxVocab / PIECE;
-constexpr int kList = 8192;
+constexpr int kList = 6144, kFewTop = 512, kTable = 16384;
+constexpr int kTieBit = 54;  // of a table entry: an equal of the last key (a piece's weights sum to 2^53 at most)
 
 // A logit's key: an unsigned integer that orders as the logits do, equal for
 // -0 and 0 (its magnitude's bits under its sign, moved up by half the range).
@@ -86,31 +92,48 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   else return (float)__builtin_bit_cast(T, (unsigned short)b);
 }
 
+// 2^(j / 512), by its Taylor series at compile time.
+constexpr int kSteps = 512;
+struct Exp2Table {
+  double v[kSteps];
+};
+constexpr Exp2Table exp2_table() {
+  Exp2Table t{};
+  for (int j = 0; j < kSteps; ++j) {
+    const double z = 0.69314718055994530942 * j / kSteps;
+    double p = 1.0;
+    for (int n = 22; n >= 1; --n) p = 1.0 + p * z / n;
+    t.v[j] = p;
+  }
+  return t;
+}
+__constant__ const Exp2Table kExp2 = exp2_table();
+
 // The weights of a row: round(2^shift * 2^y), y = (v - max) * log2(e) / T.
 struct Weights {
-  double rate32;  // 32 log2(e) / T
-  double xmax;
+  double rate;    // log2(e) / T, in steps of the table
+  double top;     // the largest logit
+  float xmax, least;  // values below `least` have weight 0
   int shift;
-  const double* table;  // 2^(j / 32)
-  int infinite;         // the largest logit is (in a scalar register)
+  const double* table;
+  int infinite;  // the largest logit is (in a scalar register)
 
-  __device__ __forceinline__ uint64_t one() const { return 1ull << shift; }
   __device__ __forceinline__ uint64_t of(float v) const {
-    if (infinite) return (double)v == xmax ? one() : 0;
-    // k = round(32 y), from the low bits of y + 1.5 * 2^52; 2^(r / 32) by its
-    // Taylor series, |r ln 2 / 32| <= 0.0109: the first term left out is below 2^-48
-    const double y = fmax(((double)v - xmax) * rate32, -32.0 * 120);
+    if (infinite) return v == xmax ? 1ull << shift : 0;
+    // k = round(y), from the low bits of y + 1.5 * 2^52; 2^(r / 512) by its
+    // series, |r ln 2 / 512| <= 6.8e-4: the first term left out is below 2^-46
+    const double y = ((double)fmaxf(v, least) - top) * rate;
     const double t = y + 0x1.8p52, r = y - (t - 0x1.8p52);
-    const int k = (int)__double2loint(t);
-    constexpr double z = 0.69314718055994530942 / 32;
-    double p = z * z * z * z * z / 120;
-    p = __builtin_fma(p, r, z * z * z * z / 24);
-    p = __builtin_fma(p, r, z * z * z / 6);
-    p = __builtin_fma(p, r, z * z / 2);
+    const int k = __double2loint(t);
+    constexpr double z = 0.69314718055994530942 / kSteps;
+    double p = __builtin_fma(z * z * z / 6, r, z * z / 2);
     p = __builtin_fma(p, r, z);
     p = __builtin_fma(p, r, 1.0);
-    const double w = __builtin_ldexp(table[k & 31] * p, (k >> 5) + shift) + 0x1p52;  // (rounds; below 2^51)
-    return (uint64_t)__double_as_longlong(w) & 0xfffffffffffffull;
+    p *= table[k & (kSteps - 1)];
+    // times 2^(k / 512 + shift) in its exponent; the sum rounds it (below 2^51)
+    const int e = (k >> 9) + shift;
+    p = __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p)) + 0x1p52;
+    return (uint64_t)__double_as_longlong(p) & 0xfffffffffffffull;
   }
 };
 
@@ -141,25 +164,30 @@ __device__ __forceinline__ uint64_t fraction64(float f) {
 
 struct Shared {
   union {
-    uint32_t count2[32768];         // 16-bit counts of the upper 16 bits of a key, two a word
-    unsigned long long bin[16384];  // weights by the upper 14 bits
+    uint32_t count2[32768];            // 16-bit counts of the upper 16 bits of a key, two a word
+    unsigned long long bin[16384];     // weights by the upper 14 bits
+    unsigned long long table[kTable];  // weight of a value by its key
     unsigned long long mass[256][64];  // radix descent: a column a lane
     uint32_t count[256][64];
     struct {
-      uint32_t key[kList];
       unsigned long long weight[kList];
+      uint32_t key[kList], index[kList];
     } list;
+    uint32_t kept[NW][PIECE];
+  };
+  union {
     struct {
       unsigned long long sum[kMaxPieces];  // kept weight of a piece, less its equals of the last key
       uint32_t ties[kMaxPieces];
-      uint32_t kept[NW][PIECE];
     } piece;
+    struct {
+      unsigned long long weight[NT];  // of 64 values each
+      uint32_t count[NT];
+    } group;
   };
-  unsigned long long group[NT];  // of 64 bins each: their weight,
-  uint32_t group_count[NT];      // their count
-  double table[32];
+  double exp2[kSteps];
+  unsigned long long digit[256];
   unsigned long long part[NW];
-  uint32_t upart[NW];
   uint32_t key, listed;
   unsigned long long above;
 };
@@ -224,14 +252,14 @@ __device__ __forceinline__ void load_groups(const T* x, int i0, int step, int vo
   }
 }
 
-// f(key) for the logits of a row (and for a few keys 0, which none has).
+// f(key, index) for the logits of a row (and for a few keys 0, which none has).
 template <int U, typename T, typename F>
 __device__ __forceinline__ void each_key(const T* x, int vocab, F&& f) {
   const int lanes = (vocab + 7) >> 3, wave0 = threadIdx.x & ~63;
   for (int i0 = wave0; i0 < lanes; i0 += NT * U)  // (a wave stays together)
-    load_groups<U>(x, i0 + (threadIdx.x & 63), NT, vocab, [&](const uint32_t (&key)[8], int) {
+    load_groups<U>(x, i0 + (threadIdx.x & 63), NT, vocab, [&](const uint32_t (&key)[8], int j) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f(key[e]);
+      for (int e = 0; e < 8; ++e) f(key[e], (i0 + (int)(threadIdx.x & 63) + j * NT) * 8 + e);
     });
 }
 
@@ -267,53 +295,115 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   const int vocab = a.vocab;
   constexpr int KB = Key<T>::bits;
 
-  if (threadIdx.x < 32) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 32);
+  if (threadIdx.x < kSteps) sh.exp2[threadIdx.x] = kExp2.v[threadIdx.x];
 
-  // the largest logit; NaNs have keys over inf's or under -inf's
+  int k = a.top_k ? a.top_k[row] : a.k;
+  float p = a.top_p ? a.top_p[row] : a.p, mp = a.min_p ? a.min_p[row] : a.m;
+  float t = a.temperature ? a.temperature[row] : a.t;
+  if (!(t > 0.f)) {  // the first of the largest
+    t = 1.f;
+    k = 1;
+    p = 1.f;
+    mp = 0.f;
+  }
+  bool need_k = k > 0 && k < vocab, need_p = !(p >= 1.f);
+
+  // Largest and smallest key: NaNs have keys over inf's or under -inf's.
   uint32_t top = 0, low = 0xffffffffu;
-  each_key<4>(x, vocab, [&](uint32_t key) {
-    top = max(top, key);
-    low = min(low, key - 1);  // (0, no key, goes past every other)
-  });
+  auto extremes = [&]() {  // of the workgroup from the threads'
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-    low = min(low, (uint32_t)__shfl_xor((int)low, o, 64));
-  }
-  if (lane == 0) sh.part[w] = ((unsigned long long)top << 32) | low;
-  __syncthreads();
+    for (int o = 32; o >= 1; o >>= 1) {
+      top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+      low = min(low, (uint32_t)__shfl_xor((int)low, o, 64));
+    }
+    if (lane == 0) sh.part[w] = ((unsigned long long)top << 32) | low;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    top = max(top, (uint32_t)(sh.part[i] >> 32));
-    low = min(low, (uint32_t)sh.part[i]);
+    for (int i = 0; i < NW; ++i) {
+      top = max(top, (uint32_t)(sh.part[i] >> 32));
+      low = min(low, (uint32_t)sh.part[i]);
+    }
+  };
+  // The key, from `hi` down, at which the weights of the workgroup's entries
+  // over it and its own first reach the goal, with `above` over hi; to within
+  // 2^slack.  each(f) calls f(key, weight) for a thread's entries.  Eight bits
+  // of the distance from lo (which the goal is reached at) a round.
+  auto radix = [&](uint32_t lo, uint32_t hi, int slack, uint64_t goal, uint64_t& above, auto&& each) {
+    const int bits = 32 - __builtin_clz((hi - lo) | 1);
+    for (int b = max(bits - 8, 0);; b = max(b - 8, 0)) {
+      __syncthreads();
+      if (threadIdx.x < 256) sh.digit[threadIdx.x] = 0;
+      __syncthreads();
+      each([&](uint32_t key, uint64_t weight) {
+        if (key >= lo && key <= hi) atomicAdd(&sh.digit[(key - lo) >> b], (unsigned long long)weight);
+      });
+      __syncthreads();
+      uint64_t own[4], sum = 0;  // (every wave the same)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += own[j] = sh.digit[255 - 4 * lane - j];
+      const uint64_t incl = above + scan64(sum);
+      const int at = __ffsll((unsigned long long)__ballot(incl >= goal)) - 1;
+      uint64_t over = incl - sum;
+      int j = 0;
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (j == i && over + own[i] < goal) {
+          over += own[i];
+          ++j;
+        }
+      const uint32_t digit = __builtin_amdgcn_readlane(255 - 4 * lane - j, at);
+      above = shfl64(over, at);
+      lo += digit << b;
+      hi = min(hi, lo + ((1u << b) - 1));
+      if (b <= slack) return lo;
+    }
+  };
+
+  // Appends the tokens of a wave that `take` says to the list: one atomic for
+  // all (a row whose every logit is the same puts all of them here).
+  auto put = [&](bool take, uint32_t key, int i) {
+    const uint64_t m = __ballot(take);
+    if (!m) return;
+    uint32_t at = 0;
+    if (lane == __ffsll((unsigned long long)m) - 1) at = atomicAdd(&sh.listed, (uint32_t)__popcll(m));
+    at = __builtin_amdgcn_readlane(at, __ffsll((unsigned long long)m) - 1) +
+         __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    if (take && at < kList) {
+      sh.list.key[at] = key;
+      sh.list.index[at] = i;
+    }
+  };
+  uint32_t bound = 1;   // no less than k keys are as large
+  uint32_t listed = 0;  // tokens on the list, all that the top k can hold among them; 0: no list
+  if (need_k && k <= kFewTop) {
+    uint32_t own = 0;
+    each_key<4>(x, min(vocab, (vocab / 4 + 8 * NT - 1) & ~(8 * NT - 1)), [&](uint32_t key, int) { own = max(own, key); });
+    // (any bound below the k-th largest does; a thread without a token has key 0)
+    uint64_t above = 0;
+    bound = max(radix(0, KB == 16 ? 0xffffu : 0xffffffffu, KB == 16 ? 0 : 16, k, above, [&](auto&& f) { f(own, 1); }), 1u);
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    each_key<4>(x, vocab, [&](uint32_t key, int i) {
+      low = min(low, key - 1);  // (0, no key, goes past every other)
+      put(key >= bound, key, i);
+    });
+    __syncthreads();
+    listed = sh.listed;
+    if (listed > kList) listed = 0;
+    for (uint32_t i = threadIdx.x; i < listed; i += NT) top = max(top, sh.list.key[i]);
   }
+  if (!listed) each_key<8>(x, vocab, [&](uint32_t key, int) {
+      top = max(top, key);
+      low = min(low, key - 1);
+    });
+  extremes();
   constexpr uint32_t kInf = Key<T>::zero + Key<T>::inf, kMinusInf = Key<T>::zero - Key<T>::inf;
   if (top > kInf || low + 1 < kMinusInf || top == kMinusInf) {
     if (threadIdx.x == 0) a.token[row] = -1;
     return;
   }
   const float xmax = value_of<T>(top);
-  const float t = a.temperature ? a.temperature[row] : a.t;
-  if (!(t > 0.f)) {  // the first of the largest
-    if (threadIdx.x == 0) sh.key = 0xffffffffu;
-    __syncthreads();
-    for (int i = threadIdx.x; i < (vocab + 7) >> 3; i += NT) {
-      uint32_t key[8];
-      load_keys(x, i, vocab, key);
-#pragma unroll
-      for (int e = 7; e >= 0; --e)
-        if (key[e] == top) atomicMin(&sh.key, (uint32_t)(i * 8 + e));
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) a.token[row] = (int64_t)sh.key;
-    return;
-  }
-  const double rate = 1.44269504088896340736 / (double)t;
-  const Weights weights{rate * 32, (double)xmax, a.shift, sh.table,
-                        __builtin_amdgcn_readfirstlane(xmax == INFINITY)};
-  // Logits with keys below `cut` have a weight that rounds to 0: they change no
-  // sum, and whether the top k holds some of them changes nothing.  (Any value
-  // under the rounding of a bound is under the bound.)
+  const double rate = 1.44269504088896340736 / (double)fminf(t, 1e30f);  // (an infinite T leaves -inf its weight, 0)
   auto key_from = [&](double v) {  // the key from which logits are at least v (of a NaN: all)
     const float f = (float)v;
     if constexpr (KB == 32) return f != f ? 1u : max(1u, Key<float>::of(f));
@@ -323,8 +413,13 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
       return f != f ? 1u : max(1u, Key<T>::of(h));
     }
   };
+  // Logits with keys below `cut` have a weight that rounds to 0: they change no
+  // sum, and whether the top k holds some of them changes nothing.  (Any value
+  // under the rounding of a bound is under the bound.)
   const uint32_t cut = min(top, key_from((double)xmax - (a.shift + 3) / rate * 1.000001));
-
+  // (`least` two steps of the weights lower: y stays above -100 bits)
+  const Weights weights{rate * kSteps, (double)xmax, xmax, (float)((double)xmax - (a.shift + 20) / rate),
+                        a.shift, sh.exp2, __builtin_amdgcn_readfirstlane(xmax == INFINITY)};
   // Descends to the key at which the counts (or weights) from the largest key
   // down first reach `goal`; `above`: what lies over that key.
   auto descend = [&](auto COUNT_, uint64_t goal, uint64_t& above) {
@@ -338,7 +433,7 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
         else ((unsigned long long*)sh.mass)[i] = 0;
       }
       __syncthreads();
-      each_key<1>(x, vocab, [&](uint32_t key) {
+      each_key<1>(x, vocab, [&](uint32_t key, int) {
         if (key < cut || (b + 8 < KB && key >> (b + 8) != prefix)) return;
         if constexpr (COUNT) atomicAdd(&sh.count[(key >> b) & 255][lane], 1u);
         else atomicAdd(&sh.mass[(key >> b) & 255][lane], (unsigned long long)weights.of(value_of<T>(key)));
@@ -394,7 +489,7 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     for (int i = threadIdx.x; i < 32768 / 4; i += NT) z[i] = int4v{};
     __syncthreads();
     uint32_t mine = 0;
-    each_key<4>(x, vocab, [&](uint32_t key) {
+    each_key<4>(x, vocab, [&](uint32_t key, int) {
       if (key < cut) return;
       const uint32_t bin = key >> (KB - 16);
       atomicAdd(&sh.count2[bin >> 1], 1u + (bin & 1) * 0xffffu);
@@ -431,9 +526,6 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
 
   // Kept: keys over `tau`, and the first `equal` tokens whose key is tau.
   uint32_t tau = 0, equal = 0;
-  const int k = a.top_k ? a.top_k[row] : a.k;
-  const float p = a.top_p ? a.top_p[row] : a.p;
-  bool need_k = k > 0 && k < vocab, need_p = !(p >= 1.f);
   const uint64_t pf = fraction64(p > 0.f ? fminf(p, 0x1.fffffep-1f) : 0.f);
   auto goal_of = [&](uint64_t whole) {  // ceil(p * whole), at least 1
     const uint64_t g = __umul64hi(pf, whole) + (pf * whole != 0);
@@ -446,46 +538,51 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     return (uint32_t)min((goal - above + wt - 1) / wt, (uint64_t)0xffffffffu);
   };
 
-  // List in LDS of the keys that `in` takes: their number (over kList: not all are there).
+  // List of the tokens whose key `in` takes: their number (over kList: not all are there).
   auto make_list = [&](auto&& in) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    each_key<4>(x, vocab, [&](uint32_t key) {
-      if (key >= cut && in(key)) {
-        const uint32_t at = atomicAdd(&sh.listed, 1u);
-        if (at < kList) sh.list.key[at] = key;
-      }
+    each_key<4>(x, vocab, [&](uint32_t key, int i) {
+      put(key >= cut && in(key), key, i);
     });
     __syncthreads();
-    const uint32_t n = sh.listed;
-    if (n <= kList)
-      for (uint32_t i = threadIdx.x; i < n; i += NT) sh.list.weight[i] = weights.of(value_of<T>(sh.list.key[i]));
-    __syncthreads();
-    return n;
+    return sh.listed;
   };
-  auto list_count = [&](uint32_t n, uint32_t from) {  // listed keys >= from
-    uint32_t c = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += NT) c += sh.list.key[i] >= from;
-    return block_sum(c, sh);
+  auto list_weights = [&](uint32_t n) {
+    for (uint32_t i = threadIdx.x; i < n; i += NT) sh.list.weight[i] = weights.of(value_of<T>(sh.list.key[i]));
+  };  // (each thread reads its own entries)
+  // A thread's entries of a list of n tokens.
+  auto list_keys = [&](uint32_t n) {
+    return [&, n](auto&& f) {
+      for (uint32_t i = threadIdx.x; i < n; i += NT) f(sh.list.key[i], 1);
+    };
   };
-  auto list_weight = [&](uint32_t n, uint32_t over) {  // weight of the listed keys > over
-    uint64_t c = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += NT) c += sh.list.key[i] > over ? sh.list.weight[i] : 0;
-    return block_sum(c, sh);
+  auto list_masses = [&](uint32_t n) {
+    return [&, n](auto&& f) {
+      for (uint32_t i = threadIdx.x; i < n; i += NT) f(sh.list.key[i], sh.list.weight[i]);
+    };
   };
-  // The largest key from lo to hi down to which the list's weight, with
-  // `base`, reaches the goal (at lo it does).
-  auto list_key = [&](uint32_t n, uint32_t lo, uint32_t hi, uint64_t base, uint64_t goal) {
-    while (lo < hi) {
-      const uint32_t mid = lo + ((hi - lo + 1) >> 1);
-      if (base + list_weight(n, mid - 1) >= goal) lo = mid;
-      else hi = mid - 1;
+  // Both thresholds from a list of n tokens that holds the top k, keys from lo on.
+  auto list_thresholds = [&](uint32_t n, uint32_t lo) {
+    uint64_t above = 0;
+    tau = radix(lo, top, 0, k, above, list_keys(n));
+    equal = (uint32_t)(k - above);
+    list_weights(n);
+    if (need_p) {
+      uint64_t own = 0;
+      list_masses(n)([&](uint32_t key, uint64_t wf) { own += key > tau ? wf : 0; });
+      const uint64_t goal = goal_of(block_sum(own, sh) + equal * weights.of(value_of<T>(tau)));
+      above = 0;
+      tau = radix(tau, top, 0, goal, above, list_masses(n));
+      equal = equals_of(goal, above);
     }
-    return lo;
+    need_k = need_p = false;
   };
 
-  if constexpr (KB == 16) {
+  if (listed) {
+    list_thresholds(listed, bound);
+  } else if constexpr (KB == 16) {
     if ((need_k || need_p) && count_keys()) {
       if (need_k && (uint64_t)k < counted) {
         uint64_t above;
@@ -498,17 +595,17 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
           return c ? c * weights.of(value_of<T>(bin)) : 0;
         };
         // each wave takes every 16th group of 64 bins, those that hold something
-        sh.group_count[threadIdx.x] = (uint32_t)count_own;
+        sh.group.count[threadIdx.x] = (uint32_t)count_own;
         __syncthreads();
-        const uint32_t some = sh.group_count[lane * NW + w];
-        if (some == 0) sh.group[lane * NW + w] = 0;
+        const uint32_t some = sh.group.count[lane * NW + w];
+        if (some == 0) sh.group.weight[lane * NW + w] = 0;
         for (uint64_t left = __ballot(some != 0); left; left &= left - 1) {
           const int g = (__ffsll((unsigned long long)left) - 1) * NW + w;
           const uint64_t sum = scan64(masses(64u * (NT - 1 - g) + lane));
-          if (lane == 63) sh.group[g] = sum;
+          if (lane == 63) sh.group.weight[g] = sum;
         }
         __syncthreads();
-        const uint64_t own = sh.group[threadIdx.x];
+        const uint64_t own = sh.group.weight[threadIdx.x];
         uint64_t whole, above;
         const uint64_t incl = block_scan(own, sh, whole), goal = goal_of(whole);
         tau = find_bin(incl, own, goal, above, masses);
@@ -528,17 +625,8 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
         const uint32_t bin =
             find_bin(count_incl, count_own, (uint64_t)k, above, [&](uint32_t b) -> uint64_t { return count_of(b); });
         if (above + count_of(bin) <= kList) {
-          const uint32_t n = make_list([&](uint32_t key) { return key >> 16 >= bin; });
-          tau = bin << 16;
-          for (int b = 15; b >= 0; --b)
-            if (list_count(n, tau | 1u << b) >= (uint64_t)k) tau |= 1u << b;
-          equal = (uint32_t)(k - list_count(n, tau + 1));  // (tau is no key past +inf's)
-          if (need_p) {
-            const uint64_t goal = goal_of(list_weight(n, tau) + equal * weights.of(value_of<T>(tau)));
-            tau = list_key(n, tau, top, 0, goal);
-            equal = equals_of(goal, list_weight(n, tau));
-          }
-          need_k = need_p = false;
+          listed = make_list([&](uint32_t key) { return key >> 16 >= bin; });
+          list_thresholds(listed, bin << 16);
         }
       }
     }
@@ -546,9 +634,16 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
       __syncthreads();
       for (int i = threadIdx.x; i < 16384; i += NT) sh.bin[i] = 0;
       __syncthreads();
-      each_key<1>(x, vocab, [&](uint32_t key) {
-        if (key >= cut) atomicAdd(&sh.bin[key >> 18], (unsigned long long)weights.of(value_of<T>(key)));
-      });
+      const int lanes = (vocab + 7) >> 3;
+      for (int i0 = w * 64; i0 < lanes; i0 += NT)
+        load_groups<1>(x, i0 + lane, NT, vocab, [&](const uint32_t (&key)[8], int) {
+          uint64_t wf[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) wf[e] = weights.of(value_of<T>(key[e]));  // (side by side)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (key[e] >= cut) atomicAdd(&sh.bin[key[e] >> 18], (unsigned long long)wf[e]);
+        });
       __syncthreads();
       uint64_t own = 0, whole;
       const uint32_t b0 = 16u * (NT - 1 - threadIdx.x);  // (threads from the largest keys down)
@@ -567,8 +662,10 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
       const uint64_t above = sh.above;
       const uint32_t n = make_list([&](uint32_t key) { return key >> 18 == bin; });
       if (n <= kList) {
-        tau = list_key(n, bin << 18, min(bin << 18 | 0x3ffffu, top), above, goal);
-        equal = equals_of(goal, above + list_weight(n, tau));
+        list_weights(n);
+        uint64_t over = above;
+        tau = radix(bin << 18, min(bin << 18 | 0x3ffffu, top), 0, goal, over, list_masses(n));
+        equal = equals_of(goal, over);
         need_p = false;
       }
     }
@@ -586,7 +683,7 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   auto sum_pieces = [&](uint64_t least, uint32_t from) {
     __syncthreads();
     constexpr int U = 4;
-    uint32_t* const kept = sh.piece.kept[w];
+    uint32_t* const kept = sh.kept[w];
     const uint32_t over = max(tau, from - 1);
     for (int c0 = w; c0 < pieces; c0 += NW * U)
       load_groups<U>(x, c0 * 64 + lane, NW * 64, vocab, [&](const uint32_t (&key)[8], int j) {
@@ -602,9 +699,10 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
           ties += __popcll(__ballot(key[e] == tau));
         }
         uint64_t sum = 0;
-        for (int i = lane; i < some; i += 64) {
-          const uint64_t wf = weights.of(value_of<T>(kept[i]));
-          sum += wf >= least ? wf : 0;
+        for (int i = lane; i < some; i += 128) {  // (two evaluations side by side)
+          const uint64_t w0 = weights.of(value_of<T>(kept[i])), w1 = weights.of(value_of<T>(kept[min(i + 64, some - 1)]));
+          sum += w0 >= least ? w0 : 0;
+          sum += i + 64 < some && w1 >= least ? w1 : 0;
         }
         if (some) sum = scan64(sum);
         if (lane == 63) {
@@ -636,12 +734,51 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     equal = equals_of(goal, above);
   }
 
-  const float mp = a.min_p ? a.min_p[row] : a.m;
   const double m = mp > 0.f ? (double)fminf(mp, 1.f) : 0.0;
   const uint64_t least = (uint64_t)__builtin_rint(__builtin_ldexp(m, a.shift));
   // (logits below `from` are below min_p or have weight 0)
   const uint32_t from = m > 0.0 ? max(cut, min(top, key_from((double)xmax + (log2(m) * 1.000001 - 1e-5) / rate))) : cut;
-  sum_pieces(least, from);
+  const uint32_t base = max(tau, from) - 1;
+  if (listed) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < pieces; i += NT) {
+      sh.piece.sum[i] = 0;
+      sh.piece.ties[i] = 0;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < listed; i += NT) {
+      const uint32_t key = sh.list.key[i], c = sh.list.index[i] / PIECE;
+      if (key > tau && sh.list.weight[i] >= least) atomicAdd(&sh.piece.sum[c], sh.list.weight[i]);
+      if (key == tau) atomicAdd(&sh.piece.ties[c], 1u);
+    }
+    __syncthreads();
+  } else if (KB == 16 && top - base < kTable) {
+    // every kept value's weight by its key: an addition a token
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i <= top - base; i += NT) {
+      const uint64_t wf = i ? weights.of(value_of<T>(base + i)) : 0;
+      sh.table[i] = base + i == tau ? 1ull << kTieBit : wf >= least ? wf : 0;
+    }
+    if (threadIdx.x == 0) sh.table[0] = 0;
+    __syncthreads();
+    constexpr int U = 4;
+    for (int c0 = w; c0 < pieces; c0 += NW * U)
+      load_groups<U>(x, c0 * 64 + lane, NW * 64, vocab, [&](const uint32_t (&key)[8], int j) {
+        const int c = c0 + j * NW;
+        if (c >= pieces) return;
+        uint64_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += sh.table[max(key[e], base) - base];
+        sum = scan64(sum);
+        if (lane == 63) {
+          sh.piece.sum[c] = sum & ((1ull << kTieBit) - 1);
+          sh.piece.ties[c] = (uint32_t)(sum >> kTieBit);
+        }
+      });
+    __syncthreads();
+  } else {
+    sum_pieces(least, from);
+  }
   if (w != 0) return;
   const uint64_t wt_all = weights.of(value_of<T>(tau)), wt = wt_all >= least ? wt_all : 0;
   uint64_t before;
@@ -709,7 +846,7 @@ hipError_t launch_sample(const SampleProblem& p, hipStream_t stream) {
   a.vocab = (int)p.vocab;
   a.shift = 62;
   while ((1ll << (62 - a.shift)) < p.vocab) --a.shift;
-  a.shift = a.shift < 50 ? a.shift : 50;
+  a.shift = a.shift < 44 ? a.shift : 44;
   a.t = p.t;
   a.k = p.k;
   a.p = p.p;

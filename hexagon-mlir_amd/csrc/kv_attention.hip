@@ -51,7 +51,8 @@ struct KArgs {
   int64_t ldq, hq, ldo, ho, ldt;
   int64_t bytes;  // of a block's codes of one head
   int requests, tokens, kv_heads, group, d, dp, lb, blocks, width;
-  int tiles, nsplit;
+  int tiles;         // of a key/value head
+  int full, nsplit;  // the first `full` tiles of all heads run whole, the others in nsplit shares of their keys
   float c;  // scale * log2(e)
 };
 
@@ -87,20 +88,33 @@ __device__ __forceinline__ float rel_exp2(float x, float top) {
   return x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - top);
 }
 
-// What a wave knows of its QT x 16 rows: O relative to 2^mv, the sum of the
-// weights (this lane's part) relative to 2^m.
+// x + lv, -inf where lv is (whatever x is).
+__device__ __forceinline__ float left_out(float x, float lv) { return lv == -INFINITY ? -INFINITY : x + lv; }
+
+// A page's V scale as the weights take it: its logarithm, and its inverse for
+// the sum.  A page of zeros (scale 0) may take any scale: the smallest one that
+// pages have, which leaves the maximum to the others.  A page that is not
+// there, or whose keys are all masked, has logarithm -inf.
+__device__ __forceinline__ void value_scale(float vs, float& lv, float& rv) {
+  vs = vs == 0.f ? 0x1p-100f : vs;
+  lv = __builtin_amdgcn_logf(vs);
+  rv = __builtin_amdgcn_rcpf(vs);
+}
+
+// What a wave knows of its QT x 16 rows: O and the sum of the p_j (this lane's
+// part), both relative to 2^mv.
 template <int QT, int DT>
 struct Partial {
-  static constexpr int N = QT * (DT * 4 + 3);  // floats a lane
+  static constexpr int N = QT * (DT * 4 + 2);  // floats a lane
   float4v o[QT][DT];
-  float m[QT], mv[QT], l[QT];
+  float mv[QT], l[QT];
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int a = 0; a < QT; ++a) {
 #pragma unroll
       for (int t = 0; t < DT; ++t) o[a][t] = float4v{0.f, 0.f, 0.f, 0.f};
-      m[a] = mv[a] = -INFINITY;
+      mv[a] = -INFINITY;
       l[a] = 0.f;
     }
   }
@@ -113,26 +127,97 @@ struct Partial {
       for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[a][t][i] = f((a * DT + t) * 4 + i, o[a][t][i]);
-      m[a] = f(QT * DT * 4 + a, m[a]);
-      mv[a] = f(QT * DT * 4 + QT + a, mv[a]);
-      l[a] = f(QT * DT * 4 + 2 * QT + a, l[a]);
+      mv[a] = f(QT * DT * 4 + a, mv[a]);
+      l[a] = f(QT * DT * 4 + QT + a, l[a]);
     }
   }
   __device__ __forceinline__ void add(const Partial& p) {
 #pragma unroll
     for (int a = 0; a < QT; ++a) {
-      const float mn = fmaxf(m[a], p.m[a]), vn = fmaxf(mv[a], p.mv[a]);
-      l[a] = l[a] * rel_exp2(m[a], mn) + p.l[a] * rel_exp2(p.m[a], mn);
+      const float vn = fmaxf(mv[a], p.mv[a]);
       const float x = rel_exp2(mv[a], vn), y = rel_exp2(p.mv[a], vn);
+      l[a] = l[a] * x + p.l[a] * y;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[a][t][i] = o[a][t][i] * x + p.o[a][t][i] * y;
-      m[a] = mn;
       mv[a] = vn;
     }
   }
 };
+
+// The request and rows of a tile of RT rows.  With cu, request r's tiles begin
+// at number floor(cu[r] * group / RT) + r: never more than RT rows a tile, and
+// no sums over the requests before it.  Numbers in between have no rows.
+struct Rows {
+  int r, first, n, row0, len;
+  int64_t count;
+};
+template <int RT>
+__device__ __forceinline__ bool rows_of(const KArgs& a, int tile, Rows& t) {
+  if (a.cu) {
+    int lo = 0, hi = a.requests;
+    auto start = [&](int i) { return (int64_t)min(max(a.cu[i], 0), a.tokens) * a.group / RT + i; };
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start(mid) <= tile) lo = mid;
+      else hi = mid;
+    }
+    t.r = lo;
+    t.first = min(max(a.cu[lo], 0), a.tokens);
+    t.n = min(max(a.cu[lo + 1], t.first), a.tokens) - t.first;
+    t.row0 = (int)min((tile - start(lo)) * RT, (int64_t)INT32_MAX);
+  } else {
+    const int per = (a.group + RT - 1) / RT;
+    t.r = t.first = tile / per;
+    t.n = 1;
+    t.row0 = (tile - t.r * per) * RT;
+  }
+  t.count = (int64_t)t.n * a.group;
+  if (t.row0 < 0 || t.row0 >= t.count) return false;
+  t.len = (int)min(max((int64_t)a.lens[t.r], (int64_t)0), (int64_t)a.width << (a.lb + 4));
+  return true;
+}
+
+// A workgroup's tile (of all heads) and share of its keys.
+struct Share {
+  int item, split, count;
+};
+// Workgroups go round-robin over the 8 XCDs; each XCD takes a contiguous run of
+// numbers, so the tiles that read the same keys read them through one L2.
+__device__ __forceinline__ int xcd_run(int id, int total) {
+  const int per = total >> 3, rem = total & 7, xcd = id & 7;
+  return xcd * per + (xcd < rem ? xcd : rem) + (id >> 3);
+}
+
+__device__ __forceinline__ Share share_of(const KArgs& a) {
+  const int id = blockIdx.x;
+  if (id < a.full) return Share{xcd_run(id, a.full), 0, 1};
+  const int j = xcd_run(id - a.full, gridDim.x - a.full);
+  return Share{a.full + j / a.nsplit, j % a.nsplit, a.nsplit};
+}
+
+// Eight elements of q as fp16, and what the scores are to be multiplied by.  q
+// in bf16 takes a power of two `ex` that brings the row's largest element to
+// [2^14, 2^15): what is below 2^-39 of it is lost, far under the fp32 sums.
+template <typename T>
+__device__ __forceinline__ float largest(const T (&x)[8], float top) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf((float)x[e]));
+  return top;
+}
+__device__ __forceinline__ int exponent_of(float top) {
+  const int ex = top > 0.f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+  return min(max(ex, -120), 120);
+}
+template <typename T>
+__device__ __forceinline__ half8v q_operand(const T (&x)[8], int ex) {
+  half8v h;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    h[e] = std::is_same_v<T, _Float16> ? (_Float16)(float)x[e] : (_Float16)__builtin_ldexpf((float)x[e], ex);
+  return h;
+}
 
 // DC: 64-dim pieces of a row; WHOLE: the head dim is 64 * DC.
 template <typename T, int DC, bool WHOLE, int QT>
@@ -145,44 +230,13 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lg = lane >> 4;
 
-  // Workgroups go round-robin over the 8 XCDs; each XCD takes a contiguous
-  // run of tiles, so those that read the same keys read them through one L2.
-  int id = blockIdx.x;
-  {
-    const int total = gridDim.x, per = total >> 3, rem = total & 7, xcd = id & 7;
-    id = xcd * per + (xcd < rem ? xcd : rem) + (id >> 3);
-  }
-  const int split = id % a.nsplit, item = id / a.nsplit;
-  const int kvh = item / a.tiles, tile = item - kvh * a.tiles;
-
-  // The tile's request and rows.  Request r's tiles begin at number
-  // floor(cu[r] * group / RT) + r: never more than RT rows a tile, and no sums
-  // over the requests before it.  Numbers in between have no rows.
-  int r, first, n, row0;
-  if (a.cu) {
-    int lo = 0, hi = a.requests;
-    auto start = [&](int i) {
-      return (int64_t)min(max(a.cu[i], 0), a.tokens) * a.group / RT + i;
-    };
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (start(mid) <= tile) lo = mid;
-      else hi = mid;
-    }
-    r = lo;
-    first = min(max(a.cu[r], 0), a.tokens);
-    n = min(max(a.cu[r + 1], first), a.tokens) - first;
-    row0 = (int)min((tile - start(r)) * RT, (int64_t)INT32_MAX);
-  } else {
-    const int per = (a.group + RT - 1) / RT;
-    r = tile / per;
-    first = r;
-    n = 1;
-    row0 = (tile - r * per) * RT;
-  }
-  const int64_t nrows = (int64_t)n * a.group;
-  if (row0 < 0 || row0 >= nrows) return;
-  const int len = (int)min(max((int64_t)a.lens[r], (int64_t)0), (int64_t)a.width << (a.lb + 4));
+  const Share part = share_of(a);
+  const int split = part.split, nsplit = part.count, item = part.item;
+  const int kvh = item / a.tiles;
+  Rows tile;
+  if (!rows_of<RT>(a, item - kvh * a.tiles, tile)) return;
+  const int r = tile.r, first = tile.first, n = tile.n, row0 = tile.row0, len = tile.len;
+  const int64_t nrows = tile.count;
 
   // This lane's rows (a row past the last one reads the last one's q)
   int last[QT];  // the last key the row sees
@@ -202,32 +256,19 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
       int4v v{};
       if (WHOLE || d < a.d) v = *(const int4u*)(q + d);
       __builtin_memcpy(raw[s], &v, 16);
-      if constexpr (BF16) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf((float)raw[s][e]));
-      }
+      if constexpr (BF16) top = largest(raw[s], top);
     }
-    int ex = 0;
-    if constexpr (BF16) {
-      // the row's largest element comes to [2^14, 2^15): what is below 2^-39
-      // of it is lost, far under the fp32 sums
-      top = row_max(top);
-      ex = top > 0.f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-      ex = min(max(ex, -120), 120);
-    }
+    const int ex = BF16 ? exponent_of(row_max(top)) : 0;
     c[x] = BF16 ? __builtin_ldexpf(a.c, -ex) : a.c;
 #pragma unroll
-    for (int s = 0; s < 2 * DC; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        qf[x][s][e] = BF16 ? (_Float16)__builtin_ldexpf((float)raw[s][e], ex) : (_Float16)(float)raw[s][e];
+    for (int s = 0; s < 2 * DC; ++s) qf[x][s] = q_operand(raw[s], ex);
   }
 
   // keys this tile / all of its rows see
   const int i1 = (int)min((int64_t)n - 1, ((int64_t)row0 + RT - 1) / a.group);
   const int kend = max(0, min(len, len - n + i1 + 1));
   const int kfull = max(0, min(len, len - n + row0 / a.group + 1));
-  const int groups = (kend + 63) >> 6, share = (groups + a.nsplit - 1) / a.nsplit;
+  const int groups = (kend + 63) >> 6, share = (groups + nsplit - 1) / nsplit;
   const int g1 = min(groups, (split + 1) * share);
 
   Partial<QT, DT> acc;
@@ -303,48 +344,52 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
     if (more) load_k(g + 4, bk2);
     // softmax
     const bool whole = g * 64 + 64 <= kfull && __all(there0);  // (wave-uniform)
-    const float lv = __builtin_amdgcn_logf(vs0);
+    float lv, rv;
+    value_scale(vs0, lv, rv);
     half8v p[QT][2];
 #pragma unroll
     for (int y = 0; y < QT; ++y) {
       const float cs = c[y] * ks0;
-      const int left = there0 ? last[y] - (g * 64 + lg * 16) : -1;  // keys of this lane up to this one are seen
-      float mx = -INFINITY;
+      float mx = -INFINITY, lvy = lv;
+      if (whole) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[y][t][i] *= cs;
-          if (!whole && 4 * t + i > left) s[y][t][i] = -INFINITY;
-          mx = fmaxf(mx, s[y][t][i]);
-        }
-      const float lane_max = mx;
-      const float mxv = row_max(mx == -INFINITY ? -INFINITY : mx + lv);
-      mx = row_max(mx);
-      const bool upd = mx > acc.m[y] + 8.f || mxv > acc.mv[y] + 8.f;
-      if (__any(upd)) {
-        const float mn = upd ? fmaxf(acc.m[y], mx) : acc.m[y], vn = upd ? fmaxf(acc.mv[y], mxv) : acc.mv[y];
-        acc.l[y] *= rel_exp2(acc.m[y], mn);
-        const float f = rel_exp2(acc.mv[y], vn);
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[y][t][i]);
+        mx *= cs;  // (cs >= 0)
+      } else {
+        // the scores times cs, masked ones -inf
+        const int left = there0 ? last[y] - (g * 64 + lg * 16) : -1;  // keys of this lane up to this one are seen
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[y][t][i] = 4 * t + i > left ? -INFINITY : s[y][t][i] * cs;
+            mx = fmaxf(mx, s[y][t][i]);
+          }
+        // (a page whose every key is masked takes no part, whatever its scale)
+        if (left < 0) lvy = -INFINITY;
+      }
+      const float mxv = row_max(left_out(mx, lvy));
+      if (__any(mxv > acc.mv[y] + 8.f)) {
+        const float vn = mxv > acc.mv[y] + 8.f ? mxv : acc.mv[y], f = rel_exp2(acc.mv[y], vn);
+        acc.l[y] *= f;
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc.o[y][t] *= f;
-        acc.m[y] = mn;
         acc.mv[y] = vn;
       }
-      const float m_use = acc.m[y] == -INFINITY ? 0.f : acc.m[y];
-      const float v_use = acc.mv[y] == -INFINITY ? 0.f : acc.mv[y];
-      // (a page whose every key is masked takes no part, whatever its scale;
-      // the bound keeps 0 * f at 0 for scales 2^120 apart)
-      float f = lane_max == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lv + m_use - v_use);
-      f = f > 0x1p120f ? 0x1p120f : f;
+      const float off = lvy == -INFINITY ? -INFINITY : lvy - (acc.mv[y] == -INFINITY ? 0.f : acc.mv[y]);
+      const float cw = whole ? cs : 1.f;
+      float sum = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(s[y][t][i] - m_use);
-          acc.l[y] += e;
-          p[y][t >> 1][(t & 1) * 4 + i] = (_Float16)(e * f);
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[y][t][i], cw, off));
+          sum += e;
+          p[y][t >> 1][(t & 1) * 4 + i] = (_Float16)e;
         }
+      acc.l[y] += lvy == -INFINITY ? 0.f : sum * rv;
     }
     // values
 #pragma unroll
@@ -380,14 +425,14 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
   };
   join();
 
-  if (a.nsplit > 1) {
+  if (nsplit > 1) {
     // Every share stores its part (system-coherent stores, visible to every
     // XCD once vmcnt drains) and arrives on the tile's counter; the last one
     // joins them.
     constexpr int kCoherent = 17;  // sc0 | sc1
     constexpr int PART = NV * 64 * 4;
     const __amdgpu_buffer_rsrc_t rP =
-        make_rsrc(a.ws + kWsCounterBytes + (int64_t)item * a.nsplit * PART, (uint32_t)(a.nsplit * PART));
+        make_rsrc(a.ws + kWsCounterBytes + (int64_t)(item - a.full) * nsplit * PART, (uint32_t)(nsplit * PART));
     if (w == 0) {
       acc.each([&](int i, float v) {
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rP, (uint32_t)(split * PART + (i * 64 + lane) * 4), 0,
@@ -396,17 +441,17 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
       });
       wait_vmcnt0();
       if (lane == 0) {
-        unsigned long long* cnt = (unsigned long long*)a.ws + item;  // < kWsMaxTiles (the host's check)
+        unsigned long long* cnt = (unsigned long long*)a.ws + (item - a.full);  // < kWsMaxTiles (the host's check)
         const unsigned long long before =
             __hip_atomic_fetch_add(cnt, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last_split = before + 1 == (unsigned long long)a.nsplit;
+        last_split = before + 1 == (unsigned long long)nsplit;
         if (last_split) __hip_atomic_store(cnt, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
     __syncthreads();
     if (!last_split) return;
     acc.clear();
-    for (int sp = w; sp < a.nsplit; sp += 4) {  // (in this order whichever came last)
+    for (int sp = w; sp < nsplit; sp += 4) {  // (in this order whichever came last)
       Partial<QT, DT> other;
       other.each([&](int i, float) {
         return __uint_as_float(
@@ -423,9 +468,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
   for (int x = 0; x < QT; ++x) {
     const int64_t row = (int64_t)row0 + x * 16 + lr;
     const float l = row_reduce(acc.l[x], [](float y, float z) { return y + z; });
-    // no key seen: zeros
-    const float f = l == 0.f || acc.mv[x] == -INFINITY ? (l == l ? 0.f : l)
-                                                       : __builtin_amdgcn_exp2f(acc.mv[x] - acc.m[x]) / l;
+    const float f = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
     if (row >= nrows) continue;
     const int i = (int)(row / a.group), head = kvh * a.group + (int)(row - (int64_t)i * a.group);
     T* const o = (T*)a.o + (int64_t)(first + i) * a.ldo + (int64_t)head * a.ho;
@@ -443,60 +486,383 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
   }
 }
 
-// Row tiles a workgroup takes (QT), their number and the shares of the keys:
-// from sizes alone, so the workspace can be asked for beforehand.
+// ---- rows in the hundreds ----------------------------------------------------------
+//
+// A workgroup of four waves owns 128 rows (32 a wave) and takes 64 keys at a
+// time through two LDS stages: its threads convert the codes to fp16 on the way
+// in, so a code is converted once for 128 rows (the kernel above: once for 16 or
+// 32), and codes of the next stage but one are in flight meanwhile.  Eight waves
+// of 256 rows convert half as often and were slower (289 us, 279 of four, 2350
+// rows x 32 heads over 8000 keys): one workgroup a CU has nothing to run while
+// it waits at its barriers.  Scores are D[key][row] of 32x32x16 MFMAs; row m of a 32-key block
+// reads key 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that a
+// lane's eight weights of 16 keys are eight in order, the B operand of P.V.  The
+// 16 keys are one piece of a page: K and V scales are wave-uniform.
+// D: LDS rows of K (64 or 128 dims).
+template <typename T, int D, bool WHOLE>
+__global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
+  constexpr bool BF16 = !std::is_same_v<T, _Float16>;
+  constexpr int DS = D / 16, DT = D / 32, RB = 2 * D;
+  constexpr int KB = 64 * RB, STAGE = KB + D * 128;
+  constexpr int PIECES = 64 * D / 16 / 256;  // 16-byte pieces of K (and of V) a thread converts a stage
+  constexpr int NV = DT * 16 + 2;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  __shared__ int last_split;
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 31, h = lane >> 5;
+  const Share part = share_of(a);
+  const int split = part.split, nsplit = part.count, item = part.item;
+  const int kvh = item / a.tiles;
+  Rows tile;
+  if (!rows_of<128>(a, a.tiles - 1 - (item - kvh * a.tiles), tile)) return;  // (the last rows see the most keys)
+  const int n = tile.n, len = tile.len;
+
+  // This lane's row (past the last one: the last one's q, not stored)
+  const int64_t row = (int64_t)tile.row0 + w * 32 + lr, rowq = min(row, tile.count - 1);
+  const int token = (int)(rowq / a.group), head = kvh * a.group + (int)(rowq - (int64_t)token * a.group);
+  const int last = (int)min((int64_t)len - n + token, (int64_t)len - 1);  // the last key it sees
+  half8v qf[DS];
+  float c = a.c;
+  {
+    const T* q = (const T*)a.q + (int64_t)(tile.first + token) * a.ldq + (int64_t)head * a.hq;
+    T raw[DS][8];
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      const int d = s * 16 + h * 8;
+      int4v v{};
+      if (WHOLE || d < a.d) v = *(const int4u*)(q + d);
+      __builtin_memcpy(raw[s], &v, 16);
+      if constexpr (BF16) top = largest(raw[s], top);
+    }
+    int ex = 0;
+    if constexpr (BF16) {
+      const auto t2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      ex = exponent_of(fmaxf(__uint_as_float(t2[0]), __uint_as_float(t2[1])));
+      c = __builtin_ldexpf(a.c, -ex);
+    }
+#pragma unroll
+    for (int s = 0; s < DS; ++s) qf[s] = q_operand(raw[s], ex);
+  }
+
+  // keys that some / all rows of the workgroup, and all rows of the wave, see
+  const int i1 = (int)min((int64_t)n - 1, ((int64_t)tile.row0 + 127) / a.group);
+  const int kend = max(0, min(len, len - n + i1 + 1));
+  const int wrow = tile.row0 + w * 32;
+  const int kfull = wrow < tile.count ? max(0, min(len, len - n + wrow / a.group + 1)) : 0;
+  const int stages = (kend + 63) >> 6, share = (stages + nsplit - 1) / nsplit;
+  const int c0 = split * share, c1 = min(stages, c0 + share);
+
+  const int* const table = a.table + (int64_t)tile.r * a.ldt;
+  const int64_t hb = (int64_t)kvh * a.bytes, kv_bytes = (int64_t)a.kv_heads * a.bytes;
+  const int pm = (1 << a.lb) - 1;
+  // Lane l's page of a stage: that of its 16-key piece l % 4, -1 where there is none or a bad one.
+  auto page = [&](int st) {
+    const int piece = 4 * st + (lane & 3), p = piece >> a.lb;
+    const int b = p < a.width && piece * 16 < kend ? table[p] : -1;
+    return (unsigned)b < (unsigned)a.blocks ? b : -1;
+  };
+
+  // Thread t's pieces of a stage: K, key t / 4, bytes 16 (t % 4 + 4 i); V, 16
+  // keys (the wave's) of dims t % 64 + 64 i.  Wave w's keys are 16 w .. 16 w + 15.
+  const int t = threadIdx.x;
+  int4v kc[PIECES], vc[PIECES];
+  struct Scales {  // of a lane's piece
+    int b;
+    float k, v;
+  };
+  // The codes and scales of a stage with pages `pg` (a page that is not there: block 0's, left out below).
+  auto load = [&](int st, int pg) {
+    const int piece = 4 * st + w, b = max(__builtin_amdgcn_readlane(pg, w), 0);
+    const int8_t* const kp = a.k + b * kv_bytes + hb + ((int64_t)((piece & pm) * 16 + (lane >> 2)) * a.dp + (lane & 3) * 16);
+    const int8_t* const vp = a.v + b * kv_bytes + hb + ((int64_t)(piece & pm) * a.dp + lane) * 16;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      kc[i] = WHOLE || (lane & 3) * 16 + 64 * i < a.dp ? *(const int4v*)(kp + 64 * i) : int4v{};
+      vc[i] = WHOLE || lane + 64 * i < a.dp ? *(const int4v*)(vp + 1024 * i) : int4v{};
+    }
+    const int64_t at = (int64_t)max(pg, 0) * a.kv_heads + kvh;
+    return Scales{pg, a.ks[at], a.vs[at]};
+  };
+  // 16-byte chunks of LDS rows are XOR-swizzled: the rows that one read takes
+  // 16 bytes of (16 lanes at a time) fall on different banks.
+  auto k_at = [](int key, int chunk) { return key * RB + ((chunk ^ (key / (256 / RB) & (RB / 16 - 1))) << 4); };
+  auto v_at = [](int d, int chunk) { return KB + d * 128 + ((chunk ^ (d >> 1 & 7)) << 4); };
+  // (the swizzle is an XOR of chunk bits: chunk 2 i + u of a row lies at the row's chunk 0 with those bits flipped)
+  const int k_store = k_at(t >> 2, (t & 3) * 2), v_store = v_at(lane, 2 * w);
+  // Unit j of 4 * PIECES = DS: half a piece, eight codes.
+  auto store = [&](char* base, int j) {
+    const int i = j >> 2, u = j & 1;
+    if (j & 2) *(half8v*)(base + (v_store ^ (u << 4)) + 64 * i * 128) = operand(vc[i][2 * u], vc[i][2 * u + 1]);
+    else *(half8v*)(base + (k_store ^ ((8 * i + u) << 4))) = operand(kc[i][2 * u], kc[i][2 * u + 1]);
+  };
+  static_assert(4 * PIECES == DS, "a unit a step of the scores");
+
+  float16v o[DT];
+#pragma unroll
+  for (int x = 0; x < DT; ++x) o[x] = float16v{};
+  float mv = -INFINITY, l = 0.f;
+
+  const int key = 16 * (lr >> 4) + 8 * (lr >> 2 & 1) + 4 * (lr >> 3 & 1) + (lr & 3);
+  const int k_read = k_at(key, h), v_read = v_at(lr, h);
+  Scales after{};
+  int pg = -1;
+  // Stage st in `base`, while `other` takes the next one.
+  auto compute = [&](int st, const char* base, char* other, const Scales& sc) {
+    // each lane's piece, then the four as scalars
+    float lane_lv, lane_rv;
+    value_scale(sc.v, lane_lv, lane_rv);
+    if (sc.b < 0) lane_lv = -INFINITY;
+    const float lane_ks = sc.b < 0 ? 0.f : sc.k;
+    const bool all = st * 64 + 64 <= kfull && __all(sc.b >= 0);
+    float ks[4], lv[4], rv[4];
+    auto lane_of = [](float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); };
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      ks[x] = lane_of(lane_ks, x);
+      lv[x] = lane_of(lane_lv, x);
+      rv[x] = lane_of(lane_rv, x);
+    }
+    // Fragments are read a step ahead of their MFMAs; the scheduling barriers
+    // keep the compiler from reading them all first.
+    float16v s[2];
+    half8v kf[2][2], vf[2][DT];
+    auto read_k = [&](int x) {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) kf[x & 1][nb] = *(const half8v*)(base + (k_read ^ (x << 5)) + nb * 32 * RB);
+    };
+    auto read_v = [&](int x) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) vf[x & 1][dt] = *(const half8v*)(base + (v_read ^ (x << 5)) + dt * 32 * 128);
+    };
+    read_k(0);
+#pragma unroll
+    for (int x = 0; x < DS; ++x) {
+      if (x + 1 < DS) read_k(x + 1);
+      else read_v(0);
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+        s[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[x & 1][nb], qf[x], x == 0 ? float16v{} : s[nb], 0, 0, 0);
+      if (st + 1 < c1) store(other, x);  // (conversion passes under the score MFMAs, which need few vector instructions)
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // (the codes' registers are free)
+    if (st + 2 < c1) after = load(st + 2, pg);
+    if (st + 3 < c1) pg = page(st + 3);
+    // the largest weighted score; where some keys are masked, scores times their scale with those at -inf
+    float mx = -INFINITY;
+    if (all) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float m = s[x >> 1][8 * (x & 1)];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) m = fmaxf(m, s[x >> 1][8 * (x & 1) + e]);
+        mx = fmaxf(mx, fmaf(m, c * ks[x], lv[x]));
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int left = lv[x] == -INFINITY ? -1 : last - (st * 64 + x * 16 + 8 * h);
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = e > left ? -INFINITY : s[x >> 1][8 * (x & 1) + e] * (c * ks[x]);
+          s[x >> 1][8 * (x & 1) + e] = v;
+          m = fmaxf(m, v);
+        }
+        mx = fmaxf(mx, left < 0 ? -INFINITY : m + lv[x]);
+      }
+    }
+    const auto m2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    mx = fmaxf(__uint_as_float(m2[0]), __uint_as_float(m2[1]));
+    if (__any(mx > mv + 8.f)) {
+      const float vn = mx > mv + 8.f ? mx : mv, f = rel_exp2(mv, vn);
+      l *= f;
+#pragma unroll
+      for (int x = 0; x < DT; ++x) o[x] *= f;
+      mv = vn;
+    }
+    const float m_use = mv == -INFINITY ? 0.f : mv;
+    // the weights of 16 keys while the MFMAs of the 16 before run
+    auto weights = [&](int x) {
+      const bool some = all || !(last < st * 64 + x * 16 + 8 * h || lv[x] == -INFINITY);
+      const float off = some ? lv[x] - m_use : -INFINITY, cw = all ? c * ks[x] : 1.f;
+      half8v p;
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = __builtin_amdgcn_exp2f(fmaf(s[x >> 1][8 * (x & 1) + e], cw, off));
+        sum += v;
+        p[e] = (_Float16)v;
+      }
+      l += some ? sum * rv[x] : 0.f;
+      return p;
+    };
+    half8v p = weights(0);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      half8v after = p;
+      if (x < 3) {
+        read_v(x + 1);
+        after = weights(x + 1);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x & 1][dt], p, o[dt], 0, 0, 0);
+      p = after;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if (c0 < c1) {
+    // Ahead of the stage computed: the next one's codes on their way into LDS,
+    // codes and scales of the one after, pages of the one after that.
+    Scales now = load(c0, page(c0)), next{};
+#pragma unroll
+    for (int x = 0; x < DS; ++x) store(lds, x);
+    if (c0 + 1 < c1) next = load(c0 + 1, page(c0 + 1));
+    if (c0 + 2 < c1) pg = page(c0 + 2);
+    auto step = [&](int st, char* base, char* other) {
+      __syncthreads();  // stage st is written, and nobody reads the other one
+      compute(st, base, other, now);
+      now = next;
+      next = after;
+    };
+    for (int st = c0; st < c1; st += 2) {  // (LDS addresses that differ by constants)
+      step(st, lds, lds + STAGE);
+      if (st + 1 < c1) step(st + 1, lds + STAGE, lds);
+    }
+  }
+
+  // A wave's floats: o, mv, l; a tile's shares joined as in the kernel above.
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int x = 0; x < DT; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f(x * 16 + i, [&](float v) { o[x][i] = v; }, o[x][i]);
+    f(DT * 16, [&](float v) { mv = v; }, mv);
+    f(DT * 16 + 1, [&](float v) { l = v; }, l);
+  };
+  if (nsplit > 1) {
+    constexpr int kCoherent = 17;  // sc0 | sc1
+    constexpr int PART = 4 * NV * 64 * 4;
+    const __amdgpu_buffer_rsrc_t rP =
+        make_rsrc(a.ws + kWsCounterBytes + (int64_t)(item - a.full) * nsplit * PART, (uint32_t)(nsplit * PART));
+    each([&](int i, auto&&, float v) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rP, (uint32_t)(split * PART + ((w * NV + i) * 64 + lane) * 4),
+                                            0, kCoherent);
+    });
+    wait_vmcnt0();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      unsigned long long* cnt = (unsigned long long*)a.ws + (item - a.full);  // < kWsMaxTiles (the host's check)
+      const unsigned long long before = __hip_atomic_fetch_add(cnt, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last_split = before + 1 == (unsigned long long)nsplit;
+      if (last_split) __hip_atomic_store(cnt, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last_split) return;
+    auto held = [&](int sp, int i) {
+      return __uint_as_float(
+          __builtin_amdgcn_raw_buffer_load_b32(rP, (uint32_t)(sp * PART + ((w * NV + i) * 64 + lane) * 4), 0, kCoherent));
+    };
+    mv = -INFINITY;
+    for (int sp = 0; sp < nsplit; ++sp) mv = fmaxf(mv, held(sp, DT * 16));
+    l = 0.f;
+#pragma unroll
+    for (int x = 0; x < DT; ++x) o[x] = float16v{};
+    for (int sp = 0; sp < nsplit; ++sp) {  // (in this order whichever came last)
+      const float f = rel_exp2(held(sp, DT * 16), mv);
+      l += f * held(sp, DT * 16 + 1);
+#pragma unroll
+      for (int x = 0; x < DT; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[x][i] += f * held(sp, x * 16 + i);
+    }
+  }
+
+  // O: lane holds row l % 32, dims 32 x + 8 g + 4 h + 0..3
+  const auto l2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+  const float whole = __uint_as_float(l2[0]) + __uint_as_float(l2[1]);
+  const float f = whole == 0.f ? 0.f : 1.f / whole;  // no key seen: zeros
+  if (row >= tile.count) return;
+  T* const out = (T*)a.o + (int64_t)(tile.first + token) * a.ldo + (int64_t)head * a.ho;
+#pragma unroll
+  for (int x = 0; x < DT; ++x)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = x * 32 + 8 * g + 4 * h;
+      if (!WHOLE && d >= a.d) continue;
+      T o4[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o4[j] = (T)(o[x][4 * g + j] * f);
+      int2v bits;
+      __builtin_memcpy(&bits, o4, 8);
+      *(int2u*)(out + d) = bits;
+    }
+}
+
+// Rows of a workgroup, tiles of them and the shares of the keys: from sizes
+// alone, so the workspace can be asked for beforehand.
 struct KvPlan {
-  int qt, nsplit;
-  int64_t tiles;
+  int qt, nsplit;  // qt 0: kv_attention_tiles
+  int64_t tiles, full;
 };
+int64_t part_bytes(const KvAttnProblem& p, const KvPlan& k) {  // of a tile's share
+  const int64_t dt = p.d <= 64 ? 4 : 8;
+  return k.qt ? k.qt * (dt * 4 + 2) * 64 * 4 : 4 * (dt * 8 + 2) * 64 * 4;
+}
 KvPlan plan_of(const KvAttnProblem& p) {
   KvPlan r;
   const int64_t group = p.heads / p.kv_heads;
   const int64_t rows = (p.cu ? (p.tokens + p.requests - 1) / p.requests : 1) * group;  // of a request, on average
-  r.qt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int64_t rt = 16 * r.qt;
+  r.qt = rows <= 16 ? 1 : rows <= 64 ? 2 : 0;
+  const int64_t rt = r.qt ? 16 * r.qt : 128;
   r.tiles = p.cu ? p.tokens * group / rt + p.requests : p.requests * ((group + rt - 1) / rt);
-  // Shares until 512 workgroups (two a CU) are there, of at least one group
-  // of 64 keys a wave.
-  const int64_t items = r.tiles * p.kv_heads, most = (p.width * p.block + 255) / 256;
-  int64_t n = items >= 512 ? 1 : (512 + items - 1) / items;
+  // The card takes 512 workgroups at a time, two a CU.  Whole rounds of them
+  // run unshared; the tiles that are left share their keys out until they make
+  // one more round, at least one group of 64 keys a wave (eight stages of a
+  // 128-row tile) to a share.  575 tiles of 128 rows x 8000 keys: 391 us unshared,
+  // 292 with all of them in two shares, 281 with the last 63 in eight.
+  const int64_t items = r.tiles * p.kv_heads, least = r.qt ? 256 : 512, most = (p.width * p.block + least - 1) / least;
+  const int64_t left = items % 512;
+  int64_t n = left ? 512 / left : 1;
   n = n < most ? n : most;
   r.nsplit = (int)(n < 1 ? 1 : n < 128 ? n : 128);
+  r.full = r.nsplit > 1 ? items - left : items;
   return r;
 }
 
-int64_t part_bytes(const KvAttnProblem& p, int qt) {
-  const int64_t dt = p.d <= 64 ? 4 : 8;
-  return qt * (dt * 4 + 3) * 64 * 4;
-}
-
-template <typename T, int DC, bool WHOLE>
-hipError_t launch_qt(int qt, dim3 grid, const KArgs& a, hipStream_t stream) {
-  const auto fn = qt == 1   ? kv_attention<T, DC, WHOLE, 1>
-                  : qt == 2 ? kv_attention<T, DC, WHOLE, 2>
-                            : kv_attention<T, DC, WHOLE, 4>;
-  hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream, a);
-  return hipGetLastError();
-}
 template <typename T>
 hipError_t launch_t(int64_t d, int qt, dim3 grid, const KArgs& a, hipStream_t stream) {
-  if (d == 64) return launch_qt<T, 1, true>(qt, grid, a, stream);
-  if (d == 128) return launch_qt<T, 2, true>(qt, grid, a, stream);
-  return d < 64 ? launch_qt<T, 1, false>(qt, grid, a, stream) : launch_qt<T, 2, false>(qt, grid, a, stream);
+  const bool small = d <= 64, whole = d == 64 || d == 128;
+  const auto fn = qt == 1   ? (small ? whole ? kv_attention<T, 1, true, 1> : kv_attention<T, 1, false, 1>
+                                     : whole ? kv_attention<T, 2, true, 1> : kv_attention<T, 2, false, 1>)
+                  : qt == 2 ? (small ? whole ? kv_attention<T, 1, true, 2> : kv_attention<T, 1, false, 2>
+                                     : whole ? kv_attention<T, 2, true, 2> : kv_attention<T, 2, false, 2>)
+                 : small   ? (whole ? kv_attention_tiles<T, 64, true> : kv_attention_tiles<T, 64, false>)
+                           : (whole ? kv_attention_tiles<T, 128, true> : kv_attention_tiles<T, 128, false>);
+  hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t kv_attention_workspace_bytes(const KvAttnProblem& p) {
   const KvPlan k = plan_of(p);
-  return k.nsplit > 1 ? kWsCounterBytes + k.tiles * p.kv_heads * k.nsplit * part_bytes(p, k.qt) : 0;
+  return k.nsplit > 1 ? kWsCounterBytes + (k.tiles * p.kv_heads - k.full) * k.nsplit * part_bytes(p, k) : 0;
 }
 
 hipError_t launch_kv_attention(const KvAttnProblem& p, hipStream_t stream) {
   KvPlan k = plan_of(p);
   const int64_t items = k.tiles * p.kv_heads;
-  if (k.nsplit > 1 && (!p.ws || p.ws_bytes < kv_attention_workspace_bytes(p) || items > kWsMaxTiles)) k.nsplit = 1;
-  if (items * k.nsplit >= (1ll << 31)) return hipErrorInvalidValue;
+  if (k.nsplit > 1 && (!p.ws || p.ws_bytes < kv_attention_workspace_bytes(p))) {
+    k.nsplit = 1;
+    k.full = items;
+  }
+  const int64_t grid = k.full + (items - k.full) * k.nsplit;
+  static_assert(512 <= kWsMaxTiles, "a counter for every shared tile");
+  if (grid >= (1ll << 31)) return hipErrorInvalidValue;
   KArgs a{};
   a.q = (const char*)p.q;
   a.k = p.k_codes;
@@ -524,10 +890,11 @@ hipError_t launch_kv_attention(const KvAttnProblem& p, hipStream_t stream) {
   a.blocks = (int)p.blocks;
   a.width = (int)p.width;
   a.tiles = (int)k.tiles;
+  a.full = (int)k.full;
   a.nsplit = k.nsplit;
   a.c = p.scale * kLog2e;
-  const dim3 grid((unsigned)(items * k.nsplit));
-  return p.dtype == DT_BF16 ? launch_t<__bf16>(p.d, k.qt, grid, a, stream) : launch_t<_Float16>(p.d, k.qt, grid, a, stream);
+  const dim3 blocks((unsigned)grid);
+  return p.dtype == DT_BF16 ? launch_t<__bf16>(p.d, k.qt, blocks, a, stream) : launch_t<_Float16>(p.d, k.qt, blocks, a, stream);
 }
 
 }  // namespace hxmi

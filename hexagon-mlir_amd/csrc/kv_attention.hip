@@ -644,17 +644,22 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb)
         s[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[x & 1][nb], qf[x], x == 0 ? float16v{} : s[nb], 0, 0, 0);
-      if (st + 1 < c1) store(other, x);  // (conversion passes under the score MFMAs, which need few vector instructions)
+      // (conversion passes under the score MFMAs, which need few vector
+      // instructions; past the last stage old codes go where nobody reads)
+      store(other, x);
       __builtin_amdgcn_sched_barrier(0);
     }
     // (the codes' registers are free)
     if (st + 2 < c1) after = load(st + 2, pg);
     if (st + 3 < c1) pg = page(st + 3);
-    // the largest weighted score; where some keys are masked, scores times their scale with those at -inf
+    // the largest weighted score of the keys that are seen: the first `left` + 1
+    // of a lane's eight of a piece (all of a piece: more than that)
+    int left[4];
     float mx = -INFINITY;
     if (all) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
+        left[x] = 8;
         float m = s[x >> 1][8 * (x & 1)];
 #pragma unroll
         for (int e = 1; e < 8; ++e) m = fmaxf(m, s[x >> 1][8 * (x & 1) + e]);
@@ -663,15 +668,11 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
     } else {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int left = lv[x] == -INFINITY ? -1 : last - (st * 64 + x * 16 + 8 * h);
+        left[x] = lv[x] == -INFINITY ? -1 : last - (st * 64 + x * 16 + 8 * h);
         float m = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float v = e > left ? -INFINITY : s[x >> 1][8 * (x & 1) + e] * (c * ks[x]);
-          s[x >> 1][8 * (x & 1) + e] = v;
-          m = fmaxf(m, v);
-        }
-        mx = fmaxf(mx, left < 0 ? -INFINITY : m + lv[x]);
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, e > left[x] ? -INFINITY : s[x >> 1][8 * (x & 1) + e]);
+        mx = fmaxf(mx, left[x] < 0 ? -INFINITY : fmaf(m, c * ks[x], lv[x]));
       }
     }
     const auto m2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
@@ -686,17 +687,21 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
     const float m_use = mv == -INFINITY ? 0.f : mv;
     // the weights of 16 keys while the MFMAs of the 16 before run
     auto weights = [&](int x) {
-      const bool some = all || !(last < st * 64 + x * 16 + 8 * h || lv[x] == -INFINITY);
-      const float off = some ? lv[x] - m_use : -INFINITY, cw = all ? c * ks[x] : 1.f;
+      const float off = lv[x] - m_use, cs = c * ks[x];
+      float v[8], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __builtin_amdgcn_exp2f(fmaf(s[x >> 1][8 * (x & 1) + e], cs, off));
+      if (!all) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e > left[x] ? 0.f : v[e];
+      }
       half8v p;
-      float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = __builtin_amdgcn_exp2f(fmaf(s[x >> 1][8 * (x & 1) + e], cw, off));
-        sum += v;
-        p[e] = (_Float16)v;
+        sum += v[e];
+        p[e] = (_Float16)v[e];
       }
-      l += some ? sum * rv[x] : 0.f;
+      l += sum == 0.f ? 0.f : sum * rv[x];  // (rv is of no use where nothing is seen)
       return p;
     };
     half8v p = weights(0);

@@ -156,6 +156,23 @@ __device__ __forceinline__ float wave_sum_dpp(float v) {
   return wave_reduce_dpp(v, [](float x, float y) { return x + y; });
 }
 
+// Inclusive sum over the wave in lane order, by DPP: within rows of 16 lanes,
+// then each row's last lane to the next row, then lane 31 to the upper half.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_add64(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ uint64_t scan64(uint64_t v) {
+  v = dpp_add64<0x111, 0xf>(v);  // row_shr:1
+  v = dpp_add64<0x112, 0xf>(v);
+  v = dpp_add64<0x114, 0xf>(v);
+  v = dpp_add64<0x118, 0xf>(v);
+  v = dpp_add64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  return dpp_add64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+}
+
 // Sum over aligned groups of `width` lanes (width a power of two <= 64).
 template <int width>
 __device__ __forceinline__ float group_sum(float v) {

@@ -197,7 +197,7 @@ struct AttnProblem {
 hipError_t launch_attention(const AttnProblem& p, hipStream_t stream);
 
 // Block tables and slot maps of one serving step (kvcache.hip).
-constexpr int64_t kPlanRequests = 4096;  // a call's requests (three 32-bit words of LDS each)
+constexpr int64_t kPlanRequests = 4096;  // a call's requests (five 32-bit words of LDS each)
 struct KvPlanProblem {
   const int *lens, *added;
   int *table, *stack;

@@ -36,90 +36,102 @@ struct PArgs {
   int64_t ldt;
 };
 
-// Inclusive sum over the workgroup's threads; `total` receives the whole sum.
+// Inclusive sums of two numbers over the workgroup's threads in thread order,
+// and their totals.
 template <int NT>
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t& total) {
+__device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t (*part)[NT / 64], int64_t& total_a,
+                                            int64_t& total_b) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t t = __shfl_up(v, o, 64);
-    if (lane >= o) v += t;
+  a = (int64_t)scan64((uint64_t)a);
+  b = (int64_t)scan64((uint64_t)b);
+  __syncthreads();
+  if (lane == 63) {
+    part[0][w] = a;
+    part[1][w] = b;
   }
   __syncthreads();
-  if (lane == 63) part[w] = v;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
+  total_a = total_b = 0;
 #pragma unroll
   for (int i = 0; i < NT / 64; ++i) {
-    const int64_t t = part[i];
-    if (i < w) before += t;
-    total += t;
+    const int64_t ta = part[0][i], tb = part[1][i];
+    a += i < w ? ta : 0;
+    b += i < w ? tb : 0;
+    total_a += ta;
+    total_b += tb;
   }
-  return before + v;
 }
 
 // Every workgroup takes the sums over all requests (at most kPlanRequests,
 // a few KB of lengths out of L2), then its waves take a request each: no
 // workgroup waits for another and one launch does.  What bounds it is that
-// chain: load, sums, look-ups, stores.
+// chain: load, sums, look-ups, stores.  A request's page numbers are looked up
+// 64 at a time, a lane each, before the slots that lie in them.
+// 16 requests: 10.1 us with shuffled sums and lengths read again, 3.9 us;
+// 1024 requests, 16384 rows: 18 us with a look-up a row, 8.3 us.
 template <int NT>
 __global__ __launch_bounds__(NT) void kv_plan(PArgs a) {
-  extern __shared__ int shared[];  // cu [requests + 1], first block taken (-1: not admitted), first released
-  __shared__ int64_t part[NT / 64];
-  int* const cu = shared;
-  int* const first = cu + a.requests + 1;
-  int* const freed = first + a.requests;
+  __shared__ int cu[kPlanRequests + 1], first[kPlanRequests];  // rows; first block taken (-1: not admitted)
+  __shared__ int freed[kPlanRequests];                         // first block released
+  __shared__ int lens[kPlanRequests], added[kPlanRequests];
+  __shared__ int64_t part[2][NT / 64];
+  __shared__ unsigned long long taken;
   const int64_t bs1 = (1ll << a.lb) - 1, limit = (int64_t)a.width << a.lb;
-  auto held = [&](int r) { return min(max((int64_t)a.lens[r], (int64_t)0), limit); };
+  const int lane = threadIdx.x & 63;
 
-  int64_t back_all = 0;
+  if (threadIdx.x == 0) taken = 0;
+  const int64_t had = min(max((int64_t)*a.count, (int64_t)0), (int64_t)a.capacity);
+  int64_t back_all = 0, rows = 0;
   for (int r0 = 0; r0 < a.requests; r0 += NT) {
     const int r = r0 + threadIdx.x;
     const bool in = r < a.requests;
-    const int64_t back = in && a.added[r] < 0 ? (held(r) + bs1) >> a.lb : 0;
-    int64_t total;
-    const int64_t incl = block_scan<NT>(back, part, total);
-    if (in) freed[r] = (int)(back_all + incl - back);
-    back_all += total;
-  }
-  const int64_t had = min(max((int64_t)*a.count, (int64_t)0), (int64_t)a.capacity), avail = had + back_all;
-  int64_t rows = 0, wanted = 0, taken = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += NT) {
-    const int r = r0 + threadIdx.x;
-    const bool in = r < a.requests;
-    const int64_t add = in ? max(a.added[r], 0) : 0, len = in ? held(r) : 0;
-    int64_t total;
-    const int64_t end = rows + block_scan<NT>(add, part, total);
-    rows += total;
-    const int64_t have = (len + bs1) >> a.lb, need = ((len + add + bs1) >> a.lb) - have;
-    const bool fits = add > 0 && have + need <= a.width && end <= a.tokens;
-    const int64_t want = fits ? need : 0, incl = wanted + block_scan<NT>(want, part, total);
-    wanted += total;
-    const bool admitted = fits && (want == 0 || incl <= avail);
-    int64_t unused = block_scan<NT>(admitted ? want : 0, part, total);
-    (void)unused;
-    taken += total;
+    const int add = in ? a.added[r] : 0;
+    const int64_t len = in ? min(max((int64_t)a.lens[r], (int64_t)0), limit) : 0;
+    const int64_t back = add < 0 ? (len + bs1) >> a.lb : 0, more = max(add, 0);
+    int64_t back_to = back, rows_to = more, back_total, rows_total;
+    block_scan2<NT>(back_to, rows_to, part, back_total, rows_total);
     if (in) {
-      cu[r] = (int)min(end - add, (int64_t)INT32_MAX);
-      // (the admitted ones that want blocks come first among those that want any)
-      first[r] = admitted ? (int)(incl - want) : -1;
+      lens[r] = (int)len;
+      added[r] = add;
+      freed[r] = (int)(back_all + back_to - back);
+      cu[r] = (int)min(rows + rows_to - more, (int64_t)INT32_MAX);
+    }
+    back_all += back_total;
+    rows += rows_total;
+  }
+  const int64_t avail = had + back_all;
+  const int all = (int)min(rows, (int64_t)INT32_MAX);
+  if (threadIdx.x == 0) cu[a.requests] = all;
+  __syncthreads();
+  int64_t wanted = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += NT) {
+    const int r = r0 + threadIdx.x;
+    const bool in = r < a.requests;
+    const int64_t len = in ? lens[r] : 0, add = in ? max(added[r], 0) : 0, have = (len + bs1) >> a.lb;
+    const int64_t need = ((len + add + bs1) >> a.lb) - have;
+    // (a row count that passed 2^31 passes any `tokens`)
+    const bool fits = add > 0 && have + need <= a.width && cu[in ? r : 0] + add <= a.tokens;
+    const int64_t want = fits ? need : 0;
+    int64_t to = want, unused = 0, total, none;
+    block_scan2<NT>(to, unused, part, total, none);
+    to += wanted;
+    wanted += total;
+    const bool admitted = fits && (want == 0 || to <= avail);
+    // (the admitted ones that want blocks come first among those that want any)
+    if (admitted && want > 0) atomicMax(&taken, (unsigned long long)to);
+    if (in) {
+      first[r] = admitted ? (int)(to - want) : -1;
       if (blockIdx.x == 0) {
         a.cu[r] = cu[r];
-        a.lens_out[r] = a.added[r] < 0 ? 0 : (int)(admitted ? len + add : len);
+        a.lens_out[r] = added[r] < 0 ? 0 : (int)(admitted ? len + add : len);
       }
     }
   }
-  const int all = (int)min(rows, (int64_t)INT32_MAX);
-  const int64_t left = min(avail - taken, (int64_t)a.capacity);
-  if (threadIdx.x == 0) {
-    cu[a.requests] = all;
-    if (blockIdx.x == 0) {
-      a.cu[a.requests] = all;
-      *a.count_out = (int)left;
-    }
-  }
   __syncthreads();
+  const int64_t left = min(avail - (int64_t)taken, (int64_t)a.capacity);
+  if (threadIdx.x == 0 && blockIdx.x == 0) {
+    a.cu[a.requests] = all;
+    *a.count_out = (int)left;
+  }
 
   // The block that comes i-th off the stack: one of the held ones, or one
   // that a request of this step has released (still in its table row).
@@ -136,11 +148,11 @@ __global__ __launch_bounds__(NT) void kv_plan(PArgs a) {
     return a.table[lo * a.ldt + (q - freed[lo])];
   };
 
-  const int lane = threadIdx.x & 63, waves = NT / 64 * gridDim.x;
+  const int waves = NT / 64 * gridDim.x;
   for (int r = blockIdx.x * (NT / 64) + (threadIdx.x >> 6); r < a.requests; r += waves) {
-    const int64_t len = held(r), have = (len + bs1) >> a.lb;
+    const int64_t len = lens[r], have = (len + bs1) >> a.lb;
     int* const row = a.table + r * a.ldt;
-    const int add = a.added[r];
+    const int add = added[r];
     if (add < 0) {
       for (int64_t i = lane; i < have; i += 64) {
         const int64_t p = had + freed[r] + i;
@@ -157,13 +169,27 @@ __global__ __launch_bounds__(NT) void kv_plan(PArgs a) {
       }
       continue;
     }
-    const int64_t need = ((len + add + bs1) >> a.lb) - have;
-    for (int64_t j = lane; j < need; j += 64) row[have + j] = block(at + j);
-    for (int64_t t = c0 + lane; t < c1; t += 64) {
-      const int64_t p = len + t - c0, b = p >> a.lb;
-      const int64_t id = b < have ? row[b] : block(at + b - have);
-      a.slots[t] = id < 0 ? -1 : (id << a.lb) + (p & bs1);
-      a.positions[t] = (int)p;
+    const int64_t end = len + add, p1 = (end + bs1) >> a.lb;
+    for (int64_t p0 = len >> a.lb; p0 < p1; p0 += 64) {  // pages that take rows, 64 at a time
+      const int64_t page = p0 + lane;
+      int id = -1;
+      if (page < p1) {
+        if (page < have) {
+          id = row[page];
+        } else {
+          id = block(at + page - have);
+          row[page] = id;
+        }
+      }
+      const int64_t q0 = max(len, p0 << a.lb), q1 = min(end, (p0 + 64) << a.lb);
+      for (int64_t q = q0; q < q1; q += 64) {  // (the wave together: lanes read each other's pages)
+        const int64_t pos = q + lane;
+        const int64_t b = __shfl(id, (int)((pos >> a.lb) - p0) & 63, 64);
+        if (pos < q1) {
+          a.slots[c0 + pos - len] = b < 0 ? -1 : (b << a.lb) + (pos & bs1);
+          a.positions[c0 + pos - len] = (int)pos;
+        }
+      }
     }
   }
   for (int64_t t = (int64_t)all + blockIdx.x * NT + threadIdx.x; t < a.tokens; t += (int64_t)NT * gridDim.x) {
@@ -228,23 +254,40 @@ __global__ __launch_bounds__(256) void kv_append(CArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int hv = (int)(item % (2 * a.heads)), h = hv >> 1, is_v = hv & 1;
-  const int64_t t0 = item / (2 * a.heads) * a.span, t1 = min(t0 + a.span, a.tokens);
+  const int64_t t0 = item / (2 * a.heads) * a.span;  // (a.span <= 64)
   const int bs = 1 << a.lb;
-  for (int64_t t = t0; t < t1; ++t) {
-    const int64_t slot = a.slots[t];
-    if (slot < 0 || slot >= a.cells) continue;
+  // Rows that begin a run, among this wave's span: a slot in the cache that
+  // does not follow the row before in its block.
+  int64_t slot_l = -1;
+  bool begins = false;
+  if (t0 + lane < a.tokens) {
+    slot_l = a.slots[t0 + lane];
+    const int64_t before = t0 + lane > 0 ? a.slots[t0 + lane - 1] : -1;
+    begins = slot_l >= 0 && slot_l < a.cells && ((slot_l & (bs - 1)) == 0 || before != slot_l - 1);
+  }
+  for (uint64_t runs = __ballot(begins && lane < a.span); runs; runs &= runs - 1) {
+    const int l = __ffsll((unsigned long long)runs) - 1;
+    const int64_t t = t0 + l;
+    const int64_t slot = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)slot_l, l) |
+                         (int64_t)__builtin_amdgcn_readlane((int)(slot_l >> 32), l) << 32;
     const int off = (int)(slot & (bs - 1));
-    if (off > 0 && t > 0 && a.slots[t - 1] == slot - 1) continue;
-    int n = 0;  // rows of the run
-    for (;;) {
-      const int64_t u = t + n + lane;
-      const bool in = n + lane < bs - off && u < a.tokens && a.slots[u] == slot + n + lane;
-      const uint64_t miss = __ballot(!in);
-      if (miss) {
-        n += __ffsll((unsigned long long)miss) - 1;
-        break;
-      }
-      n += 64;
+    // its rows: up to the end of its block, as far as the slots follow each other
+    int n = 0;
+    {
+      const uint64_t miss = ~(__ballot(slot_l == slot + (lane - l)) >> l);  // (lane l's own bit is 0)
+      n = l == 0 ? (miss ? __ffsll((unsigned long long)miss) - 1 : 64) : min(__ffsll((unsigned long long)miss) - 1, 64 - l);
+      if (n == 64 - l)
+        for (;;) {
+          const int64_t u = t + n + lane;
+          const bool in = n + lane < bs - off && u < a.tokens && a.slots[u] == slot + n + lane;
+          const uint64_t out = __ballot(!in);
+          if (out) {
+            n += __ffsll((unsigned long long)out) - 1;
+            break;
+          }
+          n += 64;
+        }
+      n = min(n, bs - off);
     }
     const T* const x = (const T*)a.x[is_v] + t * a.ld[is_v] + h * a.hs[is_v];
     const int64_t ld = a.ld[is_v];
@@ -335,51 +378,87 @@ __global__ __launch_bounds__(256) void kv_append(CArgs a) {
 
 // ---- kv_read ---------------------------------------------------------------------
 
-// Eight values of a row a lane; outputs [tokens, heads, d], zeros for a slot
-// outside the cache, values past the type's range at its end.
+// Outputs [tokens, heads, d], zeros for a slot outside the cache, values past
+// the type's range at its end.  A wave takes 16 rows of a head of K or of V, two
+// dims a lane, piece of 16 tokens by piece: those of a piece take their V codes
+// from one 32-byte load a lane (4500 rows of 8 x 128: 13.5 us with a load a byte,
+// 13.7 us with K and V by one wave, 11.0 us).
 template <typename T>
 __global__ __launch_bounds__(256) void kv_read(CArgs a) {
-  const int per = a.d >> 3;
-  const int64_t all = a.tokens * a.heads * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int c = (int)(i % per);
-    const int64_t th = i / per;
-    const int h = (int)(th % a.heads);
-    const int64_t t = th / a.heads, slot = a.slots[t];
-    const bool in = slot >= 0 && slot < a.cells;
-    T f[2][8] = {};
-    if (in) {
-      const int64_t blk = slot >> a.lb;
-      const int off = (int)(slot & ((1 << a.lb) - 1));
-      const int8_t* const kc = a.codes[0] + (blk * a.heads + h) * a.bytes + (int64_t)off * a.dp + c * 8;
-      const int8_t* const vc =
-          a.codes[1] + (blk * a.heads + h) * a.bytes + ((int64_t)(off >> 4) * a.dp + c * 8) * 16 + (off & 15);
-      const float ks = a.scale[0][blk * a.heads + h], vs = a.scale[1][blk * a.heads + h];
-      const float top = std::is_same_v<T, _Float16> ? 65504.f : 0x1.fep+127f;
-      const uint2 kw = *(const uint2*)kc;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float k = (float)(int8_t)((e < 4 ? kw.x : kw.y) >> (8 * (e & 3))) * ks, v = (float)vc[16 * e] * vs;
-        f[0][e] = (T)(k != k ? k : fminf(fmaxf(k, -top), top));
-        f[1][e] = (T)(v != v ? v : fminf(fmaxf(v, -top), top));
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int hv = (int)(item % (2 * a.heads)), h = hv >> 1, is_v = hv & 1;
+  const int64_t t0 = item / (2 * a.heads) * 16;
+  const float top = std::is_same_v<T, _Float16> ? 65504.f : 0x1.fep+127f;
+  const bool mine = lane < a.d >> 1;
+  char* const out = a.out[is_v] + ((t0 * a.heads + h) * a.d + 2 * lane) * 2;
+  const int64_t step = (int64_t)a.heads * a.d * 2;
+  int64_t slot = -1;
+  const bool row = lane < 16 && t0 + lane < a.tokens;
+  if (row) slot = a.slots[t0 + lane];
+  const bool in = row && slot >= 0 && slot < a.cells;
+  for (uint64_t left = __ballot(row && !in); left; left &= left - 1)
+    if (mine) *(uint32_t*)(out + (__ffsll((unsigned long long)left) - 1) * step) = 0;
+  for (uint64_t left = __ballot(in); left;) {
+    // the rows whose tokens are in the first one's piece
+    const int u0 = __ffsll((unsigned long long)left) - 1;
+    const int64_t piece = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(slot >> 4), u0) |
+                          (int64_t)__builtin_amdgcn_readlane((int)(slot >> 36), u0) << 32;
+    const uint32_t rows = (uint32_t)__ballot(in && slot >> 4 == piece);
+    left &= ~(uint64_t)rows;
+    const int lp = a.lb - 4;
+    const int64_t at = (piece >> lp) * a.heads + h, c = piece & ((1 << lp) - 1);
+    const int off = (int)slot & 15;  // (lane u: row u's token)
+    int4v v0{}, v1{};
+    uint16_t two[16] = {};  // two codes of each row
+    if (is_v) {
+      if (mine) {
+        const int8_t* const vc = a.codes[1] + at * a.bytes + (c * a.dp + 2 * lane) * 16;
+        v0 = *(const int4v*)vc;
+        v1 = *(const int4v*)(vc + 16);
       }
-    }
 #pragma unroll
-    for (int s = 0; s < 2; ++s) __builtin_memcpy(a.out[s] + i * 16, f[s], 16);
+      for (int u = 0; u < 16; ++u) {
+        const int o = __builtin_amdgcn_readlane(off, u), w = o >> 2, b = (o & 3) * 8;
+        const int x = w & 2 ? (w & 1 ? v0[3] : v0[2]) : (w & 1 ? v0[1] : v0[0]);
+        const int y = w & 2 ? (w & 1 ? v1[3] : v1[2]) : (w & 1 ? v1[1] : v1[0]);
+        two[u] = (uint16_t)((x >> b & 0xff) | (y >> b & 0xff) << 8);
+      }
+    } else if (mine) {
+      const int8_t* const kc = a.codes[0] + at * a.bytes + c * 16 * a.dp + 2 * lane;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) two[u] = *(const uint16_t*)(kc + __builtin_amdgcn_readlane(off, u) * a.dp);
+    }
+    const float scale = a.scale[is_v][at];
+    const bool inside = scale * 127.f <= top;  // (false for NaN)
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      if (!(rows >> u & 1)) continue;
+      float x = (float)(int8_t)two[u] * scale, y = (float)(int8_t)(two[u] >> 8) * scale;
+      if (!inside) {
+        x = x != x ? x : fminf(fmaxf(x, -top), top);
+        y = y != y ? y : fminf(fmaxf(y, -top), top);
+      }
+      const T f[2] = {(T)x, (T)y};
+      uint32_t bits;
+      __builtin_memcpy(&bits, f, 4);
+      if (mine) *(uint32_t*)(out + u * step) = bits;
+    }
   }
 }
 
 }  // namespace
 
 hipError_t launch_kv_plan(const KvPlanProblem& p, hipStream_t stream) {
-  constexpr int NT = 1024;
-  PArgs a{p.lens, p.added, p.table, p.stack, p.count, p.slots, p.positions, p.cu, p.lens_out, p.count_out,
-          (int)p.requests, (int)p.width, (int)p.capacity, (int)p.tokens, p.log2_block, p.ldt};
-  const int64_t lds = (3 * p.requests + 1) * 4;
+  const PArgs a{p.lens, p.added, p.table, p.stack, p.count, p.slots, p.positions, p.cu, p.lens_out, p.count_out,
+                (int)p.requests, (int)p.width, (int)p.capacity, (int)p.tokens, p.log2_block, p.ldt};
+  // a wave a request, or 256 rows; few requests: the fewer waves the sums pass over
   const int64_t work = p.requests > p.tokens / 256 ? p.requests : p.tokens / 256;
-  const int64_t wgs = (work + NT / 64 - 1) / (NT / 64);
-  hipLaunchKernelGGL(kv_plan<NT>, dim3((unsigned)(wgs < 1 ? 1 : wgs < 128 ? wgs : 128)), dim3(NT), (unsigned)lds, stream,
-                     a);
+  const int nt = work <= 64 ? 256 : 1024;
+  const int64_t wgs = (work + nt / 64 - 1) / (nt / 64);
+  const dim3 grid((unsigned)(wgs < 1 ? 1 : wgs < 128 ? wgs : 128));
+  if (nt == 256) hipLaunchKernelGGL(kv_plan<256>, grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL(kv_plan<1024>, grid, dim3(1024), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -409,11 +488,10 @@ hipError_t launch_kv_append(const KvCacheProblem& p, hipStream_t stream) {
   a.hs[0] = p.hsk;
   a.hs[1] = p.hsv;
   // a wave looks for runs in `span` rows: one while that leaves at most 8192
-  // waves, more (up to a block's) for long prompts, whose rows mostly begin none
+  // waves, more (up to 64) for long prompts, whose rows mostly begin none
   const int64_t per_row = 2 * p.kv_heads;
   int64_t span = p.tokens * per_row / 8192;
-  const int64_t bs = 1ll << p.log2_block;
-  a.span = (int)(span < 1 ? 1 : span < bs ? span : bs);
+  a.span = (int)(span < 1 ? 1 : span < 64 ? span : 64);
   const int64_t blocks = ((p.tokens + a.span - 1) / a.span * per_row + 3) / 4;
   if (blocks >= (1ll << 31)) return hipErrorInvalidValue;
   const auto fn = p.dtype == DT_BF16 ? kv_append<__bf16> : kv_append<_Float16>;
@@ -425,9 +503,10 @@ hipError_t launch_kv_read(const KvCacheProblem& p, hipStream_t stream) {
   CArgs a = cache_args(p);
   a.out[0] = (char*)p.k_out;
   a.out[1] = (char*)p.v_out;
-  const int64_t n = p.tokens * p.kv_heads * (p.d / 8), blocks = (n + 255) / 256;
+  const int64_t blocks = ((p.tokens + 15) / 16 * 2 * p.kv_heads + 3) / 4;
+  if (blocks >= (1ll << 31)) return hipErrorInvalidValue;
   const auto fn = p.dtype == DT_BF16 ? kv_read<__bf16> : kv_read<_Float16>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 

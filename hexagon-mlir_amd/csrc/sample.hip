@@ -140,22 +140,6 @@ struct Weights {
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) {
   return ((uint64_t)(uint32_t)__shfl((int)(v >> 32), lane, 64) << 32) | (uint32_t)__shfl((int)v, lane, 64);
 }
-// Inclusive sum over the wave in lane order, by DPP: within rows of 16 lanes,
-// then each row's last lane to the next row, then lane 31 to the upper half.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t dpp_add64(uint64_t v) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
-  return v + ((uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ uint64_t scan64(uint64_t v) {
-  v = dpp_add64<0x111, 0xf>(v);  // row_shr:1
-  v = dpp_add64<0x112, 0xf>(v);
-  v = dpp_add64<0x114, 0xf>(v);
-  v = dpp_add64<0x118, 0xf>(v);
-  v = dpp_add64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-  return dpp_add64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-}
 // floor(f * 2^64) of f in [0, 1)
 __device__ __forceinline__ uint64_t fraction64(float f) {
   const double g = (double)f * 0x1p32, hi = __builtin_floor(g);

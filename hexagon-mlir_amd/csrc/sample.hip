@@ -116,10 +116,10 @@ struct Weights {
   float xmax, least;  // values below `least` have weight 0
   int shift;
   const double* table;
-  int infinite;  // the largest logit is (in a scalar register)
+  int lone;  // only logits equal to the largest have a weight (in a scalar register)
 
   __device__ __forceinline__ uint64_t of(float v) const {
-    if (infinite) return v == xmax ? 1ull << shift : 0;
+    if (lone) return v == xmax ? 1ull << shift : 0;
     // k = round(y), from the low bits of y + 1.5 * 2^52; 2^(r / 512) by its
     // series, |r ln 2 / 512| <= 6.8e-4: the first term left out is below 2^-46
     const double y = ((double)fmaxf(v, least) - top) * rate;
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     return;
   }
   const float xmax = value_of<T>(top);
-  const double rate = 1.44269504088896340736 / (double)fminf(t, 1e30f);  // (an infinite T leaves -inf its weight, 0)
+  const double rate = 1.44269504088896340736 / (double)fminf(t, 1e28f);  // (an infinite T leaves -inf its weight, 0)
   auto key_from = [&](double v) {  // the key from which logits are at least v (of a NaN: all)
     const float f = (float)v;
     if constexpr (KB == 32) return f != f ? 1u : max(1u, Key<float>::of(f));
@@ -401,9 +401,15 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   // sum, and whether the top k holds some of them changes nothing.  (Any value
   // under the rounding of a bound is under the bound.)
   const uint32_t cut = min(top, key_from((double)xmax - (a.shift + 3) / rate * 1.000001));
-  // (`least` two steps of the weights lower: y stays above -100 bits)
-  const Weights weights{rate * kSteps, (double)xmax, xmax, (float)((double)xmax - (a.shift + 20) / rate),
-                        a.shift, sh.exp2, __builtin_amdgcn_readfirstlane(xmax == INFINITY)};
+  // `least`, lower by another 17 bits and rounded down: y stays above -200 bits.
+  // Where a float holds nothing between it and the largest logit (T of 1e-9 of
+  // that, or 1e28), only the largest have a weight, as where that is infinite.
+  const double under = (double)xmax - (a.shift + 20) / rate;
+  float least_x = (float)under;
+  const bool lone = xmax == INFINITY || least_x >= xmax;
+  if ((double)least_x > under) least_x = value_of<float>(Key<float>::of(least_x) - 1);
+  const Weights weights{rate * kSteps, (double)xmax, xmax, least_x, a.shift, sh.exp2,
+                        __builtin_amdgcn_readfirstlane(lone)};
   // Descends to the key at which the counts (or weights) from the largest key
   // down first reach `goal`; `above`: what lies over that key.
   auto descend = [&](auto COUNT_, uint64_t goal, uint64_t& above) {

@@ -556,11 +556,11 @@ int64_t hxmi_kv_attention_workspace_bytes(int64_t tokens, int64_t requests, int6
  *   tokens[r] = the lowest kept index whose running weight, in index order,
  *          exceeds u * (kept weight)
  * Of equal logits the lowest index comes first.  temperature 0 (or below, in
- * a row's own) takes the largest logit.  A row with a NaN or with no logit
+ * a row's own) takes the largest logit; one past 1e28 counts as 1e28.  A row with a NaN or with no logit
  * above -inf gives -1.  Parameters are per row (pointers of `rows` entries)
- * or, where NULL, the all_* value.  Weights are held as integers of 44 or
- * more fraction bits (vocab <= 2^18), so the token does not depend on an
- * order of summation.  vocab <= 2^20.
+ * or, where NULL, the all_* value.  Weights are held as integers of 44
+ * fraction bits (42 at a vocabulary of 2^20; their sum stays below 2^62), so
+ * the token does not depend on an order of summation.  vocab <= 2^20.
  * No counterpart in the reference, which takes the argmax of its logits on
  * the host (benchmark_models/run_qwen2.5-0.5b.py:224-233).
  */

@@ -308,6 +308,11 @@ def check_attention(got, q, k, v, block, table, lens, cu, scale, blocks, name=""
     want, room = attention64(q.cpu(), k, v, block, table.cpu(), lens.tolist(), cu, scale, blocks)
     got = got.cpu().double()
     live = ~torch.isnan(want)
+    # (65520 and more is infinity in fp16, whose largest number is 65504; 2^128 is in bf16)
+    top = torch.finfo(q.dtype).max * (1 + HALF[q.dtype] / 2)
+    over = live & (want.abs() - room > top)
+    assert (got[over] == want[over].sign() * math.inf).all(), name
+    live &= want.abs() + room < top
     off = (got - want).abs() - HALF[q.dtype] * want.abs() - room
     assert live.any() and off[live].max() <= 2.0 ** -25, (name, float(off[live].max()))
 
@@ -447,6 +452,30 @@ def test_attention_of_unlike_scales(pkg, dev):
         check_attention(got, small, k, v, block, table, lens, [0, 1], scale, blocks, scale)
 
 
+def test_attention_of_many_rows_over_bad_pages_and_unlike_scales(pkg, dev):
+    """As above in tiles of 128 rows: missing pages, a NaN page that only the
+    last rows see, pages whose V scales lie up to 2^60 apart."""
+    heads, kv_heads, d, block, blocks = 4, 1, 128, 16, 40
+    cache, (k, v) = filled(pkg, dev, blocks, kv_heads, d, block, 62)
+    e = torch.arange(blocks).double()
+    factor = torch.where(e % 5 == 4, 0, torch.exp2(((e * 7) % 13 - 6) * 5))
+    cache.v_scale.mul_(factor[:, None].float().to(dev))
+    v = v * factor.repeat_interleave(block)[:, None, None]
+    table = torch.randperm(blocks - 1, generator=gen(63)).to(torch.int32)[:32].view(2, 16)
+    table[0, [3, 7]] = torch.tensor([-1, blocks], dtype=torch.int32)
+    table[1, :10] = -7
+    table[1, 15] = blocks - 1
+    cache.k_scale[blocks - 1] = math.nan
+    cache.v_scale[blocks - 1] = math.nan
+    table, lens, cu = table.to(dev), ints(dev, 250, 250), [0, 200, 440]  # row 240 - 10 of the second sees key 240
+    q = normal((440, heads, d), 64, 1.5).to(dev)
+    for scale in (d ** -0.5, 2.0 ** -20):
+        got = pkg.kv_attention(q, cache, table, lens, cu=ints(dev, *cu), scale=scale)
+        nan = torch.isnan(got).flatten(1).any(1).cpu()
+        assert not nan[:430].any() and nan[430:].all()
+        check_attention(got[:430], q[:430], k, v, block, table, ints(dev, 250, 240), [0, 200, 430], scale, blocks)
+
+
 def test_attention_past_32_bit_offsets(pkg, dev):
     """A cache of more than 4 GiB of codes each: pages at its start and end."""
     heads, kv_heads, d, block, blocks = 8, 8, 128, 64, 70000
@@ -571,6 +600,42 @@ def test_sample_of_a_large_vocabulary(pkg, dev):
                      top_k=torch.randint(-1, 4000, (B,), generator=g, dtype=torch.int32),
                      top_p=torch.rand(B, generator=g) * 1.2, min_p=torch.rand(B, generator=g) * 0.01)
         check_sample(pkg, dev, x, u, top_p=0.97)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_sample_at_extreme_temperatures(pkg, dev, dtype):
+    """Temperatures so low that the next smaller logit has no weight (below
+    1e-9 of the logits too, where their difference from a bound rounds away),
+    and so high that all have the same."""
+    x = normal((6, 3000), 15, 2.5, dtype=dtype)
+    x[2] = (x[2].float() * 4000).clamp(-60000, 60000).to(dtype)
+    x[3] = -x[2].abs() - 1
+    x[4, 5:] = x[4, 0]
+    x[5] = torch.finfo(dtype).min
+    x[5, 100:200] = 0
+    u = torch.rand(6, generator=gen(16))
+    for t in (1e-38, 1e-9, 1e-7, 1e-5, 1e-3, 1e5, 1e10):
+        for kw in ({}, dict(top_k=20), dict(top_k=700), dict(top_p=0.7), dict(top_k=900, top_p=0.5), dict(top_k=9, min_p=0.3)):
+            check_sample(pkg, dev, x, u, temperature=t, **kw)
+    check_sample(pkg, dev, x[:5], u[:5], temperature=torch.full((5,), math.inf), top_k=20)
+    check_sample(pkg, dev, x[:5], u[:5], temperature=torch.full((5,), math.inf), top_p=0.4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_sample_of_crowded_values(pkg, dev, dtype):
+    """More equal (or nearly equal) logits than a 16-bit count or a list holds."""
+    V = 140000
+    g = gen(17)
+    few = torch.randint(0, 3, (V,), generator=g).float()
+    mostly = torch.where(torch.rand(V, generator=g) < 0.9, -1.0, torch.randn(V, generator=g))
+    near = 1 + torch.rand(V, generator=g) * 2.0 ** -9  # (fp32: within one of its upper 16 bits' values)
+    low = torch.full((V,), torch.finfo(dtype).min)
+    low[::17] = torch.randn(V)[::17]
+    x = torch.stack([torch.ones(V), few, mostly, near, low]).to(dtype)
+    u = torch.rand(5, generator=g)
+    for kw in ({}, dict(top_k=50), dict(top_k=600), dict(top_k=70001), dict(top_p=0.9), dict(top_k=100000, top_p=0.6),
+               dict(top_k=20, top_p=0.6), dict(min_p=0.2, top_p=0.95)):
+        check_sample(pkg, dev, x, u, **kw)
 
 
 def test_sample_of_other_shapes(pkg, dev):

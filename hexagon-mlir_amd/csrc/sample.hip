@@ -27,14 +27,23 @@
 //     weight a value.  Tokens so far below the largest that their weight is 0
 //     take no part;
 //   * fp32 logits otherwise: counted by the upper 16 bits, those of the top k's
-//     bins on the list; without top-k the weights are summed by the upper 14
-//     bits and the list is the threshold's bin;
+//     bins on the list; without top-k the weights are summed in 16384 bins by
+//     distance from the largest logit and the list is the threshold's bin;
 //   * where a count passes 16 bits (more than 65535 equal values) or a list
 //     its room, a radix descent over the row, 8 bits a pass with a column of
 //     the histogram for each lane, takes their place.
 // Then the kept weights are summed by pieces of 512 tokens (from the list, from
 // a table of the weight of every kept value, or evaluated), the piece that
 // reaches u * sum is found and the token in it.
+//
+// What bounds it is one CU's work on its row, not memory (rows of 151936 logits
+// in us, at 64 rows and about the same up to 256): bf16 top-p 53 (pass for the
+// largest 11, counts and threshold 23, table and sums 15), every token kept 59
+// (a weight each, 44), fp32 top-k of 400 56 (two passes of 600 KB and the list),
+// fp32 top-p 107 (a weight each into bins, the kept ones again); one row of
+// 32000 with top-k 18.  A radix descent over the row for every threshold took
+// 314 us for the first of them, 375 for fp32.  More workgroups a row would need
+// a wait across them, or several launches.
 #include "hxmi_common.h"
 #include "hxmi_internal.h"
 
@@ -60,7 +69,7 @@ struct SArgs {
 
 constexpr int NT = 1024, NW = NT / 64, PIECE = 512;
 constexpr int kMaxPieces = kSampleMaxVocab / PIECE;
-constexpr int kList = 6144, kFewTop = 512, kTable = 16384;
+constexpr int kList = 6144, kFewTop = 512, kTable = 16384, kBins = 16384;
 constexpr int kTieBit = 54;  // of a table entry: an equal of the last key (a piece's weights sum to 2^53 at most)
 
 // A logit's key: an unsigned integer that orders as the logits do, equal for
@@ -149,15 +158,15 @@ __device__ __forceinline__ uint64_t fraction64(float f) {
 struct Shared {
   union {
     uint32_t count2[32768];            // 16-bit counts of the upper 16 bits of a key, two a word
-    unsigned long long bin[16384];     // weights by the upper 14 bits
+    unsigned long long bin[kBins];     // weights by the distance from the largest logit
     unsigned long long table[kTable];  // weight of a value by its key
     unsigned long long mass[256][64];  // radix descent: a column a lane
     uint32_t count[256][64];
     struct {
       unsigned long long weight[kList];
       uint32_t key[kList], index[kList];
+      uint32_t kept[NW][PIECE];  // (a wave's own)
     } list;
-    uint32_t kept[NW][PIECE];
   };
   union {
     struct {
@@ -570,6 +579,73 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     need_k = need_p = false;
   };
 
+  const double m = mp > 0.f ? (double)fminf(mp, 1.f) : 0.0;
+  const uint64_t least = (uint64_t)__builtin_rint(__builtin_ldexp(m, a.shift));
+  // (logits below `from` are below min_p or have weight 0)
+  const uint32_t from = m > 0.0 ? max(cut, min(top, key_from((double)xmax + (log2(m) * 1.000001 - 1e-5) / rate))) : cut;
+  // What each piece keeps: the weights (of at least `least`) of its keys over
+  // `last` and from `from` on, and the number of its equals of `last`; or, with
+  // LIST, tokens with keys from `low` to `last` go onto the list.  Where there
+  // is a bound, the wave first gathers those keys: 64 at a time then take one
+  // evaluation.
+  const int pieces = (vocab + PIECE - 1) / PIECE;
+  auto sum_pieces = [&](auto LIST_, uint64_t least, uint32_t from, uint32_t last, uint32_t low) {
+    constexpr bool LIST = decltype(LIST_)::value;
+    __syncthreads();
+    if (LIST && threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    constexpr int U = 4;
+    uint32_t* const kept = sh.list.kept[w];
+    const uint32_t over = max(last, from - 1);
+    const bool dense = last == 0 && from == cut;  // (few are left out)
+    for (int c0 = w; c0 < pieces; c0 += NW * U)
+      load_groups<U>(x, c0 * 64 + lane, NW * 64, vocab, [&](const uint32_t (&key)[8], int j) {
+        const int c = c0 + j * NW;
+        if (c >= pieces) return;
+        int some = 0, ties = 0;
+        uint64_t sum = 0;
+        if (!LIST && dense) {
+          uint64_t wf[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) wf[e] = weights.of(value_of<T>(key[e]));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum += key[e] > over && wf[e] >= least ? wf[e] : 0;
+          some = PIECE;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint64_t m = __ballot(key[e] > over);
+            if (key[e] > over)
+              kept[some + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = key[e];
+            some += __popcll(m);
+            if constexpr (LIST) put(key[e] >= low && key[e] <= last, key[e], (c * 64 + lane) * 8 + e);
+            else ties += __popcll(__ballot(key[e] == last));
+          }
+          for (int i = lane; i < some; i += 128) {  // (two evaluations side by side)
+            const uint64_t w0 = weights.of(value_of<T>(kept[i])), w1 = weights.of(value_of<T>(kept[min(i + 64, some - 1)]));
+            sum += w0 >= least ? w0 : 0;
+            sum += i + 64 < some && w1 >= least ? w1 : 0;
+          }
+        }
+        if (some) sum = scan64(sum);
+        if (lane == 63) {
+          sh.piece.sum[c] = sum;
+          sh.piece.ties[c] = (uint32_t)ties;
+        }
+      });
+    __syncthreads();
+  };
+  // Adds what is kept of a list of n tokens to its pieces.
+  auto add_list = [&](uint32_t n) {
+    for (uint32_t i = threadIdx.x; i < n; i += NT) {
+      const uint32_t key = sh.list.key[i], c = sh.list.index[i] / PIECE;
+      if (key > tau && sh.list.weight[i] >= least) atomicAdd(&sh.piece.sum[c], sh.list.weight[i]);
+      if (key == tau) atomicAdd(&sh.piece.ties[c], 1u);
+    }
+    __syncthreads();
+  };
+  bool summed = false;  // the pieces are
+
   if (listed) {
     list_thresholds(listed, bound);
   } else if constexpr (KB == 16) {
@@ -622,41 +698,75 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     }
     if (!need_k && need_p) {
       __syncthreads();
-      for (int i = threadIdx.x; i < 16384; i += NT) sh.bin[i] = 0;
+      for (int i = threadIdx.x; i < kBins; i += NT) sh.bin[i] = 0;
       __syncthreads();
+      // Bins of equal width from the largest logit down to where weights end
+      // (by the keys' upper bits, most tokens would share a hundred bins).
+      const float per_bin = fminf((float)((kBins - 1) * rate / (a.shift + 3)), 0x1.fffffep127f), cut_x = value_of<T>(cut);
+      auto bin_of = [&](float v) {  // (v <= xmax, which may be infinite)
+        return v == xmax ? 0u : (uint32_t)fminf((xmax - v) * per_bin, (float)(kBins - 1));
+      };
       const int lanes = (vocab + 7) >> 3;
-      for (int i0 = w * 64; i0 < lanes; i0 += NT)
-        load_groups<1>(x, i0 + lane, NT, vocab, [&](const uint32_t (&key)[8], int) {
-          uint64_t wf[8];
+      auto values = [&](int i, float (&v)[8]) {  // of logits 8 i .. 8 i + 7, -inf past the row
+        if (__all(i * 8 + 8 <= vocab)) {
+          Eight<T> raw;
+          raw.load(x + i * 8);
+          __builtin_memcpy(v, raw.r, sizeof(v));
+        } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) wf[e] = weights.of(value_of<T>(key[e]));  // (side by side)
+          for (int e = 0; e < 8; ++e) v[e] = i * 8 + e < vocab ? (float)x[i * 8 + e] : -INFINITY;
+        }
+      };
+      float now[8], next[8];
+      values((int)threadIdx.x, now);
+      for (int i0 = w * 64; i0 < lanes; i0 += NT) {
+        values(i0 + lane + NT, next);
+        uint64_t wf[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (key[e] >= cut) atomicAdd(&sh.bin[key[e] >> 18], (unsigned long long)wf[e]);
-        });
+        for (int e = 0; e < 8; ++e) wf[e] = weights.of(now[e]);  // (side by side)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (now[e] >= cut_x) atomicAdd(&sh.bin[bin_of(now[e])], (unsigned long long)wf[e]);
+          now[e] = next[e];
+        }
+      }
       __syncthreads();
       uint64_t own = 0, whole;
-      const uint32_t b0 = 16u * (NT - 1 - threadIdx.x);  // (threads from the largest keys down)
-      for (int j = 0; j < 16; ++j) own += sh.bin[b0 + ((j + threadIdx.x) & 15)];
+      const uint32_t b0 = kBins / NT * threadIdx.x;
+      for (int j = 0; j < kBins / NT; ++j) own += sh.bin[b0 + ((j + threadIdx.x) & (kBins / NT - 1))];
       const uint64_t incl = block_scan(own, sh, whole), goal = goal_of(whole);
       __syncthreads();
       if (incl >= goal && incl - own < goal) {  // (one thread)
         uint64_t over = incl - own;
-        int j = 15;
-        for (; j > 0 && over + sh.bin[b0 + j] < goal; --j) over += sh.bin[b0 + j];
+        int j = 0;
+        for (; j < kBins / NT - 1 && over + sh.bin[b0 + j] < goal; ++j) over += sh.bin[b0 + j];
         sh.key = b0 + j;
         sh.above = over;
       }
       __syncthreads();
       const uint32_t bin = sh.key;
       const uint64_t above = sh.above;
-      const uint32_t n = make_list([&](uint32_t key) { return key >> 18 == bin; });
+      // Its keys: one pass lists them and sums the pieces of all above.
+      auto first_key = [&](uint32_t bin) {  // the lowest key in the bins up to it
+        uint32_t lo = cut, hi = top;
+        while (lo < hi) {
+          const uint32_t mid = lo + ((hi - lo) >> 1);
+          if (bin_of(value_of<T>(mid)) <= bin) hi = mid;
+          else lo = mid + 1;
+        }
+        return lo;
+      };
+      const uint32_t lo = first_key(bin), hi = bin ? first_key(bin - 1) - 1 : top;
+      sum_pieces(std::true_type{}, least, from, hi, lo);
+      const uint32_t n = sh.listed;
       if (n <= kList) {
         list_weights(n);
         uint64_t over = above;
-        tau = radix(bin << 18, min(bin << 18 | 0x3ffffu, top), 0, goal, over, list_masses(n));
+        tau = radix(lo, hi, 0, goal, over, list_masses(n));
         equal = equals_of(goal, over);
+        add_list(n);
         need_p = false;
+        summed = true;
       }
     }
   }
@@ -666,42 +776,6 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     equal = (uint32_t)((uint64_t)k - above);
   }
 
-  // What each piece keeps: the weights (of at least `least`) of its keys over
-  // tau and from `from` on, and the number of its equals of tau.  The wave
-  // first gathers those keys: 64 at a time then take one evaluation.
-  const int pieces = (vocab + PIECE - 1) / PIECE;
-  auto sum_pieces = [&](uint64_t least, uint32_t from) {
-    __syncthreads();
-    constexpr int U = 4;
-    uint32_t* const kept = sh.kept[w];
-    const uint32_t over = max(tau, from - 1);
-    for (int c0 = w; c0 < pieces; c0 += NW * U)
-      load_groups<U>(x, c0 * 64 + lane, NW * 64, vocab, [&](const uint32_t (&key)[8], int j) {
-        const int c = c0 + j * NW;
-        if (c >= pieces) return;
-        int some = 0, ties = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint64_t m = __ballot(key[e] > over);
-          if (key[e] > over)
-            kept[some + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = key[e];
-          some += __popcll(m);
-          ties += __popcll(__ballot(key[e] == tau));
-        }
-        uint64_t sum = 0;
-        for (int i = lane; i < some; i += 128) {  // (two evaluations side by side)
-          const uint64_t w0 = weights.of(value_of<T>(kept[i])), w1 = weights.of(value_of<T>(kept[min(i + 64, some - 1)]));
-          sum += w0 >= least ? w0 : 0;
-          sum += i + 64 < some && w1 >= least ? w1 : 0;
-        }
-        if (some) sum = scan64(sum);
-        if (lane == 63) {
-          sh.piece.sum[c] = sum;
-          sh.piece.ties[c] = (uint32_t)ties;
-        }
-      });
-    __syncthreads();
-  };
   // A wave over the pieces, each lane a run of `per`: its pieces' kept weight
   // `own` (equals of tau at wt each), the equals before its run.
   const int per = (pieces + 63) >> 6;
@@ -716,7 +790,7 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   };
 
   if (need_p) {
-    sum_pieces(0, cut);
+    sum_pieces(std::false_type{}, 0, cut, tau, 0);
     uint64_t before, above;
     const uint64_t whole = shfl64(scan64(lane_pieces(weights.of(value_of<T>(tau)), before)), 63);  // (every wave the same)
     const uint64_t goal = goal_of(whole);
@@ -724,24 +798,16 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     equal = equals_of(goal, above);
   }
 
-  const double m = mp > 0.f ? (double)fminf(mp, 1.f) : 0.0;
-  const uint64_t least = (uint64_t)__builtin_rint(__builtin_ldexp(m, a.shift));
-  // (logits below `from` are below min_p or have weight 0)
-  const uint32_t from = m > 0.0 ? max(cut, min(top, key_from((double)xmax + (log2(m) * 1.000001 - 1e-5) / rate))) : cut;
   const uint32_t base = max(tau, from) - 1;
-  if (listed) {
+  if (summed) {
+  } else if (listed) {
     __syncthreads();
     for (int i = threadIdx.x; i < pieces; i += NT) {
       sh.piece.sum[i] = 0;
       sh.piece.ties[i] = 0;
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < listed; i += NT) {
-      const uint32_t key = sh.list.key[i], c = sh.list.index[i] / PIECE;
-      if (key > tau && sh.list.weight[i] >= least) atomicAdd(&sh.piece.sum[c], sh.list.weight[i]);
-      if (key == tau) atomicAdd(&sh.piece.ties[c], 1u);
-    }
-    __syncthreads();
+    add_list(listed);
   } else if (KB == 16 && top - base < kTable) {
     // every kept value's weight by its key: an addition a token
     __syncthreads();
@@ -767,7 +833,7 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
       });
     __syncthreads();
   } else {
-    sum_pieces(least, from);
+    sum_pieces(std::false_type{}, least, from, tau, 0);
   }
   if (w != 0) return;
   const uint64_t wt_all = weights.of(value_of<T>(tau)), wt = wt_all >= least ? wt_all : 0;

@@ -1,5 +1,6 @@
 """hexagon_mlir_amd — MI355X-native replacement of Hexagon-MLIR's matmul / GEMV /
-RMSNorm / softmax hot path.
+RMSNorm / softmax hot path, and the operators of a serving loop around it
+(block tables, an 8-bit key/value cache, attention over it, sampling).
 
 Layers:
   * ``csrc/``      hand-written HIP kernels for gfx950 behind the C ABI of

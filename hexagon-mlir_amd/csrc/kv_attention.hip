@@ -3,11 +3,13 @@
 // in the cache sees keys j <= L - n + i,
 //   o = sum_j p_j vc_j vs_j / sum_j p_j,  p_j = exp(scale * ks_j (q . kc_j) - max).
 //
-// A workgroup of four waves owns 16 * QT rows (token, head of the group) of
+// A workgroup of four waves owns a tile of rows (token, head of the group) of
 // one key/value head and, where there are few such tiles, one of `nsplit`
-// shares of the keys; its waves take every fourth group of 64 keys.  Codes go
-// from memory straight to registers in the layout of the MFMA operands, so
-// nothing passes through LDS until the waves' partial results are joined:
+// shares of the keys.  Two kernels: this one for 16 rows,
+// kv_attention_tiles below for 128.  Here the waves take every fourth group of
+// 64 keys and codes go from memory straight to registers in the layout of the
+// MFMA operands, so nothing passes through LDS until the waves' partial results
+// are joined:
 //   * scores as D[key][row] = Kc . Q^T (16x16x32 MFMAs).  A lane's K codes
 //     are 16 bytes of one token; the head dims of a step may come in any
 //     order, so they feed two steps as they lie.  Tile t's row 4 g + i is key
@@ -22,11 +24,14 @@
 //   * the K scale multiplies the score.  The V scale multiplies the weight
 //     before its rounding to fp16, relative to 2^mv, the running maximum of
 //     score + log2(vs): the weights P.V sees stay in (0, 2^8] whatever the
-//     ratio of the scales, and the sum of the p_j stays apart in fp32.
+//     ratio of the scales, and the sum of the p_j is that of the fp32 weights
+//     over their V scale, relative to 2^mv as well: one maximum does for both.
 //     Weights round to 11 bits, half a step relative each, like the fp16
 //     weights of the fused attention; scores, maxima, sums and O are fp32.
-// One token a request is bound by the codes' bytes; rows in the hundreds by
-// the vector ALUs (conversion and softmax), which QT tiles of rows share.
+// One token a request is bound by the codes' bytes: 64 requests of 8192 tokens,
+// 32 heads over 8 of 128 dims, 156 us (814 MB, 5.2 TB/s); one of 131072 tokens
+// 62 us (4.3 TB/s, shares of the keys and their join).  Short ones are bound by
+// latency: 1900 tokens of one user 7 us.
 #include "hxmi_common.h"
 #include "hxmi_internal.h"
 
@@ -101,48 +106,39 @@ __device__ __forceinline__ void value_scale(float vs, float& lv, float& rv) {
   rv = __builtin_amdgcn_rcpf(vs);
 }
 
-// What a wave knows of its QT x 16 rows: O and the sum of the p_j (this lane's
+// What a wave knows of its 16 rows: O and the sum of the p_j (this lane's
 // part), both relative to 2^mv.
-template <int QT, int DT>
+template <int DT>
 struct Partial {
-  static constexpr int N = QT * (DT * 4 + 2);  // floats a lane
-  float4v o[QT][DT];
-  float mv[QT], l[QT];
+  static constexpr int N = DT * 4 + 2;  // floats a lane
+  float4v o[DT];
+  float mv, l;
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int a = 0; a < QT; ++a) {
-#pragma unroll
-      for (int t = 0; t < DT; ++t) o[a][t] = float4v{0.f, 0.f, 0.f, 0.f};
-      mv[a] = -INFINITY;
-      l[a] = 0.f;
-    }
+    for (int t = 0; t < DT; ++t) o[t] = float4v{0.f, 0.f, 0.f, 0.f};
+    mv = -INFINITY;
+    l = 0.f;
   }
   // Every float becomes f(its index, it).
   template <typename F>
   __device__ __forceinline__ void each(F&& f) {
 #pragma unroll
-    for (int a = 0; a < QT; ++a) {
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[a][t][i] = f((a * DT + t) * 4 + i, o[a][t][i]);
-      mv[a] = f(QT * DT * 4 + a, mv[a]);
-      l[a] = f(QT * DT * 4 + QT + a, l[a]);
-    }
+      for (int i = 0; i < 4; ++i) o[t][i] = f(t * 4 + i, o[t][i]);
+    mv = f(DT * 4, mv);
+    l = f(DT * 4 + 1, l);
   }
   __device__ __forceinline__ void add(const Partial& p) {
+    const float vn = fmaxf(mv, p.mv);
+    const float x = rel_exp2(mv, vn), y = rel_exp2(p.mv, vn);
+    l = l * x + p.l * y;
 #pragma unroll
-    for (int a = 0; a < QT; ++a) {
-      const float vn = fmaxf(mv[a], p.mv[a]);
-      const float x = rel_exp2(mv[a], vn), y = rel_exp2(p.mv[a], vn);
-      l[a] = l[a] * x + p.l[a] * y;
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[a][t][i] = o[a][t][i] * x + p.o[a][t][i] * y;
-      mv[a] = vn;
-    }
+      for (int i = 0; i < 4; ++i) o[t][i] = o[t][i] * x + p.o[t][i] * y;
+    mv = vn;
   }
 };
 
@@ -220,9 +216,9 @@ __device__ __forceinline__ half8v q_operand(const T (&x)[8], int ex) {
 }
 
 // DC: 64-dim pieces of a row; WHOLE: the head dim is 64 * DC.
-template <typename T, int DC, bool WHOLE, int QT>
-__global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
-  constexpr int DT = DC * 4, RT = 16 * QT, NV = Partial<QT, DT>::N;
+template <typename T, int DC, bool WHOLE>
+__global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
+  constexpr int DT = DC * 4, RT = 16, NV = Partial<DT>::N;
   constexpr bool BF16 = !std::is_same_v<T, _Float16>;
   __shared__ __attribute__((aligned(16))) float joined[3 * NV * 64];
   __shared__ int last_split;
@@ -238,16 +234,14 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
   const int r = tile.r, first = tile.first, n = tile.n, row0 = tile.row0, len = tile.len;
   const int64_t nrows = tile.count;
 
-  // This lane's rows (a row past the last one reads the last one's q)
-  int last[QT];  // the last key the row sees
-  half8v qf[QT][2 * DC];
-  float c[QT];
-#pragma unroll
-  for (int x = 0; x < QT; ++x) {
-    const int64_t row = min((int64_t)row0 + x * 16 + lr, nrows - 1);
-    const int i = (int)(row / a.group), head = kvh * a.group + (int)(row - (int64_t)i * a.group);
-    last[x] = (int)min((int64_t)len - n + i, (int64_t)len - 1);
-    const T* q = (const T*)a.q + (int64_t)(first + i) * a.ldq + (int64_t)head * a.hq;
+  // This lane's row (past the last one: the last one's q, not stored)
+  const int64_t row = (int64_t)row0 + lr, rowq = min(row, nrows - 1);
+  const int token = (int)(rowq / a.group), head = kvh * a.group + (int)(rowq - (int64_t)token * a.group);
+  const int last = (int)min((int64_t)len - n + token, (int64_t)len - 1);  // the last key it sees
+  half8v qf[2 * DC];
+  float c = a.c;
+  {
+    const T* q = (const T*)a.q + (int64_t)(first + token) * a.ldq + (int64_t)head * a.hq;
     T raw[2 * DC][8];
     float top = 0.f;
 #pragma unroll
@@ -259,9 +253,9 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
       if constexpr (BF16) top = largest(raw[s], top);
     }
     const int ex = BF16 ? exponent_of(row_max(top)) : 0;
-    c[x] = BF16 ? __builtin_ldexpf(a.c, -ex) : a.c;
+    if constexpr (BF16) c = __builtin_ldexpf(a.c, -ex);
 #pragma unroll
-    for (int s = 0; s < 2 * DC; ++s) qf[x][s] = q_operand(raw[s], ex);
+    for (int s = 0; s < 2 * DC; ++s) qf[s] = q_operand(raw[s], ex);
   }
 
   // keys this tile / all of its rows see
@@ -271,7 +265,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
   const int groups = (kend + 63) >> 6, share = (groups + nsplit - 1) / nsplit;
   const int g1 = min(groups, (split + 1) * share);
 
-  Partial<QT, DT> acc;
+  Partial<DT> acc;
   acc.clear();
 
   const int ck = (lane >> 2) & 3;  // 16-key piece of a group that this lane's K rows lie in (V's and the scores': lg)
@@ -324,19 +318,15 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
   }
   for (; g < g1; g += 4) {
     // scores
-    float4v s[QT][4];
+    float4v s[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
       for (int x = 0; x < DC; ++x)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const half8v kf = operand(kr[t][x][2 * u], kr[t][x][2 * u + 1]);
-#pragma unroll
-          for (int y = 0; y < QT; ++y)
-            s[y][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                kf, qf[y][2 * x + u], x == 0 && u == 0 ? float4v{0.f, 0.f, 0.f, 0.f} : s[y][t], 0, 0, 0);
-        }
+        for (int u = 0; u < 2; ++u)
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(kr[t][x][2 * u], kr[t][x][2 * u + 1]), qf[2 * x + u],
+                                                        x == 0 && u == 0 ? float4v{0.f, 0.f, 0.f, 0.f} : s[t], 0, 0, 0);
     }
     const bool more = g + 4 < g1;
     const float ks0 = ks, vs0 = vs;
@@ -346,61 +336,54 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
     const bool whole = g * 64 + 64 <= kfull && __all(there0);  // (wave-uniform)
     float lv, rv;
     value_scale(vs0, lv, rv);
-    half8v p[QT][2];
+    half8v p[2];
+    const float cs = c * ks0;
+    float mx = -INFINITY;
+    if (whole) {
 #pragma unroll
-    for (int y = 0; y < QT; ++y) {
-      const float cs = c[y] * ks0;
-      float mx = -INFINITY, lvy = lv;
-      if (whole) {
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[y][t][i]);
-        mx *= cs;  // (cs >= 0)
-      } else {
-        // the scores times cs, masked ones -inf
-        const int left = there0 ? last[y] - (g * 64 + lg * 16) : -1;  // keys of this lane up to this one are seen
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[y][t][i] = 4 * t + i > left ? -INFINITY : s[y][t][i] * cs;
-            mx = fmaxf(mx, s[y][t][i]);
-          }
-        // (a page whose every key is masked takes no part, whatever its scale)
-        if (left < 0) lvy = -INFINITY;
-      }
-      const float mxv = row_max(left_out(mx, lvy));
-      if (__any(mxv > acc.mv[y] + 8.f)) {
-        const float vn = mxv > acc.mv[y] + 8.f ? mxv : acc.mv[y], f = rel_exp2(acc.mv[y], vn);
-        acc.l[y] *= f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) acc.o[y][t] *= f;
-        acc.mv[y] = vn;
-      }
-      const float off = lvy == -INFINITY ? -INFINITY : lvy - (acc.mv[y] == -INFINITY ? 0.f : acc.mv[y]);
-      const float cw = whole ? cs : 1.f;
-      float sum = 0.f;
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+      mx *= cs;  // (cs >= 0)
+    } else {
+      // the scores times cs, masked ones -inf
+      const int left = there0 ? last - (g * 64 + lg * 16) : -1;  // keys of this lane up to this one are seen
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[y][t][i], cw, off));
-          sum += e;
-          p[y][t >> 1][(t & 1) * 4 + i] = (_Float16)e;
+          s[t][i] = 4 * t + i > left ? -INFINITY : s[t][i] * cs;
+          mx = fmaxf(mx, s[t][i]);
         }
-      acc.l[y] += lvy == -INFINITY ? 0.f : sum * rv;
+      // (a page whose every key is masked takes no part, whatever its scale)
+      if (left < 0) lv = -INFINITY;
     }
+    const float mxv = row_max(left_out(mx, lv));
+    if (__any(mxv > acc.mv + 8.f)) {
+      const float vn = mxv > acc.mv + 8.f ? mxv : acc.mv, f = rel_exp2(acc.mv, vn);
+      acc.l *= f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) acc.o[t] *= f;
+      acc.mv = vn;
+    }
+    const float off = lv == -INFINITY ? -INFINITY : lv - (acc.mv == -INFINITY ? 0.f : acc.mv);
+    const float cw = whole ? cs : 1.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i], cw, off));
+        sum += e;
+        p[t >> 1][(t & 1) * 4 + i] = (_Float16)e;
+      }
+    acc.l += lv == -INFINITY ? 0.f : sum * rv;
     // values
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const half8v vf = operand(vr[t][2 * u], vr[t][2 * u + 1]);
-#pragma unroll
-        for (int y = 0; y < QT; ++y)
-          acc.o[y][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[y][u], acc.o[y][t], 0, 0, 0);
-      }
+      for (int u = 0; u < 2; ++u)
+        acc.o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(vr[t][2 * u], vr[t][2 * u + 1]), p[u], acc.o[t], 0, 0, 0);
     if (more) {
       load_v(g + 4, bv2);
       if (g + 8 < g1) {
@@ -418,7 +401,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
     if (w > 0) return;
 #pragma unroll
     for (int o = 0; o < 3; ++o) {
-      Partial<QT, DT> other;
+      Partial<DT> other;
       other.each([&](int i, float) { return joined[(o * NV + i) * 64 + lane]; });
       acc.add(other);
     }
@@ -452,7 +435,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
     if (!last_split) return;
     acc.clear();
     for (int sp = w; sp < nsplit; sp += 4) {  // (in this order whichever came last)
-      Partial<QT, DT> other;
+      Partial<DT> other;
       other.each([&](int i, float) {
         return __uint_as_float(
             __builtin_amdgcn_raw_buffer_load_b32(rP, (uint32_t)(sp * PART + (i * 64 + lane) * 4), 0, kCoherent));
@@ -464,25 +447,20 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
   if (w > 0) return;
 
   // O: lane holds row l % 16, dims 16 t + 4 (l / 16) + 0..3
+  const float l = row_reduce(acc.l, [](float y, float z) { return y + z; });
+  const float f = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+  if (row >= nrows) return;
+  T* const o = (T*)a.o + (int64_t)(first + token) * a.ldo + (int64_t)head * a.ho;
 #pragma unroll
-  for (int x = 0; x < QT; ++x) {
-    const int64_t row = (int64_t)row0 + x * 16 + lr;
-    const float l = row_reduce(acc.l[x], [](float y, float z) { return y + z; });
-    const float f = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
-    if (row >= nrows) continue;
-    const int i = (int)(row / a.group), head = kvh * a.group + (int)(row - (int64_t)i * a.group);
-    T* const o = (T*)a.o + (int64_t)(first + i) * a.ldo + (int64_t)head * a.ho;
+  for (int t = 0; t < DT; ++t) {
+    const int d = t * 16 + lg * 4;
+    if (!WHOLE && d >= a.d) continue;
+    T o4[4];
 #pragma unroll
-    for (int t = 0; t < DT; ++t) {
-      const int d = t * 16 + lg * 4;
-      if (!WHOLE && d >= a.d) continue;
-      T o4[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o4[j] = (T)(acc.o[x][t][j] * f);
-      int2v bits;
-      __builtin_memcpy(&bits, o4, 8);
-      *(int2u*)(o + d) = bits;
-    }
+    for (int j = 0; j < 4; ++j) o4[j] = (T)(acc.o[t][j] * f);
+    int2v bits;
+    __builtin_memcpy(&bits, o4, 8);
+    *(int2u*)(o + d) = bits;
   }
 }
 
@@ -490,11 +468,12 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void kv_attention(KArgs a) {
 //
 // A workgroup of four waves owns 128 rows (32 a wave) and takes 64 keys at a
 // time through two LDS stages: its threads convert the codes to fp16 on the way
-// in, so a code is converted once for 128 rows (the kernel above: once for 16 or
-// 32), and codes of the next stage but one are in flight meanwhile.  Eight waves
-// of 256 rows convert half as often and were slower (289 us, 279 of four, 2350
-// rows x 32 heads over 8000 keys): one workgroup a CU has nothing to run while
-// it waits at its barriers.  Scores are D[key][row] of 32x32x16 MFMAs; row m of a 32-key block
+// in, so a code is converted once for 128 rows (the kernel above: for 16), and codes of the next stage but one are in flight meanwhile.  2350 rows x
+// 32 heads over 8000 keys: 269 us (733 TFLOP/s), 507 by the kernel above; bound
+// by the vector ALUs (softmax, then conversion) of two waves a SIMD.  Eight waves
+// of 256 rows convert half as often and were slower (289 us, 279 of four at that
+// time): one workgroup a CU has nothing to run while it waits at its barriers.
+// Scores are D[key][row] of 32x32x16 MFMAs; row m of a 32-key block
 // reads key 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that a
 // lane's eight weights of 16 keys are eight in order, the B operand of P.V.  The
 // 16 keys are one piece of a page: K and V scales are wave-uniform.
@@ -810,26 +789,34 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
 // Rows of a workgroup, tiles of them and the shares of the keys: from sizes
 // alone, so the workspace can be asked for beforehand.
 struct KvPlan {
-  int qt, nsplit;  // qt 0: kv_attention_tiles
+  int rt, nsplit;  // rows of a tile: 16, or 128 (kv_attention_tiles)
   int64_t tiles, full;
 };
 int64_t part_bytes(const KvAttnProblem& p, const KvPlan& k) {  // of a tile's share
   const int64_t dt = p.d <= 64 ? 4 : 8;
-  return k.qt ? k.qt * (dt * 4 + 2) * 64 * 4 : 4 * (dt * 8 + 2) * 64 * 4;
+  return k.rt == 16 ? (dt * 4 + 2) * 64 * 4 : 4 * (dt * 8 + 2) * 64 * 4;
 }
 KvPlan plan_of(const KvAttnProblem& p) {
   KvPlan r;
   const int64_t group = p.heads / p.kv_heads;
   const int64_t rows = (p.cu ? (p.tokens + p.requests - 1) / p.requests : 1) * group;  // of a request, on average
-  r.qt = rows <= 16 ? 1 : rows <= 64 ? 2 : 0;
-  const int64_t rt = r.qt ? 16 * r.qt : 128;
+  // Tiles of 128 rows where a request has about as many and every CU would get
+  // one of 16 (us, 16 / 128 rows a tile, contexts of 4000 tokens; dims of 128, 8
+  // key/value heads, 37 requests: 80 rows 186 / 188, 112 rows 250 / 167; dims of
+  // 64, 4 heads, 48 requests: 192 rows 107 / 140, 256 rows 139 / 117; one request,
+  // 128 dims: 256 rows 28 / 30, 1024 rows 56 / 43).  Tiles of 32 rows were slower
+  // than 16 up to 100 rows and never the fastest.
+  const bool wide = rows > (p.d > 64 ? 96 : 255) && p.tokens * p.heads >= 4096;
+  r.rt = wide ? 128 : 16;
+  const int64_t rt = r.rt;
   r.tiles = p.cu ? p.tokens * group / rt + p.requests : p.requests * ((group + rt - 1) / rt);
   // The card takes 512 workgroups at a time, two a CU.  Whole rounds of them
   // run unshared; the tiles that are left share their keys out until they make
   // one more round, at least one group of 64 keys a wave (eight stages of a
-  // 128-row tile) to a share.  575 tiles of 128 rows x 8000 keys: 391 us unshared,
-  // 292 with all of them in two shares, 281 with the last 63 in eight.
-  const int64_t items = r.tiles * p.kv_heads, least = r.qt ? 256 : 512, most = (p.width * p.block + least - 1) / least;
+  // 128-row tile) to a share.  575 tiles of 128 rows x 8000 keys, before later
+  // steps: 391 us unshared, 292 with all of them in two shares, 281 with the last
+  // 63 in eight.
+  const int64_t items = r.tiles * p.kv_heads, least = wide ? 512 : 256, most = (p.width * p.block + least - 1) / least;
   const int64_t left = items % 512;
   int64_t n = left ? 512 / left : 1;
   n = n < most ? n : most;
@@ -839,14 +826,12 @@ KvPlan plan_of(const KvAttnProblem& p) {
 }
 
 template <typename T>
-hipError_t launch_t(int64_t d, int qt, dim3 grid, const KArgs& a, hipStream_t stream) {
+hipError_t launch_t(int64_t d, int rt, dim3 grid, const KArgs& a, hipStream_t stream) {
   const bool small = d <= 64, whole = d == 64 || d == 128;
-  const auto fn = qt == 1   ? (small ? whole ? kv_attention<T, 1, true, 1> : kv_attention<T, 1, false, 1>
-                                     : whole ? kv_attention<T, 2, true, 1> : kv_attention<T, 2, false, 1>)
-                  : qt == 2 ? (small ? whole ? kv_attention<T, 1, true, 2> : kv_attention<T, 1, false, 2>
-                                     : whole ? kv_attention<T, 2, true, 2> : kv_attention<T, 2, false, 2>)
-                 : small   ? (whole ? kv_attention_tiles<T, 64, true> : kv_attention_tiles<T, 64, false>)
-                           : (whole ? kv_attention_tiles<T, 128, true> : kv_attention_tiles<T, 128, false>);
+  const auto fn = rt == 16 ? (small ? whole ? kv_attention<T, 1, true> : kv_attention<T, 1, false>
+                                    : whole ? kv_attention<T, 2, true> : kv_attention<T, 2, false>)
+                           : (small ? whole ? kv_attention_tiles<T, 64, true> : kv_attention_tiles<T, 64, false>
+                                    : whole ? kv_attention_tiles<T, 128, true> : kv_attention_tiles<T, 128, false>);
   hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream, a);
   return hipGetLastError();
 }
@@ -899,7 +884,7 @@ hipError_t launch_kv_attention(const KvAttnProblem& p, hipStream_t stream) {
   a.nsplit = k.nsplit;
   a.c = p.scale * kLog2e;
   const dim3 blocks((unsigned)grid);
-  return p.dtype == DT_BF16 ? launch_t<__bf16>(p.d, k.qt, blocks, a, stream) : launch_t<_Float16>(p.d, k.qt, blocks, a, stream);
+  return p.dtype == DT_BF16 ? launch_t<__bf16>(p.d, k.rt, blocks, a, stream) : launch_t<_Float16>(p.d, k.rt, blocks, a, stream);
 }
 
 }  // namespace hxmi

@@ -366,6 +366,24 @@ def test_attention_of_ragged_rows(pkg, dev, heads, kv_heads, d, block, dtype):
             check_attention(out, q, k, v, block, table, lens, cu, d ** -0.5, blocks, rows)
 
 
+@pytest.mark.parametrize("heads, kv_heads, d, block, dtype", SHAPES)
+def test_attention_of_many_rows(pkg, dev, heads, kv_heads, d, block, dtype):
+    """Tiles of 128 rows: requests that end inside one, an empty one, a prompt
+    without a context, a context that ends inside a page; rows of no request."""
+    a = 2200 // heads + 1
+    rows, held = [a, 0, a + 3], [a + 37, 5, a + 3]
+    cu = [0] + np.cumsum(rows).tolist()
+    blocks, width = 48, -(-max(held) // block)
+    cache, (k, v) = filled(pkg, dev, blocks, kv_heads, d, block, 23)
+    table = torch.randint(0, blocks, (3, width), generator=gen(24), dtype=torch.int32).to(dev)
+    q = normal((cu[-1] + 7, heads, d), 25, 1.5, dtype=dtype).to(dev)
+    out = torch.full_like(q, 7.0)
+    lens = ints(dev, *held)
+    pkg.kv_attention(q, cache, table, lens, cu=ints(dev, *cu), out=out)
+    assert (out[cu[-1]:] == 7).all()
+    check_attention(out, q, k, v, block, table, lens, cu, d ** -0.5, blocks)
+
+
 def test_attention_of_a_prompt(pkg, dev):
     """Rows in the hundreds over a longer context: several tiles a request, in both types."""
     for dtype, heads, kv_heads, d in ((torch.float16, 8, 2, 128), (torch.bfloat16, 6, 1, 64)):
@@ -455,7 +473,7 @@ def test_attention_of_unlike_scales(pkg, dev):
 def test_attention_of_many_rows_over_bad_pages_and_unlike_scales(pkg, dev):
     """As above in tiles of 128 rows: missing pages, a NaN page that only the
     last rows see, pages whose V scales lie up to 2^60 apart."""
-    heads, kv_heads, d, block, blocks = 4, 1, 128, 16, 40
+    heads, kv_heads, d, block, blocks = 10, 1, 128, 16, 40
     cache, (k, v) = filled(pkg, dev, blocks, kv_heads, d, block, 62)
     e = torch.arange(blocks).double()
     factor = torch.where(e % 5 == 4, 0, torch.exp2(((e * 7) % 13 - 6) * 5))

@@ -23,9 +23,9 @@
 //     pass puts the tokens from it on (a few thousand) on a list in LDS, and
 //     everything else happens there;
 //   * 16-bit logits otherwise: the tokens are counted by value in LDS (65536
-//     counts of 16 bits, 128 KB); both thresholds follow from counts and one
-//     weight a value.  Tokens so far below the largest that their weight is 0
-//     take no part;
+//     counts of 16 bits, 128 KB) in the pass that finds the largest; both
+//     thresholds follow from counts and one weight a value.  Values of masks take
+//     no part, and in a second count none whose weight is 0;
 //   * fp32 logits otherwise: counted by the upper 16 bits, those of the top k's
 //     bins on the list; without top-k the weights are summed in 16384 bins by
 //     distance from the largest logit and the list is the threshold's bin;
@@ -37,8 +37,9 @@
 // reaches u * sum is found and the token in it.
 //
 // What bounds it is one CU's work on its row, not memory (rows of 151936 logits
-// in us, at 64 rows and about the same up to 256): bf16 top-p 53 (pass for the
-// largest 11, counts and threshold 23, table and sums 15), every token kept 59
+// in us, at 64 rows and about the same up to 256): bf16 top-p 47 (largest and
+// counts 19, threshold 9, table and sums 15; 53 with a pass of its own for the
+// largest), every token kept 59
 // (a weight each, 44), fp32 top-k of 400 56 (two passes of 600 KB and the list),
 // fp32 top-p 107 (a weight each into bins, the kept ones again); one row of
 // 32000 with top-k 18.  A radix descent over the row for every threshold took
@@ -385,12 +386,35 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     if (listed > kList) listed = 0;
     for (uint32_t i = threadIdx.x; i < listed; i += NT) top = max(top, sh.list.key[i]);
   }
-  if (!listed) each_key<8>(x, vocab, [&](uint32_t key, int) {
+  constexpr uint32_t kInf = Key<T>::zero + Key<T>::inf, kMinusInf = Key<T>::zero - Key<T>::inf;
+  // Counts the tokens with keys from `least` on by their upper 16 bits:
+  // `in_bins` of them by this thread.
+  uint32_t in_bins = 0;
+  auto count_pass = [&](uint32_t least) {
+    __syncthreads();
+    int4v* const z = (int4v*)sh.count2;
+    for (int i = threadIdx.x; i < 32768 / 4; i += NT) z[i] = int4v{};
+    __syncthreads();
+    in_bins = 0;
+    each_key<4>(x, vocab, [&](uint32_t key, int) {
+      top = max(top, key);
+      low = min(low, key - 1);
+      if (key < least) return;
+      const uint32_t bin = key >> (KB - 16);
+      atomicAdd(&sh.count2[bin >> 1], 1u + (bin & 1) * 0xffffu);
+      ++in_bins;
+    });
+  };
+  // 16-bit logits: counted in the pass that finds the largest, all but -inf and
+  // the lowest finite value (masks, which could be more than a count holds).
+  constexpr uint32_t kMasks = kMinusInf + 2;
+  const bool early = KB == 16 && !listed && (need_k || need_p);
+  if (early) count_pass(kMasks);
+  else if (!listed) each_key<8>(x, vocab, [&](uint32_t key, int) {
       top = max(top, key);
       low = min(low, key - 1);
     });
   extremes();
-  constexpr uint32_t kInf = Key<T>::zero + Key<T>::inf, kMinusInf = Key<T>::zero - Key<T>::inf;
   if (top > kInf || low + 1 < kMinusInf || top == kMinusInf) {
     if (threadIdx.x == 0) a.token[row] = -1;
     return;
@@ -481,20 +505,12 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   // from the largest keys down.
   const uint32_t bin0 = 64u * (NT - 1 - threadIdx.x);
   auto count_of = [&](uint32_t bin) -> uint32_t { return sh.count2[bin >> 1] >> (16 * (bin & 1)) & 0xffffu; };
-  // Counts the tokens with a weight (`counted` in all); false if a count passed 16 bits.
+  // Counts the tokens with a weight (`counted` in all; where the masks have none,
+  // the early counts do); false if a count passed 16 bits.
   uint64_t counted = 0, count_incl = 0, count_own = 0;
-  auto count_keys = [&]() {
-    int4v* const z = (int4v*)sh.count2;
-    for (int i = threadIdx.x; i < 32768 / 4; i += NT) z[i] = int4v{};
-    __syncthreads();
-    uint32_t mine = 0;
-    each_key<4>(x, vocab, [&](uint32_t key, int) {
-      if (key < cut) return;
-      const uint32_t bin = key >> (KB - 16);
-      atomicAdd(&sh.count2[bin >> 1], 1u + (bin & 1) * 0xffffu);
-      ++mine;
-    });
-    counted = block_sum(mine, sh);
+  auto count_keys = [&](bool again) {
+    if (again) count_pass(cut);
+    counted = block_sum(in_bins, sh);
     count_own = 0;
     for (int j = 0; j < 32; ++j) {
       const uint32_t two = sh.count2[(bin0 >> 1) + ((j + threadIdx.x) & 31)];  // (banks apart)
@@ -649,7 +665,7 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   if (listed) {
     list_thresholds(listed, bound);
   } else if constexpr (KB == 16) {
-    if ((need_k || need_p) && count_keys()) {
+    if ((need_k || need_p) && ((early && cut >= kMasks && count_keys(false)) || count_keys(true))) {
       if (need_k && (uint64_t)k < counted) {
         uint64_t above;
         tau = find_bin(count_incl, count_own, (uint64_t)k, above, [&](uint32_t bin) -> uint64_t { return count_of(bin); });
@@ -683,7 +699,7 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     }
   } else {
     if (need_k) {
-      const bool ok = count_keys();
+      const bool ok = count_keys(true);
       if ((uint64_t)k >= counted) {
         need_k = false;
       } else if (ok) {

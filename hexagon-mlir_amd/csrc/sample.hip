@@ -39,8 +39,8 @@
 // What bounds it is one CU's work on its row, not memory (rows of 151936 logits
 // in us, at 64 rows and about the same up to 256): bf16 top-p 47 (largest and
 // counts 19, threshold 9, table and sums 15; 53 with a pass of its own for the
-// largest), every token kept 59
-// (a weight each, 44), fp32 top-k of 400 56 (two passes of 600 KB and the list),
+// largest), every token kept 42
+// (59 with a weight evaluated for each), fp32 top-k of 400 56 (two passes of 600 KB and the list),
 // fp32 top-p 107 (a weight each into bins, the kept ones again); one row of
 // 32000 with top-k 18.  A radix descent over the row for every threshold took
 // 314 us for the first of them, 375 for fp32.  More workgroups a row would need
@@ -815,6 +815,16 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   }
 
   const uint32_t base = max(tau, from) - 1;
+  // 16-bit logits of both signs can have more keys than a table holds: then
+  // those next to zero, where the fewest logits are, are a gap in it.
+  uint32_t gap0 = top + 1, gap = 0;
+  if (KB == 16 && top - base >= kTable) {
+    const uint32_t half = (top - base - kTable + 2) / 2;
+    if (half <= top - min(top, Key<T>::zero) && half < Key<T>::zero - min(Key<T>::zero, base)) {
+      gap0 = Key<T>::zero - half;
+      gap = 2 * half;
+    }
+  }
   if (summed) {
   } else if (listed) {
     __syncthreads();
@@ -824,29 +834,48 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     }
     __syncthreads();
     add_list(listed);
-  } else if (KB == 16 && top - base < kTable) {
-    // every kept value's weight by its key: an addition a token
+  } else if (KB == 16 && top - base - gap < kTable) {
+    // every kept value's weight by its key: an addition a token (and an
+    // evaluation in the gap)
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i <= top - base; i += NT) {
-      const uint64_t wf = i ? weights.of(value_of<T>(base + i)) : 0;
-      sh.table[i] = base + i == tau ? 1ull << kTieBit : wf >= least ? wf : 0;
+    for (uint32_t i = threadIdx.x; i <= top - base - gap; i += NT) {
+      const uint32_t key = base + i + (base + i >= gap0 ? gap : 0);
+      const uint64_t wf = i ? weights.of(value_of<T>(key)) : 0;
+      sh.table[i] = key == tau ? 1ull << kTieBit : wf >= least ? wf : 0;
     }
     if (threadIdx.x == 0) sh.table[0] = 0;
     __syncthreads();
     constexpr int U = 4;
-    for (int c0 = w; c0 < pieces; c0 += NW * U)
-      load_groups<U>(x, c0 * 64 + lane, NW * 64, vocab, [&](const uint32_t (&key)[8], int j) {
-        const int c = c0 + j * NW;
-        if (c >= pieces) return;
-        uint64_t sum = 0;
+    auto add_up = [&](auto GAP_) {
+      for (int c0 = w; c0 < pieces; c0 += NW * U)
+        load_groups<U>(x, c0 * 64 + lane, NW * 64, vocab, [&](const uint32_t (&key)[8], int j) {
+          const int c = c0 + j * NW;
+          if (c >= pieces) return;
+          uint64_t sum = 0;
+          if constexpr (decltype(GAP_)::value) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += sh.table[max(key[e], base) - base];
-        sum = scan64(sum);
-        if (lane == 63) {
-          sh.piece.sum[c] = sum & ((1ull << kTieBit) - 1);
-          sh.piece.ties[c] = (uint32_t)(sum >> kTieBit);
-        }
-      });
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t k = max(key[e], base);
+              if (k - gap0 < gap) {
+                const uint64_t wf = weights.of(value_of<T>(k));
+                sum += k == tau ? 1ull << kTieBit : wf >= least ? wf : 0;
+              } else {
+                sum += sh.table[k - base - (k >= gap0 ? gap : 0)];
+              }
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += sh.table[max(key[e], base) - base];
+          }
+          sum = scan64(sum);
+          if (lane == 63) {
+            sh.piece.sum[c] = sum & ((1ull << kTieBit) - 1);
+            sh.piece.ties[c] = (uint32_t)(sum >> kTieBit);
+          }
+        });
+    };
+    if (gap) add_up(std::true_type{});
+    else add_up(std::false_type{});
     __syncthreads();
   } else {
     sum_pieces(std::false_type{}, least, from, tau, 0);

@@ -39,12 +39,12 @@
 // What bounds it is one CU's work on its row, not memory (rows of 151936 logits
 // in us, at 64 rows and about the same up to 256): bf16 top-p 47 (largest and
 // counts 19, threshold 9, table and sums 15; 53 with a pass of its own for the
-// largest), every token kept 42
-// (59 with a weight evaluated for each), fp32 top-k of 400 56 (two passes of 600 KB and the list),
-// fp32 top-p 107 (a weight each into bins, the kept ones again); one row of
-// 32000 with top-k 18.  A radix descent over the row for every threshold took
-// 314 us for the first of them, 375 for fp32.  More workgroups a row would need
-// a wait across them, or several launches.
+// largest), every token kept 42 (59 with a weight evaluated for each), fp32
+// top-k of 400 56 (two passes of 600 KB and the list), fp32 top-p 107 (a weight
+// each into bins, the kept ones again); one row of 32000 with top-k 18.  A radix
+// descent over the row for every threshold took 314 us for the first of them,
+// 375 for fp32.  More workgroups a row would need a wait across them, or several
+// launches.
 #include "hxmi_common.h"
 #include "hxmi_internal.h"
 

@@ -22,10 +22,13 @@
 //     fp16 under a power of two a row, exact for all that counts beside the
 //     row's largest element;
 //   * the K scale multiplies the score.  The V scale multiplies the weight
-//     before its rounding to fp16, relative to 2^mv, the running maximum of
+//     before its rounding to fp16, relative to 2^m, the running maximum of
 //     score + log2(vs): the weights P.V sees stay in (0, 2^8] whatever the
-//     ratio of the scales, and the sum of the p_j is that of the fp32 weights
-//     over their V scale, relative to 2^mv as well: one maximum does for both.
+//     ratio of the scales.  The sum of the p_j is that of the fp32 weights over
+//     their V scale, relative to 2^m as well: one maximum does for both while
+//     the V scales leave what counts in fp32's range (near_one).  A wave (in the
+//     kernel below, a workgroup) that meets any other takes its keys again with
+//     the sum relative to a maximum of its own (Frame).
 //     Weights round to 11 bits, half a step relative each, like the fp16
 //     weights of the fused attention; scores, maxima, sums and O are fp32.
 // One token a request is bound by the codes' bytes: 64 requests of 8192 tokens,
@@ -97,27 +100,85 @@ __device__ __forceinline__ float rel_exp2(float x, float top) {
 __device__ __forceinline__ float left_out(float x, float lv) { return lv == -INFINITY ? -INFINITY : x + lv; }
 
 // A page's V scale as the weights take it: its logarithm, and its inverse for
-// the sum.  A page of zeros (scale 0) may take any scale: the smallest one that
-// pages have, which leaves the maximum to the others.  A page that is not
-// there, or whose keys are all masked, has logarithm -inf.
-__device__ __forceinline__ void value_scale(float vs, float& lv, float& rv) {
-  vs = vs == 0.f ? 0x1p-100f : vs;
+// the sum.  A page that is not there, or whose keys are all masked, has
+// logarithm -inf.  A page of zeros (scale 0) counts in the sum alone: with sums
+// of their own (apart) it has logarithm -inf too, otherwise it takes 2^-64, so
+// that whatever its codes are they are lost beside any page that is near_one.
+__device__ __forceinline__ void value_scale(float vs, bool apart, float& lv, float& rv) {
+  vs = vs == 0.f && !apart ? 0x1p-64f : vs;
   lv = __builtin_amdgcn_logf(vs);
   rv = __builtin_amdgcn_rcpf(vs);
 }
+// Whether the sum can be taken from a page's weighted scores, 2^(score + log2(vs)
+// - m): m is at most 10 above the largest score then, so that the weighted
+// scores of keys of zeros 2^45 below that are still normal numbers, and at most
+// 64 + 8 below it.
+__device__ __forceinline__ bool near_one(float vs) { return vs == 0.f || (vs >= 0x1p-30f && vs <= 0x1p10f); }
 
-// What a wave knows of its 16 rows: O and the sum of the p_j (this lane's
-// part), both relative to 2^mv.
+// a * b, rounded (never part of an fma).
+__device__ __forceinline__ float times(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
+// What a row's numbers are relative to: the sum l of its p_j to 2^m, O to
+// 2^(m + d).  d is 0 and m the running maximum of score + log2(vs) (within 8), or,
+// with sums of their own, m the largest score and d the running maximum of
+// score - m + log2(vs): -inf where nothing has been added to O.
+struct Frame {
+  float m, d;
+
+  // The largest score is now at least `top`: what l is to be multiplied by.
+  __device__ __forceinline__ float raise(float top) {
+    const float now = fmaxf(m, top), f = rel_exp2(m, now);
+    d = m == -INFINITY ? -INFINITY : d + (m - now);
+    m = now;
+    return f;
+  }
+  // The maximum of score - m + log2(vs) is now at least `cand`: what O is to be multiplied by.
+  __device__ __forceinline__ float raise_o(float cand) {
+    const float now = cand > d + 8.f ? cand : d, f = rel_exp2(d, now);
+    d = now;
+    return f;
+  }
+  // Relative to a larger m.
+  __device__ __forceinline__ Frame from(float now) const {
+    const float to = m == -INFINITY ? -INFINITY : m - now;
+    return Frame{to, d + to};
+  }
+  // What O is to be multiplied by at the end (l: the whole sum, 0 if no key was seen).
+  __device__ __forceinline__ float over(float l) const { return l == 0.f ? 0.f : __builtin_amdgcn_exp2f(d) / l; }
+};
+
+// Frames joined into the first: what l and O of each are to be multiplied by.
+template <int N>
+__device__ __forceinline__ void join_frames(Frame (&at)[N], float (&fl)[N], float (&fo)[N]) {
+  float m = at[0].m, d = -INFINITY;
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, at[i].m);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    at[i] = at[i].from(m);
+    fl[i] = __builtin_amdgcn_exp2f(at[i].m);
+    d = fmaxf(d, at[i].d);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) fo[i] = rel_exp2(at[i].d, d);
+  at[0] = Frame{m, d};
+}
+
+// What a wave knows of its 16 rows: O and the sum of the p_j (this lane's part).
 template <int DT>
 struct Partial {
-  static constexpr int N = DT * 4 + 2;  // floats a lane
+  static constexpr int N = DT * 4 + 3;  // floats a lane
   float4v o[DT];
-  float mv, l;
+  Frame at;
+  float l;
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = float4v{0.f, 0.f, 0.f, 0.f};
-    mv = -INFINITY;
+    at = Frame{-INFINITY, 0.f};
     l = 0.f;
   }
   // Every float becomes f(its index, it).
@@ -127,18 +188,29 @@ struct Partial {
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[t][i] = f(t * 4 + i, o[t][i]);
-    mv = f(DT * 4, mv);
-    l = f(DT * 4 + 1, l);
+    at.m = f(DT * 4, at.m);
+    at.d = f(DT * 4 + 1, at.d);
+    l = f(DT * 4 + 2, l);
   }
-  __device__ __forceinline__ void add(const Partial& p) {
-    const float vn = fmaxf(mv, p.mv);
-    const float x = rel_exp2(mv, vn), y = rel_exp2(p.mv, vn);
-    l = l * x + p.l * y;
+  template <int N>
+  __device__ __forceinline__ void add(const Partial (&p)[N]) {
+    Frame f[N + 1] = {at};
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+    for (int j = 0; j < N; ++j) f[j + 1] = p[j].at;
+    float fl[N + 1], fo[N + 1];
+    join_frames(f, fl, fo);
+    at = f[0];
+    l *= fl[0];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[t][i] = o[t][i] * x + p.o[t][i] * y;
-    mv = vn;
+    for (int t = 0; t < DT; ++t) o[t] *= fo[0];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      l += p[j].l * fl[j + 1];
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][i] += p[j].o[t][i] * fo[j + 1];
+    }
   }
 };
 
@@ -266,7 +338,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
   const int g1 = min(groups, (split + 1) * share);
 
   Partial<DT> acc;
-  acc.clear();
+  bool odd = false;  // a page's scale was not near_one (wave-uniform)
 
   const int ck = (lane >> 2) & 3;  // 16-key piece of a group that this lane's K rows lie in (V's and the scores': lg)
   const int* const table = a.table + (int64_t)r * a.ldt;
@@ -304,94 +376,128 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
     vs = there ? a.vs[(int64_t)b * a.kv_heads + kvh] : 0.f;
   };
 
-  int g = split * share + w;
-  int bk = -1, bv = -1, bk2 = -1, bv2 = -1;
-  if (g < g1) {
-    bk = page(4 * g + ck);
-    bv = page(4 * g + lg);
-    load_k(g, bk);
-    load_v(g, bv);
-    if (g + 4 < g1) {
-      bk2 = page(4 * (g + 4) + ck);
-      bv2 = page(4 * (g + 4) + lg);
+  // The wave's keys; APART: with sums of their own, and loads as they are needed.
+  auto pass = [&](auto APART_) {
+    constexpr bool APART = decltype(APART_)::value;
+    acc.clear();
+    int g = split * share + w;
+    int bk2 = -1, bv2 = -1;
+    if (!APART && g < g1) {
+      const int bk = page(4 * g + ck), bv = page(4 * g + lg);
+      load_k(g, bk);
+      load_v(g, bv);
+      if (g + 4 < g1) {
+        bk2 = page(4 * (g + 4) + ck);
+        bv2 = page(4 * (g + 4) + lg);
+      }
     }
-  }
-  for (; g < g1; g += 4) {
-    // scores
-    float4v s[4];
+    for (; g < g1; g += 4) {
+      if constexpr (APART) {
+        const int bk = page(4 * g + ck), bv = page(4 * g + lg);
+        load_k(g, bk);
+        load_v(g, bv);
+      }
+      // scores
+      float4v s[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+      for (int t = 0; t < 4; ++t) {
 #pragma unroll
-      for (int x = 0; x < DC; ++x)
+        for (int x = 0; x < DC; ++x)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(kr[t][x][2 * u], kr[t][x][2 * u + 1]), qf[2 * x + u],
-                                                        x == 0 && u == 0 ? float4v{0.f, 0.f, 0.f, 0.f} : s[t], 0, 0, 0);
-    }
-    const bool more = g + 4 < g1;
-    const float ks0 = ks, vs0 = vs;
-    const bool there0 = there;
-    if (more) load_k(g + 4, bk2);
-    // softmax
-    const bool whole = g * 64 + 64 <= kfull && __all(there0);  // (wave-uniform)
-    float lv, rv;
-    value_scale(vs0, lv, rv);
-    half8v p[2];
-    const float cs = c * ks0;
-    float mx = -INFINITY;
-    if (whole) {
+          for (int u = 0; u < 2; ++u)
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(kr[t][x][2 * u], kr[t][x][2 * u + 1]), qf[2 * x + u],
+                                                          x == 0 && u == 0 ? float4v{0.f, 0.f, 0.f, 0.f} : s[t], 0, 0, 0);
+      }
+      const bool more = !APART && g + 4 < g1;
+      const float ks0 = ks, vs0 = vs;
+      const bool there0 = there;
+      if (more) load_k(g + 4, bk2);
+      // softmax
+      const bool whole = g * 64 + 64 <= kfull && __all(there0);  // (wave-uniform)
+      float lv, rv;
+      value_scale(vs0, APART, lv, rv);
+      half8v p[2];
+      const float cs = c * ks0;
+      float mx = -INFINITY;
+      if (whole && !APART) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
-      mx *= cs;  // (cs >= 0)
-    } else {
-      // the scores times cs, masked ones -inf
-      const int left = there0 ? last - (g * 64 + lg * 16) : -1;  // keys of this lane up to this one are seen
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+        mx *= cs;  // (cs >= 0)
+        odd |= !__all(near_one(vs0));
+      } else {
+        // the scores times cs, masked ones -inf
+        const int left = there0 ? last - (g * 64 + lg * 16) : -1;  // keys of this lane up to this one are seen
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[t][i] = 4 * t + i > left ? -INFINITY : times(s[t][i], cs);
+            mx = fmaxf(mx, s[t][i]);
+          }
+        // (a page whose every key is masked takes no part, whatever its scale)
+        if (left < 0) lv = -INFINITY;
+        odd |= !__all(left < 0 || near_one(vs0));
+      }
+      float ref, f = 1.f;  // a weight is relative to 2^ref
+      bool up = true;
+      if constexpr (APART) {
+        acc.l *= acc.at.raise(row_max(mx));
+        const float m = acc.at.m == -INFINITY ? 0.f : acc.at.m;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[t][i] -= m;
+            acc.l += __builtin_amdgcn_exp2f(s[t][i]);
+          }
+        f = acc.at.raise_o(row_max(left_out(mx - m, lv)));
+        ref = acc.at.d;
+      } else {
+        const float mxv = row_max(left_out(mx, lv));
+        up = __any(mxv > acc.at.m + 8.f);
+        if (up) {
+          const float now = mxv > acc.at.m + 8.f ? mxv : acc.at.m;
+          f = rel_exp2(acc.at.m, now);
+          acc.l *= f;
+          acc.at.m = now;
+        }
+        ref = acc.at.m;
+      }
+      if (up) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) acc.o[t] *= f;
+      }
+      const float off = lv == -INFINITY ? -INFINITY : lv - (ref == -INFINITY ? 0.f : ref);
+      const float cw = whole && !APART ? cs : 1.f;
+      float sum = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[t][i] = 4 * t + i > left ? -INFINITY : s[t][i] * cs;
-          mx = fmaxf(mx, s[t][i]);
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i], cw, off));
+          sum += e;
+          p[t >> 1][(t & 1) * 4 + i] = (_Float16)e;
         }
-      // (a page whose every key is masked takes no part, whatever its scale)
-      if (left < 0) lv = -INFINITY;
-    }
-    const float mxv = row_max(left_out(mx, lv));
-    if (__any(mxv > acc.mv + 8.f)) {
-      const float vn = mxv > acc.mv + 8.f ? mxv : acc.mv, f = rel_exp2(acc.mv, vn);
-      acc.l *= f;
+      if (!APART) acc.l += lv == -INFINITY ? 0.f : sum * rv;
+      // values
 #pragma unroll
-      for (int t = 0; t < DT; ++t) acc.o[t] *= f;
-      acc.mv = vn;
-    }
-    const float off = lv == -INFINITY ? -INFINITY : lv - (acc.mv == -INFINITY ? 0.f : acc.mv);
-    const float cw = whole ? cs : 1.f;
-    float sum = 0.f;
+      for (int t = 0; t < DT; ++t)
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i], cw, off));
-        sum += e;
-        p[t >> 1][(t & 1) * 4 + i] = (_Float16)e;
-      }
-    acc.l += lv == -INFINITY ? 0.f : sum * rv;
-    // values
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        acc.o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(vr[t][2 * u], vr[t][2 * u + 1]), p[u], acc.o[t], 0, 0, 0);
-    if (more) {
-      load_v(g + 4, bv2);
-      if (g + 8 < g1) {
-        bk2 = page(4 * (g + 8) + ck);
-        bv2 = page(4 * (g + 8) + lg);
+        for (int u = 0; u < 2; ++u)
+          acc.o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(vr[t][2 * u], vr[t][2 * u + 1]), p[u], acc.o[t], 0, 0, 0);
+      if (more) {
+        load_v(g + 4, bv2);
+        if (g + 8 < g1) {
+          bk2 = page(4 * (g + 8) + ck);
+          bv2 = page(4 * (g + 8) + lg);
+        }
       }
     }
-  }
+  };
+  pass(std::false_type{});
+  if (odd) pass(std::true_type{});
 
   // Join the waves' parts: waves 1..3 through LDS into wave 0.
   auto join = [&]() {
@@ -399,12 +505,10 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
     if (w > 0) acc.each([&](int i, float v) { return joined[((w - 1) * NV + i) * 64 + lane] = v; });
     __syncthreads();
     if (w > 0) return;
+    Partial<DT> other[3];
 #pragma unroll
-    for (int o = 0; o < 3; ++o) {
-      Partial<DT> other;
-      other.each([&](int i, float) { return joined[(o * NV + i) * 64 + lane]; });
-      acc.add(other);
-    }
+    for (int o = 0; o < 3; ++o) other[o].each([&](int i, float) { return joined[(o * NV + i) * 64 + lane]; });
+    acc.add(other);
   };
   join();
 
@@ -435,8 +539,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
     if (!last_split) return;
     acc.clear();
     for (int sp = w; sp < nsplit; sp += 4) {  // (in this order whichever came last)
-      Partial<DT> other;
-      other.each([&](int i, float) {
+      Partial<DT> other[1];
+      other[0].each([&](int i, float) {
         return __uint_as_float(
             __builtin_amdgcn_raw_buffer_load_b32(rP, (uint32_t)(sp * PART + (i * 64 + lane) * 4), 0, kCoherent));
       });
@@ -448,7 +552,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
 
   // O: lane holds row l % 16, dims 16 t + 4 (l / 16) + 0..3
   const float l = row_reduce(acc.l, [](float y, float z) { return y + z; });
-  const float f = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+  const float f = acc.at.over(l);
   if (row >= nrows) return;
   T* const o = (T*)a.o + (int64_t)(first + token) * a.ldo + (int64_t)head * a.ho;
 #pragma unroll
@@ -484,9 +588,9 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
   constexpr int DS = D / 16, DT = D / 32, RB = 2 * D;
   constexpr int KB = 64 * RB, STAGE = KB + D * 128;
   constexpr int PIECES = 64 * D / 16 / 256;  // 16-byte pieces of K (and of V) a thread converts a stage
-  constexpr int NV = DT * 16 + 2;
+  constexpr int NV = DT * 16 + 3;
   __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-  __shared__ int last_split;
+  __shared__ int last_split, odd;  // odd: a page's scale was not near_one
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, h = lane >> 5;
@@ -579,22 +683,24 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
   static_assert(4 * PIECES == DS, "a unit a step of the scores");
 
   float16v o[DT];
-#pragma unroll
-  for (int x = 0; x < DT; ++x) o[x] = float16v{};
-  float mv = -INFINITY, l = 0.f;
+  Frame at;
+  float l;
 
   const int key = 16 * (lr >> 4) + 8 * (lr >> 2 & 1) + 4 * (lr >> 3 & 1) + (lr & 3);
   const int k_read = k_at(key, h), v_read = v_at(lr, h);
   Scales after{};
   int pg = -1;
   // Stage st in `base`, while `other` takes the next one.
-  auto compute = [&](int st, const char* base, char* other, const Scales& sc) {
+  auto compute = [&](auto APART_, int st, const char* base, char* other, const Scales& sc) {
+    constexpr bool APART = decltype(APART_)::value;
     // each lane's piece, then the four as scalars
     float lane_lv, lane_rv;
-    value_scale(sc.v, lane_lv, lane_rv);
+    value_scale(sc.v, APART, lane_lv, lane_rv);
     if (sc.b < 0) lane_lv = -INFINITY;
     const float lane_ks = sc.b < 0 ? 0.f : sc.k;
-    const bool all = st * 64 + 64 <= kfull && __all(sc.b >= 0);
+    const uint64_t there = __ballot(sc.b >= 0);
+    if (!APART && !__all(sc.b < 0 || near_one(sc.v)) && lane == 0) odd = 1;
+    const bool all = !APART && st * 64 + 64 <= kfull && there == ~0ull;
     float ks[4], lv[4], rv[4];
     auto lane_of = [](float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); };
 #pragma unroll
@@ -647,26 +753,65 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
     } else {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        left[x] = lv[x] == -INFINITY ? -1 : last - (st * 64 + x * 16 + 8 * h);
+        left[x] = there >> x & 1 ? last - (st * 64 + x * 16 + 8 * h) : -1;
         float m = -INFINITY;
+        if constexpr (APART) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, e > left[x] ? -INFINITY : s[x >> 1][8 * (x & 1) + e]);
-        mx = fmaxf(mx, left[x] < 0 ? -INFINITY : fmaf(m, c * ks[x], lv[x]));
+          for (int e = 0; e < 8; ++e) {
+            const float v = e > left[x] ? -INFINITY : times(s[x >> 1][8 * (x & 1) + e], c * ks[x]);
+            s[x >> 1][8 * (x & 1) + e] = v;
+            mx = fmaxf(mx, v);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = fmaxf(m, e > left[x] ? -INFINITY : s[x >> 1][8 * (x & 1) + e]);
+          mx = fmaxf(mx, left[x] < 0 ? -INFINITY : fmaf(m, c * ks[x], lv[x]));
+        }
       }
     }
-    const auto m2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-    mx = fmaxf(__uint_as_float(m2[0]), __uint_as_float(m2[1]));
-    if (__any(mx > mv + 8.f)) {
-      const float vn = mx > mv + 8.f ? mx : mv, f = rel_exp2(mv, vn);
-      l *= f;
+    auto both = [](float v) {  // the maximum of the two lanes of a row
+      const auto v2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+      return fmaxf(__uint_as_float(v2[0]), __uint_as_float(v2[1]));
+    };
+    mx = both(mx);
+    float ref, f = 1.f;  // a weight is relative to 2^ref
+    bool up = true;
+    if constexpr (APART) {
+      l *= at.raise(mx);
+      const float m = at.m == -INFINITY ? 0.f : at.m;
+      float cand = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = s[x >> 1][8 * (x & 1) + e] - m;
+          s[x >> 1][8 * (x & 1) + e] = v;
+          most = fmaxf(most, v);
+          l += __builtin_amdgcn_exp2f(v);
+        }
+        cand = fmaxf(cand, left[x] < 0 ? -INFINITY : left_out(most, lv[x]));
+      }
+      f = at.raise_o(both(cand));
+      ref = at.d;
+    } else {
+      up = __any(mx > at.m + 8.f);
+      if (up) {
+        const float now = mx > at.m + 8.f ? mx : at.m;
+        f = rel_exp2(at.m, now);
+        l *= f;
+        at.m = now;
+      }
+      ref = at.m;
+    }
+    if (up) {
 #pragma unroll
       for (int x = 0; x < DT; ++x) o[x] *= f;
-      mv = vn;
     }
-    const float m_use = mv == -INFINITY ? 0.f : mv;
+    ref = ref == -INFINITY ? 0.f : ref;
     // the weights of 16 keys while the MFMAs of the 16 before run
     auto weights = [&](int x) {
-      const float off = lv[x] - m_use, cs = c * ks[x];
+      const float off = lv[x] - ref, cs = APART ? 1.f : c * ks[x];
       float v[8], sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = __builtin_amdgcn_exp2f(fmaf(s[x >> 1][8 * (x & 1) + e], cs, off));
@@ -680,7 +825,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
         sum += v[e];
         p[e] = (_Float16)v[e];
       }
-      l += sum == 0.f ? 0.f : sum * rv[x];  // (rv is of no use where nothing is seen)
+      if (!APART) l += sum == 0.f ? 0.f : sum * rv[x];  // (rv is of no use where nothing is seen)
       return p;
     };
     half8v p = weights(0);
@@ -698,7 +843,12 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
     }
   };
 
-  if (c0 < c1) {
+  auto pass = [&](auto APART) {
+    at = Frame{-INFINITY, 0.f};
+    l = 0.f;
+#pragma unroll
+    for (int x = 0; x < DT; ++x) o[x] = float16v{};
+    if (c0 >= c1) return;
     // Ahead of the stage computed: the next one's codes on their way into LDS,
     // codes and scales of the one after, pages of the one after that.
     Scales now = load(c0, page(c0)), next{};
@@ -708,7 +858,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
     if (c0 + 2 < c1) pg = page(c0 + 2);
     auto step = [&](int st, char* base, char* other) {
       __syncthreads();  // stage st is written, and nobody reads the other one
-      compute(st, base, other, now);
+      compute(APART, st, base, other, now);
       now = next;
       next = after;
     };
@@ -716,16 +866,21 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
       step(st, lds, lds + STAGE);
       if (st + 1 < c1) step(st + 1, lds + STAGE, lds);
     }
-  }
+  };
+  if (t == 0) odd = 0;
+  pass(std::false_type{});
+  __syncthreads();  // (nobody reads a stage any more)
+  if (odd) pass(std::true_type{});
 
-  // A wave's floats: o, mv, l; a tile's shares joined as in the kernel above.
+  // A wave's floats: o, its frame, l; a tile's shares joined as in the kernel above.
   auto each = [&](auto&& f) {
 #pragma unroll
     for (int x = 0; x < DT; ++x)
 #pragma unroll
       for (int i = 0; i < 16; ++i) f(x * 16 + i, [&](float v) { o[x][i] = v; }, o[x][i]);
-    f(DT * 16, [&](float v) { mv = v; }, mv);
-    f(DT * 16 + 1, [&](float v) { l = v; }, l);
+    f(DT * 16, [&](float v) { at.m = v; }, at.m);
+    f(DT * 16 + 1, [&](float v) { at.d = v; }, at.d);
+    f(DT * 16 + 2, [&](float v) { l = v; }, l);
   };
   if (nsplit > 1) {
     constexpr int kCoherent = 17;  // sc0 | sc1
@@ -750,14 +905,17 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
       return __uint_as_float(
           __builtin_amdgcn_raw_buffer_load_b32(rP, (uint32_t)(sp * PART + ((w * NV + i) * 64 + lane) * 4), 0, kCoherent));
     };
-    mv = -INFINITY;
-    for (int sp = 0; sp < nsplit; ++sp) mv = fmaxf(mv, held(sp, DT * 16));
+    auto frame = [&](int sp) { return Frame{held(sp, DT * 16), held(sp, DT * 16 + 1)}; };
+    at = Frame{-INFINITY, -INFINITY};
+    for (int sp = 0; sp < nsplit; ++sp) at.m = fmaxf(at.m, held(sp, DT * 16));
+    for (int sp = 0; sp < nsplit; ++sp) at.d = fmaxf(at.d, frame(sp).from(at.m).d);
     l = 0.f;
 #pragma unroll
     for (int x = 0; x < DT; ++x) o[x] = float16v{};
     for (int sp = 0; sp < nsplit; ++sp) {  // (in this order whichever came last)
-      const float f = rel_exp2(held(sp, DT * 16), mv);
-      l += f * held(sp, DT * 16 + 1);
+      const Frame to = frame(sp).from(at.m);
+      const float f = rel_exp2(to.d, at.d);
+      l += __builtin_amdgcn_exp2f(to.m) * held(sp, DT * 16 + 2);
 #pragma unroll
       for (int x = 0; x < DT; ++x)
 #pragma unroll
@@ -768,7 +926,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
   // O: lane holds row l % 32, dims 32 x + 8 g + 4 h + 0..3
   const auto l2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
   const float whole = __uint_as_float(l2[0]) + __uint_as_float(l2[1]);
-  const float f = whole == 0.f ? 0.f : 1.f / whole;  // no key seen: zeros
+  const float f = at.over(whole);
   if (row >= tile.count) return;
   T* const out = (T*)a.o + (int64_t)(tile.first + token) * a.ldo + (int64_t)head * a.ho;
 #pragma unroll
@@ -794,7 +952,7 @@ struct KvPlan {
 };
 int64_t part_bytes(const KvAttnProblem& p, const KvPlan& k) {  // of a tile's share
   const int64_t dt = p.d <= 64 ? 4 : 8;
-  return k.rt == 16 ? (dt * 4 + 2) * 64 * 4 : 4 * (dt * 8 + 2) * 64 * 4;
+  return k.rt == 16 ? (dt * 4 + 3) * 64 * 4 : 4 * (dt * 8 + 3) * 64 * 4;
 }
 KvPlan plan_of(const KvAttnProblem& p) {
   KvPlan r;

@@ -27,8 +27,9 @@
 //     ratio of the scales.  The sum of the p_j is that of the fp32 weights over
 //     their V scale, relative to 2^m as well: one maximum does for both while
 //     the V scales leave what counts in fp32's range (near_one).  A wave (in the
-//     kernel below, a workgroup) that meets any other takes its keys again with
-//     the sum relative to a maximum of its own (Frame).
+//     kernel below, a workgroup) that meets any other, or scores in the thousands
+//     (kFar), takes its keys again with the sum relative to a maximum of its own
+//     (Frame).
 //     Weights round to 11 bits, half a step relative each, like the fp16
 //     weights of the fused attention; scores, maxima, sums and O are fp32.
 // One token a request is bound by the codes' bytes: 64 requests of 8192 tokens,
@@ -114,6 +115,12 @@ __device__ __forceinline__ void value_scale(float vs, bool apart, float& lv, flo
 // scores of keys of zeros 2^45 below that are still normal numbers, and at most
 // 64 + 8 below it.
 __device__ __forceinline__ bool near_one(float vs) { return vs == 0.f || (vs >= 0x1p-30f && vs <= 0x1p10f); }
+
+// A running maximum of this magnitude or more has no bits left for log2(vs) - m
+// beside a weight's 11 (2^-13 at this one; at 2^27 it is off by powers of two
+// that fp16 does not hold): such rows take their keys again with sums of their
+// own too, where scores are rounded and subtracted before log2(vs) comes to them.
+constexpr float kFar = 4096.f;
 
 // a * b, rounded (never part of an fma).
 __device__ __forceinline__ float times(float a, float b) {
@@ -338,7 +345,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
   const int g1 = min(groups, (split + 1) * share);
 
   Partial<DT> acc;
-  bool odd = false;  // a page's scale was not near_one (wave-uniform)
+  bool odd = false;  // a page's scale was not near_one, or a maximum far from 0 (wave-uniform)
 
   const int ck = (lane >> 2) & 3;  // 16-key piece of a group that this lane's K rows lie in (V's and the scores': lg)
   const int* const table = a.table + (int64_t)r * a.ldt;
@@ -458,6 +465,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
         const float mxv = row_max(left_out(mx, lv));
         up = __any(mxv > acc.at.m + 8.f);
         if (up) {
+          odd |= __any(mxv > acc.at.m + 8.f && fabsf(mxv) >= kFar);
           const float now = mxv > acc.at.m + 8.f ? mxv : acc.at.m;
           f = rel_exp2(acc.at.m, now);
           acc.l *= f;
@@ -590,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
   constexpr int PIECES = 64 * D / 16 / 256;  // 16-byte pieces of K (and of V) a thread converts a stage
   constexpr int NV = DT * 16 + 3;
   __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-  __shared__ int last_split, odd;  // odd: a page's scale was not near_one
+  __shared__ int last_split, odd;  // odd: a page's scale was not near_one, or a maximum far from 0
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, h = lane >> 5;
@@ -797,6 +805,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
     } else {
       up = __any(mx > at.m + 8.f);
       if (up) {
+        if (__any(mx > at.m + 8.f && fabsf(mx) >= kFar) && lane == 0) odd = 1;
         const float now = mx > at.m + 8.f ? mx : at.m;
         f = rel_exp2(at.m, now);
         l *= f;

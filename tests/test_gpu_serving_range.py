@@ -1,5 +1,6 @@
 """Attention over the 8-bit cache at the ends of its range: pages whose value
-scales lie far apart or are zero, against the definition in 64 bits."""
+scales lie far apart or are zero, scores of any size, against the definition in
+64 bits."""
 import pytest
 import torch
 
@@ -57,3 +58,49 @@ def test_attention_over_value_scales_far_apart(pkg, dev, rows, heads, d, block, 
                             blocks, (powers, i))
     else:
         check_attention(got, q, k, v, block, table, lens, cu, d ** -0.5, blocks, powers)
+
+
+@pytest.mark.parametrize("rows, heads", ROWS)
+@pytest.mark.parametrize("d, block", [(64, 16), (128, 32)])
+@pytest.mark.parametrize("power, dtype", [(14, torch.float16), (19, torch.float16), (23, torch.float16), (27, torch.float16),
+                                          (33, torch.float16), (37, torch.float16), (30, torch.bfloat16), (90, torch.bfloat16)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_of_large_scores(pkg, dev, rows, heads, d, block, power, dtype, sign):
+    """Scores that are whole multiples of 2^power: the keys of a row's largest
+    one share it, on pages of unlike value scales, and no weight overflows."""
+    blocks = max(5, 600 // block)
+    n = blocks * block
+    kc, vc = torch.zeros((n, 1, d)), codes((n, 1, d), 12)
+    kc[..., 0] = torch.randint(-9, 10, (n, 1), generator=gen(11)).float()
+    vs = torch.exp2(torch.arange(blocks) % 4 - 6.0)[:, None]
+    cache, (k, v) = cache_of(pkg, dev, kc, vc, torch.ones((blocks, 1)), vs, block)
+    table = torch.randperm(blocks, generator=gen(13)).to(torch.int32).view(1, blocks).to(dev)
+    half = min(power // 2, 15)
+    q = torch.zeros((rows, heads, d))
+    q[..., 0] = sign * 2.0 ** half
+    q[..., 1:] = normal((rows, heads, d - 1), 14, dtype=torch.float32)  # (meets zero codes)
+    q, scale = q.to(dtype).to(dev), 2.0 ** (power - half)
+    got = pkg.kv_attention(q, cache, table, ints(dev, n - 3), cu=ints(dev, 0, rows), scale=scale)
+    for i in {0, rows // 2, rows - 1}:
+        check_attention(got[i:i + 1], q[i:i + 1], k, v, block, table, ints(dev, n - 3 - rows + i + 1), [0, 1], scale, blocks,
+                        (power, i))
+
+
+def test_attention_of_rows_with_infinities(pkg, dev):
+    """An infinity or a NaN in a row of q makes that row NaN and no other."""
+    heads, d, block, blocks = 10, 128, 32, 16
+    kc, vc = codes((blocks * block, 1, d), 15), codes((blocks * block, 1, d), 16)
+    ones = torch.full((blocks, 1), 2.0 ** -6)
+    cache, (k, v) = cache_of(pkg, dev, kc, vc, ones, ones, block)
+    table = torch.arange(blocks, dtype=torch.int32, device=dev).view(1, blocks)
+    for dtype in (torch.float16, torch.bfloat16):
+        for rows in (3, 450):
+            q = normal((rows, heads, d), 17, 1.5, dtype=dtype).to(dev)
+            want = pkg.kv_attention(q, cache, table, ints(dev, 500), cu=ints(dev, 0, rows))
+            q[0, 3, 5], q[1, 0, 127], q[rows - 1, 9, 0] = float("inf"), float("nan"), float("-inf")
+            got = pkg.kv_attention(q, cache, table, ints(dev, 500), cu=ints(dev, 0, rows))
+            bad = torch.zeros((rows, heads), dtype=torch.bool, device=dev)
+            bad[0, 3] = bad[1, 0] = bad[rows - 1, 9] = True
+            assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all(), (dtype, rows)
+            off = (got[~bad].double() - want[~bad].double()).abs()
+            assert (off <= 2.0 ** -7 * want[~bad].double().abs() + 2.0 ** -9).all(), (dtype, rows)

@@ -22,16 +22,18 @@
 //     fp16 under a power of two a row, exact for all that counts beside the
 //     row's largest element;
 //   * the K scale multiplies the score.  The V scale multiplies the weight
-//     before its rounding to fp16, relative to 2^m, the running maximum of
-//     score + log2(vs): the weights P.V sees stay in (0, 2^8] whatever the
-//     ratio of the scales.  The sum of the p_j is that of the fp32 weights over
+//     before its rounding to fp16, relative to 2^m, m following the running
+//     maximum of score + log2(vs) from 7 to 15 below it: the largest weight P.V
+//     sees lies in [2^7, 2^15] whatever the ratio of the scales.  The sum of the p_j is that of the fp32 weights over
 //     their V scale, relative to 2^m as well: one maximum does for both while
 //     the V scales leave what counts in fp32's range (near_one).  A wave (in the
 //     kernel below, a workgroup) that meets any other, or scores in the thousands
 //     (kFar), takes its keys again with the sum relative to a maximum of its own
 //     (Frame).
-//     Weights round to 11 bits, half a step relative each, like the fp16
-//     weights of the fused attention; scores, maxima, sums and O are fp32.
+//     Weights from 2^-21 of the row's largest on round to 11 bits, smaller ones
+//     to multiples of 2^-31 of it (fp16 below 2^-14), so that the others keep
+//     their part beside one key far above them; scores, maxima, sums and O are
+//     fp32.
 // One token a request is bound by the codes' bytes: 64 requests of 8192 tokens,
 // 32 heads over 8 of 128 dims, 156 us (814 MB, 5.2 TB/s); one of 131072 tokens
 // 62 us (4.3 TB/s, shares of the keys and their join).  Short ones are bound by
@@ -113,7 +115,7 @@ __device__ __forceinline__ void value_scale(float vs, bool apart, float& lv, flo
 // Whether the sum can be taken from a page's weighted scores, 2^(score + log2(vs)
 // - m): m is at most 10 above the largest score then, so that the weighted
 // scores of keys of zeros 2^45 below that are still normal numbers, and at most
-// 64 + 8 below it.
+// 64 + 15 below it.
 __device__ __forceinline__ bool near_one(float vs) { return vs == 0.f || (vs >= 0x1p-30f && vs <= 0x1p10f); }
 
 // A running maximum of this magnitude or more has no bits left for log2(vs) - m
@@ -129,9 +131,12 @@ __device__ __forceinline__ float times(float a, float b) {
 }
 
 // What a row's numbers are relative to: the sum l of its p_j to 2^m, O to
-// 2^(m + d).  d is 0 and m the running maximum of score + log2(vs) (within 8), or,
-// with sums of their own, m the largest score and d the running maximum of
-// score - m + log2(vs): -inf where nothing has been added to O.
+// 2^(m + d).  d is 0 and m kLow to kHigh below the running maximum of score +
+// log2(vs), or, with sums of their own, m is the largest score and d that far
+// below the running maximum of score - m + log2(vs): -inf where nothing has been
+// added to O.  (kLow 0 and kHigh 8 would leave the upper half of fp16's range
+// unused: a key 24 bits above all others cost these a third of their part.)
+constexpr float kLow = 7.f, kHigh = 15.f;
 struct Frame {
   float m, d;
 
@@ -144,7 +149,7 @@ struct Frame {
   }
   // The maximum of score - m + log2(vs) is now at least `cand`: what O is to be multiplied by.
   __device__ __forceinline__ float raise_o(float cand) {
-    const float now = cand > d + 8.f ? cand : d, f = rel_exp2(d, now);
+    const float now = cand > d + kHigh ? cand - kLow : d, f = rel_exp2(d, now);
     d = now;
     return f;
   }
@@ -463,10 +468,10 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
         ref = acc.at.d;
       } else {
         const float mxv = row_max(left_out(mx, lv));
-        up = __any(mxv > acc.at.m + 8.f);
+        up = __any(mxv > acc.at.m + kHigh);
         if (up) {
-          odd |= __any(mxv > acc.at.m + 8.f && fabsf(mxv) >= kFar);
-          const float now = mxv > acc.at.m + 8.f ? mxv : acc.at.m;
+          odd |= __any(mxv > acc.at.m + kHigh && fabsf(mxv) >= kFar);
+          const float now = mxv > acc.at.m + kHigh ? mxv - kLow : acc.at.m;
           f = rel_exp2(acc.at.m, now);
           acc.l *= f;
           acc.at.m = now;
@@ -803,10 +808,10 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
       f = at.raise_o(both(cand));
       ref = at.d;
     } else {
-      up = __any(mx > at.m + 8.f);
+      up = __any(mx > at.m + kHigh);
       if (up) {
-        if (__any(mx > at.m + 8.f && fabsf(mx) >= kFar) && lane == 0) odd = 1;
-        const float now = mx > at.m + 8.f ? mx : at.m;
+        if (__any(mx > at.m + kHigh && fabsf(mx) >= kFar) && lane == 0) odd = 1;
+        const float now = mx > at.m + kHigh ? mx - kLow : at.m;
         f = rel_exp2(at.m, now);
         l *= f;
         at.m = now;

@@ -1,11 +1,11 @@
 """Attention over the 8-bit cache at the ends of its range: pages whose value
-scales lie far apart or are zero, scores of any size, against the definition in
-64 bits."""
+scales lie far apart or are zero, scores of any size, keys far above the others,
+against the definition in 64 bits."""
 import pytest
 import torch
 
 from gpu_util import gen, normal
-from test_gpu_serving import check_attention, ints
+from test_gpu_serving import HALF, check_attention, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +104,48 @@ def test_attention_of_rows_with_infinities(pkg, dev):
             assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all(), (dtype, rows)
             off = (got[~bad].double() - want[~bad].double()).abs()
             assert (off <= 2.0 ** -7 * want[~bad].double().abs() + 2.0 ** -9).all(), (dtype, rows)
+
+
+def weights64(q, k, n, scale):
+    return (q.double() @ k[:n, 0].T * scale).softmax(-1)
+
+
+@pytest.mark.parametrize("tiles", [16, 128])
+@pytest.mark.parametrize("spread", [0.0, 0.3])
+@pytest.mark.parametrize("bits", [12, 18, 20, 22, 24.4])
+@pytest.mark.parametrize("n", [1000, 8000])
+def test_attention_of_one_key_far_above_the_rest(pkg, dev, tiles, spread, bits, n):
+    """One key `bits` bits above all others whose values are zero, as a first
+    token often is: the others carry the output, and keep their weights' bits.
+    A weight is rounded to 11 bits, or to 2^-32 of the row's largest weight times
+    value scale; no term grows with the number of keys beyond that."""
+    d, block, group = 64, 64, 8
+    blocks = -(-n // block)
+    # 64 requests of a row and a key head for each query head, or one of many rows (keys up to them)
+    requests, rows, kv_heads = (64, 1, 8) if tiles == 16 else (1, min(n, 4200), 1)
+    kc, vc = (codes((blocks * block, 1, d), 21) * (spread / 8)).round(), codes((blocks * block, 1, d), 22, 12) + 60
+    kc[..., 0], kc[0], vc[0] = 0, 0, 0
+    kc[0, 0, 0] = 127
+    every = lambda t: t.expand(-1, kv_heads, *t.shape[2:]).contiguous()  # noqa: E731
+    one = torch.full((blocks, 1), 2.0 ** -6)
+    cache, (k, v) = cache_of(pkg, dev, every(kc), every(vc), every(one), every(one), block)
+    q = normal((1, 1, d), 23, dtype=torch.float32).expand(requests * rows, group, d).clone()
+    scale = 0.125
+    q[..., 0] = bits * 0.6931471805599453 / (127 / 64 * scale)
+    q = q.half().to(dev)
+    table = torch.arange(blocks, dtype=torch.int32, device=dev).expand(requests, blocks).contiguous()
+    lens = torch.full((requests,), n, dtype=torch.int32, device=dev)
+    cu = torch.arange(0, requests * rows + 1, rows, dtype=torch.int32, device=dev)
+    got = pkg.kv_attention(q, cache, table, lens, cu=None if tiles == 16 else cu, scale=scale).cpu().double()
+    qh = q[0, 0].cpu()
+    for t in ([0, 63] if tiles == 16 else [rows // 2, rows - 2, rows - 1]):
+        keys = n if tiles == 16 else n - rows + t + 1
+        w, x = weights64(qh, k, keys, scale), v[:keys, 0]
+        assert w[0] / w[1:].max() > 2.0 ** (bits - 2)
+        want = w @ x
+        # the output's half step; scores (fp32 sums of 64 products up to 20: 2^-13) and weights
+        # (half a step of 11 bits); weights below 2^-14 of fp16 in steps of 2^-24, times up to 127
+        room = HALF[torch.float16] * want.abs() + (2.0 ** -11 + 2.0 ** -13) * (w @ x.abs()) + \
+            2.0 ** -32 * w.max() * x.abs().sum(0) + 2.0 ** -25
+        off = (got[t] - want).abs() - room
+        assert off.max() <= 0, (t, float(((got[t] - want).abs() / want.abs()).max()))

@@ -19,25 +19,27 @@
 //   * those 16 weights are the B operand of P.V as they are, and 16 bytes of
 //     V (16 tokens of one head dim) the A operand: D[dim][row];
 //   * codes become fp16 exactly (conversion below).  q in bf16 is brought to
-//     fp16 under a power of two a row, exact for all that counts beside the
-//     row's largest element;
+//     fp16 under a power of two a row: multiples of 2^-38 of its largest element;
 //   * the K scale multiplies the score.  The V scale multiplies the weight
 //     before its rounding to fp16, relative to 2^m, m following the running
 //     maximum of score + log2(vs) from 7 to 15 below it: the largest weight P.V
-//     sees lies in [2^7, 2^15] whatever the ratio of the scales.  The sum of the p_j is that of the fp32 weights over
-//     their V scale, relative to 2^m as well: one maximum does for both while
-//     the V scales leave what counts in fp32's range (near_one).  A wave (in the
-//     kernel below, a workgroup) that meets any other, or scores in the thousands
-//     (kFar), takes its keys again with the sum relative to a maximum of its own
-//     (Frame).
+//     sees lies in [2^7, 2^15] whatever the ratio of the scales.  The sum of the
+//     p_j is that of the fp32 weights over their V scale, relative to 2^m as
+//     well: one maximum does for both while the V scales leave what counts in
+//     fp32's range (near_one).  A wave (in the kernel below, a workgroup) that
+//     meets any other, or scores in the thousands (kFar), takes its keys again
+//     with the sum relative to a maximum of its own (Frame).
 //     Weights from 2^-21 of the row's largest on round to 11 bits, smaller ones
 //     to multiples of 2^-31 of it (fp16 below 2^-14), so that the others keep
 //     their part beside one key far above them; scores, maxima, sums and O are
 //     fp32.
 // One token a request is bound by the codes' bytes: 64 requests of 8192 tokens,
-// 32 heads over 8 of 128 dims, 156 us (814 MB, 5.2 TB/s); one of 131072 tokens
-// 62 us (4.3 TB/s, shares of the keys and their join).  Short ones are bound by
-// latency: 1900 tokens of one user 7 us.
+// 32 heads over 8 of 128 dims, 157 us (814 MB, 5.2 TB/s); one of 131072 tokens
+// 63 us (268 MB, 4.3 TB/s; 55 where the call before has left part of them in the
+// last-level cache).  Short ones are bound by latency: 1900 tokens of one user
+// 7.3 us, over a table as wide as that (plan_of).  Keys taken again cost their
+// time again: scales far apart all over, 64 x 8192 183 -> 364 us and prompt chunks
+// 366 -> 834 (random codes throughout).
 #include "hxmi_common.h"
 #include "hxmi_internal.h"
 
@@ -279,7 +281,7 @@ __device__ __forceinline__ Share share_of(const KArgs& a) {
 
 // Eight elements of q as fp16, and what the scores are to be multiplied by.  q
 // in bf16 takes a power of two `ex` that brings the row's largest element to
-// [2^14, 2^15): what is below 2^-39 of it is lost, far under the fp32 sums.
+// [2^14, 2^15): the row's elements become multiples of 2^-24, at most 2^-38 of it.
 template <typename T>
 __device__ __forceinline__ float largest(const T (&x)[8], float top) {
 #pragma unroll
@@ -586,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
 // A workgroup of four waves owns 128 rows (32 a wave) and takes 64 keys at a
 // time through two LDS stages: its threads convert the codes to fp16 on the way
 // in, so a code is converted once for 128 rows (the kernel above: for 16), and codes of the next stage but one are in flight meanwhile.  2350 rows x
-// 32 heads over 8000 keys: 269 us (733 TFLOP/s), 507 by the kernel above; bound
+// 32 heads over 8000 keys: 271 us (727 TFLOP/s), 507 by the kernel above; bound
 // by the vector ALUs (softmax, then conversion) of two waves a SIMD.  Eight waves
 // of 256 rows convert half as often and were slower (289 us, 279 of four at that
 // time): one workgroup a CU has nothing to run while it waits at its barriers.
@@ -977,7 +979,11 @@ KvPlan plan_of(const KvAttnProblem& p) {
   // key/value heads, 37 requests: 80 rows 186 / 188, 112 rows 250 / 167; dims of
   // 64, 4 heads, 48 requests: 192 rows 107 / 140, 256 rows 139 / 117; one request,
   // 128 dims: 256 rows 28 / 30, 1024 rows 56 / 43).  Tiles of 32 rows were slower
-  // than 16 up to 100 rows and never the fastest.
+  // than 16 up to 100 rows and never the fastest.  The average is over requests
+  // that have no rows or one as well, so a call that mixes decoding requests and
+  // a prompt's chunk runs both on tiles that suit one of them: over 8192 keys,
+  // 63 rows and a chunk of 2048 732 us in one call, 181 + 287 in two; 256 rows and
+  // a chunk of 512 925 us, 708 + 112 in two.
   const bool wide = rows > (p.d > 64 ? 96 : 255) && p.tokens * p.heads >= 4096;
   r.rt = wide ? 128 : 16;
   const int64_t rt = r.rt;
@@ -987,7 +993,9 @@ KvPlan plan_of(const KvAttnProblem& p) {
   // one more round, at least one group of 64 keys a wave (eight stages of a
   // 128-row tile) to a share.  575 tiles of 128 rows x 8000 keys, before later
   // steps: 391 us unshared, 292 with all of them in two shares, 281 with the last
-  // 63 in eight.
+  // 63 in eight.  The table's width stands for the lengths, which only the GPU
+  // knows: shares past a request's keys are joined for nothing (one user of 1900
+  // tokens: 7.7 us with a table of 30 pages, 10.6 with 128, 24 with 512 or more).
   const int64_t items = r.tiles * p.kv_heads, least = wide ? 512 : 256, most = (p.width * p.block + least - 1) / least;
   const int64_t left = items % 512;
   int64_t n = left ? 512 / left : 1;

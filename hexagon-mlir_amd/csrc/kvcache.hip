@@ -246,9 +246,11 @@ struct CArgs {
 // block) of one head of K or V: the largest magnitude of its rows, the
 // block's scale, the block's earlier codes again if the scale has grown, its
 // own codes.  A run is found by its first row: the row before it does not go
-// to the slot before.  Latency bounds it at one token a request (three
-// dependent loads: slot, scale and row, codes), the loads and stores at a
-// prompt's length.
+// to the slot before.  Latency bounds it at one token a request (slot, scale and
+// row, and where the scale grows the codes, there and back): 128 requests, 8 x
+// 128 bf16, 12.6 us into blocks not touched before (about a fifth of the scales grow),
+// 5 us once they have.  A prompt's rows are loaded twice, for the largest value
+// and for the codes (V two bytes at a time): 6853 of 4 x 64 fp16 14 us.
 template <typename T>
 __global__ __launch_bounds__(256) void kv_append(CArgs a) {
   const int lane = threadIdx.x & 63;

@@ -520,9 +520,12 @@ int hxmi_kv_read(int is_bf16, const int8_t* k_codes, const int8_t* v_codes, cons
  * cache, these rows' own among them: row i of n sees keys j <= lens[r] - n + i,
  *   o = softmax_j(scale * q . K_j) . V_j,
  * K_j and V_j the held values of page block_table[r][j / block_size], fp32
- * scores, softmax and accumulation.  Keys of a page outside the cache are
- * left out; a row that sees no key gives zeros; rows of no request are not
- * written.  scale > 0 and finite.
+ * scores, sums and accumulation.  Two operands have fewer bits: a weight times
+ * its page's V scale goes into the product with V_j in 11 bits, or as a multiple
+ * of 2^-31 of the row's largest such number where that is coarser; and the
+ * elements of a bf16 row of q are multiples of 2^-38 of its largest.  Keys of a
+ * page outside the cache are left out; a row that sees no key gives zeros; rows
+ * of no request are not written.  scale > 0 and finite.
  * workspace: as for hxmi_gemm_f16 (zeroed once after allocation, left zeroed,
  * one call at a time), hxmi_kv_attention_workspace_bytes() bytes; with few
  * rows the keys are shared out over workgroups that join their parts there.

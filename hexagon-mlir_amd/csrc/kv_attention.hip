@@ -37,7 +37,7 @@
 // 32 heads over 8 of 128 dims, 157 us (814 MB, 5.2 TB/s); one of 131072 tokens
 // 63 us (268 MB, 4.3 TB/s; 55 where the call before has left part of them in the
 // last-level cache).  Short ones are bound by latency: 1900 tokens of one user
-// 7.3 us, over a table as wide as that (plan_of).  Keys taken again cost their
+// 7.2 us, over a table as wide as that (plan_of).  Keys taken again cost their
 // time again: scales far apart all over, 64 x 8192 183 -> 364 us and prompt chunks
 // 366 -> 834 (random codes throughout).
 #include "hxmi_common.h"
@@ -118,7 +118,10 @@ __device__ __forceinline__ void value_scale(float vs, bool apart, float& lv, flo
 // - m): m is at most 10 above the largest score then, so that the weighted
 // scores of keys of zeros 2^45 below that are still normal numbers, and at most
 // 64 + 15 below it.
-__device__ __forceinline__ bool near_one(float vs) { return vs == 0.f || (vs >= 0x1p-30f && vs <= 0x1p10f); }
+__device__ __forceinline__ bool near_one(float vs) {  // 0, or from 2^-30 to 2^10
+  const uint32_t b = __float_as_uint(vs), lo = (127 - 30) << 23, hi = (127 + 10) << 23;
+  return b - lo <= hi - lo || b == 0;
+}
 
 // A running maximum of this magnitude or more has no bits left for log2(vs) - m
 // beside a weight's 11 (2^-13 at this one; at 2^27 it is off by powers of two
@@ -301,9 +304,10 @@ __device__ __forceinline__ half8v q_operand(const T (&x)[8], int ex) {
   return h;
 }
 
-// DC: 64-dim pieces of a row; WHOLE: the head dim is 64 * DC.
+// DC: 64-dim pieces of a row; WHOLE: the head dim is 64 * DC.  (Waves a SIMD: as the
+// first pass over the keys allows; the second one's registers would take one.)
 template <typename T, int DC, bool WHOLE>
-__global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
+__global__ __launch_bounds__(256, DC == 1 ? 4 : 2) void kv_attention(KArgs a) {
   constexpr int DT = DC * 4, RT = 16, NV = Partial<DT>::N;
   constexpr bool BF16 = !std::is_same_v<T, _Float16>;
   __shared__ __attribute__((aligned(16))) float joined[3 * NV * 64];
@@ -352,7 +356,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
   const int g1 = min(groups, (split + 1) * share);
 
   Partial<DT> acc;
-  bool odd = false;  // a page's scale was not near_one, or a maximum far from 0 (wave-uniform)
+  bool odd = false;  // a page's scale was not near_one, or a maximum far from 0 (a lane's)
 
   const int ck = (lane >> 2) & 3;  // 16-key piece of a group that this lane's K rows lie in (V's and the scores': lg)
   const int* const table = a.table + (int64_t)r * a.ldt;
@@ -439,7 +443,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
         mx *= cs;  // (cs >= 0)
-        odd |= !__all(near_one(vs0));
+        odd |= !near_one(vs0);
       } else {
         // the scores times cs, masked ones -inf
         const int left = there0 ? last - (g * 64 + lg * 16) : -1;  // keys of this lane up to this one are seen
@@ -452,7 +456,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
           }
         // (a page whose every key is masked takes no part, whatever its scale)
         if (left < 0) lv = -INFINITY;
-        odd |= !__all(left < 0 || near_one(vs0));
+        odd |= left >= 0 && !near_one(vs0);
       }
       float ref, f = 1.f;  // a weight is relative to 2^ref
       bool up = true;
@@ -472,7 +476,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
         const float mxv = row_max(left_out(mx, lv));
         up = __any(mxv > acc.at.m + kHigh);
         if (up) {
-          odd |= __any(mxv > acc.at.m + kHigh && fabsf(mxv) >= kFar);
+          odd |= mxv > acc.at.m + kHigh && fabsf(mxv) >= kFar;
           const float now = mxv > acc.at.m + kHigh ? mxv - kLow : acc.at.m;
           f = rel_exp2(acc.at.m, now);
           acc.l *= f;
@@ -512,7 +516,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
     }
   };
   pass(std::false_type{});
-  if (odd) pass(std::true_type{});
+  if (__any(odd)) pass(std::true_type{});
 
   // Join the waves' parts: waves 1..3 through LDS into wave 0.
   auto join = [&]() {
@@ -596,9 +600,9 @@ __global__ __launch_bounds__(256, 2) void kv_attention(KArgs a) {
 // reads key 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that a
 // lane's eight weights of 16 keys are eight in order, the B operand of P.V.  The
 // 16 keys are one piece of a page: K and V scales are wave-uniform.
-// D: LDS rows of K (64 or 128 dims).
+// D: LDS rows of K (64 or 128 dims; with 64, two waves a SIMD were 8 % slower than three).
 template <typename T, int D, bool WHOLE>
-__global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attention_tiles(KArgs a) {
   constexpr bool BF16 = !std::is_same_v<T, _Float16>;
   constexpr int DS = D / 16, DT = D / 32, RB = 2 * D;
   constexpr int KB = 64 * RB, STAGE = KB + D * 128;
@@ -700,6 +704,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
   float16v o[DT];
   Frame at;
   float l;
+  bool bad = false;  // (a lane's)
 
   const int key = 16 * (lr >> 4) + 8 * (lr >> 2 & 1) + 4 * (lr >> 3 & 1) + (lr & 3);
   const int k_read = k_at(key, h), v_read = v_at(lr, h);
@@ -714,7 +719,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
     if (sc.b < 0) lane_lv = -INFINITY;
     const float lane_ks = sc.b < 0 ? 0.f : sc.k;
     const uint64_t there = __ballot(sc.b >= 0);
-    if (!APART && !__all(sc.b < 0 || near_one(sc.v)) && lane == 0) odd = 1;
+    if (!APART) bad |= sc.b >= 0 && !near_one(sc.v);
     const bool all = !APART && st * 64 + 64 <= kfull && there == ~0ull;
     float ks[4], lv[4], rv[4];
     auto lane_of = [](float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); };
@@ -812,7 +817,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
     } else {
       up = __any(mx > at.m + kHigh);
       if (up) {
-        if (__any(mx > at.m + kHigh && fabsf(mx) >= kFar) && lane == 0) odd = 1;
+        bad |= mx > at.m + kHigh && fabsf(mx) >= kFar;
         const float now = mx > at.m + kHigh ? mx - kLow : at.m;
         f = rel_exp2(at.m, now);
         l *= f;
@@ -886,6 +891,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
   if (t == 0) odd = 0;
   pass(std::false_type{});
   __syncthreads();  // (nobody reads a stage any more)
+  if (bad) odd = 1;
+  __syncthreads();
   if (odd) pass(std::true_type{});
 
   // A wave's floats: o, its frame, l; a tile's shares joined as in the kernel above.
@@ -922,9 +929,14 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tiles(KArgs a) {
           __builtin_amdgcn_raw_buffer_load_b32(rP, (uint32_t)(sp * PART + ((w * NV + i) * 64 + lane) * 4), 0, kCoherent));
     };
     auto frame = [&](int sp) { return Frame{held(sp, DT * 16), held(sp, DT * 16 + 1)}; };
-    at = Frame{-INFINITY, -INFINITY};
-    for (int sp = 0; sp < nsplit; ++sp) at.m = fmaxf(at.m, held(sp, DT * 16));
-    for (int sp = 0; sp < nsplit; ++sp) at.d = fmaxf(at.d, frame(sp).from(at.m).d);
+    at = Frame{-INFINITY, 0.f};
+#pragma unroll 4
+    for (int sp = 0; sp < nsplit; ++sp) {
+      Frame two[2] = {at, frame(sp)};
+      float fl[2], fo[2];
+      join_frames(two, fl, fo);
+      at = two[0];
+    }
     l = 0.f;
 #pragma unroll
     for (int x = 0; x < DT; ++x) o[x] = float16v{};

@@ -39,7 +39,7 @@
 // last-level cache).  Short ones are bound by latency: 1900 tokens of one user
 // 7.2 us, over a table as wide as that (plan_of).  Keys taken again cost their
 // time again: scales far apart all over, 64 x 8192 183 -> 364 us and prompt chunks
-// 366 -> 834 (random codes throughout).
+// 362 -> 832 (random codes throughout).
 #include "hxmi_common.h"
 #include "hxmi_internal.h"
 
@@ -994,8 +994,8 @@ KvPlan plan_of(const KvAttnProblem& p) {
   // than 16 up to 100 rows and never the fastest.  The average is over requests
   // that have no rows or one as well, so a call that mixes decoding requests and
   // a prompt's chunk runs both on tiles that suit one of them: over 8192 keys,
-  // 63 rows and a chunk of 2048 732 us in one call, 181 + 287 in two; 256 rows and
-  // a chunk of 512 925 us, 708 + 112 in two.
+  // 63 rows and a chunk of 2048 722 us in one call, 180 + 283 in two; 256 rows and
+  // a chunk of 512 928 us, 711 + 110 in two.
   const bool wide = rows > (p.d > 64 ? 96 : 255) && p.tokens * p.heads >= 4096;
   r.rt = wide ? 128 : 16;
   const int64_t rt = r.rt;
@@ -1007,7 +1007,7 @@ KvPlan plan_of(const KvAttnProblem& p) {
   // steps: 391 us unshared, 292 with all of them in two shares, 281 with the last
   // 63 in eight.  The table's width stands for the lengths, which only the GPU
   // knows: shares past a request's keys are joined for nothing (one user of 1900
-  // tokens: 7.7 us with a table of 30 pages, 10.6 with 128, 24 with 512 or more).
+  // tokens: 7.5 us with a table of 30 pages, 10.6 with 128, 24 with 512 or more).
   const int64_t items = r.tiles * p.kv_heads, least = wide ? 512 : 256, most = (p.width * p.block + least - 1) / least;
   const int64_t left = items % 512;
   int64_t n = left ? 512 / left : 1;

@@ -1,6 +1,7 @@
 """hexagon_mlir_amd — MI355X-native replacement of Hexagon-MLIR's matmul / GEMV /
 RMSNorm / softmax hot path, and the operators of a serving loop around it
-(block tables, an 8-bit key/value cache, attention over it, sampling).
+(block tables, rotation of queries and keys, key/value caches of 8 and 4 bits,
+attention over them, sampling, verification of drafted tokens).
 
 Layers:
   * ``csrc/``      hand-written HIP kernels for gfx950 behind the C ABI of
@@ -18,6 +19,7 @@ from .hxmi import (
     HxmiError,
     HxmiNotBuiltError,
     KVCache,
+    KVCache4,
     KVPlan,
     attention,
     bgemm,
@@ -32,9 +34,11 @@ from .hxmi import (
     linear,
     load_library,
     pack_gate_up,
+    qk_rope,
     quantize_int8,
     rms_norm,
     rms_norm_linear,
+    rope_frequencies,
     sample,
     set_tuning,
     softmax,
@@ -48,6 +52,7 @@ __all__ = [
     "HxmiError",
     "HxmiNotBuiltError",
     "KVCache",
+    "KVCache4",
     "KVPlan",
     "attention",
     "bgemm",
@@ -62,9 +67,11 @@ __all__ = [
     "linear",
     "load_library",
     "pack_gate_up",
+    "qk_rope",
     "quantize_int8",
     "rms_norm",
     "rms_norm_linear",
+    "rope_frequencies",
     "sample",
     "set_tuning",
     "softmax",

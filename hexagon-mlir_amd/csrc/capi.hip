@@ -718,7 +718,8 @@ int hxmi_kv_plan(const int32_t* lens, const int32_t* added, int32_t* block_table
 
 // The cache's own arguments, which every call on it takes.
 static int cache_check(const char* name, const void* k_codes, const void* v_codes, const void* k_scale,
-                       const void* v_scale, int64_t blocks, int64_t kv_heads, int64_t head_dim, int64_t block_size) {
+                       const void* v_scale, int64_t blocks, int64_t kv_heads, int64_t head_dim, int64_t block_size,
+                       bool scale_bytes) {
   REQUIRE(kv_heads > 0 && head_dim > 0 && blocks >= 0, "%s: sizes must be positive", name);
   REQUIRE(log2_block(block_size) >= 0, "%s: block_size must be a power of two from 16 to 256, got %lld", name,
           (long long)block_size);
@@ -727,22 +728,26 @@ static int cache_check(const char* name, const void* k_codes, const void* v_code
   REQUIRE(kv_heads < (1 << 20) && blocks < (1ll << 31), "%s: too many heads or blocks", name);
   REQUIRE(blocks == 0 || (k_codes && v_codes && k_scale && v_scale), "%s: null cache pointer", name);
   REQUIRE((uintptr_t)k_codes % 16 == 0 && (uintptr_t)v_codes % 16 == 0, "%s: codes must be 16-byte aligned", name);
+  REQUIRE(!scale_bytes || ((uintptr_t)k_scale % 16 == 0 && (uintptr_t)v_scale % 16 == 0),
+          "%s: scales must be 16-byte aligned", name);
   return HXMI_OK;
 }
 
-int hxmi_kv_append(int is_bf16, const void* k, const void* v, const int64_t* slots, int8_t* k_codes, int8_t* v_codes,
-                   float* k_scale, float* v_scale, int64_t tokens, int64_t blocks, int64_t kv_heads, int64_t head_dim,
-                   int64_t block_size, int64_t ldk, int64_t head_stride_k, int64_t ldv, int64_t head_stride_v,
-                   void* stream) {
-  const char* name = "hxmi_kv_append";
+// Writes to, reads from and attention over either cache (P: its problem, launch: its launcher).
+extern "C++" template <typename P, typename Code, typename Scale, typename Launch>
+static int cache_append(const char* name, Launch launch, int is_bf16, const void* k, const void* v,
+                        const int64_t* slots, Code* k_codes, Code* v_codes, Scale* k_scale, Scale* v_scale,
+                        int64_t tokens, int64_t blocks, int64_t kv_heads, int64_t head_dim, int64_t block_size,
+                        int64_t ldk, int64_t head_stride_k, int64_t ldv, int64_t head_stride_v, void* stream) {
   REQUIRE(is_bf16 == 0 || is_bf16 == 1, "%s: is_bf16 must be 0 or 1", name);
   REQUIRE(tokens >= 0 && tokens < (1ll << 31), "%s: bad number of tokens %lld", name, (long long)tokens);
-  if (const int rc = cache_check(name, k_codes, v_codes, k_scale, v_scale, blocks, kv_heads, head_dim, block_size))
+  if (const int rc = cache_check(name, k_codes, v_codes, k_scale, v_scale, blocks, kv_heads, head_dim, block_size,
+                                 sizeof(Scale) == 1))
     return rc;
   if (tokens == 0 || blocks == 0) return ok();
   REQUIRE(k && v && slots, "%s: null pointer", name);
   REQUIRE(ldk >= 0 && head_stride_k >= 0 && ldv >= 0 && head_stride_v >= 0, "%s: negative stride", name);
-  hxmi::KvCacheProblem p{};
+  P p{};
   p.k_codes = k_codes;
   p.v_codes = v_codes;
   p.k_scale = k_scale;
@@ -760,24 +765,26 @@ int hxmi_kv_append(int is_bf16, const void* k, const void* v, const int64_t* slo
   p.hsv = head_stride_v;
   p.log2_block = log2_block(block_size);
   p.dtype = is_bf16 ? hxmi::DT_BF16 : hxmi::DT_F16;
-  return from_hip(hxmi::launch_kv_append(p, (hipStream_t)stream), name);
+  return from_hip(launch(p, (hipStream_t)stream), name);
 }
 
-int hxmi_kv_read(int is_bf16, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
-                 const int64_t* slots, void* k, void* v, int64_t tokens, int64_t blocks, int64_t kv_heads,
-                 int64_t head_dim, int64_t block_size, void* stream) {
-  const char* name = "hxmi_kv_read";
+extern "C++" template <typename P, typename Code, typename Scale, typename Launch>
+static int cache_read(const char* name, Launch launch, int is_bf16, const Code* k_codes, const Code* v_codes,
+                      const Scale* k_scale, const Scale* v_scale, const int64_t* slots, void* k, void* v,
+                      int64_t tokens, int64_t blocks, int64_t kv_heads, int64_t head_dim, int64_t block_size,
+                      void* stream) {
   REQUIRE(is_bf16 == 0 || is_bf16 == 1, "%s: is_bf16 must be 0 or 1", name);
   REQUIRE(tokens >= 0 && tokens < (1ll << 31), "%s: bad number of tokens %lld", name, (long long)tokens);
-  if (const int rc = cache_check(name, k_codes, v_codes, k_scale, v_scale, blocks, kv_heads, head_dim, block_size))
+  if (const int rc = cache_check(name, k_codes, v_codes, k_scale, v_scale, blocks, kv_heads, head_dim, block_size,
+                                 sizeof(Scale) == 1))
     return rc;
   if (tokens == 0) return ok();
   REQUIRE(k && v && slots, "%s: null pointer", name);
-  hxmi::KvCacheProblem p{};
-  p.k_codes = const_cast<int8_t*>(k_codes);
-  p.v_codes = const_cast<int8_t*>(v_codes);
-  p.k_scale = const_cast<float*>(k_scale);
-  p.v_scale = const_cast<float*>(v_scale);
+  P p{};
+  p.k_codes = const_cast<Code*>(k_codes);
+  p.v_codes = const_cast<Code*>(v_codes);
+  p.k_scale = const_cast<Scale*>(k_scale);
+  p.v_scale = const_cast<Scale*>(v_scale);
   p.slots = slots;
   p.k_out = k;
   p.v_out = v;
@@ -787,16 +794,50 @@ int hxmi_kv_read(int is_bf16, const int8_t* k_codes, const int8_t* v_codes, cons
   p.d = head_dim;
   p.log2_block = log2_block(block_size);
   p.dtype = is_bf16 ? hxmi::DT_BF16 : hxmi::DT_F16;
-  return from_hip(hxmi::launch_kv_read(p, (hipStream_t)stream), name);
+  return from_hip(launch(p, (hipStream_t)stream), name);
 }
 
-int64_t hxmi_kv_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
-                                          int64_t head_dim, int64_t block_size, int64_t width, int ragged) {
+int hxmi_kv_append(int is_bf16, const void* k, const void* v, const int64_t* slots, int8_t* k_codes, int8_t* v_codes,
+                   float* k_scale, float* v_scale, int64_t tokens, int64_t blocks, int64_t kv_heads, int64_t head_dim,
+                   int64_t block_size, int64_t ldk, int64_t head_stride_k, int64_t ldv, int64_t head_stride_v,
+                   void* stream) {
+  return cache_append<hxmi::KvCacheProblem>("hxmi_kv_append", hxmi::launch_kv_append, is_bf16, k, v, slots, k_codes,
+                                            v_codes, k_scale, v_scale, tokens, blocks, kv_heads, head_dim, block_size,
+                                            ldk, head_stride_k, ldv, head_stride_v, stream);
+}
+
+int hxmi_kv4_append(int is_bf16, const void* k, const void* v, const int64_t* slots, uint8_t* k_codes,
+                    uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int64_t tokens, int64_t blocks,
+                    int64_t kv_heads, int64_t head_dim, int64_t block_size, int64_t ldk, int64_t head_stride_k,
+                    int64_t ldv, int64_t head_stride_v, void* stream) {
+  return cache_append<hxmi::Kv4CacheProblem>("hxmi_kv4_append", hxmi::launch_kv4_append, is_bf16, k, v, slots, k_codes,
+                                             v_codes, k_scale, v_scale, tokens, blocks, kv_heads, head_dim, block_size,
+                                             ldk, head_stride_k, ldv, head_stride_v, stream);
+}
+
+int hxmi_kv_read(int is_bf16, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                 const int64_t* slots, void* k, void* v, int64_t tokens, int64_t blocks, int64_t kv_heads,
+                 int64_t head_dim, int64_t block_size, void* stream) {
+  return cache_read<hxmi::KvCacheProblem>("hxmi_kv_read", hxmi::launch_kv_read, is_bf16, k_codes, v_codes, k_scale,
+                                          v_scale, slots, k, v, tokens, blocks, kv_heads, head_dim, block_size, stream);
+}
+
+int hxmi_kv4_read(int is_bf16, const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scale,
+                  const uint8_t* v_scale, const int64_t* slots, void* k, void* v, int64_t tokens, int64_t blocks,
+                  int64_t kv_heads, int64_t head_dim, int64_t block_size, void* stream) {
+  return cache_read<hxmi::Kv4CacheProblem>("hxmi_kv4_read", hxmi::launch_kv4_read, is_bf16, k_codes, v_codes, k_scale,
+                                           v_scale, slots, k, v, tokens, blocks, kv_heads, head_dim, block_size,
+                                           stream);
+}
+
+extern "C++" template <typename P, typename Bytes>
+static int64_t attention_bytes(Bytes bytes, int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
+                               int64_t head_dim, int64_t block_size, int64_t width, int ragged) {
   if (tokens <= 0 || requests <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 ||
       head_dim > 128 || log2_block(block_size) < 0 || width < 0)
     return 0;
   static const int one = 0;
-  hxmi::KvAttnProblem p{};
+  P p{};
   p.tokens = tokens;
   p.requests = requests;
   p.heads = heads;
@@ -805,19 +846,32 @@ int64_t hxmi_kv_attention_workspace_bytes(int64_t tokens, int64_t requests, int6
   p.block = block_size;
   p.width = width;
   p.cu = ragged ? &one : nullptr;
-  return hxmi::kv_attention_workspace_bytes(p);
+  return bytes(p);
 }
 
-int hxmi_kv_attention(int is_bf16, const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
-                      const float* v_scale, const int32_t* block_table, const int32_t* lens, const int32_t* cu,
-                      void* o, int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                      int64_t block_size, int64_t blocks, int64_t width, int64_t ld_table, int64_t ldq,
-                      int64_t head_stride_q, int64_t ldo, int64_t head_stride_o, float scale, void* workspace,
-                      int64_t workspace_bytes, void* stream) {
-  const char* name = "hxmi_kv_attention";
+int64_t hxmi_kv_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
+                                          int64_t head_dim, int64_t block_size, int64_t width, int ragged) {
+  return attention_bytes<hxmi::KvAttnProblem>(hxmi::kv_attention_workspace_bytes, tokens, requests, heads, kv_heads,
+                                              head_dim, block_size, width, ragged);
+}
+
+int64_t hxmi_kv4_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
+                                           int64_t head_dim, int64_t block_size, int64_t width, int ragged) {
+  return attention_bytes<hxmi::Kv4AttnProblem>(hxmi::kv4_attention_workspace_bytes, tokens, requests, heads, kv_heads,
+                                               head_dim, block_size, width, ragged);
+}
+
+extern "C++" template <typename P, typename Code, typename Scale, typename Launch>
+static int cache_attention(const char* name, Launch launch, int is_bf16, const void* q, const Code* k_codes,
+                           const Code* v_codes, const Scale* k_scale, const Scale* v_scale, const int32_t* block_table,
+                           const int32_t* lens, const int32_t* cu, void* o, int64_t tokens, int64_t requests,
+                           int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t block_size, int64_t blocks,
+                           int64_t width, int64_t ld_table, int64_t ldq, int64_t head_stride_q, int64_t ldo,
+                           int64_t head_stride_o, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
   REQUIRE(is_bf16 == 0 || is_bf16 == 1, "%s: is_bf16 must be 0 or 1", name);
   REQUIRE(tokens >= 0 && requests >= 0 && heads >= 0 && width >= 0, "%s: negative size", name);
-  if (const int rc = cache_check(name, k_codes, v_codes, k_scale, v_scale, blocks, kv_heads, head_dim, block_size))
+  if (const int rc = cache_check(name, k_codes, v_codes, k_scale, v_scale, blocks, kv_heads, head_dim, block_size,
+                                 sizeof(Scale) == 1))
     return rc;
   REQUIRE(heads % kv_heads == 0, "%s: heads must be a multiple of kv_heads (%lld, %lld)", name, (long long)heads,
           (long long)kv_heads);
@@ -833,7 +887,7 @@ int hxmi_kv_attention(int is_bf16, const void* q, const int8_t* k_codes, const i
   REQUIRE(ld_table >= width, "%s: ld_table below the table's width", name);
   REQUIRE(ldq >= 0 && head_stride_q >= 0 && ldo >= 0 && head_stride_o >= 0, "%s: negative stride", name);
   REQUIRE(!workspace || al(workspace, 256), "%s: workspace must be 256-byte aligned", name);
-  hxmi::KvAttnProblem p{};
+  P p{};
   p.q = q;
   p.k_codes = k_codes;
   p.v_codes = v_codes;
@@ -860,7 +914,94 @@ int hxmi_kv_attention(int is_bf16, const void* q, const int8_t* k_codes, const i
   p.hso = head_stride_o;
   p.scale = scale;
   p.dtype = is_bf16 ? hxmi::DT_BF16 : hxmi::DT_F16;
-  return from_hip(hxmi::launch_kv_attention(p, (hipStream_t)stream), name);
+  return from_hip(launch(p, (hipStream_t)stream), name);
+}
+
+int hxmi_kv_attention(int is_bf16, const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
+                      const float* v_scale, const int32_t* block_table, const int32_t* lens, const int32_t* cu,
+                      void* o, int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                      int64_t block_size, int64_t blocks, int64_t width, int64_t ld_table, int64_t ldq,
+                      int64_t head_stride_q, int64_t ldo, int64_t head_stride_o, float scale, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  return cache_attention<hxmi::KvAttnProblem>("hxmi_kv_attention", hxmi::launch_kv_attention, is_bf16, q, k_codes,
+                                              v_codes, k_scale, v_scale, block_table, lens, cu, o, tokens, requests,
+                                              heads, kv_heads, head_dim, block_size, blocks, width, ld_table, ldq,
+                                              head_stride_q, ldo, head_stride_o, scale, workspace, workspace_bytes,
+                                              stream);
+}
+
+int hxmi_kv4_attention(int is_bf16, const void* q, const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scale,
+                      const uint8_t* v_scale, const int32_t* block_table, const int32_t* lens, const int32_t* cu,
+                      void* o, int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                      int64_t block_size, int64_t blocks, int64_t width, int64_t ld_table, int64_t ldq,
+                      int64_t head_stride_q, int64_t ldo, int64_t head_stride_o, float scale, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  return cache_attention<hxmi::Kv4AttnProblem>("hxmi_kv4_attention", hxmi::launch_kv4_attention, is_bf16, q, k_codes,
+                                              v_codes, k_scale, v_scale, block_table, lens, cu, o, tokens, requests,
+                                              heads, kv_heads, head_dim, block_size, blocks, width, ld_table, ldq,
+                                              head_stride_q, ldo, head_stride_o, scale, workspace, workspace_bytes,
+                                              stream);
+}
+
+int hxmi_qk_rope(int is_bf16, const void* q, const void* k, void* q_out, void* k_out, const void* positions,
+                 int pos_is_64, const double* inv_freq, const int32_t* axis, const void* q_weight,
+                 const void* k_weight, int weight_is_f32, int64_t tokens, int64_t heads, int64_t kv_heads,
+                 int64_t head_dim, int64_t rotary_dim, int64_t axes, int64_t ld_pos, int64_t ldq,
+                 int64_t head_stride_q, int64_t ldk, int64_t head_stride_k, int64_t ldq_out,
+                 int64_t head_stride_q_out, int64_t ldk_out, int64_t head_stride_k_out, int interleaved, float eps,
+                 float scale, void* stream) {
+  const char* name = "hxmi_qk_rope";
+  REQUIRE((is_bf16 == 0 || is_bf16 == 1) && (pos_is_64 == 0 || pos_is_64 == 1) &&
+              (weight_is_f32 == 0 || weight_is_f32 == 1) && (interleaved == 0 || interleaved == 1),
+          "%s: a flag must be 0 or 1", name);
+  REQUIRE(tokens >= 0 && tokens < (1ll << 31) && heads >= 0 && kv_heads >= 0 && heads + kv_heads < (1 << 20),
+          "%s: bad number of tokens or heads", name);
+  REQUIRE(head_dim > 0 && head_dim % 8 == 0 && head_dim <= hxmi::kRopeMaxDim,
+          "%s: head_dim must be a multiple of 8 up to %lld, got %lld", name, (long long)hxmi::kRopeMaxDim,
+          (long long)head_dim);
+  REQUIRE(rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim,
+          "%s: rotary_dim must be even and at most head_dim, got %lld", name, (long long)rotary_dim);
+  REQUIRE(axes >= 1 && axes < (1 << 20) && (ld_pos >= tokens || axes == 1), "%s: bad number of axes or ld_pos", name);
+  REQUIRE(eps >= 0.f && eps < __builtin_inff() && scale - scale == 0.f, "%s: eps and scale must be finite, eps >= 0", name);
+  REQUIRE(ldq >= 0 && head_stride_q >= 0 && ldk >= 0 && head_stride_k >= 0 && ldq_out >= 0 && head_stride_q_out >= 0 &&
+              ldk_out >= 0 && head_stride_k_out >= 0,
+          "%s: negative stride", name);
+  if (tokens == 0 || heads + kv_heads == 0) return ok();
+  REQUIRE((q && q_out) || !heads, "%s: null q", name);
+  REQUIRE((k && k_out) || !kv_heads, "%s: null k", name);
+  REQUIRE((positions && inv_freq) || !rotary_dim, "%s: null positions or inv_freq", name);
+  hxmi::RopeProblem p{};
+  p.q = q;
+  p.k = k;
+  p.q_out = q_out;
+  p.k_out = k_out;
+  p.positions = positions;
+  p.inv_freq = inv_freq;
+  p.axis = axis;
+  p.q_weight = q_weight;
+  p.k_weight = k_weight;
+  p.tokens = tokens;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.d = head_dim;
+  p.rotary = rotary_dim;
+  p.axes = axes;
+  p.ldp = ld_pos;
+  p.ldq = ldq;
+  p.hsq = head_stride_q;
+  p.ldk = ldk;
+  p.hsk = head_stride_k;
+  p.ldqo = ldq_out;
+  p.hsqo = head_stride_q_out;
+  p.ldko = ldk_out;
+  p.hsko = head_stride_k_out;
+  p.pos64 = pos_is_64;
+  p.w32 = weight_is_f32;
+  p.interleaved = interleaved;
+  p.eps = eps;
+  p.scale = scale;
+  p.dtype = is_bf16 ? hxmi::DT_BF16 : hxmi::DT_F16;
+  return from_hip(hxmi::launch_qk_rope(p, (hipStream_t)stream), name);
 }
 
 int hxmi_sample(int dtype, const void* logits, const float* u, const float* temperature, const int32_t* top_k,

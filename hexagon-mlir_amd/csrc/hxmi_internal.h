@@ -223,11 +223,39 @@ struct KvCacheProblem {
 hipError_t launch_kv_append(const KvCacheProblem& p, hipStream_t stream);
 hipError_t launch_kv_read(const KvCacheProblem& p, hipStream_t stream);
 
-// Attention over the 8-bit cache (kv_attention.hip).
-struct KvAttnProblem {
+// The 4-bit cache (kv4_cache.hip), as the 8-bit one above.
+struct Kv4CacheProblem {
+  uint8_t *k_codes, *v_codes, *k_scale, *v_scale;
+  const int64_t* slots;
+  const void *k, *v;
+  void *k_out, *v_out;
+  int64_t tokens, blocks, kv_heads, d;
+  int64_t ldk, hsk, ldv, hsv;  // row and head strides of k and v
+  int log2_block, dtype;
+};
+hipError_t launch_kv4_append(const Kv4CacheProblem& p, hipStream_t stream);
+hipError_t launch_kv4_read(const Kv4CacheProblem& p, hipStream_t stream);
+
+// Norms of queries and keys, and their rotation (rope.hip).
+struct RopeProblem {
+  const void *q, *k;  // k: with kv_heads 0, none
+  void *q_out, *k_out;
+  const void* positions;
+  const double* inv_freq;
+  const int* axis;                  // of each pair, or null: 0
+  const void *q_weight, *k_weight;  // or null
+  int64_t tokens, heads, kv_heads, d, rotary, axes, ldp;
+  int64_t ldq, hsq, ldk, hsk, ldqo, hsqo, ldko, hsko;
+  int pos64, w32, interleaved;
+  float eps, scale;
+  int dtype;
+};
+constexpr int64_t kRopeMaxDim = 256;
+hipError_t launch_qk_rope(const RopeProblem& p, hipStream_t stream);
+
+// Attention over a cache: all but the cache's own tensors.
+struct KvAttnSizes {
   const void* q;
-  const int8_t *k_codes, *v_codes;
-  const float *k_scale, *v_scale;
   const int *table, *lens;
   const int* cu;  // null: one row a request
   void* o;
@@ -238,8 +266,19 @@ struct KvAttnProblem {
   float scale;
   int dtype;
 };
+// Over the 8-bit cache (kv_attention.hip).
+struct KvAttnProblem : KvAttnSizes {
+  const int8_t *k_codes, *v_codes;
+  const float *k_scale, *v_scale;
+};
 int64_t kv_attention_workspace_bytes(const KvAttnProblem& p);
 hipError_t launch_kv_attention(const KvAttnProblem& p, hipStream_t stream);
+// Over the 4-bit cache (kv4_attention.hip).
+struct Kv4AttnProblem : KvAttnSizes {
+  const uint8_t *k_codes, *v_codes, *k_scale, *v_scale;
+};
+int64_t kv4_attention_workspace_bytes(const Kv4AttnProblem& p);
+hipError_t launch_kv4_attention(const Kv4AttnProblem& p, hipStream_t stream);
 
 // A token a row from logits (sample.hip).
 constexpr int64_t kSampleMaxVocab = 1 << 20;

@@ -1,0 +1,423 @@
+// Attention over the 4-bit key/value cache (numbers and layout: kv4.h), causal over
+// ragged requests, grouped heads: row i of a request with n rows and L tokens
+// in the cache sees keys j <= L - n + i,
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q . k_j - max).
+//
+// A workgroup of four waves owns a tile of 16 rows (token, head of the group) of
+// one key/value head and, where there are few such tiles, one of `nsplit`
+// shares of the keys.  The waves take every fourth group of 64 keys; numbers go
+// from memory straight to registers, and what the cache holds is exact in fp16
+// (number * scale, two instructions for two values), so both products take it
+// as it is:
+//   * scores as D[key][row] = K . Q^T (16x16x32 MFMAs).  The dims of a step may
+//     come in any order, so a lane takes 16 (of 64) or 32 (of 128) dims of a key
+//     that lie together, under one scale.  Row m of tile t is key 4 m + t of the
+//     group: a lane's four keys have their scales in one word, and its 16 scores
+//     (row l % 16, g = l / 16) are keys 16 g .. 16 g + 15, one page's;
+//   * those 16 weights are the B operand of P.V as they are.  A lane's V numbers
+//     are two dims of those 16 tokens, tiles 2 c and 2 c + 1 of 32 dims (row m is
+//     dim 2 m or 2 m + 1), so that a lane ends with eight dims that lie together;
+//   * q in bf16 is brought to fp16 under a power of two a row: multiples of 2^-38
+//     of its largest element;
+//   * weights are relative to 2^m, m from 7 to 15 below the running maximum, in
+//     11 bits or multiples of 2^-31 of the row's largest (fp16 below 2^-14);
+//     scores, maxima, sums and O are fp32.
+#include "kv4.h"
+#include "kv_attention_impl.h"
+
+namespace hxmi {
+namespace {
+
+using namespace kv4;
+
+struct KArgs : TileArgs {
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  int64_t sbytes;  // of a block's scales of one head
+};
+
+// Weights are 2^(score - m): m stays until a score is more than kHigh above it,
+// then follows to kLow below the largest.
+constexpr float kLow = 7.f, kHigh = 15.f;
+
+// Eight numbers times their scales (pairs) as one MFMA operand.
+template <typename F>
+__device__ __forceinline__ half8v operand(uint32_t w, F&& scale) {
+  const half2v a = numbers<0>(w) * scale(0), b = numbers<1>(w) * scale(1), c = numbers<2>(w) * scale(2),
+               d = numbers<3>(w) * scale(3);
+  return half8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// Scales of eight values in a row (words w0 and w1), pair by pair.
+struct Pairs {
+  half2v p[4];
+  __device__ __forceinline__ Pairs(uint32_t w0, uint32_t w1)
+      : p{scale_pair<0>(w0), scale_pair<1>(w0), scale_pair<0>(w1), scale_pair<1>(w1)} {}
+};
+// Bytes of word x (of four) that belong to the first n of 16.
+__device__ __forceinline__ uint32_t first_bytes(int n, int x) {
+  const int c = min(max(n - 4 * x, 0), 4);
+  return c == 4 ? ~0u : (1u << (8 * c)) - 1;
+}
+
+// Bytes of a word of scales that hold no finite number (kv4_append writes none), as 255.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  const uint32_t e = ((w >> 3) & 0x1f1f1f1fu) ^ 0x1f1f1f1fu;  // 0 where all exponent bits are set
+  return ((~(e + 0x1f1f1f1fu) & 0x20202020u) >> 5) * 255u;
+}
+
+// What a wave knows of its 16 rows: O and the sum of the weights (this lane's part).
+template <int DT>
+struct Partial {
+  static constexpr int N = DT * 4 + 2;  // floats a lane
+  float4v o[DT];
+  float m, l;
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = float4v{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+  }
+  // Every float becomes f(its index, it).
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[t][i] = f(t * 4 + i, o[t][i]);
+    m = f(DT * 4, m);
+    l = f(DT * 4 + 1, l);
+  }
+  template <int M>
+  __device__ __forceinline__ void add(const Partial (&p)[M]) {
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < M; ++j) top = fmaxf(top, p[j].m);
+    const float f = rel_exp2(m, top);
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] *= f;
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const float g = rel_exp2(p[j].m, top);
+      l += p[j].l * g;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][i] += p[j].o[t][i] * g;
+    }
+  }
+};
+
+// DC: 64-dim pieces of a row; WHOLE: the head dim is 64 * DC.
+template <typename T, int DC, bool WHOLE>
+__global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
+  constexpr int DT = DC * 4, G = DC * 2, RT = 16, NV = Partial<DT>::N, KD = 16 * DC;  // KD: dims of a lane's keys
+  constexpr bool BF16 = !std::is_same_v<T, _Float16>;
+  __shared__ __attribute__((aligned(16))) float joined[3 * NV * 64];
+  __shared__ int last_split;
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+
+  const Share part = share_of(a);
+  const int split = part.split, nsplit = part.count, item = part.item;
+  const int kvh = item / a.tiles;
+  Rows tile;
+  if (!rows_of<RT>(a, item - kvh * a.tiles, tile)) return;
+  const int r = tile.r, first = tile.first, n = tile.n, row0 = tile.row0, len = tile.len;
+  const int64_t nrows = tile.count;
+
+  // This lane's row (past the last one: the last one's q, not stored)
+  const int64_t row = (int64_t)row0 + lr, rowq = min(row, nrows - 1);
+  const int token = (int)(rowq / a.group), head = kvh * a.group + (int)(rowq - (int64_t)token * a.group);
+  const int last = (int)min((int64_t)len - n + token, (int64_t)len - 1);  // the last key it sees
+  half8v qf[2 * DC];
+  float c = a.c;
+  {
+    const T* q = (const T*)a.q + (int64_t)(first + token) * a.ldq + (int64_t)head * a.hq;
+    T raw[2 * DC][8];
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2 * DC; ++s) {
+      const int d = lg * KD + s * 8;
+      int4v v{};
+      if (WHOLE || d < a.d) v = *(const int4u*)(q + d);
+      __builtin_memcpy(raw[s], &v, 16);
+      if constexpr (BF16) top = largest(raw[s], top);
+    }
+    const int ex = BF16 ? exponent_of(row_max(top)) : 0;
+    if constexpr (BF16) c = __builtin_ldexpf(a.c, -ex);
+#pragma unroll
+    for (int s = 0; s < 2 * DC; ++s) qf[s] = q_operand(raw[s], ex);
+  }
+
+  // keys this tile / all of its rows see
+  const int i1 = (int)min((int64_t)n - 1, ((int64_t)row0 + RT - 1) / a.group);
+  const int kend = max(0, min(len, len - n + i1 + 1));
+  const int kfull = max(0, min(len, len - n + row0 / a.group + 1));
+  const int groups = (kend + 63) >> 6, share = (groups + nsplit - 1) / nsplit;
+  const int g1 = min(groups, (split + 1) * share);
+
+  Partial<DT> acc;
+  acc.clear();
+
+  const int ck = lr >> 2;  // 16-key piece of a group that this lane's K rows lie in (V's and the scores': lg)
+  const int* const table = a.table + (int64_t)r * a.ldt;
+  const int64_t hb = (int64_t)kvh * a.bytes, kv_bytes = (int64_t)a.kv_heads * a.bytes;
+  const int pm = (1 << a.lb) - 1;  // 16-key pieces of a page, less one
+  // The block of 16-key piece `piece`, -1 where there is none or a bad one.
+  auto page = [&](int piece) {
+    const int p = piece >> a.lb;
+    const int b = p < a.width && piece * 16 < kend ? table[p] : -1;
+    return (unsigned)b < (unsigned)a.blocks ? b : -1;
+  };
+  uint32_t kr[4][2 * DC], ksw = 0;
+  int4v vr[G], vsw[G];
+  bool there;
+  // (a piece that is not there reads block 0's numbers, which its mask leaves out)
+  auto load_k = [&](int g, int b) {
+    const int64_t blk = max(b, 0);
+    const int at = ((4 * g + ck) & pm) * 16 + 4 * (lr & 3);
+    const uint8_t* p = a.k + blk * kv_bytes + hb + (int64_t)at * (a.dp >> 1) + lg * (KD / 2);
+    const bool in = WHOLE || lg * KD < a.dp;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if constexpr (DC == 1) {
+        const uint2 v = in ? *(const uint2*)(p + t * (a.dp >> 1)) : uint2{};
+        kr[t][0] = v.x;
+        kr[t][1] = v.y;
+      } else {
+        const uint4 v = in ? *(const uint4*)(p + t * (a.dp >> 1)) : uint4{};
+        kr[t][0] = v.x;
+        kr[t][1] = v.y;
+        kr[t][2] = v.z;
+        kr[t][3] = v.w;
+      }
+    }
+    if (in) ksw = *(const uint32_t*)(a.ks + (blk * a.kv_heads + kvh) * a.sbytes + ((int64_t)(lg * KD / 32) << (a.lb + 4)) + at);
+  };
+  auto load_v = [&](int g, int b) {
+    const int64_t blk = max(b, 0);
+    const int piece = (4 * g + lg) & pm;
+    const uint8_t* p = a.v + blk * kv_bytes + hb + ((int64_t)piece * a.dp + 2 * lr) * 8;
+    const uint8_t* s = a.vs + (blk * a.kv_heads + kvh) * a.sbytes + piece * 16;
+#pragma unroll
+    for (int x = 0; x < G; ++x) {
+      const bool in = WHOLE || x * 32 < a.dp;
+      vr[x] = in ? *(const int4v*)(p + x * 256) : int4v{};
+      vsw[x] = in ? *(const int4v*)(s + ((int64_t)x << (a.lb + 4))) : int4v{};
+    }
+    there = b >= 0;
+  };
+
+  int g = split * share + w, bk2 = -1, bv2 = -1;
+  if (g < g1) {
+    const int bk = page(4 * g + ck), bv = page(4 * g + lg);
+    load_k(g, bk);
+    load_v(g, bv);
+    if (g + 4 < g1) {
+      bk2 = page(4 * (g + 4) + ck);
+      bv2 = page(4 * (g + 4) + lg);
+    }
+  }
+  for (; g < g1; g += 4) {
+    // scores
+    float4v s[4];
+    static_for<4>([&](auto t) {
+      const half2v sc = scale_twice<t>(ksw);
+#pragma unroll
+      for (int x = 0; x < 2 * DC; ++x)
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(kr[t][x], [&](int) { return sc; }), qf[x],
+                                                      x == 0 ? float4v{0.f, 0.f, 0.f, 0.f} : s[t], 0, 0, 0);
+    });
+    const bool more = g + 4 < g1;
+    const bool there0 = there;
+    if (more) load_k(g + 4, bk2);
+    // softmax
+    const bool whole = g * 64 + 64 <= kfull && __all(there0);  // (wave-uniform)
+    float mx = -INFINITY;
+    if (!whole) {
+      const int left = there0 ? last - (g * 64 + lg * 16) : -1;  // keys of this lane up to this one are seen
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][i] = 4 * i + t > left ? -INFINITY : s[t][i];
+      // A weight of 0 has to leave nothing behind whatever the scale is: those of
+      // keys past all rows' are 0, and so are others that are not finite, which
+      // make the rows that see them NaN by their sum.
+      const int held = there0 ? kend - (g * 64 + lg * 16) : 0;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t mask = first_bytes(held, y);
+        uint32_t bad = 0;
+#pragma unroll
+        for (int x = 0; x < G; ++x) {
+          const uint32_t b = not_finite((uint32_t)vsw[x][y]) & mask;
+          vsw[x][y] &= (int)(mask & ~b);
+          bad |= b;
+        }
+        if (bad & first_bytes(left + 1, y)) acc.l = NAN;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
+    mx = row_max(mx) * c;  // (c > 0)
+    if (__any(mx > acc.m + kHigh)) {
+      const float now = mx > acc.m + kHigh ? mx - kLow : acc.m, f = rel_exp2(acc.m, now);
+      acc.m = now;
+      acc.l *= f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) acc.o[t] *= f;
+    }
+    const float off = acc.m == -INFINITY ? 0.f : -acc.m;
+    half8v p[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[j & 3][2 * u + (j >> 2)], c, off));
+        acc.l += e;
+        p[u][j] = (_Float16)e;
+      }
+    // values
+#pragma unroll
+    for (int x = 0; x < G; ++x) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const Pairs sc((uint32_t)vsw[x][2 * u], (uint32_t)vsw[x][2 * u + 1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          acc.o[2 * x + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              operand((uint32_t)vr[x][2 * e + u], [&](int i) { return sc.p[i]; }), p[u], acc.o[2 * x + e], 0, 0, 0);
+      }
+    }
+    if (more) {
+      load_v(g + 4, bv2);
+      if (g + 8 < g1) {
+        bk2 = page(4 * (g + 8) + ck);
+        bv2 = page(4 * (g + 8) + lg);
+      }
+    }
+  }
+
+  // Join the waves' parts: waves 1..3 through LDS into wave 0.
+  auto join = [&]() {
+    __syncthreads();
+    if (w > 0) acc.each([&](int i, float v) { return joined[((w - 1) * NV + i) * 64 + lane] = v; });
+    __syncthreads();
+    if (w > 0) return;
+    Partial<DT> other[3];
+#pragma unroll
+    for (int o = 0; o < 3; ++o) other[o].each([&](int i, float) { return joined[(o * NV + i) * 64 + lane]; });
+    acc.add(other);
+  };
+  join();
+
+  if (nsplit > 1) {
+    // Every share stores its part (system-coherent stores, visible to every
+    // XCD once vmcnt drains) and arrives on the tile's counter; the last one
+    // joins them.
+    constexpr int kCoherent = 17;  // sc0 | sc1
+    constexpr int PART = NV * 64 * 4;
+    const __amdgpu_buffer_rsrc_t rP =
+        make_rsrc(a.ws + kWsCounterBytes + (int64_t)(item - a.full) * nsplit * PART, (uint32_t)(nsplit * PART));
+    if (w == 0) {
+      acc.each([&](int i, float v) {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rP, (uint32_t)(split * PART + (i * 64 + lane) * 4), 0,
+                                              kCoherent);
+        return v;
+      });
+      wait_vmcnt0();
+      if (lane == 0) {
+        unsigned long long* cnt = (unsigned long long*)a.ws + (item - a.full);  // < kWsMaxTiles (the host's check)
+        const unsigned long long before =
+            __hip_atomic_fetch_add(cnt, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last_split = before + 1 == (unsigned long long)nsplit;
+        if (last_split) __hip_atomic_store(cnt, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+    __syncthreads();
+    if (!last_split) return;
+    acc.clear();
+    for (int sp = w; sp < nsplit; sp += 4) {  // (in this order whichever came last)
+      Partial<DT> other[1];
+      other[0].each([&](int i, float) {
+        return __uint_as_float(
+            __builtin_amdgcn_raw_buffer_load_b32(rP, (uint32_t)(sp * PART + (i * 64 + lane) * 4), 0, kCoherent));
+      });
+      acc.add(other);
+    }
+    join();
+  }
+  if (w > 0) return;
+
+  // O: lane holds row l % 16, dims 32 x + 8 (l / 16) + 0..7
+  const float l = row_reduce(acc.l, [](float y, float z) { return y + z; });
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  if (row >= nrows) return;
+  T* const o = (T*)a.o + (int64_t)(first + token) * a.ldo + (int64_t)head * a.ho;
+#pragma unroll
+  for (int x = 0; x < G; ++x) {
+    const int d = x * 32 + lg * 8;
+    if (!WHOLE && d >= a.d) continue;
+    T o8[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o8[j] = (T)(acc.o[2 * x + (j & 1)][j >> 1] * f);
+    int4v bits;
+    __builtin_memcpy(&bits, o8, 16);
+    *(int4u*)(o + d) = bits;
+  }
+}
+
+int64_t part_bytes(const KvAttnSizes& p, const KvPlan& k) {  // of a tile's share
+  const int64_t dt = p.d <= 64 ? 4 : 8;
+  return (dt * 4 + 2) * 64 * 4;
+}
+KvPlan plan4_of(const KvAttnSizes& p) { return plan_of(p, false); }
+
+template <typename T>
+hipError_t launch_t(int64_t d, int rt, dim3 grid, const KArgs& a, hipStream_t stream) {
+  const bool small = d <= 64, whole = d == 64 || d == 128;
+  const auto fn = small ? whole ? kv4_attention<T, 1, true> : kv4_attention<T, 1, false>
+                        : whole ? kv4_attention<T, 2, true> : kv4_attention<T, 2, false>;
+  hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t kv4_attention_workspace_bytes(const Kv4AttnProblem& p) {
+  const KvPlan k = plan4_of(p);
+  return k.nsplit > 1 ? kWsCounterBytes + (k.tiles * p.kv_heads - k.full) * k.nsplit * part_bytes(p, k) : 0;
+}
+
+hipError_t launch_kv4_attention(const Kv4AttnProblem& p, hipStream_t stream) {
+  KvPlan k = plan4_of(p);
+  const int64_t items = k.tiles * p.kv_heads;
+  if (k.nsplit > 1 && (!p.ws || p.ws_bytes < kv4_attention_workspace_bytes(p))) {
+    k.nsplit = 1;
+    k.full = items;
+  }
+  const int64_t grid = k.full + (items - k.full) * k.nsplit;
+  static_assert(512 <= kWsMaxTiles, "a counter for every shared tile");
+  if (grid >= (1ll << 31)) return hipErrorInvalidValue;
+  KArgs a{};
+  a.k = p.k_codes;
+  a.v = p.v_codes;
+  a.ks = p.k_scale;
+  a.vs = p.v_scale;
+  a.dp = (int)((p.d + 31) / 32 * 32);
+  a.bytes = p.block * a.dp / 2;
+  a.sbytes = p.block * a.dp / 32;
+  tile_args(p, k, a);
+  const dim3 blocks((unsigned)grid);
+  return p.dtype == DT_BF16 ? launch_t<__bf16>(p.d, k.rt, blocks, a, stream) : launch_t<_Float16>(p.d, k.rt, blocks, a, stream);
+}
+
+}  // namespace hxmi

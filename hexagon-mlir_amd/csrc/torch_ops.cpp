@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/hxmi.h"
 
@@ -489,8 +490,11 @@ PyObject* op_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// The tensors of a cache: (k, v, k_scale, v_scale, head_dim) from args[0] on.
+// The tensors of a cache of 8 or (FOUR) 4 bits: (k, v, k_scale, v_scale, head_dim) from args[0] on.
+template <bool FOUR>
 struct Cache {
+  using Code = std::conditional_t<FOUR, uint8_t, int8_t>;
+  using Scale = std::conditional_t<FOUR, uint8_t, float>;
   const Tensor *k, *v, *ks, *vs;
   long d = 0;
   int64_t blocks = 0, heads = 0, block = 0;
@@ -498,17 +502,23 @@ struct Cache {
 
   Cache(Operands& in, PyObject* const* args)
       : k(in.get(args[0])), v(in.get(args[1])), ks(in.get(args[2])), vs(in.get(args[3])) {
-    if (!in.ok || !number(args[4], d) || k->dim() != 4 || k->scalar_type() != at::kChar ||
-        v->scalar_type() != at::kChar || ks->scalar_type() != at::kFloat || vs->scalar_type() != at::kFloat)
+    constexpr at::ScalarType codes = FOUR ? at::kByte : at::kChar, scales = FOUR ? at::kByte : at::kFloat;
+    if (!in.ok || !number(args[4], d) || k->dim() != 4 || k->scalar_type() != codes || v->scalar_type() != codes ||
+        ks->scalar_type() != scales || vs->scalar_type() != scales)
       return;
     blocks = k->size(0);
     heads = k->size(1);
     block = k->size(2);
-    const int64_t dp = (d + 15) / 16 * 16;
-    ok = heads > 0 && k->size(3) == dp && v->sizes() == at::IntArrayRef({blocks, heads, block / 16, dp, 16}) &&
-         ks->sizes() == at::IntArrayRef({blocks, heads}) && vs->sizes() == ks->sizes() && k->is_contiguous() &&
-         v->is_contiguous() && ks->is_contiguous() && vs->is_contiguous();
+    const int64_t dp = FOUR ? (d + 31) / 32 * 32 : (d + 15) / 16 * 16;
+    ok = heads > 0 && k->size(3) == (FOUR ? dp / 2 : dp) &&
+         v->sizes() == at::IntArrayRef({blocks, heads, block / 16, dp, FOUR ? 8 : 16}) &&
+         (FOUR ? ks->sizes() == at::IntArrayRef({blocks, heads, dp / 32, block})
+               : ks->sizes() == at::IntArrayRef({blocks, heads})) &&
+         vs->sizes() == ks->sizes() && k->is_contiguous() && v->is_contiguous() && ks->is_contiguous() &&
+         vs->is_contiguous();
   }
+  Code* codes(const Tensor* t) const { return (Code*)ptr(t); }
+  Scale* scales(const Tensor* t) const { return (Scale*)ptr(t); }
 };
 
 // Rows [tokens, heads, d] with unit last stride.
@@ -555,11 +565,12 @@ PyObject* op_kv_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // kv_append(*cache, k, v, slots): True once done
-PyObject* op_kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+template <bool FOUR>
+PyObject* kv_append(PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   NOT_PLAIN_UNLESS(n == 8);
   Operands in;
-  const Cache c(in, args);
+  const Cache<FOUR> c(in, args);
   const Tensor *k = in.get(args[5]), *v = in.get(args[6]), *slots = in.get(args[7]);
   NOT_PLAIN_UNLESS(in.ok && c.ok && half_type(*k) && v->scalar_type() == k->scalar_type() &&
                    head_rows(*k, c.heads, c.d) && head_rows(*v, c.heads, c.d) && v->size(0) == k->size(0) &&
@@ -567,9 +578,13 @@ PyObject* op_kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const c10::DeviceGuard guard(k->device());
   void* s = in.stream();
   const int rc = unlocked([&] {
-    return hxmi_kv_append(bf16(*k), ptr(k), ptr(v), (const int64_t*)ptr(slots), (int8_t*)ptr(c.k), (int8_t*)ptr(c.v),
-                          (float*)ptr(c.ks), (float*)ptr(c.vs), k->size(0), c.blocks, c.heads, c.d, c.block,
-                          k->stride(0), k->stride(1), v->stride(0), v->stride(1), s);
+    const auto call = [&](auto fn) {
+      return fn(bf16(*k), ptr(k), ptr(v), (const int64_t*)ptr(slots), c.codes(c.k), c.codes(c.v), c.scales(c.ks),
+                c.scales(c.vs), k->size(0), c.blocks, c.heads, c.d, c.block, k->stride(0), k->stride(1), v->stride(0),
+                v->stride(1), s);
+    };
+    if constexpr (FOUR) return call(hxmi_kv4_append);
+    else return call(hxmi_kv_append);
   });
   if (rc != HXMI_OK) Py_RETURN_NONE;
   Py_RETURN_TRUE;
@@ -577,11 +592,12 @@ PyObject* op_kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // kv_read(*cache, slots, bf16)
-PyObject* op_kv_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+template <bool FOUR>
+PyObject* kv_read(PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   NOT_PLAIN_UNLESS(n == 7);
   Operands in;
-  const Cache c(in, args);
+  const Cache<FOUR> c(in, args);
   const Tensor* slots = in.get(args[5]);
   NOT_PLAIN_UNLESS(in.ok && c.ok && slots->dim() == 1 && vec(slots, slots->size(0), at::kLong));
   const bool b16 = PyObject_IsTrue(args[6]);
@@ -590,9 +606,12 @@ PyObject* op_kv_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor k = fresh(*slots, {T, c.heads, c.d}, b16 ? at::kBFloat16 : at::kHalf), v = at::empty_like(k);
   void* s = in.stream();
   const int rc = unlocked([&] {
-    return hxmi_kv_read(b16, (const int8_t*)ptr(c.k), (const int8_t*)ptr(c.v), (const float*)ptr(c.ks),
-                        (const float*)ptr(c.vs), (const int64_t*)ptr(slots), ptr(&k), ptr(&v), T, c.blocks, c.heads, c.d,
-                        c.block, s);
+    const auto call = [&](auto fn) {
+      return fn(b16, c.codes(c.k), c.codes(c.v), c.scales(c.ks), c.scales(c.vs), (const int64_t*)ptr(slots), ptr(&k),
+                ptr(&v), T, c.blocks, c.heads, c.d, c.block, s);
+    };
+    if constexpr (FOUR) return call(hxmi_kv4_read);
+    else return call(hxmi_kv_read);
   });
   if (rc != HXMI_OK) Py_RETURN_NONE;
   return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
@@ -600,12 +619,13 @@ PyObject* op_kv_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // kv_attention(q, *cache, table, lens, cu or None, scale or None, out or None): an out apart from every operand
-PyObject* op_kv_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+template <bool FOUR>
+PyObject* kv_attention(PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   NOT_PLAIN_UNLESS(n == 11);
   Operands in;
   const Tensor* q = in.get(args[0]);
-  const Cache c(in, args + 1);
+  const Cache<FOUR> c(in, args + 1);
   const Tensor *tab = in.get(args[6]), *lens = in.get(args[7]), *cu = in.get(args[8], true), *o = in.get(args[10], true);
   NOT_PLAIN_UNLESS(in.ok && c.ok && half_type(*q) && q->dim() == 3 && q->size(1) % c.heads == 0 &&
                    head_rows(*q, q->size(1), c.d) && lens->dim() == 1);
@@ -620,18 +640,98 @@ PyObject* op_kv_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
                           !(cu && overlap(*o, *cu))));
   const c10::DeviceGuard guard(q->device());
   const Tensor out = o ? *o : like(*q, q->sizes());
-  const Workspace ws(hxmi_kv_attention_workspace_bytes(T, R, H, c.heads, c.d, c.block, tab->size(1), cu != nullptr), *q);
+  const Workspace ws((FOUR ? hxmi_kv4_attention_workspace_bytes : hxmi_kv_attention_workspace_bytes)(
+                         T, R, H, c.heads, c.d, c.block, tab->size(1), cu != nullptr),
+                     *q);
   if (!ws.ok) return nullptr;
   void* s = in.stream();
   return result(unlocked([&] {
-                  return hxmi_kv_attention(bf16(*q), ptr(q), (const int8_t*)ptr(c.k), (const int8_t*)ptr(c.v),
-                                           (const float*)ptr(c.ks), (const float*)ptr(c.vs), (const int32_t*)ptr(tab),
-                                           (const int32_t*)ptr(lens), (const int32_t*)ptr(cu), ptr(&out), T, R, H,
-                                           c.heads, c.d, c.block, c.blocks, tab->size(1), ldt, q->stride(0),
-                                           q->stride(1), out.stride(0), out.stride(1), (float)scale, ws.data, ws.bytes,
-                                           s);
+                  const auto call = [&](auto fn) {
+                    return fn(bf16(*q), ptr(q), c.codes(c.k), c.codes(c.v), c.scales(c.ks), c.scales(c.vs),
+                              (const int32_t*)ptr(tab), (const int32_t*)ptr(lens), (const int32_t*)ptr(cu), ptr(&out), T,
+                              R, H, c.heads, c.d, c.block, c.blocks, tab->size(1), ldt, q->stride(0), q->stride(1),
+                              out.stride(0), out.stride(1), (float)scale, ws.data, ws.bytes, s);
+                  };
+                  if constexpr (FOUR) return call(hxmi_kv4_attention);
+                  else return call(hxmi_kv_attention);
                 }),
                 out);
+  END_HANDLE_TH_ERRORS
+}
+
+// The two kinds of cache.
+#define CACHE_OP(name)                                                                                            \
+  PyObject* op_kv_##name(PyObject*, PyObject* const* args, Py_ssize_t n) { return kv_##name<false>(args, n); } \
+  PyObject* op_kv4_##name(PyObject*, PyObject* const* args, Py_ssize_t n) { return kv_##name<true>(args, n); }
+CACHE_OP(append)
+CACHE_OP(read)
+CACHE_OP(attention)
+
+// Rows [tokens, heads, d] with unit last stride, strides as the C ABI takes them, that share no elements.
+bool own_head_rows(const Tensor& t) {
+  const int64_t T = t.size(0), H = t.size(1), d = t.size(2), s0 = t.stride(0), s1 = t.stride(1);
+  return t.stride(2) == 1 && (T == 1 || s0 >= (H - 1) * s1 + d || (s0 >= d && (H == 1 || s1 >= (T - 1) * s0 + d))) &&
+         (H == 1 || s1 >= d);
+}
+// Two ranges of heads of the same rows.
+bool heads_apart(const Tensor& a, const Tensor& b) {
+  const int64_t row = a.stride(0), size = (int64_t)a.element_size();
+  const int64_t by = ((intptr_t)b.data_ptr() - (intptr_t)a.data_ptr()) / size, at = ((by % row) + row) % row;
+  return b.stride(0) == row && at >= (a.size(1) - 1) * a.stride(1) + a.size(2) &&
+         at + (b.size(1) - 1) * b.stride(1) + b.size(2) <= row;
+}
+
+// qk_rope(q, k or None, positions, inv_freq, axis or None, scale, q_weight or None, k_weight or None, eps, interleaved,
+// q_out or None, k_out or None): outputs that are new or the operands themselves
+PyObject* op_qk_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NOT_PLAIN_UNLESS(n == 12);
+  Operands in;
+  const Tensor *q = in.get(args[0]), *k = in.get(args[1], true), *pos = in.get(args[2]), *freq = in.get(args[3]),
+               *axis = in.get(args[4], true), *qw = in.get(args[6], true), *kw = in.get(args[7], true),
+               *oq = in.get(args[10], true), *ok = in.get(args[11], true);
+  double scale, eps;
+  NOT_PLAIN_UNLESS(in.ok && number(args[5], scale) && number(args[8], eps) && PyBool_Check(args[9]));
+  NOT_PLAIN_UNLESS(half_type(*q) && q->dim() == 3 && q->stride(2) == 1 && q->numel() > 0);
+  const int64_t T = q->size(0), H = q->size(1), d = q->size(2), K = k ? k->size(k->dim() > 1 ? 1 : 0) : 0;
+  NOT_PLAIN_UNLESS(!k || (k->dim() == 3 && k->size(0) == T && k->size(2) == d && k->stride(2) == 1 &&
+                          k->scalar_type() == q->scalar_type() && K > 0));
+  NOT_PLAIN_UNLESS(freq->dim() == 1 && vec(freq, freq->size(0), at::kDouble));
+  const int64_t pairs = freq->size(0);
+  const bool wide = pos->scalar_type() == at::kLong;
+  NOT_PLAIN_UNLESS((wide || pos->scalar_type() == at::kInt) && pos->is_contiguous() &&
+                   (pos->dim() == 1 || (pos->dim() == 2 && (axis ? pos->size(0) > 0 : pos->size(0) == 1))) &&
+                   pos->size(-1) == T && vec(axis, pairs, at::kInt));
+  const at::ScalarType wt = qw ? qw->scalar_type() : kw ? kw->scalar_type() : at::kFloat;
+  NOT_PLAIN_UNLESS((wt == at::kFloat || wt == q->scalar_type()) && vec(qw, d, wt) && vec(kw, d, wt));
+  // (in place: nothing else that is read may lie in the outputs)
+  const bool placed = oq || ok;
+  NOT_PLAIN_UNLESS(!placed || (oq && (ok != nullptr) == (k != nullptr) && oq->data_ptr() == q->data_ptr() &&
+                               oq->sizes() == q->sizes() && oq->strides() == q->strides() &&
+                               oq->scalar_type() == q->scalar_type() && own_head_rows(*oq) && q->stride(0) > 0));
+  NOT_PLAIN_UNLESS(!ok || (ok->data_ptr() == k->data_ptr() && ok->sizes() == k->sizes() &&
+                           ok->strides() == k->strides() && ok->scalar_type() == k->scalar_type() &&
+                           own_head_rows(*ok) && (!overlap(*q, *k) || heads_apart(*q, *k))));
+  if (placed)
+    for (const Tensor* o : {oq, ok})
+      for (const Tensor* t : {pos, freq, axis, qw, kw})
+        NOT_PLAIN_UNLESS(!o || !t || t->numel() == 0 || !overlap(*o, *t));
+  const c10::DeviceGuard guard(q->device());
+  const Tensor yq = oq ? *oq : like(*q, q->sizes());
+  Tensor yk;
+  if (k) yk = ok ? *ok : like(*k, k->sizes());
+  void* s = in.stream();
+  const bool next = args[9] == Py_True;
+  const int rc = unlocked([&] {
+    return hxmi_qk_rope(bf16(*q), ptr(q), ptr(k), ptr(&yq), k ? ptr(&yk) : nullptr, ptr(pos), wide,
+                        (const double*)ptr(freq), (const int32_t*)ptr(axis), ptr(qw), ptr(kw), wt == at::kFloat, T, H, K,
+                        d, 2 * pairs, pos->dim() == 2 ? pos->size(0) : 1, T, q->stride(0), q->stride(1),
+                        k ? k->stride(0) : 0, k ? k->stride(1) : 0, yq.stride(0), yq.stride(1), k ? yk.stride(0) : 0,
+                        k ? yk.stride(1) : 0, next, (float)eps, (float)scale, s);
+  });
+  if (rc != HXMI_OK) Py_RETURN_NONE;
+  if (!k) return Py_BuildValue("(NO)", THPVariable_Wrap(yq), Py_None);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(yq), THPVariable_Wrap(yk));
   END_HANDLE_TH_ERRORS
 }
 
@@ -680,6 +780,7 @@ PyObject* op_sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef kMethods[] = {ENTRY(gemm),         ENTRY(bgemm),    ENTRY(linear),  ENTRY(rms_norm_linear), ENTRY(gemv),
                           ENTRY(w8a16_linear), ENTRY(rms_norm), ENTRY(softmax), ENTRY(attention),
                           ENTRY(kv_plan),      ENTRY(kv_append), ENTRY(kv_read), ENTRY(kv_attention),  ENTRY(sample),
+                          ENTRY(kv4_append),   ENTRY(kv4_read), ENTRY(kv4_attention), ENTRY(qk_rope),
                           {"set_workspace", set_workspace, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "hxmi_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

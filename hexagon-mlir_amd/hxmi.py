@@ -16,7 +16,7 @@ import importlib.util
 import math
 import pathlib
 import warnings
-from typing import NamedTuple, Optional, Union
+from typing import NamedTuple, Optional, Sequence, Union
 
 import torch
 
@@ -75,6 +75,11 @@ SIGNATURES = {
     "hxmi_kv_read": ([_I] + [_P] * 7 + [_I64] * 5 + [_P], _I),
     "hxmi_kv_attention": ([_I] + [_P] * 9 + [_I64] * 13 + [_F, _P, _I64, _P], _I),
     "hxmi_kv_attention_workspace_bytes": ([_I64] * 7 + [_I], _I64),
+    "hxmi_kv4_append": ([_I] + [_P] * 7 + [_I64] * 9 + [_P], _I),
+    "hxmi_kv4_read": ([_I] + [_P] * 7 + [_I64] * 5 + [_P], _I),
+    "hxmi_kv4_attention": ([_I] + [_P] * 9 + [_I64] * 13 + [_F, _P, _I64, _P], _I),
+    "hxmi_kv4_attention_workspace_bytes": ([_I64] * 7 + [_I], _I64),
+    "hxmi_qk_rope": ([_I] + [_P] * 5 + [_I] + [_P] * 4 + [_I] + [_I64] * 15 + [_I, _F, _F, _P], _I),
     "hxmi_sample": ([_I] + [_P] * 6 + [_F, ctypes.c_int32, _F, _F, _P] + [_I64] * 3 + [_P], _I),
     "hxmi_lwp_record": ([_P, _I64, ctypes.c_uint32, _P], _I),
     "hxmi_lwp_clock_hz": ([], _I64),
@@ -968,7 +973,172 @@ def decode_status(device: Optional[torch.device] = None, clear: bool = True) -> 
     return status
 
 
-# ---- serving: an 8-bit key/value cache, attention over it, sampling ---------------------
+# ---- serving: queries and keys at their positions ----------------------------------------
+
+def rope_frequencies(rotary_dim: int, theta: float = 10000.0, *, sections: Optional[Sequence[int]] = None,
+                     device="cuda") -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(inv_freq, axis) for qk_rope: theta^(-2 i / rotary_dim) for each pair i
+    (fp64) and, with sections, the axis of each pair (int32): the first
+    sections[0] pairs turn with axis 0's positions, the next sections[1] with axis
+    1's and so on."""
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise HxmiError(f"rotary_dim must be even, got {rotary_dim}")
+    n = rotary_dim // 2
+    inv_freq = theta ** (-torch.arange(n, dtype=torch.float64) / max(n, 1))
+    axis = None
+    if sections is not None:
+        if sum(sections) != n or min(sections) < 0:
+            raise HxmiError(f"sections must add up to the {n} pairs of {rotary_dim} dimensions, got {tuple(sections)}")
+        axis = torch.repeat_interleave(torch.arange(len(sections), dtype=torch.int32), torch.tensor(sections)).to(device)
+    return inv_freq.to(device), axis
+
+
+def _rope_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dtype not in (torch.float16, torch.bfloat16):
+        raise HxmiError(f"qk_rope takes fp16 or bf16 q and k, got {t.dtype} for {name}")
+    if t.dim() != 3:
+        raise HxmiError(f"{name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _apart(t: torch.Tensor) -> bool:
+    """Whether no two of the [rows, heads, dims] elements of t share memory."""
+    T, H, d = t.shape
+    s0, s1, _ = t.stride()
+    return (T == 1 or s0 >= (H - 1) * s1 + d or (s0 >= d and (H == 1 or s1 >= (T - 1) * s0 + d))) \
+        and (H == 1 or s1 >= d)
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors may share elements; false for two ranges of heads of
+    the same rows (q and k of one projection), whose address ranges meet."""
+    if not _overlap(a, b):
+        return False
+    if a.dim() != 3 or b.dim() != 3 or a.stride(0) != b.stride(0) or a.element_size() != b.element_size() \
+            or a.stride(2) != 1 or b.stride(2) != 1:
+        return True
+    row, size = a.stride(0), a.element_size()
+    wide = [(t.shape[1] - 1) * t.stride(1) + t.shape[2] for t in (a, b)]
+    if row <= 0 or (b.data_ptr() - a.data_ptr()) % size:
+        return True
+    at = (b.data_ptr() - a.data_ptr()) // size % row
+    return not (at >= wide[0] and at + wide[1] <= row)
+
+
+def qk_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
+            axis: Optional[torch.Tensor] = None, scale: float = 1.0, q_weight: Optional[torch.Tensor] = None,
+            k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+            out: Optional[tuple] = None) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (fp16 or
+    bf16, any row and head strides; k may be None) at their positions, in one pass.
+
+    With q_weight / k_weight [head_dim] (q's type or fp32) each head is normalised
+    first: x * rsqrt(mean(x^2) + eps) * weight.  Then the first 2 * n dimensions
+    turn, n = len(inv_freq): pair i is dimensions i and i + n, or with interleaved
+    2 i and 2 i + 1, and becomes scale * (a cos t - b sin t, b cos t + a sin t)
+    at t = position * inv_freq[i] (fp64).  positions: [tokens] (int32 or int64, as
+    kv_plan gives them), or [axes, tokens] with axis [n] (int32), the row of positions that
+    each pair turns with (rope_frequencies makes both).  Everything is computed in
+    32 bits, angles in 64, and rounded once.  head_dim is a multiple of 8 up to 256.
+
+    Returns (q, k), contiguous, or writes to out = (q, k), which may be the
+    operands themselves."""
+    oq, ok = (None, None) if out is None else out
+    y = _ops.qk_rope(q, k, positions, inv_freq, axis, scale, q_weight, k_weight, eps, interleaved, oq, ok)
+    if y is not None:
+        return y if out is None else (oq, ok)
+    _require_gpu(q, k, positions, inv_freq, axis, q_weight, k_weight, oq, ok)
+    x = _rope_rows(q, "q")
+    T, H, d = x.shape
+    z = None
+    if k is not None:
+        z = _rope_rows(k, "k")
+        if z.shape[0] != T or z.shape[2] != d or z.dtype != x.dtype:
+            raise HxmiError(f"k must be {x.dtype} [{T}, kv_heads, {d}], got {z.dtype} {tuple(z.shape)}")
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64:
+        raise HxmiError("inv_freq must be a 1-D torch.float64 tensor")
+    n = inv_freq.numel()
+    if 2 * n > d:
+        raise HxmiError(f"{n} pairs do not fit in head_dim {d}")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) or positions.shape[-1] != T:
+        raise HxmiError(f"positions must be int32 or int64 [{T}] or [axes, {T}], got {positions.dtype} "
+                        f"{tuple(positions.shape)}")
+    if axis is None:
+        if positions.dim() == 2 and positions.shape[0] != 1:
+            raise HxmiError("positions of several axes need axis, the axis of each pair")
+    else:
+        axis = _ints(axis, n, "axis")
+    if positions.dim() == 2 and positions.shape[0] == 0:
+        raise HxmiError("positions must have at least one axis")
+    pos = positions if T <= 1 or positions.stride(-1) == 1 else positions.contiguous()
+    if pos.dim() == 2 and pos.shape[0] > 1 and pos.stride(0) < T:
+        pos = pos.contiguous()
+    weights = [None if w is None else _rope_weight(w, d, x.dtype, name)
+               for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight"))]
+    if len({w.dtype for w in weights if w is not None}) == 2:
+        weights = [w.float() for w in weights]
+    if not 0 <= eps < math.inf or not math.isfinite(scale):
+        raise HxmiError(f"eps and scale must be finite and eps >= 0, got {eps} and {scale}")
+    results = []
+    for t, o, name in ((x, oq, "q"), (z, ok, "k")):
+        if t is None:
+            if o is not None:
+                raise HxmiError("out has a k and the call has none")
+            results.append(None)
+        elif o is None:
+            if out is not None:
+                raise HxmiError(f"out must hold a tensor for {name}")
+            results.append(torch.empty(t.shape, dtype=t.dtype, device=t.device))
+        else:
+            if o.shape != t.shape or o.dtype != t.dtype:
+                raise HxmiError(f"out's {name} must be {t.dtype} {tuple(t.shape)}, got {o.dtype} {tuple(o.shape)}")
+            if not _apart(o):
+                raise HxmiError(f"the rows of out's {name} must not share elements (strides {o.stride()})")
+            results.append(o)
+    if out is not None and T:
+        given = [t for t in results if t is not None and t.numel()]
+        if len(given) == 2 and _meet(*given):
+            raise HxmiError("out's q and k must not share elements")
+        # an output that meets an operand, other than its own in place, waits for its copy
+        others = [t for t in (q, k, positions, inv_freq, axis, q_weight, k_weight) if t is not None and t.numel()]
+        free = True
+        for o, own in ((oq, q), (ok, k)):
+            if o is None or o.numel() == 0:
+                continue
+            in_place = o.data_ptr() == own.data_ptr() and o.stride() == own.stride()
+            free = free and o.stride(2) == 1 and not any(_meet(o, t) for t in others if not (t is own and in_place))
+        if not free:
+            new = qk_rope(q, k, positions, inv_freq, axis=axis, scale=scale, q_weight=q_weight, k_weight=k_weight,
+                          eps=eps, interleaved=interleaved)
+            for o, v in zip((oq, ok), new):
+                if o is not None:
+                    o.copy_(v)
+            return oq, ok
+    strides = lambda t: (0, 0) if t is None else (t.stride(0), t.stride(1))  # noqa: E731
+    with _on(x):
+        _check(load_library().hxmi_qk_rope(
+            int(x.dtype == torch.bfloat16), x.data_ptr(), _ptr(z), results[0].data_ptr(), _ptr(results[1]),
+            pos.data_ptr(), int(pos.dtype == torch.int64), inv_freq.contiguous().data_ptr(), _ptr(axis), _ptr(weights[0]),
+            _ptr(weights[1]), int(any(w is not None and w.dtype == torch.float32 for w in weights)), T, H,
+            0 if z is None else z.shape[1], d, 2 * n, pos.shape[0] if pos.dim() == 2 else 1,
+            pos.stride(0) if pos.dim() == 2 and pos.shape[0] > 1 else T, *strides(x), *strides(z), *strides(results[0]),
+            *strides(results[1]), int(bool(interleaved)), eps, scale, _stream(x)))
+    return results[0], results[1]
+
+
+def _rope_weight(w: torch.Tensor, d: int, dtype: torch.dtype, name: str) -> torch.Tensor:
+    if w.dim() != 1 or w.numel() != d or w.dtype not in (dtype, torch.float32):
+        raise HxmiError(f"{name} must be a 1-D {dtype} or torch.float32 tensor of {d} elements")
+    return w.contiguous()
+
+# ---- serving: key/value caches of 8 and 4 bits, attention over them, sampling ---------------------
+
+def _cache_sizes(head_dim: int, block_size: int, of: str = "") -> None:
+    if block_size not in (16, 32, 64, 128, 256):
+        raise HxmiError(f"{of}block_size must be a power of two from 16 to 256, got {block_size}")
+    if head_dim % 8 or not 8 <= head_dim <= 128:
+        raise HxmiError(f"{of}head_dim must be a multiple of 8 up to 128, got {head_dim}")
+
 
 @dataclasses.dataclass
 class KVCache:
@@ -989,14 +1159,50 @@ class KVCache:
     @classmethod
     def empty(cls, blocks: int, kv_heads: int, head_dim: int, block_size: int = 64, device="cuda") -> "KVCache":
         """A cache that holds nothing yet."""
-        if block_size not in (16, 32, 64, 128, 256):
-            raise HxmiError(f"block_size must be a power of two from 16 to 256, got {block_size}")
-        if head_dim % 8 or not 8 <= head_dim <= 128:
-            raise HxmiError(f"head_dim must be a multiple of 8 up to 128, got {head_dim}")
+        _cache_sizes(head_dim, block_size)
         dp = (head_dim + 15) // 16 * 16
         zeros = lambda *shape, dtype=torch.int8: torch.zeros(shape, dtype=dtype, device=device)  # noqa: E731
         return cls(zeros(blocks, kv_heads, block_size, dp), zeros(blocks, kv_heads, block_size // 16, dp, 16),
                    zeros(blocks, kv_heads, dtype=torch.float32), zeros(blocks, kv_heads, dtype=torch.float32), head_dim)
+
+    @property
+    def blocks(self) -> int:
+        return self.k.shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.k.shape[1]
+
+    @property
+    def block_size(self) -> int:
+        return self.k.shape[2]
+
+
+@dataclasses.dataclass
+class KVCache4:
+    """The keys and values of a serving loop in 4 bits, in blocks of tokens, with
+    a scale of 8 bits for every 32 dimensions of each token and head
+    (include/hxmi.h): 4.25 bits a value, half of what a KVCache holds.
+
+    k uint8 [blocks, kv_heads, block_size, Dp / 2], v uint8 [blocks, kv_heads,
+    block_size / 16, Dp, 8] (Dp = head_dim rounded up to 32), k_scale and v_scale
+    uint8 [blocks, kv_heads, Dp / 32, block_size]; what is held fp16 and bf16
+    hold exactly.  block_size, head_dim and slots as a KVCache's; kv_append,
+    kv_read and kv_attention take either."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    head_dim: int
+
+    @classmethod
+    def empty(cls, blocks: int, kv_heads: int, head_dim: int, block_size: int = 64, device="cuda") -> "KVCache4":
+        """A cache that holds nothing yet."""
+        _cache_sizes(head_dim, block_size)
+        dp = (head_dim + 31) // 32 * 32
+        zeros = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device=device)  # noqa: E731
+        return cls(zeros(blocks, kv_heads, block_size, dp // 2), zeros(blocks, kv_heads, block_size // 16, dp, 8),
+                   zeros(blocks, kv_heads, dp // 32, block_size), zeros(blocks, kv_heads, dp // 32, block_size), head_dim)
 
     @property
     def blocks(self) -> int:
@@ -1043,29 +1249,40 @@ def _table(t: torch.Tensor, requests: int) -> int:
     return _rowmajor(t, "block_table")
 
 
-def _cache_args(c: KVCache) -> tuple:
+def _cache_args(c) -> tuple:
     """(pointers, (blocks, kv_heads, head_dim, block_size)) of a cache."""
-    if not isinstance(c, KVCache):
-        raise HxmiError(f"cache must be a KVCache, got {type(c).__name__}")
+    if not isinstance(c, (KVCache, KVCache4)):
+        raise HxmiError(f"cache must be a KVCache or a KVCache4, got {type(c).__name__}")
     _require_gpu(c.k, c.v, c.k_scale, c.v_scale)
-    d = c.head_dim
+    d, four = c.head_dim, isinstance(c, KVCache4)
     if c.k.dim() != 4:
-        raise HxmiError(f"cache.k must be [blocks, kv_heads, block_size, Dp], got shape {tuple(c.k.shape)}")
-    n, h, b, dp = c.k.shape
-    if b not in (16, 32, 64, 128, 256):
-        raise HxmiError(f"the cache's block_size must be a power of two from 16 to 256, got {b}")
-    if d % 8 or not 8 <= d <= 128:
-        raise HxmiError(f"the cache's head_dim must be a multiple of 8 up to 128, got {d}")
-    if dp != (d + 15) // 16 * 16 or c.v.shape != (n, h, b // 16, dp, 16) or c.k_scale.shape != (n, h) \
-            or c.v_scale.shape != (n, h) or h < 1:
+        raise HxmiError(f"cache.k must be [blocks, kv_heads, block_size, {'Dp / 2' if four else 'Dp'}], got shape "
+                        f"{tuple(c.k.shape)}")
+    n, h, b, row = c.k.shape
+    _cache_sizes(d, b, "the cache's ")
+    if four:
+        dp = (d + 31) // 32 * 32
+        shapes = (n, h, b, dp // 2), (n, h, b // 16, dp, 8), (n, h, dp // 32, b)
+    else:
+        dp = (d + 15) // 16 * 16
+        shapes = (n, h, b, dp), (n, h, b // 16, dp, 16), (n, h)
+    if c.k.shape != shapes[0] or c.v.shape != shapes[1] or c.k_scale.shape != shapes[2] \
+            or c.v_scale.shape != shapes[2] or h < 1:
         raise HxmiError(f"the cache's tensors do not belong together: k {tuple(c.k.shape)}, v {tuple(c.v.shape)}, "
                         f"scales {tuple(c.k_scale.shape)} and {tuple(c.v_scale.shape)}, head_dim {d}")
-    if c.k.dtype != torch.int8 or c.v.dtype != torch.int8 or c.k_scale.dtype != torch.float32 \
-            or c.v_scale.dtype != torch.float32:
-        raise HxmiError("a cache holds int8 codes and fp32 scales")
+    codes, scales = (torch.uint8, torch.uint8) if four else (torch.int8, torch.float32)
+    if c.k.dtype != codes or c.v.dtype != codes or c.k_scale.dtype != scales or c.v_scale.dtype != scales:
+        raise HxmiError("a 4-bit cache holds uint8 codes and scales" if four else
+                        "a cache holds int8 codes and fp32 scales")
     if not all(t.is_contiguous() for t in (c.k, c.v, c.k_scale, c.v_scale)):
         raise HxmiError("the cache's tensors must be contiguous")
     return (c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr()), (n, h, d, b)
+
+
+def _of_cache(cache, op: str):
+    """The native entry and the library's function `op` for this kind of cache."""
+    op = op.replace("kv_", "kv4_") if isinstance(cache, KVCache4) else op
+    return getattr(_ops, op), "hxmi_" + op
 
 
 def kv_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
@@ -1106,15 +1323,18 @@ def kv_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, fr
     return out
 
 
-def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+def kv_append(cache: Union[KVCache, KVCache4], k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Write k and v rows [tokens, kv_heads, head_dim] (fp16 or bf16) to the
     given slots [tokens] (int64; those outside the cache are skipped).  Rows of
     one block are consecutive rows with consecutive slots, as kv_plan gives
-    them.  A block and head's scale is what its largest value needs: it grows
-    with later rows (earlier codes are rounded again) and starts anew when the
-    block's first token is written."""
-    if isinstance(cache, KVCache) and _ops.kv_append(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim,
-                                                     k, v, slots):
+    them.  In a KVCache a block and head's scale is what its largest value needs:
+    it grows with later rows (earlier codes are rounded again) and starts anew
+    when the block's first token is written.  In a KVCache4 every 32 dimensions
+    of a row have a scale of their own and what is there already does not change;
+    values past 61440, infinities and NaN among them, are held as 61440."""
+    native, name = _of_cache(cache, "kv_append")
+    if isinstance(cache, (KVCache, KVCache4)) and native(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim,
+                                                         k, v, slots):
         return
     ptrs, (n, h, d, b) = _cache_args(cache)
     _require_gpu(cache.k, k, v, slots)
@@ -1125,17 +1345,19 @@ def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Ten
     slots = _ints(slots, k.shape[0], "slots", torch.int64)
     k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (k, v))
     with _on(k):
-        _check(load_library().hxmi_kv_append(
+        _check(getattr(load_library(), name)(
             int(k.dtype == torch.bfloat16), k.data_ptr(), v.data_ptr(), slots.data_ptr(), *ptrs, k.shape[0], n, h, d, b,
             k.stride(0), k.stride(1), v.stride(0), v.stride(1), _stream(k)))
 
 
-def kv_read(cache: KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
+def kv_read(cache: Union[KVCache, KVCache4], slots: torch.Tensor,
+            dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values held at slots [tokens] (int64), rounded to fp16 or
-    bf16: two tensors [tokens, kv_heads, head_dim], zeros for slots outside the
-    cache."""
-    if isinstance(cache, KVCache) and dtype in (torch.float16, torch.bfloat16):
-        y = _ops.kv_read(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim, slots, dtype == torch.bfloat16)
+    bf16 (of a KVCache4: as they are): two tensors [tokens, kv_heads, head_dim],
+    zeros for slots outside the cache."""
+    native, name = _of_cache(cache, "kv_read")
+    if isinstance(cache, (KVCache, KVCache4)) and dtype in (torch.float16, torch.bfloat16):
+        y = native(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim, slots, dtype == torch.bfloat16)
         if y is not None:
             return y
     ptrs, (n, h, d, b) = _cache_args(cache)
@@ -1145,12 +1367,12 @@ def kv_read(cache: KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.floa
     slots = _ints(slots, None, "slots", torch.int64)
     k, v = (torch.empty((slots.numel(), h, d), dtype=dtype, device=slots.device) for _ in range(2))
     with _on(slots):
-        _check(load_library().hxmi_kv_read(int(dtype == torch.bfloat16), *ptrs, slots.data_ptr(), k.data_ptr(),
-                                           v.data_ptr(), slots.numel(), n, h, d, b, _stream(slots)))
+        _check(getattr(load_library(), name)(int(dtype == torch.bfloat16), *ptrs, slots.data_ptr(), k.data_ptr(),
+                                             v.data_ptr(), slots.numel(), n, h, d, b, _stream(slots)))
     return k, v
 
 
-def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, *,
+def kv_attention(q: torch.Tensor, cache: Union[KVCache, KVCache4], block_table: torch.Tensor, lens: torch.Tensor, *,
                  cu: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of q [tokens, heads, head_dim] (fp16 or bf16) over the
@@ -1160,8 +1382,9 @@ def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, len
     heads may be a multiple of the cache's kv_heads.  A row that sees no key
     gets zeros; pages outside the cache are left out; rows that belong to no
     request are not written (in a new result they hold nothing)."""
-    if isinstance(cache, KVCache):
-        y = _ops.kv_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim, block_table, lens, cu,
+    native, name = _of_cache(cache, "kv_attention")
+    if isinstance(cache, (KVCache, KVCache4)):
+        y = native(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim, block_table, lens, cu,
                               scale, out)
         if y is not None:
             return out if out is not None else y
@@ -1190,20 +1413,17 @@ def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, len
     else:
         if out.shape != q.shape or out.dtype != q.dtype:
             raise HxmiError(f"out must be {q.dtype} {tuple(q.shape)}")
-        s0, s1, s2 = out.stride()
-        apart = (T == 1 or s0 >= (H - 1) * s1 + d or (s0 >= d and (H == 1 or s1 >= (T - 1) * s0 + d))) \
-            and (H == 1 or s1 >= d)
         same = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()  # (a tile has read its rows by then)
         others = [t for t in (block_table, lens, cu, cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
-        if not apart:
+        if not _apart(out):
             raise HxmiError(f"the rows of out must not share elements (strides {out.stride()})")
-        if s2 != 1 or (_overlap(q, out) and not same) or any(_overlap(t, out) for t in others):
+        if out.stride(2) != 1 or (_overlap(q, out) and not same) or any(_overlap(t, out) for t in others):
             return out.copy_(kv_attention(q, cache, block_table, lens, cu=cu, scale=scale))
     lib = load_library()
     with _on(q):
-        ws = _workspace(lib.hxmi_kv_attention_workspace_bytes(T, R, H, h, d, b, block_table.shape[1],
-                                                              int(cu is not None)), q.device)
-        _check(lib.hxmi_kv_attention(
+        ws = _workspace(getattr(lib, name + "_workspace_bytes")(T, R, H, h, d, b, block_table.shape[1],
+                                                                int(cu is not None)), q.device)
+        _check(getattr(lib, name)(
             int(q.dtype == torch.bfloat16), q.data_ptr(), *ptrs, block_table.data_ptr(), lens.data_ptr(), _ptr(cu),
             o.data_ptr(), T, R, H, h, d, b, n, block_table.shape[1], ldt, q.stride(0), q.stride(1), o.stride(0),
             o.stride(1), scale, _ptr(ws), 0 if ws is None else ws.numel() * 4, _stream(q)))

@@ -543,6 +543,84 @@ int hxmi_kv_attention(int is_bf16, const void* q, const int8_t* k_codes, const i
 int64_t hxmi_kv_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
                                           int64_t head_dim, int64_t block_size, int64_t width, int ragged);
 
+/*
+ * Queries and keys at their positions.  q [tokens, heads, head_dim] and k
+ * [tokens, kv_heads, head_dim] (fp16, or bf16 with is_bf16 = 1; any row and head
+ * strides, unit last stride; kv_heads 0: no k) become, head by head,
+ *   y = x * rsqrt(mean(x^2) + eps) * weight        (where a weight is given)
+ *   (a, b) -> scale * (a cos t - b sin t, b cos t + a sin t)
+ * for the rotary_dim / 2 pairs of the first rotary_dim dimensions: pair i is
+ * dimensions i and i + rotary_dim / 2, with interleaved = 1 dimensions 2 i and
+ * 2 i + 1.  Its angle is t = positions[axis[i]][token] * inv_freq[i]: positions
+ * int32 or (pos_is_64 = 1) int64 [axes, tokens] (row stride ld_pos), inv_freq fp64,
+ * axis int32 (NULL: 0; values outside 0 to axes - 1 count as the nearest).  Angles are
+ * taken in 64 bits, the rest in 32, each value rounded once.  Weights [head_dim]
+ * have the type of q and k, or fp32 with weight_is_f32 = 1; NULL: none.  head_dim
+ * is a multiple of 8 up to 256, rotary_dim even (0: no rotation).  q_out and k_out
+ * may be q and k themselves (same pointer and strides); otherwise outputs and
+ * inputs lie apart.
+ * No counterpart in the reference, whose one-token run is at position 0
+ * (benchmark_models/run_qwen2.5-0.5b.py:171-173, 224-233).
+ */
+int hxmi_qk_rope(int is_bf16, const void* q, const void* k, void* q_out, void* k_out, const void* positions,
+                 int pos_is_64, const double* inv_freq, const int32_t* axis, const void* q_weight,
+                 const void* k_weight, int weight_is_f32, int64_t tokens, int64_t heads, int64_t kv_heads,
+                 int64_t head_dim, int64_t rotary_dim, int64_t axes, int64_t ld_pos, int64_t ldq,
+                 int64_t head_stride_q, int64_t ldk, int64_t head_stride_k, int64_t ldq_out,
+                 int64_t head_stride_q_out, int64_t ldk_out, int64_t head_stride_k_out, int interleaved, float eps,
+                 float scale, void* stream);
+
+/*
+ * The cache in 4 bits: as above with Dp = head_dim rounded up to 32 and
+ *   k_codes uint8 [blocks, kv_heads, block_size, Dp / 2]  (dimension 2 j in the
+ *           lower half of byte j, 2 j + 1 in its upper half)
+ *   v_codes uint8 [blocks, kv_heads, block_size / 16, Dp, 8]  (tokens 16 c + 2 j
+ *           and 16 c + 2 j + 1 of a block, dimension d at [c, d, j])
+ *   k_scale, v_scale uint8 [blocks, kv_heads, Dp / 32, block_size]
+ * A code has a sign (its upper bit) and a magnitude 0, 1/2, 1, 3/2, 2, 3, 4 or 6;
+ * a scale's byte is bits 7 to 14 of a positive fp16 number (five exponent bits,
+ * three of mantissa); a held value is their product, which fp16 and bf16 hold
+ * exactly.  Each token and head has a scale for every 32 dimensions.
+ */
+
+/*
+ * hxmi_kv_append for the 4-bit cache; rows of one piece of 16 tokens (not block)
+ * must be consecutive rows with consecutive slots.  For every 32 dimensions of a row:
+ *   scale = the smallest of the scales s with 6 s >= the largest magnitude
+ *   code  = the magnitude nearest to |value| / scale (half way: the one whose
+ *           code is even), with the value's sign
+ * so a value is off by at most half the distance of the two magnitudes around
+ * it, and nothing else in the cache changes.  Values past 61440 (6 times the
+ * largest scale, 10240), infinities and NaN among them, are held as 61440 with
+ * their sign (NaN: positive); magnitudes up to 2^-19 next to nothing larger are held as 0.
+ */
+int hxmi_kv4_append(int is_bf16, const void* k, const void* v, const int64_t* slots, uint8_t* k_codes,
+                    uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int64_t tokens, int64_t blocks,
+                    int64_t kv_heads, int64_t head_dim, int64_t block_size, int64_t ldk, int64_t head_stride_k,
+                    int64_t ldv, int64_t head_stride_v, void* stream);
+
+/* hxmi_kv_read for the 4-bit cache: the held values themselves. */
+int hxmi_kv4_read(int is_bf16, const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scale,
+                  const uint8_t* v_scale, const int64_t* slots, void* k, void* v, int64_t tokens, int64_t blocks,
+                  int64_t kv_heads, int64_t head_dim, int64_t block_size, void* stream);
+
+/*
+ * hxmi_kv_attention over the 4-bit cache.  Keys and values go into the products
+ * as they are held; a weight goes in with 11 bits, or as a multiple of 2^-31 of the
+ * row's largest where that is coarser; the elements of a bf16 row of q are
+ * multiples of 2^-38 of its largest.
+ */
+int hxmi_kv4_attention(int is_bf16, const void* q, const uint8_t* k_codes, const uint8_t* v_codes,
+                       const uint8_t* k_scale, const uint8_t* v_scale, const int32_t* block_table,
+                       const int32_t* lens, const int32_t* cu, void* o, int64_t tokens, int64_t requests,
+                       int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t block_size, int64_t blocks,
+                       int64_t width, int64_t ld_table, int64_t ldq, int64_t head_stride_q, int64_t ldo,
+                       int64_t head_stride_o, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of hxmi_kv4_attention (as hxmi_kv_attention_workspace_bytes). */
+int64_t hxmi_kv4_attention_workspace_bytes(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
+                                           int64_t head_dim, int64_t block_size, int64_t width, int ragged);
+
 /* Types of hxmi_sample's logits. */
 #define HXMI_SAMPLE_F16 0
 #define HXMI_SAMPLE_BF16 1

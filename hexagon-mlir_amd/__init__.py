@@ -21,6 +21,7 @@ from .hxmi import (
     KVCache,
     KVCache4,
     KVPlan,
+    Verified,
     attention,
     bgemm,
     fold_rms_weight,
@@ -43,6 +44,7 @@ from .hxmi import (
     set_tuning,
     softmax,
     tuning,
+    verify,
     w8a16_linear,
 )
 
@@ -54,6 +56,7 @@ __all__ = [
     "KVCache",
     "KVCache4",
     "KVPlan",
+    "Verified",
     "attention",
     "bgemm",
     "fold_rms_weight",
@@ -76,5 +79,6 @@ __all__ = [
     "set_tuning",
     "softmax",
     "tuning",
+    "verify",
     "w8a16_linear",
 ]

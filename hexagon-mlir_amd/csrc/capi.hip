@@ -1004,13 +1004,11 @@ int hxmi_qk_rope(int is_bf16, const void* q, const void* k, void* q_out, void* k
   return from_hip(hxmi::launch_qk_rope(p, (hipStream_t)stream), name);
 }
 
-int hxmi_sample(int dtype, const void* logits, const float* u, const float* temperature, const int32_t* top_k,
-                const float* top_p, const float* min_p, float all_temperature, int32_t all_top_k, float all_top_p,
-                float all_min_p, int64_t* tokens, int64_t rows, int64_t vocab, int64_t ldx, void* stream) {
-  const char* name = "hxmi_sample";
-  REQUIRE(dtype >= HXMI_SAMPLE_F16 && dtype <= HXMI_SAMPLE_F32, "%s: unknown dtype %d", name, dtype);
-  REQUIRE(rows >= 0 && rows < (1ll << 31), "%s: bad number of rows %lld", name, (long long)rows);
-  if (rows == 0) return ok();
+// The arguments that sampling and verification share, checked and put into p.
+static int sample_args(const char* name, int dtype, const void* logits, const float* u, const float* temperature,
+                       const int32_t* top_k, const float* top_p, const float* min_p, float all_temperature,
+                       int32_t all_top_k, float all_top_p, float all_min_p, int64_t* tokens, int64_t rows, int64_t vocab,
+                       int64_t ldx, hxmi::SampleProblem& p) {
   REQUIRE(vocab > 0 && vocab <= hxmi::kSampleMaxVocab, "%s: vocab must be 1 to %lld, got %lld", name,
           (long long)hxmi::kSampleMaxVocab, (long long)vocab);
   REQUIRE(ldx >= vocab || rows == 1, "%s: leading dimension below vocab", name);
@@ -1020,7 +1018,6 @@ int hxmi_sample(int dtype, const void* logits, const float* u, const float* temp
           "%s: temperature must be finite and >= 0", name);
   REQUIRE(top_p || all_top_p == all_top_p, "%s: top_p must be a number", name);
   REQUIRE(min_p || all_min_p == all_min_p, "%s: min_p must be a number", name);
-  hxmi::SampleProblem p{};
   p.logits = logits;
   p.u = u;
   p.temperature = temperature;
@@ -1036,7 +1033,65 @@ int hxmi_sample(int dtype, const void* logits, const float* u, const float* temp
   p.p = all_top_p;
   p.m = all_min_p;
   p.dtype = dtype;
+  return HXMI_OK;
+}
+
+int hxmi_sample(int dtype, const void* logits, const float* u, const float* temperature, const int32_t* top_k,
+                const float* top_p, const float* min_p, float all_temperature, int32_t all_top_k, float all_top_p,
+                float all_min_p, int64_t* tokens, int64_t rows, int64_t vocab, int64_t ldx, void* stream) {
+  const char* name = "hxmi_sample";
+  REQUIRE(dtype >= HXMI_SAMPLE_F16 && dtype <= HXMI_SAMPLE_F32, "%s: unknown dtype %d", name, dtype);
+  REQUIRE(rows >= 0 && rows < (1ll << 31), "%s: bad number of rows %lld", name, (long long)rows);
+  if (rows == 0) return ok();
+  hxmi::SampleProblem p{};
+  if (const int rc = sample_args(name, dtype, logits, u, temperature, top_k, top_p, min_p, all_temperature, all_top_k,
+                                 all_top_p, all_min_p, tokens, rows, vocab, ldx, p))
+    return rc;
   return from_hip(hxmi::launch_sample(p, (hipStream_t)stream), name);
+}
+
+int64_t hxmi_verify_workspace_bytes(int64_t rows) { return rows > 0 ? hxmi::verify_workspace_bytes(rows) : 0; }
+
+int hxmi_verify(int dtype, const void* logits, const int64_t* drafts, const float* u, const float* draw,
+                const int32_t* cu, const void* draft_probs, int probs_dtype, const float* temperature,
+                const int32_t* top_k, const float* top_p, const float* min_p, float all_temperature,
+                int32_t all_top_k, float all_top_p, float all_min_p, int64_t* tokens, int32_t* counts, int64_t rows,
+                int64_t requests, int64_t vocab, int64_t ldx, int64_t ld_probs, void* workspace,
+                int64_t workspace_bytes, void* stream) {
+  const char* name = "hxmi_verify";
+  REQUIRE(dtype >= HXMI_SAMPLE_F16 && dtype <= HXMI_SAMPLE_F32, "%s: unknown dtype %d", name, dtype);
+  REQUIRE(probs_dtype >= HXMI_SAMPLE_F16 && probs_dtype <= HXMI_SAMPLE_F32, "%s: unknown probs_dtype %d", name, probs_dtype);
+  REQUIRE(rows >= 0 && rows < (1ll << 31) && requests >= 0 && requests < (1ll << 31),
+          "%s: bad number of rows %lld or requests %lld", name, (long long)rows, (long long)requests);
+  REQUIRE(cu || (requests ? rows % requests == 0 : rows == 0), "%s: without cu every request has the same number of rows",
+          name);
+  if (requests == 0 && rows == 0) return ok();
+  REQUIRE(requests > 0, "%s: rows without a request", name);
+  REQUIRE(draw && counts, "%s: null draw or counts", name);
+  hxmi::VerifyProblem p{};
+  if (rows) {
+    if (const int rc = sample_args(name, dtype, logits, u, temperature, top_k, top_p, min_p, all_temperature, all_top_k,
+                                   all_top_p, all_min_p, tokens, rows, vocab, ldx, p))
+      return rc;
+    REQUIRE(drafts, "%s: null drafts", name);
+    REQUIRE(!draft_probs || ld_probs >= vocab || rows == 1, "%s: leading dimension of draft_probs below vocab", name);
+    REQUIRE((uintptr_t)draft_probs % (probs_dtype == HXMI_SAMPLE_F32 ? 4 : 2) == 0,
+            "%s: draft_probs must be aligned to their type", name);
+    REQUIRE(workspace && al(workspace, 256) && workspace_bytes >= hxmi::verify_workspace_bytes(rows),
+            "%s: needs a 256-byte aligned workspace of %lld bytes", name, (long long)hxmi::verify_workspace_bytes(rows));
+  }
+  p.rows = rows;
+  p.dtype = dtype;
+  p.drafts = drafts;
+  p.draw = draw;
+  p.cu = cu;
+  p.q = draft_probs;
+  p.ldq = ld_probs;
+  p.q_type = probs_dtype;
+  p.counts = counts;
+  p.ws = workspace;
+  p.requests = requests;
+  return from_hip(hxmi::launch_verify(p, (hipStream_t)stream), name);
 }
 
 int hxmi_lwp_record(uint32_t* records, int64_t slot, uint32_t id, void* stream) {

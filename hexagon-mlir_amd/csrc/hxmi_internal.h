@@ -295,6 +295,20 @@ struct SampleProblem {
 };
 constexpr int SAMPLE_F32 = 2;
 hipError_t launch_sample(const SampleProblem& p, hipStream_t stream);
+// Drafted tokens against the target's distribution (sample.hip); parameters are
+// a request's own, `tokens` and `u` a row's.
+struct VerifyProblem : SampleProblem {
+  const int64_t* drafts;
+  const float* draw;
+  const int* cu;  // null: rows / requests each
+  const void* q;  // the draft's probabilities, or null
+  int* counts;
+  void* ws;
+  int64_t requests, ldq;
+  int q_type;  // as dtype
+};
+int64_t verify_workspace_bytes(int64_t rows);
+hipError_t launch_verify(const VerifyProblem& p, hipStream_t stream);
 
 // One-token decoder step of a Llama / Qwen2 stack (persistent kernel).
 struct DecodeProblem {

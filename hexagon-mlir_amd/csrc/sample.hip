@@ -68,6 +68,27 @@ struct SArgs {
   int k;
 };
 
+// Verification of drafted tokens: rows of requests, `u` a row's number for its
+// draft, `draw` a request's for the token after the accepted ones.
+struct RowState {
+  int64_t token;  // drawn (state kDrawn)
+  uint64_t whole, least;
+  uint32_t state, tau, top, from;
+  int ties_end;  // equals of tau before this token are kept
+  float t;
+};
+enum : uint32_t { kDrawn, kAccepted, kToDraw };
+struct VArgs : SArgs {
+  const int64_t* drafts;
+  const float* draw;
+  const int* cu;  // null: `per` rows a request
+  const char* q;  // the draft's probabilities, or null: the drafted token is certain
+  int64_t ldq, rows;
+  RowState* state;
+  int* counts;
+  int requests, per, q_type;
+};
+
 constexpr int NT = 1024, NW = NT / 64, PIECE = 512;
 constexpr int kMaxPieces = kSampleMaxVocab / PIECE;
 constexpr int kList = 6144, kFewTop = 512, kTable = 16384, kBins = 16384;
@@ -146,6 +167,21 @@ struct Weights {
     return (uint64_t)__double_as_longlong(p) & 0xfffffffffffffull;
   }
 };
+
+// The weights of a row with the largest key `top` at temperature t.
+template <typename T>
+__device__ __forceinline__ Weights weights_of(uint32_t top, float t, int shift, const double* table) {
+  const float xmax = value_of<T>(top);
+  const double rate = 1.44269504088896340736 / (double)fminf(t, 1e28f);  // (an infinite T leaves -inf its weight, 0)
+  // `least`, 20 bits below where weights end and rounded down: y stays above -200 bits.
+  // Where a float holds nothing between it and the largest logit (T of 1e-9 of
+  // that, or 1e28), only the largest have a weight, as where that is infinite.
+  const double under = (double)xmax - (shift + 20) / rate;
+  float least_x = (float)under;
+  const bool lone = xmax == INFINITY || least_x >= xmax;
+  if ((double)least_x > under) least_x = value_of<float>(Key<float>::of(least_x) - 1);
+  return Weights{rate * kSteps, (double)xmax, xmax, least_x, shift, table, __builtin_amdgcn_readfirstlane(lone)};
+}
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) {
   return ((uint64_t)(uint32_t)__shfl((int)(v >> 32), lane, 64) << 32) | (uint32_t)__shfl((int)v, lane, 64);
@@ -280,20 +316,65 @@ __device__ __forceinline__ uint64_t block_sum(uint64_t v, Shared& sh) {
   return total;
 }
 
-template <typename T>
-__global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
+// Element i of a row of the draft's probabilities; NaN and negative ones count as 0.
+__device__ __forceinline__ float prob_of(const char* q, int type, int64_t i) {
+  const float f = type == SAMPLE_F32 ? ((const float*)q)[i]
+                  : type == DT_BF16  ? (float)((const __bf16*)q)[i]
+                                     : (float)((const _Float16*)q)[i];
+  return fmaxf(f, 0.f);
+}
+// floor(f * whole) for a probability f.
+__device__ __forceinline__ uint64_t share_of(float f, double whole) {
+  return (uint64_t)fmin((double)f * whole, 0x1p62);
+}
+__device__ __forceinline__ float unit(float u) { return u > 0.f ? (u < 1.f ? u : 0x1.fffffep-1f) : 0.f; }
+
+// The rows [first, end) of request r.
+__device__ __forceinline__ void rows_of(const VArgs& a, int r, int64_t& first, int64_t& end) {
+  first = a.cu ? min(max((int64_t)a.cu[r], (int64_t)0), a.rows) : (int64_t)r * a.per;
+  end = a.cu ? min(max((int64_t)a.cu[r + 1], first), a.rows) : first + a.per;
+}
+
+// A row to its token; or (VERIFY, A = VArgs) a row to whether its drafted token is
+// accepted, and if not what is drawn in its place, as far as the row's own
+// weights say: with a draft's probabilities verify_rows draws it.
+template <typename T, typename A>
+__global__ __launch_bounds__(NT) void sample_rows(A a) {
+  constexpr bool VERIFY = std::is_same_v<A, VArgs>;
   __shared__ __attribute__((aligned(16))) Shared sh;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t row = blockIdx.x;
+  int64_t owner = row;  // index of the row's settings
+  bool final = true;  // VERIFY: its request's last row, which has no draft
+  if constexpr (VERIFY) {
+    int lo = 0;
+    if (a.cu) {
+      for (int hi = a.requests; hi - lo > 1;) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid] <= row) lo = mid;
+        else hi = mid;
+      }
+    } else {
+      lo = (int)(row / a.per);
+    }
+    int64_t first, end;
+    rows_of(a, lo, first, end);
+    if (row < first || row >= end) {  // of no request
+      if (threadIdx.x == 0) a.token[row] = -1;
+      return;
+    }
+    owner = lo;
+    final = row + 1 == end;
+  }
   const T* const x = (const T*)a.x + row * a.ldx;
   const int vocab = a.vocab;
   constexpr int KB = Key<T>::bits;
 
   if (threadIdx.x < kSteps) sh.exp2[threadIdx.x] = kExp2.v[threadIdx.x];
 
-  int k = a.top_k ? a.top_k[row] : a.k;
-  float p = a.top_p ? a.top_p[row] : a.p, mp = a.min_p ? a.min_p[row] : a.m;
-  float t = a.temperature ? a.temperature[row] : a.t;
+  int k = a.top_k ? a.top_k[owner] : a.k;
+  float p = a.top_p ? a.top_p[owner] : a.p, mp = a.min_p ? a.min_p[owner] : a.m;
+  float t = a.temperature ? a.temperature[owner] : a.t;
   if (!(t > 0.f)) {  // the first of the largest
     t = 1.f;
     k = 1;
@@ -416,11 +497,15 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
     });
   extremes();
   if (top > kInf || low + 1 < kMinusInf || top == kMinusInf) {
-    if (threadIdx.x == 0) a.token[row] = -1;
+    if (threadIdx.x == 0) {
+      if constexpr (VERIFY) a.state[row] = RowState{.token = -1, .state = kDrawn};
+      else a.token[row] = -1;
+    }
     return;
   }
-  const float xmax = value_of<T>(top);
-  const double rate = 1.44269504088896340736 / (double)fminf(t, 1e28f);  // (an infinite T leaves -inf its weight, 0)
+  const Weights weights = weights_of<T>(top, t, a.shift, sh.exp2);
+  const float xmax = weights.xmax;
+  const double rate = 1.44269504088896340736 / (double)fminf(t, 1e28f);
   auto key_from = [&](double v) {  // the key from which logits are at least v (of a NaN: all)
     const float f = (float)v;
     if constexpr (KB == 32) return f != f ? 1u : max(1u, Key<float>::of(f));
@@ -434,15 +519,6 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   // sum, and whether the top k holds some of them changes nothing.  (Any value
   // under the rounding of a bound is under the bound.)
   const uint32_t cut = min(top, key_from((double)xmax - (a.shift + 3) / rate * 1.000001));
-  // `least`, lower by another 17 bits and rounded down: y stays above -200 bits.
-  // Where a float holds nothing between it and the largest logit (T of 1e-9 of
-  // that, or 1e28), only the largest have a weight, as where that is infinite.
-  const double under = (double)xmax - (a.shift + 20) / rate;
-  float least_x = (float)under;
-  const bool lone = xmax == INFINITY || least_x >= xmax;
-  if ((double)least_x > under) least_x = value_of<float>(Key<float>::of(least_x) - 1);
-  const Weights weights{rate * kSteps, (double)xmax, xmax, least_x, a.shift, sh.exp2,
-                        __builtin_amdgcn_readfirstlane(lone)};
   // Descends to the key at which the counts (or weights) from the largest key
   // down first reach `goal`; `above`: what lies over that key.
   auto descend = [&](auto COUNT_, uint64_t goal, uint64_t& above) {
@@ -883,9 +959,84 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   if (w != 0) return;
   const uint64_t wt_all = weights.of(value_of<T>(tau)), wt = wt_all >= least ? wt_all : 0;
   uint64_t before;
-  const uint64_t run = lane_pieces(wt, before), incl = scan64(run), whole = shfl64(incl, 63);
-  float u = a.u[row];
-  u = u > 0.f ? (u < 1.f ? u : 0x1.fffffep-1f) : 0.f;
+  uint64_t run = lane_pieces(wt, before), incl = scan64(run), whole = shfl64(incl, 63);
+  int64_t out = -1;    // the drafted token where that takes no part any more
+  uint64_t w_out = 0;  // its weight
+  float u = 0.f;
+  if constexpr (VERIFY) {
+    const int64_t d = final ? -1 : a.drafts[row];
+    const bool in = d >= 0 && d < vocab;
+    uint64_t wd = 0;
+    if (in) {
+      const uint32_t kd = Key<T>::of(x[d]);
+      if (kd > tau && kd >= from) {
+        const uint64_t wf = weights.of(value_of<T>(kd));
+        wd = wf >= least ? wf : 0;
+      } else if (kd == tau && wt) {
+        // its place among tau's equals
+        const int c = (int)(d / PIECE);
+        uint64_t ties = 0;
+        for (int i = lane; i < c; i += 64) ties += sh.piece.ties[i];
+        uint32_t key[8];
+        load_keys(x, c * 64 + lane, vocab, key);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ties += key[e] == tau && (c * 64 + lane) * 8 + e < d;
+        wd = shfl64(scan64(ties), 63) < equal ? wt : 0;
+      }
+    }
+    const float qd = !in ? 0.f : a.q ? prob_of(a.q + row * a.ldq * (a.q_type == SAMPLE_F32 ? 4 : 2), a.q_type, d) : 1.f;
+    const bool accepted = (double)wd > (double)unit(a.u[row]) * qd * (double)whole;
+    if (accepted || (a.q && !final)) {
+      int ties_end = vocab;  // of tau's equals, those before this token are kept
+      if (!accepted && equal > 0) {
+        uint64_t seen = 0;  // (a wave over the pieces, 64 at a time, to the one that holds the first that is not)
+        for (int c0 = 0; c0 < pieces; c0 += 64) {
+          const uint64_t ties = c0 + lane < pieces ? sh.piece.ties[c0 + lane] : 0, incl = seen + scan64(ties);
+          const uint64_t past = __ballot(incl > equal);
+          if (!past) {
+            seen = shfl64(incl, 63);
+            continue;
+          }
+          const int l = __ffsll((unsigned long long)past) - 1, c = c0 + l;
+          seen = shfl64(incl - ties, l);
+          uint32_t key[8];
+          load_keys(x, c * 64 + lane, vocab, key);
+          uint64_t mine = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mine += key[e] == tau;
+          uint64_t at = seen + scan64(mine) - mine;
+          int first = vocab;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (key[e] != tau) continue;
+            if (at >= equal && first == vocab) first = (c * 64 + lane) * 8 + e;
+            ++at;
+          }
+#pragma unroll
+          for (int o = 32; o >= 1; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
+          ties_end = first;
+          break;
+        }
+      }
+      if (lane == 0)
+        a.state[row] = RowState{-1, whole, least, accepted ? kAccepted : kToDraw, tau, top, from, ties_end, t};
+      return;
+    }
+    if (in && !a.q && !final) {
+      out = d;
+      w_out = wd;
+    }
+    u = unit(a.draw[owner]);
+  } else {
+    u = unit(a.u[row]);
+  }
+  const int out_piece = out >= 0 ? (int)(out / PIECE) : -1;
+  if (out_piece >= 0) {
+    const uint64_t less = out_piece / per == lane ? w_out : 0;
+    run -= less;
+    incl -= out_piece / per <= lane ? w_out : 0;
+    whole -= w_out;
+  }
   const uint64_t goal = __umul64hi(fraction64(u), whole);  // floor(u * whole) < whole
 
   // the lane's run, the piece, then the token whose running weight first exceeds the goal
@@ -895,7 +1046,8 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
   int at = l * per;
   for (;; ++at) {  // (every lane the same)
     const uint64_t ties = sh.piece.ties[at];
-    const uint64_t own = sh.piece.sum[at] + (before >= equal ? 0 : min(ties, (uint64_t)equal - before)) * wt;
+    uint64_t own = sh.piece.sum[at] + (before >= equal ? 0 : min(ties, (uint64_t)equal - before)) * wt;
+    if (at == out_piece) own -= w_out;
     if (sum + own > goal || at + 1 >= min((l + 1) * per, pieces)) break;
     sum += own;
     before += ties;
@@ -917,6 +1069,7 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
       own[e] = before < equal ? wt : 0;
       ++before;
     }
+    if (VERIFY && (at * 64 + lane) * 8 + e == out) own[e] = 0;
     mine += own[e];
   }
   const uint64_t s = sum + scan64(mine);
@@ -928,14 +1081,153 @@ __global__ __launch_bounds__(NT) void sample_rows(SArgs a) {
       so_far += own[e];
       if (so_far > goal) break;
     }
-    a.token[row] = (int64_t)(at * 64 + lane) * 8 + e;
+    const int64_t token = (int64_t)(at * 64 + lane) * 8 + e;
+    if constexpr (VERIFY) a.state[row] = RowState{.token = token, .state = kDrawn};
+    else a.token[row] = token;
+  }
+}
+
+// ---- verification of drafted tokens ------------------------------------------------
+//
+//   p_i    a row's kept weights over their sum, as above
+//   accept token d of a row (not its request's last) if p_d > u * q_d
+//   the first row that is not accepted draws a token from max(p - q, 0), or, with
+//   no probabilities of the draft, from p without d; the request's last row from p
+//
+// sample_rows says for every row whether its token is accepted and draws from
+// what needs the row's own weights alone; this kernel, a workgroup a request,
+// finds the row that stops it and, given q, goes over that row again: the kept
+// weights less floor(q * sum), integers as they are, by pieces of 512 tokens,
+// then the token in the piece that reaches draw * sum.
+template <typename T, typename Q>
+__global__ __launch_bounds__(NT) void verify_rows(VArgs a) {
+  struct Local {
+    uint32_t key[NW][PIECE];
+    float q[NW][PIECE];
+    unsigned long long sum[kMaxPieces];
+    double exp2[kSteps];
+    unsigned long long stop;
+  };
+  __shared__ Local sh;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = blockIdx.x, vocab = a.vocab;
+  int64_t first, end;
+  rows_of(a, r, first, end);
+  if (threadIdx.x == 0) {
+    sh.stop = (unsigned long long)end;
+    if (first == end) a.counts[r] = 0;
+  }
+  if (threadIdx.x < kSteps) sh.exp2[threadIdx.x] = kExp2.v[threadIdx.x];
+  __syncthreads();
+  for (int64_t i = first + threadIdx.x; i < end; i += NT)
+    if (a.state[i].state != kAccepted) {
+      atomicMin(&sh.stop, (unsigned long long)i);
+      break;
+    }
+  __syncthreads();
+  const int64_t stop = (int64_t)sh.stop;
+  for (int64_t i = first + threadIdx.x; i < end; i += NT)
+    if (i != stop) a.token[i] = i < stop ? a.drafts[i] : -1;
+  if (stop >= end) return;  // (without rows)
+  const RowState st = a.state[stop];
+  if (threadIdx.x == 0) {
+    a.counts[r] = (int)(stop - first + 1);
+    if (st.state == kDrawn) a.token[stop] = st.token;
+  }
+  if (st.state == kDrawn) return;
+
+  const T* const x = (const T*)a.x + stop * a.ldx;
+  const Q* const q = (const Q*)a.q + stop * a.ldq;
+  const Weights weights = weights_of<T>(st.top, st.t, a.shift, sh.exp2);
+  const int pieces = (vocab + PIECE - 1) / PIECE;
+  // what is left of a kept token's weight
+  const double whole = (double)st.whole;
+  auto left_of = [&](uint32_t key, float prob, bool with_q) {
+    const uint64_t wf = weights.of(value_of<T>(key)), take = with_q ? share_of(prob, whole) : 0;
+    return wf >= st.least && wf > take ? wf - take : 0;
+  };
+  auto kept = [&](uint32_t key, int i) {
+    return key >= st.from && (key > st.tau || (key == st.tau && i < st.ties_end));
+  };
+  auto load = [&](int i, uint32_t (&key)[8], float (&prob)[8]) {
+    if (__all(i * 8 + 8 <= vocab)) {
+      Eight<T> raw;
+      raw.load(x + i * 8);
+      raw.keys(key);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) prob[e] = fmaxf((float)q[i * 8 + e], 0.f);
+    } else {
+      load_keys(x, i, vocab, key);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) prob[e] = i * 8 + e < vocab ? fmaxf((float)q[i * 8 + e], 0.f) : 0.f;
+    }
+  };
+  bool with_q = true;
+  uint64_t whole_left = 0, incl = 0, run = 0;
+  const int per = (pieces + 63) >> 6;
+  for (;; with_q = false) {
+    for (int c = w; c < pieces; c += NW) {
+      uint32_t key[8];
+      float prob[8];
+      load(c * 64 + lane, key, prob);
+      int some = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // the kept ones together: 64 of them take one evaluation
+        const bool k = kept(key[e], (c * 64 + lane) * 8 + e);
+        const uint64_t m = __ballot(k);
+        const int at = some + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+        if (k) {
+          sh.key[w][at] = key[e];
+          sh.q[w][at] = prob[e];
+        }
+        some += __popcll(m);
+      }
+      uint64_t sum = 0;
+      for (int i = lane; i < some; i += 64) sum += left_of(sh.key[w][i], sh.q[w][i], with_q);
+      if (some) sum = scan64(sum);
+      if (lane == 63) sh.sum[c] = sum;
+    }
+    __syncthreads();
+    run = 0;  // (every wave the same)
+    for (int c = lane * per; c < min(lane * per + per, pieces); ++c) run += sh.sum[c];
+    incl = scan64(run);
+    whole_left = shfl64(incl, 63);
+    __syncthreads();
+    if (whole_left || !with_q) break;  // (nothing left: the draft's distribution covers the target's; from p then)
+  }
+  if (w != 0) return;
+  const uint64_t goal = __umul64hi(fraction64(unit(a.draw[r])), whole_left);
+  const int l = __ffsll((unsigned long long)__ballot(incl > goal)) - 1;
+  uint64_t sum = shfl64(incl - run, l);
+  int at = l * per;
+  for (;; ++at) {  // (every lane the same)
+    if (sum + sh.sum[at] > goal || at + 1 >= min((l + 1) * per, pieces)) break;
+    sum += sh.sum[at];
+  }
+  uint32_t key[8];
+  float prob[8];
+  load(at * 64 + lane, key, prob);
+  uint64_t own[8], mine = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    own[e] = kept(key[e], (at * 64 + lane) * 8 + e) ? left_of(key[e], prob[e], with_q) : 0;
+    mine += own[e];
+  }
+  const uint64_t s = sum + scan64(mine);
+  const uint64_t reach = __ballot(s > goal);
+  if (lane == __ffsll((unsigned long long)reach) - 1) {
+    uint64_t so_far = s - mine;
+    int e = 0;
+    for (; e < 7; ++e) {
+      so_far += own[e];
+      if (so_far > goal) break;
+    }
+    a.token[stop] = (int64_t)(at * 64 + lane) * 8 + e;
   }
 }
 
 }  // namespace
 
-hipError_t launch_sample(const SampleProblem& p, hipStream_t stream) {
-  SArgs a{};
+static void settings(const SampleProblem& p, SArgs& a) {
   a.x = (const char*)p.logits;
   a.u = p.u;
   a.temperature = p.temperature;
@@ -952,9 +1244,47 @@ hipError_t launch_sample(const SampleProblem& p, hipStream_t stream) {
   a.k = p.k;
   a.p = p.p;
   a.m = p.m;
-  const auto fn = p.dtype == DT_F16 ? sample_rows<_Float16> : p.dtype == DT_BF16 ? sample_rows<__bf16> : sample_rows<float>;
+}
+
+hipError_t launch_sample(const SampleProblem& p, hipStream_t stream) {
+  SArgs a{};
+  settings(p, a);
+  const auto fn = p.dtype == DT_F16    ? sample_rows<_Float16, SArgs>
+                  : p.dtype == DT_BF16 ? sample_rows<__bf16, SArgs>
+                                       : sample_rows<float, SArgs>;
   hipLaunchKernelGGL(fn, dim3((unsigned)p.rows), dim3(NT), 0, stream, a);
   return hipGetLastError();
+}
+
+int64_t verify_workspace_bytes(int64_t rows) { return kWsCounterBytes + rows * (int64_t)sizeof(RowState); }
+
+template <typename T>
+static hipError_t launch_verify_t(const VerifyProblem& p, const VArgs& a, hipStream_t stream) {
+  if (p.rows) hipLaunchKernelGGL((sample_rows<T, VArgs>), dim3((unsigned)p.rows), dim3(NT), 0, stream, a);
+  const auto fn = p.q_type == SAMPLE_F32 ? verify_rows<T, float>
+                  : p.q_type == DT_BF16  ? verify_rows<T, __bf16>
+                                         : verify_rows<T, _Float16>;
+  if (p.requests) hipLaunchKernelGGL(fn, dim3((unsigned)p.requests), dim3(NT), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_verify(const VerifyProblem& p, hipStream_t stream) {
+  VArgs a{};
+  settings(p, a);
+  a.drafts = p.drafts;
+  a.draw = p.draw;
+  a.cu = p.cu;
+  a.q = (const char*)p.q;
+  a.ldq = p.ldq;
+  a.rows = p.rows;
+  a.state = (RowState*)((char*)p.ws + kWsCounterBytes);
+  a.counts = p.counts;
+  a.requests = (int)p.requests;
+  a.per = p.requests ? (int)(p.rows / p.requests) : 0;
+  a.q_type = p.q_type;
+  return p.dtype == DT_F16    ? launch_verify_t<_Float16>(p, a, stream)
+         : p.dtype == DT_BF16 ? launch_verify_t<__bf16>(p, a, stream)
+                              : launch_verify_t<float>(p, a, stream);
 }
 
 }  // namespace hxmi

@@ -735,6 +735,35 @@ PyObject* op_qk_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// hxmi_sample's type of a tensor, -1 for none.
+int sample_type(const Tensor& t) {
+  return t.scalar_type() == at::kHalf       ? HXMI_SAMPLE_F16
+         : t.scalar_type() == at::kBFloat16 ? HXMI_SAMPLE_BF16
+         : t.scalar_type() == at::kFloat    ? HXMI_SAMPLE_F32
+                                            : -1;
+}
+// temperature, top_k, top_p and min_p: tensors of shape `lead`, or numbers for all.
+struct Settings {
+  const Tensor* own[4] = {};
+  double all[4] = {1, 0, 1, 0};
+
+  bool take(Operands& in, PyObject* const* args, at::IntArrayRef lead) {
+    for (int i = 0; i < 4; ++i) {
+      if (THPVariable_Check(args[i])) {
+        own[i] = in.get(args[i]);
+        if (!(in.ok && own[i]->sizes() == lead && own[i]->is_contiguous() &&
+              own[i]->scalar_type() == (i == 1 ? at::kInt : at::kFloat)))
+          return false;
+      } else {
+        long k;
+        if (!(i == 1 ? number(args[1], k) && k >= 0 && k < (1l << 31) : number(args[i], all[i]))) return false;
+        if (i == 1) all[1] = (double)k;
+      }
+    }
+    return true;
+  }
+};
+
 // sample(logits, u, temperature, top_k, top_p, min_p)
 PyObject* op_sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -743,36 +772,58 @@ PyObject* op_sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor *x = in.get(args[0]), *u = in.get(args[1]);
   NOT_PLAIN_UNLESS(in.ok && x->dim() >= 1 && x->numel() > 0);
   int64_t M, V, ld;
-  const int dtype = x->scalar_type() == at::kHalf       ? HXMI_SAMPLE_F16
-                    : x->scalar_type() == at::kBFloat16 ? HXMI_SAMPLE_BF16
-                    : x->scalar_type() == at::kFloat    ? HXMI_SAMPLE_F32
-                                                        : -1;
+  const int dtype = sample_type(*x);
   const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
   NOT_PLAIN_UNLESS(dtype >= 0 && as_rows(*x, M, V, ld) && u->sizes() == lead && u->is_contiguous() &&
                    u->scalar_type() == at::kFloat);
-  const Tensor* own[4] = {};
-  double all[4] = {1, 0, 1, 0};
-  for (int i = 0; i < 4; ++i) {
-    if (THPVariable_Check(args[2 + i])) {
-      own[i] = in.get(args[2 + i]);
-      NOT_PLAIN_UNLESS(in.ok && own[i]->sizes() == lead && own[i]->is_contiguous() &&
-                       own[i]->scalar_type() == (i == 1 ? at::kInt : at::kFloat));
-    } else {
-      long k;
-      NOT_PLAIN_UNLESS(i == 1 ? number(args[3], k) && k >= 0 && k < (1l << 31) : number(args[2 + i], all[i]));
-      if (i == 1) all[1] = (double)k;
-    }
-  }
+  Settings set;
+  NOT_PLAIN_UNLESS(set.take(in, args + 2, lead));
   const c10::DeviceGuard guard(x->device());
   const Tensor out = fresh(*x, lead, at::kLong);
   void* s = in.stream();
   return result(unlocked([&] {
-                  return hxmi_sample(dtype, ptr(x), (const float*)ptr(u), (const float*)ptr(own[0]),
-                                     (const int32_t*)ptr(own[1]), (const float*)ptr(own[2]), (const float*)ptr(own[3]),
-                                     (float)all[0], (int32_t)all[1], (float)all[2], (float)all[3], (int64_t*)ptr(&out),
-                                     M, V, ld, s);
+                  return hxmi_sample(dtype, ptr(x), (const float*)ptr(u), (const float*)ptr(set.own[0]),
+                                     (const int32_t*)ptr(set.own[1]), (const float*)ptr(set.own[2]),
+                                     (const float*)ptr(set.own[3]), (float)set.all[0], (int32_t)set.all[1],
+                                     (float)set.all[2], (float)set.all[3], (int64_t*)ptr(&out), M, V, ld, s);
                 }),
                 out);
+  END_HANDLE_TH_ERRORS
+}
+
+// verify(logits, drafts, u, draw, cu or None, draft_probs or None, temperature, top_k, top_p, min_p)
+PyObject* op_verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NOT_PLAIN_UNLESS(n == 10);
+  Operands in;
+  const Tensor *x = in.get(args[0]), *drafts = in.get(args[1]), *u = in.get(args[2]), *draw = in.get(args[3]),
+               *cu = in.get(args[4], true), *q = in.get(args[5], true);
+  NOT_PLAIN_UNLESS(in.ok && x->dim() == (cu ? 2 : 3) && x->numel() > 0 && draw->dim() == 1 && draw->size(0) > 0);
+  const int64_t R = draw->size(0);
+  int64_t M, V, ld, Mq, Vq, ldq = 0;
+  const int dtype = sample_type(*x), qtype = q ? sample_type(*q) : HXMI_SAMPLE_F32;
+  const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
+  NOT_PLAIN_UNLESS(dtype >= 0 && qtype >= 0 && as_rows(*x, M, V, ld) && (cu || x->size(0) == R) &&
+                   vec(cu, R + 1, at::kInt) && vec(draw, R, at::kFloat));
+  NOT_PLAIN_UNLESS(drafts->sizes() == lead && drafts->is_contiguous() && drafts->scalar_type() == at::kLong &&
+                   u->sizes() == lead && u->is_contiguous() && u->scalar_type() == at::kFloat &&
+                   (!q || (q->sizes() == x->sizes() && as_rows(*q, Mq, Vq, ldq))));
+  Settings set;
+  NOT_PLAIN_UNLESS(set.take(in, args + 6, {R}));
+  const c10::DeviceGuard guard(x->device());
+  const Tensor tokens = fresh(*x, lead, at::kLong), counts = fresh(*x, {R}, at::kInt);
+  const Workspace ws(hxmi_verify_workspace_bytes(M), *x);
+  if (!ws.ok) return nullptr;
+  void* s = in.stream();
+  const int rc = unlocked([&] {
+    return hxmi_verify(dtype, ptr(x), (const int64_t*)ptr(drafts), (const float*)ptr(u), (const float*)ptr(draw),
+                       (const int32_t*)ptr(cu), ptr(q), qtype, (const float*)ptr(set.own[0]),
+                       (const int32_t*)ptr(set.own[1]), (const float*)ptr(set.own[2]), (const float*)ptr(set.own[3]),
+                       (float)set.all[0], (int32_t)set.all[1], (float)set.all[2], (float)set.all[3],
+                       (int64_t*)ptr(&tokens), (int32_t*)ptr(&counts), M, R, V, ld, ldq, ws.data, ws.bytes, s);
+  });
+  if (rc != HXMI_OK) Py_RETURN_NONE;
+  return Py_BuildValue("(NN)", THPVariable_Wrap(tokens), THPVariable_Wrap(counts));
   END_HANDLE_TH_ERRORS
 }
 
@@ -781,6 +832,7 @@ PyMethodDef kMethods[] = {ENTRY(gemm),         ENTRY(bgemm),    ENTRY(linear),  
                           ENTRY(w8a16_linear), ENTRY(rms_norm), ENTRY(softmax), ENTRY(attention),
                           ENTRY(kv_plan),      ENTRY(kv_append), ENTRY(kv_read), ENTRY(kv_attention),  ENTRY(sample),
                           ENTRY(kv4_append),   ENTRY(kv4_read), ENTRY(kv4_attention), ENTRY(qk_rope),
+                          ENTRY(verify),
                           {"set_workspace", set_workspace, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "hxmi_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

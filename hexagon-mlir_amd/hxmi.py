@@ -81,6 +81,8 @@ SIGNATURES = {
     "hxmi_kv4_attention_workspace_bytes": ([_I64] * 7 + [_I], _I64),
     "hxmi_qk_rope": ([_I] + [_P] * 5 + [_I] + [_P] * 4 + [_I] + [_I64] * 15 + [_I, _F, _F, _P], _I),
     "hxmi_sample": ([_I] + [_P] * 6 + [_F, ctypes.c_int32, _F, _F, _P] + [_I64] * 3 + [_P], _I),
+    "hxmi_verify": ([_I] + [_P] * 6 + [_I] + [_P] * 4 + [_F, ctypes.c_int32, _F, _F, _P, _P] + [_I64] * 5 + [_P, _I64, _P], _I),
+    "hxmi_verify_workspace_bytes": ([_I64], _I64),
     "hxmi_lwp_record": ([_P, _I64, ctypes.c_uint32, _P], _I),
     "hxmi_lwp_clock_hz": ([], _I64),
     "hexkl_matmul_f16f16_f32": ([_I64, _I64, _I64, _P, _P, _P], _I),
@@ -1433,6 +1435,24 @@ def kv_attention(q: torch.Tensor, cache: Union[KVCache, KVCache4], block_table: 
 _SAMPLE_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
+def _sample_settings(given: list, lead) -> tuple[list, list, list]:
+    """Pointers (or None), values for all, and what keeps the pointers alive, of
+    temperature, top_k, top_p and min_p, each a number or a tensor of shape `lead`."""
+    ptrs, alls, keep = [], [], []
+    for name, p, dtype, neutral in zip(("temperature", "top_k", "top_p", "min_p"), given,
+                                       (torch.float32, torch.int32, torch.float32, torch.float32), (1.0, 0, 1.0, 0.0)):
+        if isinstance(p, torch.Tensor):
+            if p.shape != lead or p.dtype != dtype:
+                raise HxmiError(f"{name} must be a number or a {dtype} tensor {tuple(lead)}")
+            keep.append(p.contiguous())
+            ptrs.append(keep[-1].data_ptr())
+            alls.append(neutral)
+        else:
+            ptrs.append(None)
+            alls.append(max(-1, min(int(p), 2**31 - 1)) if dtype == torch.int32 else float(p))
+    return ptrs, alls, keep
+
+
 def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[float, torch.Tensor] = 1.0,
            top_k: Union[int, torch.Tensor] = 0, top_p: Union[float, torch.Tensor] = 1.0,
            min_p: Union[float, torch.Tensor] = 0.0) -> torch.Tensor:
@@ -1456,18 +1476,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[float, t
     rows, vocab = math.prod(lead), logits.shape[-1]
     if u.shape != lead or u.dtype != torch.float32:
         raise HxmiError(f"u must be torch.float32 {tuple(lead)}, got {u.dtype} {tuple(u.shape)}")
-    ptrs, alls, keep = [], [], []
-    for name, p, dtype, neutral in zip(("temperature", "top_k", "top_p", "min_p"), given,
-                                       (torch.float32, torch.int32, torch.float32, torch.float32), (1.0, 0, 1.0, 0.0)):
-        if isinstance(p, torch.Tensor):
-            if p.shape != lead or p.dtype != dtype:
-                raise HxmiError(f"{name} must be a number or a {dtype} tensor {tuple(lead)}")
-            keep.append(p.contiguous())
-            ptrs.append(keep[-1].data_ptr())
-            alls.append(neutral)
-        else:
-            ptrs.append(None)
-            alls.append(max(-1, min(int(p), 2**31 - 1)) if dtype == torch.int32 else float(p))
+    ptrs, alls, keep = _sample_settings(given, lead)
     out = torch.empty(lead, dtype=torch.int64, device=logits.device)
     if rows == 0:
         return out
@@ -1479,6 +1488,86 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[float, t
         _check(load_library().hxmi_sample(_SAMPLE_TYPES[x.dtype], x.data_ptr(), u.data_ptr(), *ptrs, *alls,
                                           out.data_ptr(), rows, vocab, _lead(x, "logits"), _stream(x)))
     return out
+
+
+class Verified(NamedTuple):
+    """What verify gives: tokens, in the shape of the drafts (a request's
+    accepted drafts, the token drawn after them, then -1), and counts [requests]
+    (int32), the number of a request's tokens."""
+    tokens: torch.Tensor
+    counts: torch.Tensor
+
+
+def verify(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor, draw: torch.Tensor, *,
+           cu: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None,
+           temperature: Union[float, torch.Tensor] = 1.0, top_k: Union[int, torch.Tensor] = 0,
+           top_p: Union[float, torch.Tensor] = 1.0, min_p: Union[float, torch.Tensor] = 0.0) -> Verified:
+    """Drafted tokens against the target's distribution, so that what comes out
+    is distributed as tokens that sample draws one at a time.
+
+    logits [requests, rows, vocab], or [tokens, vocab] with the requests' bounds
+    cu [requests + 1] (int32), fp16, bf16 or fp32: a row for each drafted token
+    and one more.  drafts (int64) and u (fp32, in [0, 1)) have the rows' shape
+    (a request's last row has no draft: it is not read), draw [requests] is fp32.
+    With p a row's distribution under the settings, as sample keeps and weights
+    its tokens, and q the draft's (draft_probs, the logits' shape, fp16, bf16 or
+    fp32; None: the drafted token was certain, as one copied from the prompt is), a
+    draft d is accepted while p[d] > u * q[d].  At the first that is not, a token is
+    drawn from max(p - q, 0); if all are, from the last row's p.  Each setting is a
+    number or a tensor of the requests' own [requests] (fp32, top_k int32);
+    temperature 0 accepts the largest logits.  A row with a NaN or no logit above
+    -inf accepts nothing and draws -1."""
+    y = _ops.verify(logits, drafts, u, draw, cu, draft_probs, temperature, top_k, top_p, min_p)
+    if y is not None:
+        return Verified(*y)
+    given = [temperature, top_k, top_p, min_p]
+    _require_gpu(logits, drafts, u, draw, cu, draft_probs, *(p for p in given if isinstance(p, torch.Tensor)))
+    if logits.dtype not in _SAMPLE_TYPES:
+        raise HxmiError(f"verify takes fp16, bf16 or fp32 logits, got {logits.dtype}")
+    if logits.dim() != (3 if cu is None else 2):
+        raise HxmiError(f"logits must be [requests, rows, vocab], or [tokens, vocab] with cu, got {tuple(logits.shape)}")
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    rows = math.prod(lead)
+    if draw.dim() != 1 or draw.dtype != torch.float32:
+        raise HxmiError("draw must be a 1-D torch.float32 tensor")
+    R = draw.numel()
+    if cu is None:
+        if lead[0] != R:
+            raise HxmiError(f"draw must have an entry for each of the {lead[0]} requests, got {R}")
+    else:
+        cu = _ints(cu, R + 1, "cu")
+    if drafts.shape != lead or drafts.dtype != torch.int64:
+        raise HxmiError(f"drafts must be torch.int64 {tuple(lead)}, got {drafts.dtype} {tuple(drafts.shape)}")
+    if u.shape != lead or u.dtype != torch.float32:
+        raise HxmiError(f"u must be torch.float32 {tuple(lead)}, got {u.dtype} {tuple(u.shape)}")
+    if draft_probs is not None and (draft_probs.shape != logits.shape or draft_probs.dtype not in _SAMPLE_TYPES):
+        raise HxmiError(f"draft_probs must be fp16, bf16 or fp32 {tuple(logits.shape)}, got {draft_probs.dtype} "
+                        f"{tuple(draft_probs.shape)}")
+    ptrs, alls, keep = _sample_settings(given, (R,))
+    tokens = torch.empty(lead, dtype=torch.int64, device=logits.device)
+    counts = torch.empty(R, dtype=torch.int32, device=logits.device)
+    if rows and not R:
+        raise HxmiError("rows without a request")
+
+    def flat(t):
+        t = t.reshape(rows, vocab)
+        return _own_rows(t if t.stride(1) == 1 or vocab <= 1 else t.contiguous())
+
+    drafts, u, draw = drafts.contiguous(), u.contiguous(), draw.contiguous()
+    lib = load_library()
+    with _on(logits):
+        if not rows:
+            tokens.fill_(-1)
+            counts.zero_()
+            return Verified(tokens, counts)
+        x, q = flat(logits), None if draft_probs is None else flat(draft_probs)
+        ws = _workspace(lib.hxmi_verify_workspace_bytes(rows), x.device)
+        _check(lib.hxmi_verify(
+            _SAMPLE_TYPES[x.dtype], x.data_ptr(), drafts.data_ptr(), u.data_ptr(), draw.data_ptr(), _ptr(cu), _ptr(q),
+            2 if q is None else _SAMPLE_TYPES[q.dtype], *ptrs, *alls, tokens.data_ptr(), counts.data_ptr(), rows, R, vocab,
+            _lead(x, "logits"), 0 if q is None else _lead(q, "draft_probs"), _ptr(ws), 0 if ws is None else ws.numel() * 4,
+            _stream(x)))
+    return Verified(tokens, counts)
 
 
 def release_workspaces() -> None:

@@ -650,6 +650,39 @@ int hxmi_sample(int dtype, const void* logits, const float* u, const float* temp
                 float all_min_p, int64_t* tokens, int64_t rows, int64_t vocab, int64_t ldx, void* stream);
 
 /*
+ * Drafted tokens against the target's distribution.  logits [rows, vocab] (row
+ * stride ldx, dtype as hxmi_sample's) are the rows of `requests` requests: cu[r]
+ * to cu[r+1] (cu NULL: rows / requests each).  Row i of a request is the target's
+ * answer to the tokens before its drafted token drafts[i]; the last row has no draft
+ * (drafts there is not read).  With a row's weights and kept tokens as in
+ * hxmi_sample, under its request's settings, p = kept weight / their sum and q =
+ * draft_probs [rows, vocab] (row stride ld_probs, of probs_dtype; NULL: 1 for the
+ * drafted token, 0 for all others):
+ *   a draft d is accepted if p[d] > u * q[d], u [rows] in [0, 1);
+ *   at the first row that is not, a token is drawn from max(p - q, 0) (from p
+ *   where nothing is left of that); if all are, from the last row's p: the
+ *   lowest index whose running sum, in index order, exceeds draw * (the whole),
+ *   draw [requests] in [0, 1).
+ * tokens [rows] becomes a request's accepted drafts, the drawn token after them
+ * and -1 in its other rows and in rows of no request; counts [requests] how many
+ * that are (0 for a request without rows).  A draft outside the vocabulary is not
+ * accepted; probabilities that are NaN or negative count as 0 (draft_probs need not
+ * sum to 1); a row with a NaN logit or none above -inf accepts nothing and draws -1.
+ * Settings are per request (pointers of `requests` entries) or, where NULL, the
+ * all_* value.  Weights are integers as in hxmi_sample, q * (their sum) rounded
+ * down to one.  workspace: hxmi_verify_workspace_bytes(rows) bytes, 256-byte
+ * aligned; its first HXMI_WORKSPACE_COUNTER_BYTES are left alone.  vocab <= 2^20.
+ * No counterpart in the reference.
+ */
+int hxmi_verify(int dtype, const void* logits, const int64_t* drafts, const float* u, const float* draw,
+                const int32_t* cu, const void* draft_probs, int probs_dtype, const float* temperature,
+                const int32_t* top_k, const float* top_p, const float* min_p, float all_temperature,
+                int32_t all_top_k, float all_top_p, float all_min_p, int64_t* tokens, int32_t* counts, int64_t rows,
+                int64_t requests, int64_t vocab, int64_t ldx, int64_t ld_probs, void* workspace,
+                int64_t workspace_bytes, void* stream);
+int64_t hxmi_verify_workspace_bytes(int64_t rows);
+
+/*
  * Region profiling hook: enqueues on `stream` a one-wave marker that, when it
  * runs (after every kernel enqueued before it on that stream has finished),
  * writes record `slot` of `records` -- three uint32 words {id, t low word,

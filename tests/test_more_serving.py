@@ -1,4 +1,4 @@
-"""CPU checks of qk_rope's and the 4-bit cache's entries: what they refuse
+"""CPU checks of qk_rope's, the 4-bit cache's and verify's entries: what they refuse
 before any launch, empty calls, workspace sizes and the cache's layout."""
 import pytest
 import torch
@@ -79,7 +79,34 @@ def test_attention_refuses(pkg, bad, msg):
     assert msg in last(pkg) and "hxmi_kv4_attention" in last(pkg)
 
 
+def verify(pkg, dtype=0, x=P, d=P, u=P, draw=P, cu=P, q=P, q_type=2, t=1.0, k=0, p=1.0, m=0.0, out=P, counts=P, rows=6,
+           requests=2, vocab=100, ld=100, ldq=100, ws=P, ws_bytes=1 << 20):
+    return pkg.load_library().hxmi_verify(dtype, x, d, u, draw, cu, q, q_type, None, None, None, None, t, k, p, m, out, counts,
+                                          rows, requests, vocab, ld, ldq, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("bad, msg", [
+    (dict(dtype=3), "dtype"), (dict(q_type=-1), "probs_dtype"), (dict(rows=-1), "rows"), (dict(requests=-1), "requests"),
+    (dict(requests=0), "without a request"), (dict(cu=None, rows=5), "same number"), (dict(vocab=0), "vocab"),
+    (dict(vocab=(1 << 20) + 1, ld=1 << 21, ldq=1 << 21), "vocab"), (dict(ld=99), "leading dimension"),
+    (dict(ldq=99), "draft_probs"), (dict(x=None), "null"), (dict(u=None), "null"), (dict(d=None), "null drafts"),
+    (dict(draw=None), "null draw"), (dict(counts=None), "counts"), (dict(out=None), "null"), (dict(x=P + 1), "aligned"),
+    (dict(q=P + 2), "aligned"), (dict(t=-0.5), "temperature"), (dict(t=float("nan")), "temperature"),
+    (dict(p=float("nan")), "top_p"), (dict(m=float("nan")), "min_p"), (dict(ws=None), "workspace"),
+    (dict(ws=P + 16), "workspace"), (dict(ws_bytes=16384), "workspace"),
+])
+def test_verify_refuses(pkg, bad, msg):
+    assert verify(pkg, **bad) == 1
+    assert msg in last(pkg)
+
+
+def test_verify_workspace(pkg):
+    need = pkg.load_library().hxmi_verify_workspace_bytes
+    assert need(0) == need(-1) == 0 and need(1) > 16384 and need(100) - need(1) == 99 * (need(2) - need(1))
+
+
 def test_empty_calls_do_nothing(pkg):
+    assert verify(pkg, rows=0, requests=0, x=None, draw=None) == 0
     assert rope(pkg, tokens=0, q=None, k=None, pos=None) == 0 and rope(pkg, heads=0, kv_heads=0, q=None, k=None) == 0
     assert append(pkg, tokens=0, ptr=None) == 0 and append(pkg, blocks=0, codes=None, scale=None) == 0
     assert read(pkg, tokens=0, ptr=None) == 0
@@ -123,6 +150,7 @@ def test_ops_refuse_cpu_tensors(pkg):
     x, i = torch.zeros(2, 1, 64, dtype=torch.float16), torch.zeros(2, dtype=torch.int32)
     table, freq = torch.zeros(2, 1, dtype=torch.int32), torch.zeros(32, dtype=torch.float64)
     for call in (lambda: pkg.kv_append(c, x, x, i.long()), lambda: pkg.kv_read(c, i.long()),
-                 lambda: pkg.kv_attention(x, c, table, i), lambda: pkg.qk_rope(x, x, i, freq)):
+                 lambda: pkg.kv_attention(x, c, table, i), lambda: pkg.qk_rope(x, x, i, freq),
+                 lambda: pkg.verify(x, torch.zeros(2, 1, dtype=torch.int64), torch.zeros(2, 1), torch.zeros(2))):
         with pytest.raises(pkg.HxmiError, match="GPU"):
             call()

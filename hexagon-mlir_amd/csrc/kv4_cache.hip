@@ -10,6 +10,7 @@ namespace {
 using namespace kv4;
 
 typedef uint32_t uint1u __attribute__((aligned(2)));  // (rows start anywhere)
+typedef int int4u __attribute__((ext_vector_type(4), aligned(2)));
 
 struct CArgs {
   const char* x[2];  // rows of k and of v
@@ -45,17 +46,41 @@ __device__ __forceinline__ float quotient(float x, float inv) {
 // What is held for x: infinities and NaN as the largest value.
 __device__ __forceinline__ float held(float x) { return x != x ? kMost : fminf(fmaxf(x, -kMost), kMost); }
 
+template <int CTRL, int BANKS = 0xf>
+__device__ __forceinline__ uint32_t dpp(uint32_t old, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, 0xf, BANKS, false);
+}
+// Eight lanes l % 8 hold a row of eight 4-bit numbers each: lane j's become the
+// numbers j of all of them, lane 0's first.  Halves, quarters and eighths of the words in turn
+// go to the lane 4, 2 and 1 away.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t o = dpp<0x104, 0x5>(0, v);  // row_shl:4, for lanes without bit 2
+  o = dpp<0x114, 0xa>(o, v);           // row_shr:4, for the others
+  v = threadIdx.x & 4 ? __builtin_amdgcn_perm(v, o, 0x07060302u) : __builtin_amdgcn_perm(o, v, 0x05040100u);
+  o = dpp<0x4e>(0, v);  // lane l ^ 2
+  v = threadIdx.x & 2 ? __builtin_amdgcn_perm(v, o, 0x07030501u) : __builtin_amdgcn_perm(o, v, 0x06020400u);
+  o = dpp<0xb1>(0, v);  // lane l ^ 1
+  return threadIdx.x & 1 ? (v & 0xf0f0f0f0u) | (o >> 4 & 0x0f0f0f0fu) : (v & 0x0f0f0f0fu) | (o << 4 & 0xf0f0f0f0u);
+}
+
 // A wave writes one run (up to 16 rows of the call that go to consecutive slots
-// of one piece of 16 tokens) of one head of K or V, two dims a lane: 16 lanes'
-// largest magnitude gives a scale, and nothing that is in the cache already
-// changes.  A run is found by its first row: the row before it does not go to
-// the slot before, or to another piece.
+// of one piece of 16 tokens) of one head of K or V.  A run is found by its first
+// row: the row before it does not go to the slot before, or to another piece.  Lane l takes
+// token l % 8 of half a piece and eight dims of 64, so four lanes (l, l + 8, l +
+// 16, l + 24) have a scale in common; K's eight numbers are a word of the
+// cache, V's become one by an exchange between the eight tokens' lanes.  Nothing that
+// is in the cache already changes.
+// The code is kept short: a wave meets it cold, and with a run's rows unrolled (two
+// dims a lane, 1900 instructions) fetching them cost more than all loads and
+// stores (8900 rows of 4 x 64: 17.7 us).
 template <typename T>
 __global__ __launch_bounds__(256) void kv4_append(CArgs a) {
   const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int hv = (int)(item % (2 * a.heads)), h = hv >> 1, is_v = hv & 1;
-  const int64_t t0 = item / (2 * a.heads) * a.span;  // (a.span <= 48: a run that begins there ends within 64 rows)
+  // item: rows, head, 64 dims, K or V
+  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wide = a.dp > 64;
+  const uint32_t parts = 2u * a.heads << wide, group = item / parts, part = item - group * parts;
+  const int is_v = part & 1, h = (int)(part >> (1 + wide)), d = (lane & ~7) + (part >> 1 & wide) * 64, token = lane & 7;
+  const int64_t t0 = (int64_t)group * a.span;  // (a.span <= 48: a run that begins there ends within 64 rows)
   int64_t slot_l = -1;
   bool begins = false;
   if (t0 + lane < a.tokens) {
@@ -63,7 +88,9 @@ __global__ __launch_bounds__(256) void kv4_append(CArgs a) {
     const int64_t before = t0 + lane > 0 ? a.slots[t0 + lane - 1] : -1;
     begins = slot_l >= 0 && slot_l < a.cells && ((slot_l & 15) == 0 || before != slot_l - 1);
   }
-  const bool mine = 2 * lane < a.dp, filled = 2 * lane < a.d;
+  const int64_t ld = a.ld[is_v];
+  const bool mine = d < a.dp;
+#pragma unroll 1
   for (uint64_t runs = __ballot(begins && lane < a.span); runs; runs &= runs - 1) {
     const int l = __ffsll((unsigned long long)runs) - 1;
     const int64_t slot = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)slot_l, l) |
@@ -71,108 +98,116 @@ __global__ __launch_bounds__(256) void kv4_append(CArgs a) {
     const int off = (int)(slot & 15);
     const uint64_t miss = ~(__ballot(lane >= l && slot_l == slot + (lane - l)) >> l);  // (lane l's own bit is 0)
     const int n = min(16 - off, miss ? __ffsll((unsigned long long)miss) - 1 : 64);
-    const T* const x = (const T*)a.x[is_v] + (t0 + l) * a.ld[is_v] + h * a.hs[is_v] + 2 * lane;
-    const int64_t ld = a.ld[is_v], at = slot & ((1 << a.lb) - 1), cell = (slot >> a.lb) * a.heads + h;
-
-    uint32_t raw[16], byte[16], sb = 0;
+    const int64_t at = (slot & ((1 << a.lb) - 1)) - off, cell = (slot >> a.lb) * a.heads + h;  // the piece
+    // (token i of the piece is row i - off of the run)
+    const T* const x = (const T*)a.x[is_v] + (t0 + l - off + token) * ld + h * a.hs[is_v] + d;
+    uint8_t* const scale = a.scale[is_v] + (((cell * (a.dp >> 5) + (d >> 5)) << a.lb) + at) + token;
+    uint8_t* const keys = a.codes[0] + ((cell << a.lb) + at + token) * (a.dp >> 1) + (d >> 1);
+    const uint32_t held_by = (uint32_t)(0xffff >> (16 - n) << off);  // a bit a token
+    int4v raw[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      raw[i] = 0;
-      if (i < n && filled) raw[i] = *(const uint1u*)(x + i * ld);
+    for (int i = 0; i < 2; ++i) {
+      raw[i] = int4v{};
+      if (d < a.d && held_by >> (8 * i + token) & 1) raw[i] = *(const int4u*)(x + 8 * i * ld);
     }
+    uint64_t both = 0;
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      if (!(held_by >> (8 * i) & 0xff)) continue;
+      const int4v r = i ? raw[1] : raw[0];
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      byte[i] = 0;
-      if (i >= n) continue;  // (uniform)
-      T two[2];
-      __builtin_memcpy(two, &raw[i], 4);
-      const float x0 = held((float)two[0]), x1 = held((float)two[1]);
-      const float most = wave_reduce_dpp<16>(fmaxf(fabsf(x0), fabsf(x1)), [](float p, float q) { return fmaxf(p, q); });
-      const uint32_t b = scale_byte(most);
-      const float inv = b ? 1.f / scale_value(b) : 0.f;
-      byte[i] = (uint32_t)__builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, quotient(x0, inv), quotient(x1, inv), 1.f, 0) & 0xffu;
-      sb = (lane & 15) == i ? b : sb;
-    }
-    // scales: lane 16 g + i has row i's of group g
-    if (mine && (lane & 15) < n) a.scale[is_v][(((cell * (a.dp >> 5) + (lane >> 4)) << a.lb) + at) + (lane & 15)] = (uint8_t)sb;
-    if (!is_v) {
-      uint8_t* const dst = a.codes[0] + ((cell << a.lb) + at) * (a.dp >> 1) + lane;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < n && mine) dst[i * (a.dp >> 1)] = (uint8_t)byte[i];
-    } else if (mine) {
-      // row i is token off + i of the piece: two dims' sixteen halves of bytes
-      uint64_t d0 = 0, d1 = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        d0 |= (uint64_t)(byte[i] & 15) << (4 * i);
-        d1 |= (uint64_t)(byte[i] >> 4) << (4 * i);
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t b = (uint32_t)r[e] & 0x7fff7fffu;
+        top = max(top, max(b & 0xffffu, b >> 16));
       }
-      uint64_t* const dst = (uint64_t*)(a.codes[1] + (((cell << (a.lb - 4)) + (at >> 4)) * a.dp + 2 * lane) * 8);
+      top = max(top, dpp<0x128>(0, top));  // row_ror:8
+      const auto r16 = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+      top = max((uint32_t)r16[0], (uint32_t)r16[1]);
+      const float amax = (float)__builtin_bit_cast(T, (unsigned short)top);
+      const bool past = !(amax <= kMost);  // (or no number)
+      const uint32_t sb = scale_byte(past ? kMost : amax);
+      const float inv = sb ? __builtin_amdgcn_rcpf(scale_value(sb)) : 0.f;
+      T f[8];
+      __builtin_memcpy(f, &r, 16);
+      float q[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = (float)f[e];
+      if (__any(past)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = held(q[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = quotient(q[e], inv);
+      uint32_t word = 0;
+      static_for<4>([&](auto e) {
+        word = (uint32_t)__builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, q[2 * e], q[2 * e + 1], 1.f, e);
+      });
+      const bool in = mine && held_by >> (8 * i + token) & 1;
+      if (in && (lane & 24) == 0) scale[8 * i] = (uint8_t)sb;
+      if (!is_v) {
+        if (in) *(uint32_t*)(keys + 8 * i * (a.dp >> 1)) = word;
+      } else {
+        both |= (uint64_t)transpose8(word) << (32 * i);
+      }
+    }
+    if (is_v && mine) {
+      // this lane's dim is d + token: sixteen tokens
       const uint64_t mask = (n == 16 ? ~0ull : (1ull << (4 * n)) - 1) << (4 * off);
-      d0 <<= 4 * off;
-      d1 <<= 4 * off;
-      if (n < 16) {
-        d0 |= dst[0] & ~mask;
-        d1 |= dst[1] & ~mask;
-      }
-      dst[0] = d0;
-      dst[1] = d1;
+      uint64_t* const dst = (uint64_t*)(a.codes[1] + (((cell << (a.lb - 4)) + (at >> 4)) * a.dp + d + token) * 8);
+      both &= mask;
+      if (n < 16) both |= *dst & ~mask;
+      *dst = both;
     }
   }
 }
 
 // ---- kv4_read --------------------------------------------------------------------
 
-// Outputs [tokens, heads, d], zeros for a slot outside the cache.  A wave takes 16
-// rows of a head of K or of V, two dims a lane, piece of 16 tokens by piece: those
-// of a piece take their V numbers from one 16-byte load a lane.
+// Outputs [tokens, heads, d], zeros for a slot outside the cache.  A lane takes eight
+// dims of a row: of K four bytes, of V their piece's 64 bytes (the other rows of the
+// piece take the same ones out of the cache next to the CU), a number of each eight.
+// 2^log lanes a row; one row a lane: two or four in flight were slower (4336 rows
+// of 8 x 128: 8.8 us, 9.4 and 11.0).
 template <typename T>
-__global__ __launch_bounds__(256) void kv4_read(CArgs a) {
+__global__ __launch_bounds__(256) void kv4_read(CArgs a, int log) {
   const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int hv = (int)(item % (2 * a.heads)), h = hv >> 1, is_v = hv & 1;
-  const int64_t t0 = item / (2 * a.heads) * 16;
-  const bool mine = 2 * lane < a.d;
-  char* const out = a.out[is_v] + ((t0 * a.heads + h) * a.d + 2 * lane) * 2;
-  const int64_t step = (int64_t)a.heads * a.d * 2;
-  int64_t slot = -1;
-  const bool row = lane < 16 && t0 + lane < a.tokens;
-  if (row) slot = a.slots[t0 + lane];
-  const bool in = row && slot >= 0 && slot < a.cells;
-  for (uint64_t left = __ballot(row && !in); left; left &= left - 1)
-    if (mine) *(uint32_t*)(out + (__ffsll((unsigned long long)left) - 1) * step) = 0;
-  for (uint64_t left = __ballot(in); left;) {
-    // the rows whose tokens are in the first one's piece
-    const int u0 = __ffsll((unsigned long long)left) - 1;
-    const int64_t piece = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(slot >> 4), u0) |
-                          (int64_t)__builtin_amdgcn_readlane((int)(slot >> 36), u0) << 32;
-    const uint32_t rows = (uint32_t)__ballot(in && slot >> 4 == piece);
-    left &= ~(uint64_t)rows;
-    const int lp = a.lb - 4;
-    const int64_t cell = (piece >> lp) * a.heads + h, at = (piece & ((1 << lp) - 1)) * 16;
-    const int off = (int)slot & 15;  // (lane u: row u's token)
-    if (!mine) continue;
-    const uint8_t* const sc = a.scale[is_v] + (((cell * (a.dp >> 5) + (lane >> 4)) << a.lb) + at);
-    uint64_t d0 = 0, d1 = 0;
-    const uint8_t* const kc = a.codes[0] + ((cell << a.lb) + at) * (a.dp >> 1) + lane;
-    if (is_v) {
-      const uint64_t* const vc = (const uint64_t*)(a.codes[1] + ((cell << lp) * a.dp + (at >> 4) * a.dp + 2 * lane) * 8);
-      d0 = vc[0];
-      d1 = vc[1];
-    }
+  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), parts = 2u * a.heads;
+  const uint32_t group = item / parts, hv = item - group * parts;
+  const int h = (int)(hv >> 1), is_v = hv & 1, d = (lane & ((1 << log) - 1)) * 8;
+  const int64_t t = ((int64_t)group << (6 - log)) + (lane >> log);
+  if (d >= a.d || t >= a.tokens) return;
+  const int64_t slot = a.slots[t];
+  T f[8] = {};
+  if (slot >= 0 && slot < a.cells) {
+    const int64_t cell = (slot >> a.lb) * a.heads + h, at = slot & ((1 << a.lb) - 1);
+    const uint32_t sb = a.scale[is_v][((cell * (a.dp >> 5) + (d >> 5)) << a.lb) + at];
+    uint32_t word = 0;
+    if (!is_v) {
+      word = *(const uint32_t*)(a.codes[0] + ((cell << a.lb) + at) * (a.dp >> 1) + (d >> 1));
+    } else {
+      const int4v* const p = (const int4v*)(a.codes[1] + (((cell << (a.lb - 4)) + (at >> 4)) * a.dp + d) * 8);
+      const int o = 4 * ((int)at & 7);
+      const bool hi = at & 8;
+      int4v v[4];
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
-      if (!(rows >> u & 1)) continue;
-      const int o = __builtin_amdgcn_readlane(off, u);
-      const uint32_t byte = is_v ? (uint32_t)(d0 >> (4 * o) & 15) | (uint32_t)(d1 >> (4 * o) & 15) << 4 : kc[o * (a.dp >> 1)];
-      const half2v v = numbers<0>(byte) * scale_twice<0>(sc[o]);
-      const T f[2] = {(T)(float)v[0], (T)(float)v[1]};
-      uint32_t bits;
-      __builtin_memcpy(&bits, f, 4);
-      *(uint32_t*)(out + u * step) = bits;
+      for (int j = 0; j < 4; ++j) v[j] = p[j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x = (uint32_t)(hi ? v[j][1] : v[j][0]) >> o & 15, y = (uint32_t)(hi ? v[j][3] : v[j][2]) >> o & 15;
+        word |= (x | y << 4) << (8 * j);
+      }
     }
+    const half2v s = scale_twice<0>(sb);
+    static_for<4>([&](auto j) {
+      const half2v v = numbers<j>(word) * s;
+      f[2 * j] = (T)(float)v[0];
+      f[2 * j + 1] = (T)(float)v[1];
+    });
   }
+  int4v bits;
+  __builtin_memcpy(&bits, f, 16);
+  *(int4u*)((T*)a.out[is_v] + (t * a.heads + h) * a.d + d) = bits;
 }
 
 CArgs cache_args(const Kv4CacheProblem& p) {
@@ -203,11 +238,11 @@ hipError_t launch_kv4_append(const Kv4CacheProblem& p, hipStream_t stream) {
   a.hs[1] = p.hsv;
   // a wave looks for runs in `span` rows: one while that leaves at most 8192
   // waves, more for long prompts, whose rows mostly begin none
-  const int64_t per_row = 2 * p.kv_heads;
+  const int64_t per_row = p.d > 64 ? 4 * p.kv_heads : 2 * p.kv_heads;
   const int64_t span = p.tokens * per_row / 8192;
   a.span = (int)(span < 1 ? 1 : span < 48 ? span : 48);
   const int64_t blocks = ((p.tokens + a.span - 1) / a.span * per_row + 3) / 4;
-  if (blocks >= (1ll << 31)) return hipErrorInvalidValue;
+  if (blocks >= (1ll << 30)) return hipErrorInvalidValue;
   const auto fn = p.dtype == DT_BF16 ? kv4_append<__bf16> : kv4_append<_Float16>;
   hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
@@ -217,10 +252,12 @@ hipError_t launch_kv4_read(const Kv4CacheProblem& p, hipStream_t stream) {
   CArgs a = cache_args(p);
   a.out[0] = (char*)p.k_out;
   a.out[1] = (char*)p.v_out;
-  const int64_t blocks = ((p.tokens + 15) / 16 * 2 * p.kv_heads + 3) / 4;
-  if (blocks >= (1ll << 31)) return hipErrorInvalidValue;
+  int log = 0;
+  while (8 << log < p.d) ++log;
+  const int64_t per = 64 >> log, blocks = ((p.tokens + per - 1) / per * 2 * p.kv_heads + 3) / 4;
+  if (blocks >= (1ll << 30)) return hipErrorInvalidValue;
   const auto fn = p.dtype == DT_BF16 ? kv4_read<__bf16> : kv4_read<_Float16>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), 0, stream, a, log);
   return hipGetLastError();
 }
 

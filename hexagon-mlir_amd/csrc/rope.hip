@@ -21,6 +21,7 @@ namespace hxmi {
 namespace {
 
 typedef int int4u __attribute__((ext_vector_type(4), aligned(2)));  // (rows start anywhere)
+typedef int int4f __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kMaxPairs = 256;  // of a workgroup's tokens
 
@@ -36,7 +37,7 @@ struct RArgs {
   int heads, all, d, pairs, axes;  // heads of q, of both
   int tb;                          // tokens of a workgroup
   int pos64, w32;
-  float eps, scale;
+  float eps, scale, inv_d;
 };
 
 // Cosine and sine of 2 pi `turns`.
@@ -59,8 +60,7 @@ __device__ __forceinline__ float2 cos_sin(double turns) {
 }
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  const int4v raw = *(const int4u*)p;
+__device__ __forceinline__ void floats(const int4v& raw, float (&f)[8]) {
   T t[8];
   __builtin_memcpy(t, &raw, 16);
 #pragma unroll
@@ -89,6 +89,40 @@ __global__ __launch_bounds__(256) void qk_rope(RArgs a, int log) {
   __shared__ __attribute__((aligned(16))) float cs[kMaxPairs], sn[kMaxPairs];
   const int64_t t0 = (int64_t)blockIdx.x * a.tb;
   const int nt = (int)min((int64_t)a.tb, a.tokens - t0), pairs = a.pairs;
+  const int u = threadIdx.x & ((1 << log) - 1), slot = threadIdx.x >> log, slots = 256 >> log;
+  const int half = pairs, rot = 2 * pairs;
+  // the lane's values: d0 on, and (kWhole) their partners d1 on
+  const int whole = pairs >> 3;
+  const bool turned = FORM == kWhole ? u < whole : u * 8 < rot;
+  const int d0 = FORM == kWhole ? (turned ? u * 8 : rot + (u - whole) * 8) : u * 8;
+  const bool in = d0 < a.d;
+  constexpr int NV = FORM == kWhole ? 16 : 8;
+  float wq[NV], wk[NV];
+
+  // Head i of the workgroup's: its pieces, loaded a head ahead (what is in flight
+  // belongs to no head that is written meanwhile, in place or not).
+  struct Head {
+    int t, h;  // h: k's heads after q's
+  };
+  auto after = [&](Head n) {
+    n.h += slots;
+    while (n.h >= a.all) {
+      n.h -= a.all;
+      ++n.t;
+    }
+    return n;
+  };
+  auto row = [&](const Head& n) {
+    const int is_k = n.h >= a.heads;
+    return (const T*)a.x[is_k] + (t0 + n.t) * a.ld[is_k] + (n.h - (is_k ? a.heads : 0)) * a.hs[is_k];
+  };
+  int4v v_raw{}, w_raw{};
+  auto load = [&](const T* x) {
+    if (in) v_raw = *(const int4u*)(x + d0);
+    if (FORM == kWhole && turned) w_raw = *(const int4u*)(x + half + d0);
+  };
+  Head now = after(Head{0, slot - slots});
+  if (now.t < nt) load(row(now));
   for (int i = threadIdx.x; i < nt * pairs; i += 256) {
     const int t = i / pairs, p = i - t * pairs;
     const int ax = a.axis ? min(max(a.axis[p], 0), a.axes - 1) : 0;
@@ -100,37 +134,40 @@ __global__ __launch_bounds__(256) void qk_rope(RArgs a, int log) {
   }
   __syncthreads();
 
-  const int u = threadIdx.x & ((1 << log) - 1), slot = threadIdx.x >> log, slots = 256 >> log;
-  const int half = pairs, rot = 2 * pairs;
-  // the lane's values: d0 on, and (kWhole) their partners d1 on
-  const int whole = pairs >> 3;
-  const bool turned = FORM == kWhole ? u < whole : u * 8 < rot;
-  const int d0 = FORM == kWhole ? (turned ? u * 8 : rot + (u - whole) * 8) : u * 8;
-  const bool in = d0 < a.d;
-  constexpr int NV = FORM == kWhole ? 16 : 8;
-  float wq[NV], wk[NV];
   if constexpr (NORM) {
+    auto eight = [&](const char* w, int d, float* f) {
+      float t[8];
+      if (a.w32) {
+        const int4v lo = *(const int4f*)(w + 4 * d), hi = *(const int4f*)(w + 4 * d + 16);
+        __builtin_memcpy(t, &lo, 16);
+        __builtin_memcpy(t + 4, &hi, 16);
+      } else {
+        floats<T>(*(const int4u*)(w + 2 * d), t);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = t[e];
+    };
     auto weights = [&](const char* w, float (&f)[NV]) {
 #pragma unroll
-      for (int e = 0; e < NV; ++e) {
-        const int d = e < 8 ? d0 + e : half + d0 + e - 8;
-        f[e] = 1.f;
-        if (w && in && (e < 8 || turned)) f[e] = a.w32 ? ((const float*)w)[d] : (float)((const T*)w)[d];
-      }
+      for (int e = 0; e < NV; ++e) f[e] = 1.f;
+      if (w && in) eight(w, d0, f);
+      if (FORM == kWhole && w && turned) eight(w, half + d0, f + NV - 8);
     };
     weights(a.w[0], wq);
     weights(a.w[1], wk);
   }
 
-  for (int i = slot; i < nt * a.all; i += slots) {  // (a head's lanes stay together)
-    const int t = i / a.all, h = i - t * a.all, is_k = h >= a.heads, hh = is_k ? h - a.heads : h;
-    const T* const x = (const T*)a.x[is_k] + (t0 + t) * a.ld[is_k] + hh * a.hs[is_k];
-    T* const y = (T*)a.y[is_k] + (t0 + t) * a.ldo[is_k] + hh * a.hso[is_k];
-    const float *const c = cs + t * pairs, *const s = sn + t * pairs;
+  for (Head next; now.t < nt; now = next) {  // (a head's lanes stay together)
+    const int is_k = now.h >= a.heads;
+    T* const y = (T*)a.y[is_k] + (t0 + now.t) * a.ldo[is_k] + (now.h - (is_k ? a.heads : 0)) * a.hso[is_k];
+    const float *const c = cs + now.t * pairs, *const s = sn + now.t * pairs;
     float v[8] = {}, w[8] = {};
-    if (in) load8(x + d0, v);
-    if (FORM == kWhole && turned) load8(x + half + d0, w);
+    if (in) floats<T>(v_raw, v);
+    if (FORM == kWhole && turned) floats<T>(w_raw, w);
+    next = after(now);
+    if (next.t < nt) load(row(next));
     if constexpr (FORM == kSplit) {
+      const T* const x = row(now);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int d = d0 + e;
@@ -146,7 +183,7 @@ __global__ __launch_bounds__(256) void qk_rope(RArgs a, int log) {
       }
       for (int o = 1; o < 1 << log; o <<= 1) sum += __shfl_xor(sum, o, 64);
       const bool has = a.w[is_k] != nullptr;
-      const float f = has ? __builtin_amdgcn_rsqf(sum / (float)a.d + a.eps) : 1.f;
+      const float f = has ? __builtin_amdgcn_rsqf(fmaf(sum, a.inv_d, a.eps)) : 1.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[e] *= f * (is_k ? wk[e] : wq[e]);
@@ -162,10 +199,14 @@ __global__ __launch_bounds__(256) void qk_rope(RArgs a, int log) {
       if (turned) {
         float o[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float ce = c[d0 + e], se = s[d0 + e], p = v[e];
-          v[e] = p * ce - w[e] * se;
-          o[e] = w[e] * ce + p * se;
+        for (int x = 0; x < 8; x += 4) {
+          const float4v ce = *(const float4v*)(c + d0 + x), se = *(const float4v*)(s + d0 + x);  // (pairs: a multiple of 8)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = v[x + j], r = w[x + j];
+            v[x + j] = p * ce[j] - r * se[j];
+            o[x + j] = r * ce[j] + p * se[j];
+          }
         }
         store8(y + half + d0, o);
       }
@@ -230,6 +271,7 @@ hipError_t launch_qk_rope(const RopeProblem& p, hipStream_t stream) {
   a.pos64 = p.pos64;
   a.w32 = p.w32;
   a.eps = p.eps;
+  a.inv_d = 1.f / (float)p.d;
   a.scale = p.scale;
   const int form = p.interleaved ? kNext : p.rotary % 16 == 0 ? kWhole : kSplit;
   const int units = form == kWhole ? (int)(p.rotary / 16 + (p.d - p.rotary) / 8) : (int)(p.d / 8);

@@ -375,17 +375,346 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
   }
 }
 
+// ---- rows in the hundreds ----------------------------------------------------------
+//
+// A workgroup of four waves owns 128 rows (32 a wave) and takes 64 keys at a
+// time through two LDS stages: its threads bring the numbers to fp16 on the way
+// in, once for 128 rows (the kernel above: for 16), under the score MFMAs, and
+// those of the next stage but one are in flight meanwhile.  Scores are
+// D[key][row] of 32x32x16 MFMAs; row m of a 32-key block reads key 16 (m / 16) +
+// 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that a lane's eight weights of 16 keys
+// are eight in order, the B operand of P.V.
+// D: LDS rows of K (64 or 128 dims).
+template <typename T, int D, bool WHOLE>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArgs a) {
+  constexpr bool BF16 = !std::is_same_v<T, _Float16>;
+  constexpr int DS = D / 16, DT = D / 32, RB = 2 * D;
+  constexpr int KB = 64 * RB, STAGE = KB + D * 128;
+  constexpr int KW = D / 32, VD = D / 64;  // words of K, dims of V (of 16 keys) a thread converts a stage
+  constexpr int NV = DT * 16 + 2;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  __shared__ uint32_t unheld[2][4];  // of a stage's pieces: keys with a value that is no number, a bit each
+  __shared__ int last_split;
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 31, h = lane >> 5;
+  const Share part = share_of(a);
+  const int split = part.split, nsplit = part.count, item = part.item;
+  const int kvh = item / a.tiles;
+  Rows tile;
+  if (!rows_of<128>(a, a.tiles - 1 - (item - kvh * a.tiles), tile)) return;  // (the last rows see the most keys)
+  const int n = tile.n, len = tile.len;
+
+  // This lane's row (past the last one: the last one's q, not stored)
+  const int64_t row = (int64_t)tile.row0 + w * 32 + lr, rowq = min(row, tile.count - 1);
+  const int token = (int)(rowq / a.group), head = kvh * a.group + (int)(rowq - (int64_t)token * a.group);
+  const int last = (int)min((int64_t)len - n + token, (int64_t)len - 1);  // the last key it sees
+  half8v qf[DS];
+  float c = a.c;
+  {
+    const T* q = (const T*)a.q + (int64_t)(tile.first + token) * a.ldq + (int64_t)head * a.hq;
+    T raw[DS][8];
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      const int d = s * 16 + h * 8;
+      int4v v{};
+      if (WHOLE || d < a.d) v = *(const int4u*)(q + d);
+      __builtin_memcpy(raw[s], &v, 16);
+      if constexpr (BF16) top = largest(raw[s], top);
+    }
+    int ex = 0;
+    if constexpr (BF16) {
+      const auto t2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      ex = exponent_of(fmaxf(__uint_as_float(t2[0]), __uint_as_float(t2[1])));
+      c = __builtin_ldexpf(a.c, -ex);
+    }
+#pragma unroll
+    for (int s = 0; s < DS; ++s) qf[s] = q_operand(raw[s], ex);
+  }
+
+  // keys that some / all rows of the workgroup, and all rows of the wave, see
+  const int i1 = (int)min((int64_t)n - 1, ((int64_t)tile.row0 + 127) / a.group);
+  const int kend = max(0, min(len, len - n + i1 + 1));
+  const int kall = max(0, min(len, len - n + tile.row0 / a.group + 1));
+  const int wrow = tile.row0 + w * 32;
+  const int kfull = wrow < tile.count ? max(0, min(len, len - n + wrow / a.group + 1)) : 0;
+  const int stages = (kend + 63) >> 6, share = (stages + nsplit - 1) / nsplit;
+  const int c0 = split * share, c1 = min(stages, c0 + share);
+
+  const int* const table = a.table + (int64_t)tile.r * a.ldt;
+  const int64_t hb = (int64_t)kvh * a.bytes, kv_bytes = (int64_t)a.kv_heads * a.bytes;
+  const int pm = (1 << a.lb) - 1;
+  // Lane l's page of a stage: that of its 16-key piece l % 4, -1 where there is none or a bad one.
+  auto page = [&](int st) {
+    const int piece = 4 * st + (lane & 3), p = piece >> a.lb;
+    const int b = p < a.width && piece * 16 < kend ? table[p] : -1;
+    return (unsigned)b < (unsigned)a.blocks ? b : -1;
+  };
+
+  // Thread t's part of a stage: K, key t / 4 (one of the wave's 16), dims 8 KW (t %
+  // 4) on, under one scale; V, the wave's 16 keys of dims VD (t % 64) on.
+  const int t = threadIdx.x, kd = (lane & 3) * 8 * KW, vd = lane * VD;
+  uint32_t kc[KW], vc[2 * VD], ksw = 0;
+  int4v vsw{};
+  // The numbers and scales of a stage with pages `pg` (a page that is not there: block 0's, left out below).
+  auto load = [&](int st, int pg) {
+    const int b = __builtin_amdgcn_readlane(pg, w), at = ((4 * st + w) & pm) * 16;
+    const int64_t blk = max(b, 0), sb = (blk * a.kv_heads + kvh) * a.sbytes + at;
+    const uint8_t* const kp = a.k + blk * kv_bytes + hb + (int64_t)(at + (lane >> 2)) * (a.dp >> 1) + (kd >> 1);
+    const uint8_t* const vp = a.v + blk * kv_bytes + hb + ((int64_t)(at >> 4) * a.dp + vd) * 8;
+    const bool kin = WHOLE || kd < a.dp, vin = WHOLE || vd < a.dp;
+    if constexpr (D == 64) {
+      const uint2 k2 = kin ? *(const uint2*)kp : uint2{}, v2 = vin ? *(const uint2*)vp : uint2{};
+      kc[0] = k2.x;
+      kc[1] = k2.y;
+      vc[0] = v2.x;
+      vc[1] = v2.y;
+    } else {
+      const uint4 k4 = kin ? *(const uint4*)kp : uint4{}, v4 = vin ? *(const uint4*)vp : uint4{};
+      __builtin_memcpy(kc, &k4, 16);
+      __builtin_memcpy(vc, &v4, 16);
+    }
+    if (kin) ksw = a.ks[sb + ((int64_t)(kd >> 5) << (a.lb + 4)) + (lane >> 2)];
+    vsw = vin ? *(const int4v*)(a.vs + sb + ((int64_t)(vd >> 5) << (a.lb + 4))) : int4v{};
+    return pg;
+  };
+  // A weight of 0 has to leave nothing behind whatever a scale is: in a stage that
+  // not every row sees whole, scales of keys past all rows' are 0, and so are
+  // others that are not finite, which make the rows that see them NaN by their sum.
+  auto clear = [&](int st, int pg) {
+    const int b = __builtin_amdgcn_readlane(pg, w);
+    if (b >= 0 && st * 64 + 64 <= kall) return;
+    const int held = b >= 0 ? kend - (st * 64 + 16 * w) : 0;
+    uint32_t any = 0;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const uint32_t mask = first_bytes(held, y), bad = not_finite((uint32_t)vsw[y]) & mask;
+      vsw[y] &= (int)(mask & ~bad);
+      any |= (bad & 1) << (4 * y) | (bad >> 7 & 2) << (4 * y) | (bad >> 14 & 4) << (4 * y) | (bad >> 21 & 8) << (4 * y);
+    }
+    if (__any(any)) {
+      for (int o = 32; o >= 1; o >>= 1) any |= (uint32_t)__shfl_xor((int)any, o, 64);
+    }
+    if (lane == 0) unheld[st & 1][w] = any;
+  };
+  // 16-byte chunks of LDS rows are XOR-swizzled: the rows that one read takes
+  // 16 bytes of (16 lanes at a time) fall on different banks.
+  auto k_at = [](int key, int chunk) { return key * RB + ((chunk ^ (key / (256 / RB) & (RB / 16 - 1))) << 4); };
+  auto v_at = [](int d, int chunk) { return KB + d * 128 + ((chunk ^ (d >> 1 & 7)) << 4); };
+  // (the swizzle is an XOR of chunk bits: another chunk of a row lies at the row's chunk 0 with those bits flipped)
+  const int k_store = k_at(t >> 2, (lane & 3) * KW), v_store = v_at(vd, 2 * w);
+  // Unit j of DS: eight numbers, of K or of V.
+  auto store = [&](char* base, auto j_) {
+    constexpr int j = j_;
+    if constexpr (j < KW) {
+      const half2v sc = scale_twice<0>(ksw);
+      *(half8v*)(base + (k_store ^ (j << 4))) = operand(kc[j], [&](int) { return sc; });
+    } else {
+      constexpr int u = (j - KW) / VD, e = (j - KW) % VD;  // (both dims under the same scales)
+      const Pairs sc((uint32_t)vsw[2 * u], (uint32_t)vsw[2 * u + 1]);
+      *(half8v*)(base + (v_store ^ (u << 4)) + e * 128) = operand(vc[2 * e + u], [&](int i) { return sc.p[i]; });
+    }
+  };
+  static_assert(KW + 2 * VD == DS, "a unit a step of the scores");
+
+  float16v o[DT];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int x = 0; x < DT; ++x) o[x] = float16v{};
+
+  const int key = 16 * (lr >> 4) + 8 * (lr >> 2 & 1) + 4 * (lr >> 3 & 1) + (lr & 3);
+  const int k_read = k_at(key, h), v_read = v_at(lr, h);
+  int pg = -1, after = -1;  // pages of the stage after next, and of the one loaded
+  // Stage st (pages `here`) in `base`, while `other` takes the next one (pages `next`).
+  auto compute = [&](int st, const char* base, char* other, int here, int next) {
+    const uint64_t there = __ballot(here >= 0);
+    const bool all = st * 64 + 64 <= kfull && there == ~0ull;
+    // Fragments are read a step ahead of their MFMAs; the scheduling barriers
+    // keep the compiler from reading them all first.
+    float16v s[2];
+    half8v kf[2][2], vf[2][DT];
+    auto read_k = [&](int x) {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) kf[x & 1][nb] = *(const half8v*)(base + (k_read ^ (x << 5)) + nb * 32 * RB);
+    };
+    auto read_v = [&](int x) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) vf[x & 1][dt] = *(const half8v*)(base + (v_read ^ (x << 5)) + dt * 32 * 128);
+    };
+    if (st + 1 < c1) clear(st + 1, next);
+    read_k(0);
+    static_for<DS>([&](auto x) {
+      if (x + 1 < DS) read_k(x + 1);
+      else read_v(0);
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+        s[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[x & 1][nb], qf[x], x == 0 ? float16v{} : s[nb], 0, 0, 0);
+      // (conversion passes under the score MFMAs, which need few vector
+      // instructions; past the last stage old numbers go where nobody reads)
+      store(other, x);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    // (the numbers' registers are free)
+    if (st + 2 < c1) after = load(st + 2, pg);
+    if (st + 3 < c1) pg = page(st + 3);
+    if (!all) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        // a lane's eight keys of a piece up to this one are seen
+        const int left = there >> x & 1 ? last - (st * 64 + x * 16 + 8 * h) : -1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[x >> 1][8 * (x & 1) + e] = e > left ? -INFINITY : s[x >> 1][8 * (x & 1) + e];
+        if (st * 64 + 64 > kall && there >> x & 1) {
+          const uint32_t bad = unheld[st & 1][x] >> (8 * h) & 0xff;
+          if (bad & ((1u << min(max(left + 1, 0), 8)) - 1)) l = NAN;
+        }
+      }
+    } else if (st * 64 + 64 > kall) {  // (rows of other waves do not see it whole)
+      if (unheld[st & 1][0] | unheld[st & 1][1] | unheld[st & 1][2] | unheld[st & 1][3]) l = NAN;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[x][i]);
+    const auto m2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    mx = fmaxf(__uint_as_float(m2[0]), __uint_as_float(m2[1])) * c;  // (c > 0)
+    if (__any(mx > m + kHigh)) {
+      const float now = mx > m + kHigh ? mx - kLow : m, f = rel_exp2(m, now);
+      m = now;
+      l *= f;
+#pragma unroll
+      for (int x = 0; x < DT; ++x) o[x] *= f;
+    }
+    const float off = m == -INFINITY ? 0.f : -m;
+    // the weights of 16 keys while the MFMAs of the 16 before run
+    auto weights = [&](int x) {
+      half8v p;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = __builtin_amdgcn_exp2f(fmaf(s[x >> 1][8 * (x & 1) + e], c, off));
+        l += v;
+        p[e] = (_Float16)v;
+      }
+      return p;
+    };
+    half8v p = weights(0);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      half8v then = p;
+      if (x < 3) {
+        read_v(x + 1);
+        then = weights(x + 1);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x & 1][dt], p, o[dt], 0, 0, 0);
+      p = then;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if (c0 < c1) {
+    // Ahead of the stage computed: the next one's numbers on their way into LDS,
+    // those of the one after, pages of the one after that.
+    int now = load(c0, page(c0)), next = -1;
+    clear(c0, now);
+    static_for<DS>([&](auto x) { store(lds, x); });
+    if (c0 + 1 < c1) next = load(c0 + 1, page(c0 + 1));
+    if (c0 + 2 < c1) pg = page(c0 + 2);
+    auto step = [&](int st, char* base, char* other) {
+      __syncthreads();  // stage st is written, and nobody reads the other one
+      compute(st, base, other, now, next);
+      now = next;
+      next = after;
+    };
+    // (LDS addresses that differ by constants)
+    for (int st = c0; st < c1; st += 2) {
+      step(st, lds, lds + STAGE);
+      if (st + 1 < c1) step(st + 1, lds + STAGE, lds);
+    }
+  }
+
+  // A wave's floats: o, m, l; a tile's shares joined as in the kernel above.
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int x = 0; x < DT; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f(x * 16 + i, o[x][i]);
+    f(DT * 16, m);
+    f(DT * 16 + 1, l);
+  };
+  if (nsplit > 1) {
+    constexpr int kCoherent = 17;  // sc0 | sc1
+    constexpr int PART = 4 * NV * 64 * 4;
+    const __amdgpu_buffer_rsrc_t rP =
+        make_rsrc(a.ws + kWsCounterBytes + (int64_t)(item - a.full) * nsplit * PART, (uint32_t)(nsplit * PART));
+    each([&](int i, float v) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rP, (uint32_t)(split * PART + ((w * NV + i) * 64 + lane) * 4),
+                                            0, kCoherent);
+    });
+    wait_vmcnt0();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      unsigned long long* cnt = (unsigned long long*)a.ws + (item - a.full);  // < kWsMaxTiles (the host's check)
+      const unsigned long long before = __hip_atomic_fetch_add(cnt, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last_split = before + 1 == (unsigned long long)nsplit;
+      if (last_split) __hip_atomic_store(cnt, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last_split) return;
+    auto held = [&](int sp, int i) {
+      return __uint_as_float(
+          __builtin_amdgcn_raw_buffer_load_b32(rP, (uint32_t)(sp * PART + ((w * NV + i) * 64 + lane) * 4), 0, kCoherent));
+    };
+    m = -INFINITY;
+#pragma unroll 4
+    for (int sp = 0; sp < nsplit; ++sp) m = fmaxf(m, held(sp, DT * 16));
+    l = 0.f;
+#pragma unroll
+    for (int x = 0; x < DT; ++x) o[x] = float16v{};
+    for (int sp = 0; sp < nsplit; ++sp) {  // (in this order whichever came last)
+      const float f = rel_exp2(held(sp, DT * 16), m);
+      l += f * held(sp, DT * 16 + 1);
+#pragma unroll
+      for (int x = 0; x < DT; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[x][i] += f * held(sp, x * 16 + i);
+    }
+  }
+
+  // O: lane holds row l % 32, dims 32 x + 8 g + 4 h + 0..3
+  const auto l2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+  const float whole = __uint_as_float(l2[0]) + __uint_as_float(l2[1]), f = whole == 0.f ? 0.f : 1.f / whole;
+  if (row >= tile.count) return;
+  T* const out = (T*)a.o + (int64_t)(tile.first + token) * a.ldo + (int64_t)head * a.ho;
+#pragma unroll
+  for (int x = 0; x < DT; ++x)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = x * 32 + 8 * g + 4 * h;
+      if (!WHOLE && d >= a.d) continue;
+      T o4[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o4[j] = (T)(o[x][4 * g + j] * f);
+      int2v bits;
+      __builtin_memcpy(&bits, o4, 8);
+      *(int2u*)(out + d) = bits;
+    }
+}
+
 int64_t part_bytes(const KvAttnSizes& p, const KvPlan& k) {  // of a tile's share
   const int64_t dt = p.d <= 64 ? 4 : 8;
-  return (dt * 4 + 2) * 64 * 4;
+  return k.rt == 16 ? (dt * 4 + 2) * 64 * 4 : 4 * (dt * 8 + 2) * 64 * 4;
 }
-KvPlan plan4_of(const KvAttnSizes& p) { return plan_of(p, false); }
 
 template <typename T>
 hipError_t launch_t(int64_t d, int rt, dim3 grid, const KArgs& a, hipStream_t stream) {
   const bool small = d <= 64, whole = d == 64 || d == 128;
-  const auto fn = small ? whole ? kv4_attention<T, 1, true> : kv4_attention<T, 1, false>
-                        : whole ? kv4_attention<T, 2, true> : kv4_attention<T, 2, false>;
+  const auto fn = rt == 16 ? (small ? whole ? kv4_attention<T, 1, true> : kv4_attention<T, 1, false>
+                                    : whole ? kv4_attention<T, 2, true> : kv4_attention<T, 2, false>)
+                           : (small ? whole ? kv4_attention_tiles<T, 64, true> : kv4_attention_tiles<T, 64, false>
+                                    : whole ? kv4_attention_tiles<T, 128, true> : kv4_attention_tiles<T, 128, false>);
   hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream, a);
   return hipGetLastError();
 }
@@ -393,12 +722,12 @@ hipError_t launch_t(int64_t d, int rt, dim3 grid, const KArgs& a, hipStream_t st
 }  // namespace
 
 int64_t kv4_attention_workspace_bytes(const Kv4AttnProblem& p) {
-  const KvPlan k = plan4_of(p);
+  const KvPlan k = plan_of(p);
   return k.nsplit > 1 ? kWsCounterBytes + (k.tiles * p.kv_heads - k.full) * k.nsplit * part_bytes(p, k) : 0;
 }
 
 hipError_t launch_kv4_attention(const Kv4AttnProblem& p, hipStream_t stream) {
-  KvPlan k = plan4_of(p);
+  KvPlan k = plan_of(p);
   const int64_t items = k.tiles * p.kv_heads;
   if (k.nsplit > 1 && (!p.ws || p.ws_bytes < kv4_attention_workspace_bytes(p))) {
     k.nsplit = 1;

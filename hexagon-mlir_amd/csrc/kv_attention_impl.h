@@ -125,7 +125,7 @@ struct KvPlan {
   int rt, nsplit;  // rows of a tile: 16, or 128 (kv_attention_tiles)
   int64_t tiles, full;
 };
-inline KvPlan plan_of(const KvAttnSizes& p, bool tall = true) {  // tall: there are tiles of 128 rows
+inline KvPlan plan_of(const KvAttnSizes& p) {
   KvPlan r;
   const int64_t group = p.heads / p.kv_heads;
   const int64_t rows = (p.cu ? (p.tokens + p.requests - 1) / p.requests : 1) * group;  // of a request, on average
@@ -139,7 +139,7 @@ inline KvPlan plan_of(const KvAttnSizes& p, bool tall = true) {  // tall: there 
   // a prompt's chunk runs both on tiles that suit one of them: over 8192 keys,
   // 63 rows and a chunk of 2048 722 us in one call, 180 + 283 in two; 256 rows and
   // a chunk of 512 928 us, 711 + 110 in two.
-  const bool wide = tall && rows > (p.d > 64 ? 96 : 255) && p.tokens * p.heads >= 4096;
+  const bool wide = rows > (p.d > 64 ? 96 : 255) && p.tokens * p.heads >= 4096;
   r.rt = wide ? 128 : 16;
   const int64_t rt = r.rt;
   r.tiles = p.cu ? p.tokens * group / rt + p.requests : p.requests * ((group + rt - 1) / rt);

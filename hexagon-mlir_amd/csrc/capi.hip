@@ -1050,7 +1050,9 @@ int hxmi_sample(int dtype, const void* logits, const float* u, const float* temp
   return from_hip(hxmi::launch_sample(p, (hipStream_t)stream), name);
 }
 
-int64_t hxmi_verify_workspace_bytes(int64_t rows) { return rows > 0 ? hxmi::verify_workspace_bytes(rows) : 0; }
+int64_t hxmi_verify_workspace_bytes(int64_t rows, int64_t requests, int64_t vocab) {
+  return rows > 0 && requests > 0 && vocab > 0 ? hxmi::verify_workspace_bytes(rows, requests, vocab) : 0;
+}
 
 int hxmi_verify(int dtype, const void* logits, const int64_t* drafts, const float* u, const float* draw,
                 const int32_t* cu, const void* draft_probs, int probs_dtype, const float* temperature,
@@ -1077,8 +1079,8 @@ int hxmi_verify(int dtype, const void* logits, const int64_t* drafts, const floa
     REQUIRE(!draft_probs || ld_probs >= vocab || rows == 1, "%s: leading dimension of draft_probs below vocab", name);
     REQUIRE((uintptr_t)draft_probs % (probs_dtype == HXMI_SAMPLE_F32 ? 4 : 2) == 0,
             "%s: draft_probs must be aligned to their type", name);
-    REQUIRE(workspace && al(workspace, 256) && workspace_bytes >= hxmi::verify_workspace_bytes(rows),
-            "%s: needs a 256-byte aligned workspace of %lld bytes", name, (long long)hxmi::verify_workspace_bytes(rows));
+    REQUIRE(workspace && al(workspace, 256) && workspace_bytes >= hxmi::verify_workspace_bytes(rows, requests, vocab),
+            "%s: needs a 256-byte aligned workspace of %lld bytes", name, (long long)hxmi::verify_workspace_bytes(rows, requests, vocab));
   }
   p.rows = rows;
   p.dtype = dtype;

@@ -307,7 +307,7 @@ struct VerifyProblem : SampleProblem {
   int64_t requests, ldq;
   int q_type;  // as dtype
 };
-int64_t verify_workspace_bytes(int64_t rows);
+int64_t verify_workspace_bytes(int64_t rows, int64_t requests, int64_t vocab);
 hipError_t launch_verify(const VerifyProblem& p, hipStream_t stream);
 
 // One-token decoder step of a Llama / Qwen2 stack (persistent kernel).

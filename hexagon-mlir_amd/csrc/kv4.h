@@ -30,11 +30,14 @@ template <int N>
 __device__ __forceinline__ half2v numbers(uint32_t w) {
   return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, N);
 }
-// A byte of scales as a pair of equal numbers.
+// A byte of scales as a pair of equal numbers: byte n by twice_byte(n).
+__device__ __forceinline__ constexpr uint32_t twice_byte(uint32_t n) { return 0x0c000c00u | n << 16 | n; }  // (0x0c: zero)
+__device__ __forceinline__ half2v scale_twice(uint32_t w, uint32_t byte) {
+  return __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0u, w, byte) << 7);
+}
 template <int N>
 __device__ __forceinline__ half2v scale_twice(uint32_t w) {
-  constexpr uint32_t sel = 0x0c000c00u | N << 16 | N;  // (0x0c: zero)
-  return __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0u, w, sel) << 7);
+  return scale_twice(w, twice_byte(N));
 }
 // Bytes 2 N and 2 N + 1 of a word of scales as a pair.
 template <int N>

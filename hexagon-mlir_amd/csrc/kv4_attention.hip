@@ -49,6 +49,13 @@ __device__ __forceinline__ half8v operand(uint32_t w, F&& scale) {
                d = numbers<3>(w) * scale(3);
   return half8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+// l + the sum of eight weights, as P.V takes them (two an instruction).
+__device__ __forceinline__ float sum_of(const half8v& p, float l) {
+  const half2v one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) l = __builtin_amdgcn_fdot2(half2v{p[e], p[e + 1]}, one, l, false);
+  return l;
+}
 // Scales of eight values in a row (words w0 and w1), pair by pair.
 struct Pairs {
   half2v p[4];
@@ -165,6 +172,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
   Partial<DT> acc;
   acc.clear();
 
+  const uint32_t kbyte = twice_byte(lr & 3);  // (of the words of scales, those of this lane's keys)
   const int ck = lr >> 2;  // 16-key piece of a group that this lane's K rows lie in (V's and the scores': lg)
   const int* const table = a.table + (int64_t)r * a.ldt;
   const int64_t hb = (int64_t)kvh * a.bytes, kv_bytes = (int64_t)a.kv_heads * a.bytes;
@@ -175,30 +183,30 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
     const int b = p < a.width && piece * 16 < kend ? table[p] : -1;
     return (unsigned)b < (unsigned)a.blocks ? b : -1;
   };
-  uint32_t kr[4][2 * DC], ksw = 0;
-  int4v vr[G], vsw[G];
+  uint32_t kr[4][2 * DC];
+  int4v ksw{}, vr[G], vsw[G];
   bool there;
   // (a piece that is not there reads block 0's numbers, which its mask leaves out)
   auto load_k = [&](int g, int b) {
     const int64_t blk = max(b, 0);
-    const int at = ((4 * g + ck) & pm) * 16 + 4 * (lr & 3);
-    const uint8_t* p = a.k + blk * kv_bytes + hb + (int64_t)at * (a.dp >> 1) + lg * (KD / 2);
+    const int at = ((4 * g + ck) & pm) * 16;
+    const uint8_t* p = a.k + blk * kv_bytes + hb + (int64_t)(at + (lr & 3)) * (a.dp >> 1) + lg * (KD / 2);
     const bool in = WHOLE || lg * KD < a.dp;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if constexpr (DC == 1) {
-        const uint2 v = in ? *(const uint2*)(p + t * (a.dp >> 1)) : uint2{};
+        const uint2 v = in ? *(const uint2*)(p + 4 * t * (a.dp >> 1)) : uint2{};
         kr[t][0] = v.x;
         kr[t][1] = v.y;
       } else {
-        const uint4 v = in ? *(const uint4*)(p + t * (a.dp >> 1)) : uint4{};
+        const uint4 v = in ? *(const uint4*)(p + 4 * t * (a.dp >> 1)) : uint4{};
         kr[t][0] = v.x;
         kr[t][1] = v.y;
         kr[t][2] = v.z;
         kr[t][3] = v.w;
       }
     }
-    if (in) ksw = *(const uint32_t*)(a.ks + (blk * a.kv_heads + kvh) * a.sbytes + ((int64_t)(lg * KD / 32) << (a.lb + 4)) + at);
+    if (in) ksw = *(const int4v*)(a.ks + (blk * a.kv_heads + kvh) * a.sbytes + ((int64_t)(lg * KD / 32) << (a.lb + 4)) + at);
   };
   auto load_v = [&](int g, int b) {
     const int64_t blk = max(b, 0);
@@ -228,7 +236,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
     // scores
     float4v s[4];
     static_for<4>([&](auto t) {
-      const half2v sc = scale_twice<t>(ksw);
+      const half2v sc = scale_twice((uint32_t)ksw[int(t)], kbyte);
 #pragma unroll
       for (int x = 0; x < 2 * DC; ++x)
         s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(kr[t][x], [&](int) { return sc; }), qf[x],
@@ -245,7 +253,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][i] = 4 * i + t > left ? -INFINITY : s[t][i];
+        for (int i = 0; i < 4; ++i) s[t][i] = 4 * t + i > left ? -INFINITY : s[t][i];
       // A weight of 0 has to leave nothing behind whatever the scale is: those of
       // keys past all rows' are 0, and so are others that are not finite, which
       // make the rows that see them NaN by their sum.
@@ -278,13 +286,14 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
     const float off = acc.m == -INFINITY ? 0.f : -acc.m;
     half8v p[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[j & 3][2 * u + (j >> 2)], c, off));
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[2 * u + (j >> 2)][j & 3], c, off));
         acc.l += e;
         p[u][j] = (_Float16)e;
       }
+    }
     // values
 #pragma unroll
     for (int x = 0; x < G; ++x) {
@@ -558,20 +567,22 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
     // (the numbers' registers are free)
     if (st + 2 < c1) after = load(st + 2, pg);
     if (st + 3 < c1) pg = page(st + 3);
+    // a lane's eight keys of a piece up to this one are seen
+    auto left_of = [&](int x) { return there >> x & 1 ? last - (st * 64 + x * 16 + 8 * h) : -1; };
     if (!all) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        // a lane's eight keys of a piece up to this one are seen
-        const int left = there >> x & 1 ? last - (st * 64 + x * 16 + 8 * h) : -1;
+        const int left = left_of(x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[x >> 1][8 * (x & 1) + e] = e > left ? -INFINITY : s[x >> 1][8 * (x & 1) + e];
-        if (st * 64 + 64 > kall && there >> x & 1) {
-          const uint32_t bad = unheld[st & 1][x] >> (8 * h) & 0xff;
-          if (bad & ((1u << min(max(left + 1, 0), 8)) - 1)) l = NAN;
-        }
       }
-    } else if (st * 64 + 64 > kall) {  // (rows of other waves do not see it whole)
-      if (unheld[st & 1][0] | unheld[st & 1][1] | unheld[st & 1][2] | unheld[st & 1][3]) l = NAN;
+    }
+    if (st * 64 + 64 > kall) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (there >> x & 1) bad |= unheld[st & 1][x] >> (8 * h) & ((1u << min(max(left_of(x) + 1, 0), 8)) - 1);
+      l = bad ? NAN : l;
     }
     float mx = s[0][0];
 #pragma unroll
@@ -592,11 +603,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
     auto weights = [&](int x) {
       half8v p;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = __builtin_amdgcn_exp2f(fmaf(s[x >> 1][8 * (x & 1) + e], c, off));
-        l += v;
-        p[e] = (_Float16)v;
-      }
+      for (int e = 0; e < 8; ++e)
+        p[e] = (_Float16)__builtin_amdgcn_exp2f(fmaf(s[x >> 1][8 * (x & 1) + e], c, off));
+      l = sum_of(p, l);
       return p;
     };
     half8v p = weights(0);
@@ -703,6 +712,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
     }
 }
 
+// The card takes four workgroups a CU of the kernel for 16 rows at up to 64 dims (the
+// 8-bit one is planned for two): 64 requests of 8192 tokens over 4 heads 35.0 us in
+// two shares a tile, 31.5 in four.  Fewer tiles have their keys shared out as far
+// as it pays either way (64 tiles of 4000 keys: 10.0 us in eight, 11.4 in sixteen).
+KvPlan plan4_of(const KvAttnSizes& p) {
+  const int64_t group = p.heads / p.kv_heads;
+  const int64_t tiles = p.cu ? p.tokens * group / 16 + p.requests : p.requests * ((group + 15) / 16);
+  return plan_of(p, p.d <= 64 && tiles * p.kv_heads >= 128 ? 1024 : 512);
+}
 int64_t part_bytes(const KvAttnSizes& p, const KvPlan& k) {  // of a tile's share
   const int64_t dt = p.d <= 64 ? 4 : 8;
   return k.rt == 16 ? (dt * 4 + 2) * 64 * 4 : 4 * (dt * 8 + 2) * 64 * 4;
@@ -722,19 +740,19 @@ hipError_t launch_t(int64_t d, int rt, dim3 grid, const KArgs& a, hipStream_t st
 }  // namespace
 
 int64_t kv4_attention_workspace_bytes(const Kv4AttnProblem& p) {
-  const KvPlan k = plan_of(p);
+  const KvPlan k = plan4_of(p);
   return k.nsplit > 1 ? kWsCounterBytes + (k.tiles * p.kv_heads - k.full) * k.nsplit * part_bytes(p, k) : 0;
 }
 
 hipError_t launch_kv4_attention(const Kv4AttnProblem& p, hipStream_t stream) {
-  KvPlan k = plan_of(p);
+  KvPlan k = plan4_of(p);
   const int64_t items = k.tiles * p.kv_heads;
   if (k.nsplit > 1 && (!p.ws || p.ws_bytes < kv4_attention_workspace_bytes(p))) {
     k.nsplit = 1;
     k.full = items;
   }
   const int64_t grid = k.full + (items - k.full) * k.nsplit;
-  static_assert(512 <= kWsMaxTiles, "a counter for every shared tile");
+  static_assert(1024 <= kWsMaxTiles, "a counter for every shared tile");
   if (grid >= (1ll << 31)) return hipErrorInvalidValue;
   KArgs a{};
   a.k = p.k_codes;

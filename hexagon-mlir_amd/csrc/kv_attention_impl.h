@@ -125,7 +125,7 @@ struct KvPlan {
   int rt, nsplit;  // rows of a tile: 16, or 128 (kv_attention_tiles)
   int64_t tiles, full;
 };
-inline KvPlan plan_of(const KvAttnSizes& p) {
+inline KvPlan plan_of(const KvAttnSizes& p, int64_t slots = 512) {  // slots: workgroups for 16 rows on the card at a time
   KvPlan r;
   const int64_t group = p.heads / p.kv_heads;
   const int64_t rows = (p.cu ? (p.tokens + p.requests - 1) / p.requests : 1) * group;  // of a request, on average
@@ -152,8 +152,9 @@ inline KvPlan plan_of(const KvAttnSizes& p) {
   // knows: shares past a request's keys are joined for nothing (one user of 1900
   // tokens: 7.5 us with a table of 30 pages, 10.6 with 128, 24 with 512 or more).
   const int64_t items = r.tiles * p.kv_heads, least = wide ? 512 : 256, most = (p.width * p.block + least - 1) / least;
-  const int64_t left = items % 512;
-  int64_t n = left ? 512 / left : 1;
+  if (wide) slots = 512;
+  const int64_t left = items % slots;
+  int64_t n = left ? slots / left : 1;
   n = n < most ? n : most;
   r.nsplit = (int)(n < 1 ? 1 : n < 128 ? n : 128);
   r.full = r.nsplit > 1 ? items - left : items;

@@ -85,8 +85,10 @@ struct VArgs : SArgs {
   const char* q;  // the draft's probabilities, or null: the drafted token is certain
   int64_t ldq, rows;
   RowState* state;
+  uint64_t* sums;               // [requests, pieces]: what is left of a stopping row's weight
+  unsigned long long* arrived;  // [requests] shares that are done: 0 before and after
   int* counts;
-  int requests, per, q_type;
+  int requests, per, q_type, shares;
 };
 
 constexpr int NT = 1024, NW = NT / 64, PIECE = 512;
@@ -1099,41 +1101,41 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
 // finds the row that stops it and, given q, goes over that row again: the kept
 // weights less floor(q * sum), integers as they are, by pieces of 512 tokens,
 // then the token in the piece that reaches draw * sum.
+// A request's pieces go to a.shares workgroups of four waves, which store their
+// sums; the last to arrive draws.  Each finds the stopping row for itself.
+constexpr int VW = 4;
 template <typename T, typename Q>
-__global__ __launch_bounds__(NT) void verify_rows(VArgs a) {
+__global__ __launch_bounds__(64 * VW) void verify_rows(VArgs a) {
   struct Local {
-    uint32_t key[NW][PIECE];
-    float q[NW][PIECE];
-    unsigned long long sum[kMaxPieces];
+    uint32_t key[VW][PIECE];
+    float q[VW][PIECE];
     double exp2[kSteps];
-    unsigned long long stop;
+    unsigned long long sum[kMaxPieces];
+    int last;
   };
   __shared__ Local sh;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = blockIdx.x, vocab = a.vocab;
+  for (int i = threadIdx.x; i < kSteps; i += 64 * VW) sh.exp2[i] = kExp2.v[i];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, vocab = a.vocab;
+  const int r = (int)(blockIdx.x / a.shares), share = (int)(blockIdx.x - (uint32_t)r * a.shares);
   int64_t first, end;
   rows_of(a, r, first, end);
-  if (threadIdx.x == 0) {
-    sh.stop = (unsigned long long)end;
-    if (first == end) a.counts[r] = 0;
+  int64_t stop = end;
+  for (int64_t i0 = first; i0 < end && stop == end; i0 += 64) {  // (every wave the same)
+    const uint64_t m = __ballot(i0 + lane < end && a.state[min(i0 + lane, end - 1)].state != kAccepted);
+    if (m) stop = i0 + __ffsll((unsigned long long)m) - 1;
   }
-  if (threadIdx.x < kSteps) sh.exp2[threadIdx.x] = kExp2.v[threadIdx.x];
-  __syncthreads();
-  for (int64_t i = first + threadIdx.x; i < end; i += NT)
-    if (a.state[i].state != kAccepted) {
-      atomicMin(&sh.stop, (unsigned long long)i);
-      break;
-    }
-  __syncthreads();
-  const int64_t stop = (int64_t)sh.stop;
-  for (int64_t i = first + threadIdx.x; i < end; i += NT)
-    if (i != stop) a.token[i] = i < stop ? a.drafts[i] : -1;
+  if (share == 0) {
+    for (int64_t i = first + threadIdx.x; i < end; i += 64 * VW)
+      if (i != stop) a.token[i] = i < stop ? a.drafts[i] : -1;
+    if (threadIdx.x == 0) a.counts[r] = stop < end ? (int)(stop - first + 1) : 0;
+  }
   if (stop >= end) return;  // (without rows)
   const RowState st = a.state[stop];
-  if (threadIdx.x == 0) {
-    a.counts[r] = (int)(stop - first + 1);
-    if (st.state == kDrawn) a.token[stop] = st.token;
+  if (st.state == kDrawn) {
+    if (share == 0 && threadIdx.x == 0) a.token[stop] = st.token;
+    return;
   }
-  if (st.state == kDrawn) return;
+  __syncthreads();
 
   const T* const x = (const T*)a.x + stop * a.ldx;
   const Q* const q = (const Q*)a.q + stop * a.ldq;
@@ -1148,27 +1150,40 @@ __global__ __launch_bounds__(NT) void verify_rows(VArgs a) {
   auto kept = [&](uint32_t key, int i) {
     return key >= st.from && (key > st.tau || (key == st.tau && i < st.ties_end));
   };
-  auto load = [&](int i, uint32_t (&key)[8], float (&prob)[8]) {
+  struct Raw {  // eight logits and probabilities as they lie
+    Eight<T> x;
+    Eight<Q> q;
+  };
+  auto load = [&](int i, Raw& raw) {
+    if (i * 8 + 8 <= vocab) {
+      raw.x.load(x + i * 8);
+      raw.q.load(q + i * 8);
+    }
+  };
+  auto values = [&](int i, const Raw& raw, uint32_t (&key)[8], float (&prob)[8]) {
     if (__all(i * 8 + 8 <= vocab)) {
-      Eight<T> raw;
-      raw.load(x + i * 8);
-      raw.keys(key);
+      raw.x.keys(key);
+      Q p[8];
+      __builtin_memcpy(p, raw.q.r, sizeof(p));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) prob[e] = fmaxf((float)q[i * 8 + e], 0.f);
+      for (int e = 0; e < 8; ++e) prob[e] = fmaxf((float)p[e], 0.f);
     } else {
       load_keys(x, i, vocab, key);
 #pragma unroll
       for (int e = 0; e < 8; ++e) prob[e] = i * 8 + e < vocab ? fmaxf((float)q[i * 8 + e], 0.f) : 0.f;
     }
   };
-  bool with_q = true;
-  uint64_t whole_left = 0, incl = 0, run = 0;
-  const int per = (pieces + 63) >> 6;
-  for (;; with_q = false) {
-    for (int c = w; c < pieces; c += NW) {
+  constexpr int kCoherent = 17;  // sc0 | sc1
+  const __amdgpu_buffer_rsrc_t sums = make_rsrc(a.sums + (int64_t)r * pieces, (uint32_t)(pieces * 8));
+  // the sums of pieces c0 to c1
+  auto sum_up = [&](int c0, int c1, bool with_q) {
+    Raw next;
+    load((c0 + w) * 64 + lane, next);
+    for (int c = c0 + w; c < c1; c += VW) {
       uint32_t key[8];
       float prob[8];
-      load(c * 64 + lane, key, prob);
+      values(c * 64 + lane, next, key, prob);
+      if (c + VW < c1) load((c + VW) * 64 + lane, next);
       int some = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {  // the kept ones together: 64 of them take one evaluation
@@ -1184,15 +1199,43 @@ __global__ __launch_bounds__(NT) void verify_rows(VArgs a) {
       uint64_t sum = 0;
       for (int i = lane; i < some; i += 64) sum += left_of(sh.key[w][i], sh.q[w][i], with_q);
       if (some) sum = scan64(sum);
-      if (lane == 63) sh.sum[c] = sum;
+      if (lane == 63) {
+        const int2v both = {(int)(uint32_t)sum, (int)(sum >> 32)};
+        __builtin_amdgcn_raw_buffer_store_b64(both, sums, (uint32_t)c * 8, 0, kCoherent);
+      }
+    }
+    wait_vmcnt0();  // (what this wave stored is there for every XCD)
+    __syncthreads();
+  };
+  const int per_share = (pieces + a.shares - 1) / a.shares;
+  sum_up(min(share * per_share, pieces), min((share + 1) * per_share, pieces), true);
+  if (a.shares > 1) {
+    if (threadIdx.x == 0) {
+      unsigned long long* const cnt = a.arrived + r;  // (at most kWsMaxTiles requests are shared out)
+      const unsigned long long before = __hip_atomic_fetch_add(cnt, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sh.last = before + 1 == (unsigned long long)a.shares;
+      if (sh.last) __hip_atomic_store(cnt, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!sh.last) return;
+  }
+  const int per = (pieces + 63) >> 6;
+  bool with_q = true;
+  uint64_t whole_left = 0, incl = 0, run = 0;
+  for (;;) {
+    for (int c = threadIdx.x; c < pieces; c += 64 * VW) {
+      const int2v both = __builtin_amdgcn_raw_buffer_load_b64(sums, (uint32_t)c * 8, 0, kCoherent);
+      sh.sum[c] = (uint64_t)(uint32_t)both[1] << 32 | (uint32_t)both[0];
     }
     __syncthreads();
     run = 0;  // (every wave the same)
     for (int c = lane * per; c < min(lane * per + per, pieces); ++c) run += sh.sum[c];
     incl = scan64(run);
     whole_left = shfl64(incl, 63);
+    if (whole_left || !with_q) break;
+    with_q = false;  // (nothing left: the draft's distribution covers the target's; from p then)
     __syncthreads();
-    if (whole_left || !with_q) break;  // (nothing left: the draft's distribution covers the target's; from p then)
+    sum_up(0, pieces, false);
   }
   if (w != 0) return;
   const uint64_t goal = __umul64hi(fraction64(unit(a.draw[r])), whole_left);
@@ -1203,9 +1246,11 @@ __global__ __launch_bounds__(NT) void verify_rows(VArgs a) {
     if (sum + sh.sum[at] > goal || at + 1 >= min((l + 1) * per, pieces)) break;
     sum += sh.sum[at];
   }
+  Raw raw;
   uint32_t key[8];
   float prob[8];
-  load(at * 64 + lane, key, prob);
+  load(at * 64 + lane, raw);
+  values(at * 64 + lane, raw, key, prob);
   uint64_t own[8], mine = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -1256,7 +1301,10 @@ hipError_t launch_sample(const SampleProblem& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-int64_t verify_workspace_bytes(int64_t rows) { return kWsCounterBytes + rows * (int64_t)sizeof(RowState); }
+static int64_t sums_bytes(int64_t requests, int64_t vocab) { return requests * ((vocab + PIECE - 1) / PIECE) * 8; }
+int64_t verify_workspace_bytes(int64_t rows, int64_t requests, int64_t vocab) {
+  return kWsCounterBytes + sums_bytes(requests, vocab) + rows * (int64_t)sizeof(RowState);
+}
 
 template <typename T>
 static hipError_t launch_verify_t(const VerifyProblem& p, const VArgs& a, hipStream_t stream) {
@@ -1264,7 +1312,7 @@ static hipError_t launch_verify_t(const VerifyProblem& p, const VArgs& a, hipStr
   const auto fn = p.q_type == SAMPLE_F32 ? verify_rows<T, float>
                   : p.q_type == DT_BF16  ? verify_rows<T, __bf16>
                                          : verify_rows<T, _Float16>;
-  if (p.requests) hipLaunchKernelGGL(fn, dim3((unsigned)p.requests), dim3(NT), 0, stream, a);
+  if (p.requests) hipLaunchKernelGGL(fn, dim3((unsigned)(p.requests * a.shares)), dim3(64 * VW), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -1277,7 +1325,13 @@ hipError_t launch_verify(const VerifyProblem& p, hipStream_t stream) {
   a.q = (const char*)p.q;
   a.ldq = p.ldq;
   a.rows = p.rows;
-  a.state = (RowState*)((char*)p.ws + kWsCounterBytes);
+  a.arrived = (unsigned long long*)p.ws;
+  a.sums = (uint64_t*)((char*)p.ws + kWsCounterBytes);
+  a.state = (RowState*)((char*)a.sums + sums_bytes(p.requests, p.vocab));
+  // four pieces a wave, while every CU has no more than eight of these workgroups
+  const int64_t pieces = (p.vocab + PIECE - 1) / PIECE, most = p.requests <= kWsMaxTiles ? 2048 / (p.requests ? p.requests : 1) : 1;
+  const int64_t shares = p.q ? (pieces + 4 * VW - 1) / (4 * VW) : 1;
+  a.shares = (int)(shares < most ? shares : most < 1 ? 1 : most);
   a.counts = p.counts;
   a.requests = (int)p.requests;
   a.per = p.requests ? (int)(p.rows / p.requests) : 0;

@@ -812,7 +812,7 @@ PyObject* op_verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
   NOT_PLAIN_UNLESS(set.take(in, args + 6, {R}));
   const c10::DeviceGuard guard(x->device());
   const Tensor tokens = fresh(*x, lead, at::kLong), counts = fresh(*x, {R}, at::kInt);
-  const Workspace ws(hxmi_verify_workspace_bytes(M), *x);
+  const Workspace ws(hxmi_verify_workspace_bytes(M, R, V), *x);
   if (!ws.ok) return nullptr;
   void* s = in.stream();
   const int rc = unlocked([&] {

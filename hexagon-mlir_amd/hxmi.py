@@ -82,7 +82,7 @@ SIGNATURES = {
     "hxmi_qk_rope": ([_I] + [_P] * 5 + [_I] + [_P] * 4 + [_I] + [_I64] * 15 + [_I, _F, _F, _P], _I),
     "hxmi_sample": ([_I] + [_P] * 6 + [_F, ctypes.c_int32, _F, _F, _P] + [_I64] * 3 + [_P], _I),
     "hxmi_verify": ([_I] + [_P] * 6 + [_I] + [_P] * 4 + [_F, ctypes.c_int32, _F, _F, _P, _P] + [_I64] * 5 + [_P, _I64, _P], _I),
-    "hxmi_verify_workspace_bytes": ([_I64], _I64),
+    "hxmi_verify_workspace_bytes": ([_I64] * 3, _I64),
     "hxmi_lwp_record": ([_P, _I64, ctypes.c_uint32, _P], _I),
     "hxmi_lwp_clock_hz": ([], _I64),
     "hexkl_matmul_f16f16_f32": ([_I64, _I64, _I64, _P, _P, _P], _I),
@@ -1561,7 +1561,7 @@ def verify(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor, draw: to
             counts.zero_()
             return Verified(tokens, counts)
         x, q = flat(logits), None if draft_probs is None else flat(draft_probs)
-        ws = _workspace(lib.hxmi_verify_workspace_bytes(rows), x.device)
+        ws = _workspace(lib.hxmi_verify_workspace_bytes(rows, R, vocab), x.device)
         _check(lib.hxmi_verify(
             _SAMPLE_TYPES[x.dtype], x.data_ptr(), drafts.data_ptr(), u.data_ptr(), draw.data_ptr(), _ptr(cu), _ptr(q),
             2 if q is None else _SAMPLE_TYPES[q.dtype], *ptrs, *alls, tokens.data_ptr(), counts.data_ptr(), rows, R, vocab,

@@ -670,8 +670,9 @@ int hxmi_sample(int dtype, const void* logits, const float* u, const float* temp
  * sum to 1); a row with a NaN logit or none above -inf accepts nothing and draws -1.
  * Settings are per request (pointers of `requests` entries) or, where NULL, the
  * all_* value.  Weights are integers as in hxmi_sample, q * (their sum) rounded
- * down to one.  workspace: hxmi_verify_workspace_bytes(rows) bytes, 256-byte
- * aligned; its first HXMI_WORKSPACE_COUNTER_BYTES are left alone.  vocab <= 2^20.
+ * down to one.  workspace: as for hxmi_gemm_f16 (zeroed once after allocation,
+ * its counters left zeroed, one call at a time), not NULL,
+ * hxmi_verify_workspace_bytes() bytes.  vocab <= 2^20.
  * No counterpart in the reference.
  */
 int hxmi_verify(int dtype, const void* logits, const int64_t* drafts, const float* u, const float* draw,
@@ -680,7 +681,7 @@ int hxmi_verify(int dtype, const void* logits, const int64_t* drafts, const floa
                 int32_t all_top_k, float all_top_p, float all_min_p, int64_t* tokens, int32_t* counts, int64_t rows,
                 int64_t requests, int64_t vocab, int64_t ldx, int64_t ld_probs, void* workspace,
                 int64_t workspace_bytes, void* stream);
-int64_t hxmi_verify_workspace_bytes(int64_t rows);
+int64_t hxmi_verify_workspace_bytes(int64_t rows, int64_t requests, int64_t vocab);
 
 /*
  * Region profiling hook: enqueues on `stream` a one-wave marker that, when it

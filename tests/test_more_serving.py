@@ -102,7 +102,9 @@ def test_verify_refuses(pkg, bad, msg):
 
 def test_verify_workspace(pkg):
     need = pkg.load_library().hxmi_verify_workspace_bytes
-    assert need(0) == need(-1) == 0 and need(1) > 16384 and need(100) - need(1) == 99 * (need(2) - need(1))
+    assert need(0, 1, 9) == need(-1, 1, 9) == need(1, 0, 9) == need(1, 1, 0) == 0 and need(1, 1, 1) > 16384
+    assert need(100, 3, 9) - need(1, 3, 9) == 99 * (need(2, 3, 9) - need(1, 3, 9))
+    assert need(7, 3, 152000) - need(7, 2, 152000) == (152000 + 511) // 512 * 8
 
 
 def test_empty_calls_do_nothing(pkg):

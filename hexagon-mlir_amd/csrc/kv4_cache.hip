@@ -156,8 +156,9 @@ __global__ __launch_bounds__(256) void kv4_append(CArgs a) {
       const uint64_t mask = (n == 16 ? ~0ull : (1ull << (4 * n)) - 1) << (4 * off);
       uint64_t* const dst = (uint64_t*)(a.codes[1] + (((cell << (a.lb - 4)) + (at >> 4)) * a.dp + d + token) * 8);
       both &= mask;
-      if (n < 16) both |= *dst & ~mask;
-      *dst = both;
+      // (other runs may write other tokens of the piece meanwhile)
+      if (n < 16) __hip_atomic_fetch_xor(dst, both ^ (*dst & mask), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      else *dst = both;
     }
   }
 }

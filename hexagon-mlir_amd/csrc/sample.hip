@@ -1131,8 +1131,8 @@ __global__ __launch_bounds__(64 * VW) void verify_rows(VArgs a) {
   }
   if (stop >= end) return;  // (without rows)
   const RowState st = a.state[stop];
-  if (st.state == kDrawn) {
-    if (share == 0 && threadIdx.x == 0) a.token[stop] = st.token;
+  if (st.state == kDrawn || !a.q) {  // (without q every row has drawn; only a row that two requests claim may have no state)
+    if (share == 0 && threadIdx.x == 0) a.token[stop] = st.state == kDrawn ? st.token : -1;
     return;
   }
   __syncthreads();

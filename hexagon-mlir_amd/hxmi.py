@@ -1327,13 +1327,14 @@ def kv_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, fr
 
 def kv_append(cache: Union[KVCache, KVCache4], k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Write k and v rows [tokens, kv_heads, head_dim] (fp16 or bf16) to the
-    given slots [tokens] (int64; those outside the cache are skipped).  Rows of
-    one block are consecutive rows with consecutive slots, as kv_plan gives
-    them.  In a KVCache a block and head's scale is what its largest value needs:
-    it grows with later rows (earlier codes are rounded again) and starts anew
-    when the block's first token is written.  In a KVCache4 every 32 dimensions
-    of a row have a scale of their own and what is there already does not change;
-    values past 61440, infinities and NaN among them, are held as 61440."""
+    given slots [tokens] (int64; those outside the cache are skipped; each at
+    most once).  In a KVCache rows of one block are consecutive rows with
+    consecutive slots, as kv_plan gives them, and a block and head's scale is what its
+    largest value needs: it grows with later rows (earlier codes are rounded
+    again) and starts anew when the block's first token is written.  A KVCache4
+    takes slots in any order; every 32 dimensions of a row have a scale of their
+    own and what is there already does not change; values past 61440, infinities
+    and NaN among them, are held as 61440."""
     native, name = _of_cache(cache, "kv_append")
     if isinstance(cache, (KVCache, KVCache4)) and native(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim,
                                                          k, v, slots):

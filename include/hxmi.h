@@ -584,8 +584,9 @@ int hxmi_qk_rope(int is_bf16, const void* q, const void* k, void* q_out, void* k
  */
 
 /*
- * hxmi_kv_append for the 4-bit cache; rows of one piece of 16 tokens (not block)
- * must be consecutive rows with consecutive slots.  For every 32 dimensions of a row:
+ * hxmi_kv_append for the 4-bit cache; slots may come in any order, each at most
+ * once a call (of rows with the same slot, what it holds is unspecified).  For every
+ * 32 dimensions of a row:
  *   scale = the smallest of the scales s with 6 s >= the largest magnitude
  *   code  = the magnitude nearest to |value| / scale (half way: the one whose
  *           code is even), with the value's sign

@@ -97,6 +97,21 @@ def test_append_of_many_requests(pkg, dev, tokens, heads, d, block, dtype):
         assert torch.equal(got.cpu().double(), want)
 
 
+@pytest.mark.parametrize("heads, d, block", [(2, 64, 16), (1, 128, 64), (3, 40, 32)])
+def test_append_in_any_order(pkg, dev, heads, d, block):
+    """Slots with gaps, backwards and shuffled, many of them of the same pieces in one call."""
+    g, cells = gen(27), 6 * block
+    for n, order in ((cells, "shuffled"), (cells // 2, "every other"), (cells, "backwards"), (7, "few")):
+        slots = {"shuffled": torch.randperm(cells, generator=g), "every other": torch.arange(0, cells, 2),
+                 "backwards": torch.arange(cells).flip(0), "few": torch.tensor([3, 1, 14, 15, 0, 9, 40])}[order]
+        cache, held = pkg.KVCache4.empty(6, heads, d, block, device=dev), Held(cells, heads, d)
+        for step in range(2):  # into an empty cache, then over what is there
+            k, v = torch.randn((2, n, heads, d), generator=g).half()
+            pkg.kv_append(cache, k.to(dev), v.to(dev), slots.to(dev))
+            held.append(k, v, slots.tolist())
+            held.check(pkg, cache, torch.float16, (order, step))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_append_of_every_border(pkg, dev, dtype):
     """Rows whose quotients are every magnitude, every border of two and the

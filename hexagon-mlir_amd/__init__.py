@@ -32,6 +32,7 @@ from .hxmi import (
     kv_attention,
     kv_plan,
     kv_read,
+    kv_trim,
     linear,
     load_library,
     pack_gate_up,
@@ -67,6 +68,7 @@ __all__ = [
     "kv_attention",
     "kv_plan",
     "kv_read",
+    "kv_trim",
     "linear",
     "load_library",
     "pack_gate_up",

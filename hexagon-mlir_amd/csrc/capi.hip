@@ -716,6 +716,33 @@ int hxmi_kv_plan(const int32_t* lens, const int32_t* added, int32_t* block_table
   return from_hip(hxmi::launch_kv_plan(p, (hipStream_t)stream), name);
 }
 
+int hxmi_kv_trim(int32_t* lens, const int32_t* keep, const int32_t* block_table, int32_t* free_blocks,
+                 int32_t* free_count, int64_t requests, int64_t width, int64_t ld_table, int64_t capacity,
+                 int64_t block_size, void* stream) {
+  const char* name = "hxmi_kv_trim";
+  REQUIRE(requests >= 0 && width >= 0 && capacity >= 0, "%s: negative size", name);
+  const int lb = log2_block(block_size);
+  REQUIRE(lb >= 0, "%s: block_size must be a power of two from 16 to 256, got %lld", name, (long long)block_size);
+  REQUIRE(capacity < (1ll << 31) && requests < (1ll << 31) && width <= (1ll << 30) / block_size &&
+              requests * width < (1ll << 31),
+          "%s: capacity and table entries must be below 2^31, a table row at most 2^30 tokens", name);
+  REQUIRE(ld_table >= width, "%s: ld_table below the table's width", name);
+  if (requests == 0) return ok();
+  REQUIRE(lens && keep && free_count && (block_table || !width) && (free_blocks || !capacity), "%s: null pointer", name);
+  hxmi::KvTrimProblem p{};
+  p.lens = lens;
+  p.keep = keep;
+  p.table = block_table;
+  p.stack = free_blocks;
+  p.count = free_count;
+  p.requests = requests;
+  p.width = width;
+  p.ldt = ld_table;
+  p.capacity = capacity;
+  p.log2_block = lb;
+  return from_hip(hxmi::launch_kv_trim(p, (hipStream_t)stream), name);
+}
+
 // The cache's own arguments, which every call on it takes.
 static int cache_check(const char* name, const void* k_codes, const void* v_codes, const void* k_scale,
                        const void* v_scale, int64_t blocks, int64_t kv_heads, int64_t head_dim, int64_t block_size,

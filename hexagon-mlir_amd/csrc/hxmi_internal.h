@@ -208,6 +208,15 @@ struct KvPlanProblem {
   int log2_block;
 };
 hipError_t launch_kv_plan(const KvPlanProblem& p, hipStream_t stream);
+struct KvTrimProblem {
+  int* lens;
+  const int* keep;
+  const int* table;
+  int *stack, *count;
+  int64_t requests, width, ldt, capacity;
+  int log2_block;
+};
+hipError_t launch_kv_trim(const KvTrimProblem& p, hipStream_t stream);
 
 // Rows of keys and values into the 8-bit cache (k, v) or out of it (k_out, v_out).
 struct KvCacheProblem {

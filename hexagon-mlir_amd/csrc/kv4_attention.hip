@@ -11,9 +11,9 @@
 // as it is:
 //   * scores as D[key][row] = K . Q^T (16x16x32 MFMAs).  The dims of a step may
 //     come in any order, so a lane takes 16 (of 64) or 32 (of 128) dims of a key
-//     that lie together, under one scale.  Row m of tile t is key 4 m + t of the
-//     group: a lane's four keys have their scales in one word, and its 16 scores
-//     (row l % 16, g = l / 16) are keys 16 g .. 16 g + 15, one page's;
+//     that lie together, under one scale.  Row m of tile t is key 16 (m / 4) + 4 t +
+//     m % 4 of the group (four keys in a row an access), and a lane's 16 scores
+//     (row l % 16, g = l / 16) are keys 16 g .. 16 g + 15 in order, one page's;
 //   * those 16 weights are the B operand of P.V as they are.  A lane's V numbers
 //     are two dims of those 16 tokens, tiles 2 c and 2 c + 1 of 32 dims (row m is
 //     dim 2 m or 2 m + 1), so that a lane ends with eight dims that lie together;
@@ -21,7 +21,15 @@
 //     of its largest element;
 //   * weights are relative to 2^m, m from 7 to 15 below the running maximum, in
 //     11 bits or multiples of 2^-31 of the row's largest (fp16 below 2^-14);
-//     scores, maxima, sums and O are fp32.
+//     scores, maxima, sums and O are fp32.  Scales that are part of V and K, and
+//     not of the weights, keep that one maximum valid whatever they are.
+// One token a request: 64 requests of 4096 to 8192 tokens, 32 heads over 8 of 128
+// dims, 94-100 us (422 MB at 4.2-4.5 TB/s; a copy reaches 4.98).  It is bound by the vector
+// ALUs as much as by memory: 500 instructions a wave and group, 256 of them the
+// conversion; with every V number from one block (half the bytes) it is only 10 %
+// faster.  Two groups in flight a wave, non-temporal loads, three shares a
+// tile and equal shares of fewer keys were no faster.  One token of 131072 keys 41 us, 1900
+// tokens of one user 7.1-7.5 (latency; launch, two rounds of loads, joins).
 #include "kv4.h"
 #include "kv_attention_impl.h"
 
@@ -392,7 +400,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
 // those of the next stage but one are in flight meanwhile.  Scores are
 // D[key][row] of 32x32x16 MFMAs; row m of a 32-key block reads key 16 (m / 16) +
 // 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that a lane's eight weights of 16 keys
-// are eight in order, the B operand of P.V.
+// are eight in order, the B operand of P.V.  2350 rows x 32 heads over 8000 keys of 128
+// dims: 253 us (780 TFLOP/s; 397 by the kernel above), 64 dims over 4 heads 223 us. The
+// vector ALUs bound it: softmax (an exponential is two slots, a sum of weights half
+// a one: both as v_dot2), then conversion.
 // D: LDS rows of K (64 or 128 dims).
 template <typename T, int D, bool WHOLE>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArgs a) {

@@ -228,6 +228,53 @@ struct Bits16<__bf16> {
   static constexpr uint32_t inf = 0x7f80;
 };
 
+// ---- kv_trim -------------------------------------------------------------------
+
+struct TArgs {
+  int* lens;
+  const int* keep;
+  const int* table;
+  int* stack;
+  int* count;
+  int64_t ldt;
+  int requests, width, capacity, lb;
+};
+
+// One workgroup: a thread a request, its blocks' place on the stack from a sum over the
+// requests before it.
+__global__ __launch_bounds__(1024) void kv_trim(TArgs a) {
+  __shared__ int part[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int64_t at = max(a.count[0], 0);
+  for (int r0 = 0; r0 < a.requests; r0 += 1024) {
+    const int r = r0 + (int)threadIdx.x;
+    int first = 0, n = 0;
+    if (r < a.requests) {
+      const int len = a.lens[r], keep = a.keep[r];
+      if (keep >= 0 && keep < len) {
+        auto held = [&](int tokens) { return (int)min(((int64_t)tokens + (1 << a.lb) - 1) >> a.lb, (int64_t)a.width); };
+        first = held(keep);
+        n = held(len) - first;
+        a.lens[r] = keep;
+      }
+    }
+    const int incl = (int)scan64((uint64_t)n);  // (at most requests * width: below 2^31)
+    __syncthreads();
+    if (lane == 63) part[w] = incl;
+    __syncthreads();
+    int64_t before = at + incl - n;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      before += i < w ? part[i] : 0;
+      at += part[i];
+    }
+    for (int j = 0; j < n; ++j)
+      if (before + j < a.capacity) a.stack[before + j] = a.table[(int64_t)r * a.ldt + first + j];
+  }
+  __syncthreads();  // (everyone has read the count)
+  if (threadIdx.x == 0) a.count[0] = (int)min(at, (int64_t)a.capacity);
+}
+
 // ---- kv_append -------------------------------------------------------------------
 
 struct CArgs {
@@ -461,6 +508,12 @@ hipError_t launch_kv_plan(const KvPlanProblem& p, hipStream_t stream) {
   const dim3 grid((unsigned)(wgs < 1 ? 1 : wgs < 128 ? wgs : 128));
   if (nt == 256) hipLaunchKernelGGL(kv_plan<256>, grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL(kv_plan<1024>, grid, dim3(1024), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_trim(const KvTrimProblem& p, hipStream_t stream) {
+  const TArgs a{p.lens, p.keep, p.table, p.stack, p.count, p.ldt, (int)p.requests, (int)p.width, (int)p.capacity, p.log2_block};
+  hipLaunchKernelGGL(kv_trim, dim3(1), dim3(1024), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -13,7 +13,10 @@
 //
 // A workgroup takes a few tokens: a thread computes each pair's cosine and
 // sine into LDS, once for all heads, then groups of lanes take heads, a lane the
-// same eight pairs (16 values) of every one.
+// same eight pairs (16 values) of every one, the next head's in flight meanwhile.
+// Memory bounds it: 16384 tokens of 40 heads of 128 dims with norms 74 us (336 MB at 4.5
+// TB/s; 98 without the head ahead); one token of 36 heads of 64 2.9 us, a launch
+// and three dependent loads.
 #include "hxmi_common.h"
 #include "hxmi_internal.h"
 
@@ -83,7 +86,7 @@ enum Form {
   kNext,   // four pairs of neighbours
 };
 
-// LOG: 2^LOG lanes a head.
+// 2^log lanes a head.
 template <typename T, int FORM, bool NORM>
 __global__ __launch_bounds__(256) void qk_rope(RArgs a, int log) {
   __shared__ __attribute__((aligned(16))) float cs[kMaxPairs], sn[kMaxPairs];

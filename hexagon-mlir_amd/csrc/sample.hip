@@ -1102,7 +1102,9 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
 // weights less floor(q * sum), integers as they are, by pieces of 512 tokens,
 // then the token in the piece that reaches draw * sum.
 // A request's pieces go to a.shares workgroups of four waves, which store their
-// sums; the last to arrive draws.  Each finds the stopping row for itself.
+// sums; the last to arrive draws.  Each finds the stopping row for itself.  64
+// requests over 151936 tokens, top-p: 18 us in 19 shares (22 in ten, 48 by one
+// workgroup of sixteen waves), after 64 us of sample_rows (190 rows, a CU each).
 constexpr int VW = 4;
 template <typename T, typename Q>
 __global__ __launch_bounds__(64 * VW) void verify_rows(VArgs a) {

@@ -71,6 +71,7 @@ SIGNATURES = {
     "hxmi_decode_workspace_bytes": ([_I64, _I64, _I64], _I64),
     "hxmi_decode_status": ([_P, _I, ctypes.POINTER(_I), _P], _I),
     "hxmi_kv_plan": ([_P] * 10 + [_I64] * 6 + [_P], _I),
+    "hxmi_kv_trim": ([_P] * 5 + [_I64] * 5 + [_P], _I),
     "hxmi_kv_append": ([_I] + [_P] * 7 + [_I64] * 9 + [_P], _I),
     "hxmi_kv_read": ([_I] + [_P] * 7 + [_I64] * 5 + [_P], _I),
     "hxmi_kv_attention": ([_I] + [_P] * 9 + [_I64] * 13 + [_F, _P, _I64, _P], _I),
@@ -1323,6 +1324,33 @@ def kv_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, fr
             *(t.data_ptr() for t in out), n, block_table.shape[1], ldt, free_blocks.numel(), int(tokens),
             int(block_size), _stream(lens)))
     return out
+
+
+def kv_trim(lens: torch.Tensor, keep: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
+            free_count: torch.Tensor, *, block_size: int) -> None:
+    """Take tokens back from requests, on the GPU in one launch: where 0 <=
+    keep[r] < lens[r] [requests] (int32), lens[r] becomes keep[r] and the blocks
+    that only the tokens past it had go onto the stack free_blocks, whose first
+    free_count [1] entries are free, in request order.  lens, the stack and its
+    count are updated in place; block_table and the others are kv_plan's.  A step
+    that verified drafts ends with it: without it the blocks of refused drafts
+    are lost."""
+    _require_gpu(lens, keep, block_table, free_blocks, free_count)
+    for name, t in (("lens", lens), ("free_blocks", free_blocks), ("free_count", free_count)):
+        if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous():
+            raise HxmiError(f"{name} must be a contiguous 1-D torch.int32 tensor")
+    n = lens.numel()
+    keep = _ints(keep, n, "keep")
+    if free_count.numel() != 1:
+        raise HxmiError("free_count must have one element")
+    ldt = _table(block_table, n)
+    held = [t for t in (lens, free_blocks, free_count) if t.numel()]
+    if any(_overlap(a, b) for i, a in enumerate(held) for b in [*held[i + 1:], keep, block_table]):
+        raise HxmiError("lens, free_blocks and free_count are written: they must not share elements with other operands")
+    with _on(lens):
+        _check(load_library().hxmi_kv_trim(lens.data_ptr(), keep.data_ptr(), block_table.data_ptr(), free_blocks.data_ptr(),
+                                           free_count.data_ptr(), n, block_table.shape[1], ldt, free_blocks.numel(),
+                                           int(block_size), _stream(lens)))
 
 
 def kv_append(cache: Union[KVCache, KVCache4], k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:

@@ -483,6 +483,18 @@ int hxmi_kv_plan(const int32_t* lens, const int32_t* added, int32_t* block_table
                  int64_t tokens, int64_t block_size, void* stream);
 
 /*
+ * Takes tokens back from requests, in place: where 0 <= keep[r] < lens[r], lens[r]
+ * becomes keep[r] and the blocks that only tokens past it had (entries
+ * ceil(keep / block_size) to ceil(lens / block_size) of its table row) go onto the
+ * stack of free blocks, in request order; other requests stay as they are.  Other
+ * arguments as hxmi_kv_plan's; entries that the stack has no room for are dropped.
+ * What the cache holds for those tokens is no longer read and may be written over.
+ */
+int hxmi_kv_trim(int32_t* lens, const int32_t* keep, const int32_t* block_table, int32_t* free_blocks,
+                 int32_t* free_count, int64_t requests, int64_t width, int64_t ld_table, int64_t capacity,
+                 int64_t block_size, void* stream);
+
+/*
  * Writes k and v rows [tokens, kv_heads, head_dim] (fp16, or bf16 with
  * is_bf16 = 1; row strides ldk / ldv, head strides head_stride_*, elements,
  * any alignment of the type) to the given slots.  Slots outside the cache are

@@ -51,9 +51,11 @@ class Drafter:
         # row i's draft is the token that row i + 1 was given
         drafts = torch.cat([ids[1:], ids[:1]])
         got = pkg.verify(logits, drafts, u, draw, cu=p.cu, draft_probs=probs, temperature=0.9, top_k=40, top_p=0.95)
-        # the rows past the accepted drafts leave the requests again; blocks taken for them stay
-        self.lens.copy_(p.lens - (p.cu[1:] - p.cu[:-1]) + got.counts)
+        # the rows past the accepted drafts leave the requests again, their blocks go back
+        keep = torch.where(p.lens > self.lens, self.lens + got.counts, p.lens)
+        self.lens.copy_(p.lens)
         self.count.copy_(p.free_count)
+        pkg.kv_trim(self.lens, keep, self.table, self.free, self.count, block_size=self.block)
         return dict(tokens=got.tokens, counts=got.counts, logits=logits, attended=o, qkv=qkv, raw=raw, slots=p.slots, cu=p.cu,
                     positions=p.positions, drafts=drafts, lens=p.lens)
 
@@ -97,8 +99,57 @@ def test_drafting_loop(pkg, dev, dtype):
                                         None if probs is None else probs.double().numpy(), [T, [40] * 3, P, [0.0] * 3])
         assert near == 0 and out["tokens"].tolist() == tokens and out["counts"].tolist() == counts, step
         assert s.lens.tolist() == [b + n for b, n in zip(before, counts)]
+        # every block is a request's or free
+        held = [s.table[r, :-(-n // s.block)].tolist() for r, n in enumerate(s.lens.tolist())]
+        assert sorted(sum(held, []) + s.free[:int(s.count)].tolist()) == list(range(s.blocks))
         token = [tokens[cu[r] + counts[r] - 1] for r in range(3)]
         new = [1 + int(torch.randint(0, 5, (1,), generator=g)) for _ in range(3)]
+
+
+@pytest.mark.parametrize("requests, width, block, seed", [(1, 4, 16, 0), (70, 5, 32, 1), (2100, 3, 16, 2), (5000, 2, 64, 3)])
+def test_trim(pkg, dev, requests, width, block, seed):
+    """Lengths taken back by some, all, none and more than there are; a stack short of room."""
+    rng = np.random.default_rng(seed)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    lens = rng.integers(0, width * block + 1, requests)
+    keep = np.where(rng.random(requests) < 0.3, lens, rng.integers(-3, width * block + 9, requests))
+    table = rng.permutation(requests * (width + 2)).reshape(requests, width + 2)
+    held = lambda n: -(-n // block)  # noqa: E731
+    want, stack = lens.copy(), [900001, 900002]
+    for r in range(requests):
+        if 0 <= keep[r] < lens[r]:
+            stack += table[r, held(keep[r]):held(lens[r])].tolist()
+            want[r] = keep[r]
+    for room in (len(stack) + 5, max(len(stack) - 1, 2)):
+        a, free, count = i32(lens), torch.full((room,), -7, dtype=torch.int32, device=dev), i32([2])
+        free[:2] = i32([900001, 900002])
+        t = i32(table)[:, :width]
+        pkg.kv_trim(a, i32(keep), t, free, count, block_size=block)
+        assert a.tolist() == want.tolist() and count.tolist() == [min(len(stack), room)]
+        assert free.tolist() == (stack + [-7] * 5)[:room] and torch.equal(t, i32(table)[:, :width])
+
+
+def test_trim_refuses(pkg, dev):
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    lens, table, free, count = i32(5, 6), torch.zeros((2, 3), dtype=torch.int32, device=dev), i32(1, 2, 3), i32(1)
+    bad = [
+        ("lens", lambda: pkg.kv_trim(lens.long(), lens, table, free, count, block_size=16)),
+        ("keep", lambda: pkg.kv_trim(lens, lens[:1].clone(), table, free, count, block_size=16)),
+        ("share", lambda: pkg.kv_trim(lens, lens, table, free, count, block_size=16)),
+        ("share", lambda: pkg.kv_trim(lens, i32(1, 1), table, free, free[:1], block_size=16)),
+        ("block_table", lambda: pkg.kv_trim(lens, i32(1, 1), table[:1], free, count, block_size=16)),
+        ("free_blocks", lambda: pkg.kv_trim(lens, i32(1, 1), table, free[::2], count, block_size=16)),
+        ("free_count", lambda: pkg.kv_trim(lens, i32(1, 1), table, free, i32(1, 2), block_size=16)),
+        ("block_size", lambda: pkg.kv_trim(lens, i32(1, 1), table, free, count, block_size=17)),
+        ("GPU", lambda: pkg.kv_trim(lens, i32(1, 1), table.cpu(), free, count, block_size=16)),
+    ]
+    for i, (msg, call) in enumerate(bad):
+        with pytest.raises(pkg.HxmiError, match=msg):
+            call()
+            pytest.fail(f"call {i} ({msg}) was taken")
+    none = i32()
+    pkg.kv_trim(none, i32(), table[:0], free, count, block_size=16)
+    assert lens.tolist() == [5, 6] and free.tolist() == [1, 2, 3] and count.tolist() == [1]
 
 
 @pytest.mark.parametrize("bits", [4, 8])

@@ -32,6 +32,20 @@ def test_rope_refuses(pkg, bad, msg):
     assert msg in last(pkg)
 
 
+def trim(pkg, requests=4, width=4, ld=4, capacity=16, block=16, ptr=P, count=P):
+    return pkg.load_library().hxmi_kv_trim(ptr, ptr, ptr, ptr, count, requests, width, ld, capacity, block, None)
+
+
+@pytest.mark.parametrize("bad, msg", [
+    (dict(requests=-1), "negative"), (dict(width=-1), "negative"), (dict(capacity=-1), "negative"), (dict(block=24), "power of two"),
+    (dict(ld=3), "ld_table"), (dict(ptr=None), "null"), (dict(count=None), "null"), (dict(capacity=1 << 31), "2^31"),
+    (dict(width=1 << 27, ld=1 << 27), "2^30"), (dict(requests=1 << 30, width=4), "2^31"),
+])
+def test_trim_refuses(pkg, bad, msg):
+    assert trim(pkg, **bad) == 1
+    assert msg in last(pkg)
+
+
 def append(pkg, tokens=4, blocks=4, heads=2, d=64, block=16, bf16=0, ptr=P, codes=P, scale=P, ld=128, hs=64):
     return pkg.load_library().hxmi_kv4_append(bf16, ptr, ptr, ptr, codes, codes, scale, scale, tokens, blocks, heads, d,
                                               block, ld, hs, ld, hs, None)
@@ -108,7 +122,7 @@ def test_verify_workspace(pkg):
 
 
 def test_empty_calls_do_nothing(pkg):
-    assert verify(pkg, rows=0, requests=0, x=None, draw=None) == 0
+    assert verify(pkg, rows=0, requests=0, x=None, draw=None) == 0 and trim(pkg, requests=0, ptr=None) == 0
     assert rope(pkg, tokens=0, q=None, k=None, pos=None) == 0 and rope(pkg, heads=0, kv_heads=0, q=None, k=None) == 0
     assert append(pkg, tokens=0, ptr=None) == 0 and append(pkg, blocks=0, codes=None, scale=None) == 0
     assert read(pkg, tokens=0, ptr=None) == 0

@@ -151,7 +151,7 @@ inline KvPlan plan_of(const KvAttnSizes& p, int64_t slots = 512) {  // slots: wo
   // 63 in eight.  The table's width stands for the lengths, which only the GPU
   // knows: shares past a request's keys are joined for nothing (one user of 1900
   // tokens: 7.5 us with a table of 30 pages, 10.6 with 128, 24 with 512 or more).
-  const int64_t items = r.tiles * p.kv_heads, least = wide ? 512 : 256, most = (p.width * p.block + least - 1) / least;
+  const int64_t items = r.tiles * p.kv_heads, least = wide || slots > 512 ? 512 : 256, most = (p.width * p.block + least - 1) / least;
   if (wide) slots = 512;
   const int64_t left = items % slots;
   int64_t n = left ? slots / left : 1;

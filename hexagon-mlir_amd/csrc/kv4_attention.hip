@@ -49,6 +49,17 @@ struct KArgs : TileArgs {
 // Weights are 2^(score - m): m stays until a score is more than kHigh above it,
 // then follows to kLow below the largest.
 constexpr float kLow = 7.f, kHigh = 15.f;
+// From this magnitude of m on, a score's product with c is rounded before m is
+// subtracted: what fp32 leaves of m is steps of 1/8 and more, and the unrounded
+// product's distance from it would be a factor on the weights, 2^4096 at scores of 2^36.
+constexpr float kFar = 0x1p20f;
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m != -INFINITY; }
+
+// a * b, rounded (never part of an fma).
+__device__ __forceinline__ float times(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
 
 // Eight numbers times their scales (pairs) as one MFMA operand.
 template <typename F>
@@ -179,6 +190,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
 
   Partial<DT> acc;
   acc.clear();
+  bool far = false;  // some row's m is
 
   const uint32_t kbyte = twice_byte(lr & 3);  // (of the words of scales, those of this lane's keys)
   const int ck = lr >> 2;  // 16-key piece of a group that this lane's K rows lie in (V's and the scores': lg)
@@ -290,14 +302,23 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
       acc.l *= f;
 #pragma unroll
       for (int t = 0; t < DT; ++t) acc.o[t] *= f;
+      far = __any(is_far(now));
     }
     const float off = acc.m == -INFINITY ? 0.f : -acc.m;
+    float cw = c;
+    if (far) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][i] = times(s[t][i], c);
+      cw = 1.f;
+    }
     half8v p[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[2 * u + (j >> 2)][j & 3], c, off));
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[2 * u + (j >> 2)][j & 3], cw, off));
         acc.l += e;
         p[u][j] = (_Float16)e;
       }
@@ -540,6 +561,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
 
   float16v o[DT];
   float m = -INFINITY, l = 0.f;
+  bool far = false;  // some row's m is
 #pragma unroll
   for (int x = 0; x < DT; ++x) o[x] = float16v{};
 
@@ -608,14 +630,23 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
       l *= f;
 #pragma unroll
       for (int x = 0; x < DT; ++x) o[x] *= f;
+      far = __any(is_far(now));
     }
     const float off = m == -INFINITY ? 0.f : -m;
+    float cw = c;
+    if (far) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[x][i] = times(s[x][i], c);
+      cw = 1.f;
+    }
     // the weights of 16 keys while the MFMAs of the 16 before run
     auto weights = [&](int x) {
       half8v p;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        p[e] = (_Float16)__builtin_amdgcn_exp2f(fmaf(s[x >> 1][8 * (x & 1) + e], c, off));
+        p[e] = (_Float16)__builtin_amdgcn_exp2f(fmaf(s[x >> 1][8 * (x & 1) + e], cw, off));
       l = sum_of(p, l);
       return p;
     };

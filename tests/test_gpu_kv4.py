@@ -400,6 +400,40 @@ def test_attention_at_the_ends_of_its_range(pkg, dev, dtype):
     assert (got > 3e-4).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 130])  # tiles of 16 rows and of 128
+def test_attention_of_scores_far_beyond(pkg, dev, dtype, rows):
+    """Scores from 2^18 to 2^38, of either sign: the key far above the others is
+    what remains, equal ones share, and rows with a few small scores beside such stay as they are."""
+    heads, kv_heads, d, block, blocks = 32, 1, 64, 16, 16
+    n, g = blocks * block, gen(87)
+    table, lens = torch.arange(blocks, dtype=torch.int32, device=dev).view(1, blocks), ints(dev, n)
+    v = torch.randn((n, 1, d), generator=g).half()
+    for size in (96.0, 6144.0, 61440.0):
+        for sign in (1, -1):
+            k = torch.full((n, 1, d), sign * size)
+            k[::3] *= 2 / 3 if sign > 0 else 1
+            if sign < 0:
+                k[1::3] *= 2 / 3
+                k[2::3] *= 2 / 3
+            best = torch.arange(n) % 3 != 0  # the (equal) largest scores' keys
+            cache = pkg.KVCache4.empty(blocks, 1, d, block, device=dev)
+            pkg.kv_append(cache, k.half().to(dev), v.to(dev), torch.arange(n, device=dev))
+            vs = numbers(cache, "v")[:, 0]
+            q = (torch.rand((rows, heads, d), generator=g) + 0.5) * torch.exp2(torch.arange(heads).float() % 16 - 1)[:, None]
+            q[:, 5] = 2.0 ** -18  # (scores of about one beside the others' of 2^20 and more)
+            q = q.to(dtype).to(dev)
+            got = pkg.kv_attention(q, cache, table, lens, cu=ints(dev, 0, rows), scale=1.0).cpu().double()
+            for i in (0, rows - 1):
+                seen = torch.arange(n) <= n - rows + i
+                want = vs[best & seen].mean(0)
+                far = [h for h in range(heads) if h != 5]
+                # the weights are equal and their sum exact to 2^-12; other scores lie 30 and more below
+                assert ((got[i, far] - want).abs() <= HALF[dtype] * want.abs() + 2.0 ** -11 * vs.abs().mean(0) + 2.0 ** -25).all(), (size, sign, i)
+            check_attention(got[:, 5:6].to(dtype), q[:, 5:6], numbers(cache, "k"), numbers(cache, "v"), block, table, lens,
+                            [0, rows], 1.0, blocks, (size, sign))
+
+
 def test_attention_past_32_bit_offsets(pkg, dev):
     """A cache of more than 4 GiB of codes each: pages at its start and end."""
     heads, kv_heads, d, block, blocks = 8, 8, 128, 64, 140000

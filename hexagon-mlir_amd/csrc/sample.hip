@@ -76,6 +76,7 @@ struct RowState {
   uint32_t state, tau, top, from;
   int ties_end;  // equals of tau before this token are kept
   float t;
+  int owner;  // the request that the row was judged for, -1: none
 };
 enum : uint32_t { kDrawn, kAccepted, kToDraw };
 struct VArgs : SArgs {
@@ -361,8 +362,11 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
     }
     int64_t first, end;
     rows_of(a, lo, first, end);
-    if (row < first || row >= end) {  // of no request
-      if (threadIdx.x == 0) a.token[row] = -1;
+    if (row < first || row >= end) {  // of no request (or, where bounds do not ascend, one that the search passes by)
+      if (threadIdx.x == 0) {
+        a.token[row] = -1;
+        a.state[row] = RowState{.token = -1, .state = kDrawn, .owner = -1};
+      }
       return;
     }
     owner = lo;
@@ -500,7 +504,7 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
   extremes();
   if (top > kInf || low + 1 < kMinusInf || top == kMinusInf) {
     if (threadIdx.x == 0) {
-      if constexpr (VERIFY) a.state[row] = RowState{.token = -1, .state = kDrawn};
+      if constexpr (VERIFY) a.state[row] = RowState{.token = -1, .state = kDrawn, .owner = (int)owner};
       else a.token[row] = -1;
     }
     return;
@@ -1021,7 +1025,7 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
         }
       }
       if (lane == 0)
-        a.state[row] = RowState{-1, whole, least, accepted ? kAccepted : kToDraw, tau, top, from, ties_end, t};
+        a.state[row] = RowState{-1, whole, least, accepted ? kAccepted : kToDraw, tau, top, from, ties_end, t, (int)owner};
       return;
     }
     if (in && !a.q && !final) {
@@ -1084,7 +1088,7 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
       if (so_far > goal) break;
     }
     const int64_t token = (int64_t)(at * 64 + lane) * 8 + e;
-    if constexpr (VERIFY) a.state[row] = RowState{.token = token, .state = kDrawn};
+    if constexpr (VERIFY) a.state[row] = RowState{.token = token, .state = kDrawn, .owner = (int)owner};
     else a.token[row] = token;
   }
 }
@@ -1121,20 +1125,25 @@ __global__ __launch_bounds__(64 * VW) void verify_rows(VArgs a) {
   const int r = (int)(blockIdx.x / a.shares), share = (int)(blockIdx.x - (uint32_t)r * a.shares);
   int64_t first, end;
   rows_of(a, r, first, end);
+  // A row that was judged for another request, or for none, stops this one, and
+  // its token is left to that one: every row's state was written by this call, the
+  // thresholds of the one that is drawn from for this request, and no row has two writers.
   int64_t stop = end;
   for (int64_t i0 = first; i0 < end && stop == end; i0 += 64) {  // (every wave the same)
-    const uint64_t m = __ballot(i0 + lane < end && a.state[min(i0 + lane, end - 1)].state != kAccepted);
+    const RowState& s = a.state[min(i0 + lane, end - 1)];
+    const uint64_t m = __ballot(i0 + lane < end && (s.state != kAccepted || s.owner != r));
     if (m) stop = i0 + __ffsll((unsigned long long)m) - 1;
   }
   if (share == 0) {
     for (int64_t i = first + threadIdx.x; i < end; i += 64 * VW)
-      if (i != stop) a.token[i] = i < stop ? a.drafts[i] : -1;
+      if (i != stop && a.state[i].owner == r) a.token[i] = i < stop ? a.drafts[i] : -1;
     if (threadIdx.x == 0) a.counts[r] = stop < end ? (int)(stop - first + 1) : 0;
   }
   if (stop >= end) return;  // (without rows)
   const RowState st = a.state[stop];
-  if (st.state == kDrawn || !a.q) {  // (without q every row has drawn; only a row that two requests claim may have no state)
-    if (share == 0 && threadIdx.x == 0) a.token[stop] = st.state == kDrawn ? st.token : -1;
+  if (st.owner != r) return;
+  if (st.state == kDrawn) {  // (without q every row that does not accept)
+    if (share == 0 && threadIdx.x == 0) a.token[stop] = st.token;
     return;
   }
   __syncthreads();

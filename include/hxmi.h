@@ -681,6 +681,10 @@ int hxmi_sample(int dtype, const void* logits, const float* u, const float* temp
  * that are (0 for a request without rows).  A draft outside the vocabulary is not
  * accepted; probabilities that are NaN or negative count as 0 (draft_probs need not
  * sum to 1); a row with a NaN logit or none above -inf accepts nothing and draws -1.
+ * Bounds count as the nearest in [0, rows], one below the bound before it as that.
+ * A row that bounds out of order give to two requests is judged for one of them, or for
+ * none; to the others it is a row that draws -1 (in counts alone: tokens there is its own
+ * request's, -1 without one).
  * Settings are per request (pointers of `requests` entries) or, where NULL, the
  * all_* value.  Weights are integers as in hxmi_sample, q * (their sum) rounded
  * down to one.  workspace: as for hxmi_gemm_f16 (zeroed once after allocation,

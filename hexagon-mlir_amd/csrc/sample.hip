@@ -1341,8 +1341,9 @@ hipError_t launch_verify(const VerifyProblem& p, hipStream_t stream) {
   a.state = (RowState*)((char*)a.sums + sums_bytes(p.requests, p.vocab));
   // four pieces a wave, while every CU has no more than eight of these workgroups
   const int64_t pieces = (p.vocab + PIECE - 1) / PIECE, most = p.requests <= kWsMaxTiles ? 2048 / (p.requests ? p.requests : 1) : 1;
-  const int64_t shares = p.q ? (pieces + 4 * VW - 1) / (4 * VW) : 1;
-  a.shares = (int)(shares < most ? shares : most < 1 ? 1 : most);
+  int64_t shares = p.q ? (pieces + 4 * VW - 1) / (4 * VW) : 1;
+  shares = shares < most ? shares : most;
+  a.shares = (int)(shares < 1 ? 1 : shares);  // (no rows, no vocabulary: counts are still to be written)
   a.counts = p.counts;
   a.requests = (int)p.requests;
   a.per = p.requests ? (int)(p.rows / p.requests) : 0;

@@ -72,3 +72,20 @@ def test_bounds_that_do_not_ascend(pkg, dev, dtype, certain):
             earlier()
             got = pkg.verify(x, drafts, u, draw, cu=torch.tensor(cu, dtype=torch.int32, device=dev), draft_probs=probs, top_p=0.9)
             assert got.tokens.tolist() == tokens and got.counts.tolist() == counts, cu
+
+
+@pytest.mark.parametrize("with_cu", [False, True])
+@pytest.mark.parametrize("with_probs", [False, True])
+@pytest.mark.parametrize("requests", [1, 70, 3000])
+def test_requests_without_rows_get_counts_of_zero(pkg, dev, requests, with_probs, with_cu):
+    """The C entry with no rows at all: counts are written, with the draft's
+    probabilities given (never read) or not."""
+    counts = torch.full((requests + 1,), 7, dtype=torch.int32, device=dev)
+    cu, draw = torch.zeros(requests + 1, dtype=torch.int32, device=dev), torch.zeros(requests, device=dev)
+    probs = torch.zeros(8, device=dev)
+    rc = pkg.load_library().hxmi_verify(0, None, None, None, draw.data_ptr(), cu.data_ptr() if with_cu else None,
+                                        probs.data_ptr() if with_probs else None, 2, None, None, None, None, 1.0, 0, 1.0, 0.0,
+                                        None, counts.data_ptr(), 0, requests, 1000, 1000, 1000, None, 0,
+                                        torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, pkg.load_library().hxmi_last_error().decode()
+    assert counts.tolist() == [0] * requests + [7]

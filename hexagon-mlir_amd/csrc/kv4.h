@@ -4,8 +4,8 @@
 // A value is number * scale.  Numbers have a sign, two exponent bits and one of
 // mantissa (0, 1/2, 1, 3/2, 2, 3, 4, 6); 32 dims of a token of a head share a
 // scale, a positive number of five exponent bits and three of mantissa held in a
-// byte: the upper bits of an fp16 number.  So a value has six significant bits:
-// fp16 and bf16 hold it as it is, and what goes into a matrix product is what
+// byte: the upper bits of an fp16 number, up to 10240.  So a value has six significant
+// bits: fp16 and bf16 hold it as it is, and what goes into a matrix product is what
 // the cache holds.
 //
 // Layout (blocks of B tokens, Dp = head dim rounded up to 32):
@@ -20,7 +20,8 @@
 namespace hxmi {
 namespace kv4 {
 
-constexpr float kMost = 61440.f;  // the largest value: 6 * 10240, the largest scale that fp16 holds six of
+constexpr float kMost = 61440.f;       // the largest value: 6 * 10240, the largest scale that fp16 holds six of
+constexpr uint32_t kMostScale = 0xe2;  // that scale's byte
 
 __device__ __forceinline__ float scale_value(uint32_t byte) {
   return (float)__builtin_bit_cast(_Float16, (unsigned short)(byte << 7));

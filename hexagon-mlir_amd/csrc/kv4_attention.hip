@@ -87,10 +87,12 @@ __device__ __forceinline__ uint32_t first_bytes(int n, int x) {
   return c == 4 ? ~0u : (1u << (8 * c)) - 1;
 }
 
-// Bytes of a word of scales that hold no finite number (kv4_append writes none), as 255.
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  const uint32_t e = ((w >> 3) & 0x1f1f1f1fu) ^ 0x1f1f1f1fu;  // 0 where all exponent bits are set
-  return ((~(e + 0x1f1f1f1fu) & 0x20202020u) >> 5) * 255u;
+// Bytes of a word of scales past the largest, as 255: fp16 holds no six of them, or
+// not even one, so a product may be infinite (kv4_append writes none).
+__device__ __forceinline__ uint32_t past_largest(uint32_t w) {
+  // the byte's upper bit set, and its lower seven at least 99: that and 29 reach the upper bit
+  const uint32_t b = ((w & 0x7f7f7f7fu) + (0x7f - (kMostScale & 0x7f)) * 0x01010101u) & w & 0x80808080u;
+  return (b >> 7) * 255u;
 }
 
 // What a wave knows of its 16 rows: O and the sum of the weights (this lane's part).
@@ -275,8 +277,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[t][i] = 4 * t + i > left ? -INFINITY : s[t][i];
       // A weight of 0 has to leave nothing behind whatever the scale is: those of
-      // keys past all rows' are 0, and so are others that are not finite, which
-      // make the rows that see them NaN by their sum.
+      // keys past all rows' are 0, and so are others that may make an infinite
+      // product, which make the rows that see them NaN by their sum.
       const int held = there0 ? kend - (g * 64 + lg * 16) : 0;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
@@ -284,7 +286,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
         uint32_t bad = 0;
 #pragma unroll
         for (int x = 0; x < G; ++x) {
-          const uint32_t b = not_finite((uint32_t)vsw[x][y]) & mask;
+          const uint32_t b = past_largest((uint32_t)vsw[x][y]) & mask;
           vsw[x][y] &= (int)(mask & ~b);
           bad |= b;
         }
@@ -521,8 +523,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
     return pg;
   };
   // A weight of 0 has to leave nothing behind whatever a scale is: in a stage that
-  // not every row sees whole, scales of keys past all rows' are 0, and so are
-  // others that are not finite, which make the rows that see them NaN by their sum.
+  // not every row sees whole, scales of keys past all rows' are 0, and so are others
+  // that may make an infinite product, which make the rows that see them NaN by their sum.
   auto clear = [&](int st, int pg) {
     const int b = __builtin_amdgcn_readlane(pg, w);
     if (b >= 0 && st * 64 + 64 <= kall) return;
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
     uint32_t any = 0;
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const uint32_t mask = first_bytes(held, y), bad = not_finite((uint32_t)vsw[y]) & mask;
+      const uint32_t mask = first_bytes(held, y), bad = past_largest((uint32_t)vsw[y]) & mask;
       vsw[y] &= (int)(mask & ~bad);
       any |= (bad & 1) << (4 * y) | (bad >> 7 & 2) << (4 * y) | (bad >> 14 & 4) << (4 * y) | (bad >> 21 & 8) << (4 * y);
     }

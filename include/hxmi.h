@@ -591,8 +591,10 @@ int hxmi_qk_rope(int is_bf16, const void* q, const void* k, void* q_out, void* k
  *   k_scale, v_scale uint8 [blocks, kv_heads, Dp / 32, block_size]
  * A code has a sign (its upper bit) and a magnitude 0, 1/2, 1, 3/2, 2, 3, 4 or 6;
  * a scale's byte is bits 7 to 14 of a positive fp16 number (five exponent bits,
- * three of mantissa); a held value is their product, which fp16 and bf16 hold
- * exactly.  Each token and head has a scale for every 32 dimensions.
+ * three of mantissa) and at most 226, 10240; a held value is their product, which
+ * fp16 and bf16 hold exactly.  Each token and head has a scale for every 32
+ * dimensions.  Bytes past 226 are not written by hxmi_kv4_append; in a cache that has
+ * some, what they stand for is unspecified, and rows that do not see them are as without.
  */
 
 /*

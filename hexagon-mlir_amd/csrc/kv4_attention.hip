@@ -61,6 +61,14 @@ __device__ __forceinline__ float times(float a, float b) {
   return a * b;
 }
 
+// What the products of K and a row of q (times 2^ex) are to be multiplied by.  They are
+// below 2^40 and, where not 0, above 2^-45: from 2^-126 down they are all alike, and
+// from 2^80 up any two lie further apart than weights reach, so that c can stop there. In
+// between it is neither 0 nor infinite, and a masked key's -inf stays one, 0 stays 0.
+__device__ __forceinline__ float score_scale(float c, int ex) {
+  return fminf(fmaxf(__builtin_ldexpf(c, -ex), 0x1p-126f), 0x1p80f);
+}
+
 // Eight numbers times their scales (pairs) as one MFMA operand.
 template <typename F>
 __device__ __forceinline__ half8v operand(uint32_t w, F&& scale) {
@@ -164,7 +172,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
   const int token = (int)(rowq / a.group), head = kvh * a.group + (int)(rowq - (int64_t)token * a.group);
   const int last = (int)min((int64_t)len - n + token, (int64_t)len - 1);  // the last key it sees
   half8v qf[2 * DC];
-  float c = a.c;
+  float c;
   {
     const T* q = (const T*)a.q + (int64_t)(first + token) * a.ldq + (int64_t)head * a.hq;
     T raw[2 * DC][8];
@@ -178,7 +186,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention(KArgs a) {
       if constexpr (BF16) top = largest(raw[s], top);
     }
     const int ex = BF16 ? exponent_of(row_max(top)) : 0;
-    if constexpr (BF16) c = __builtin_ldexpf(a.c, -ex);
+    c = score_scale(a.c, ex);
 #pragma unroll
     for (int s = 0; s < 2 * DC; ++s) qf[s] = q_operand(raw[s], ex);
   }
@@ -453,7 +461,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
   const int token = (int)(rowq / a.group), head = kvh * a.group + (int)(rowq - (int64_t)token * a.group);
   const int last = (int)min((int64_t)len - n + token, (int64_t)len - 1);  // the last key it sees
   half8v qf[DS];
-  float c = a.c;
+  float c;
   {
     const T* q = (const T*)a.q + (int64_t)(tile.first + token) * a.ldq + (int64_t)head * a.hq;
     T raw[DS][8];
@@ -470,8 +478,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
     if constexpr (BF16) {
       const auto t2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       ex = exponent_of(fmaxf(__uint_as_float(t2[0]), __uint_as_float(t2[1])));
-      c = __builtin_ldexpf(a.c, -ex);
     }
+    c = score_scale(a.c, ex);
 #pragma unroll
     for (int s = 0; s < DS; ++s) qf[s] = q_operand(raw[s], ex);
   }

@@ -1,5 +1,6 @@
 """Attention over the 4-bit cache at the ends of what it can be given: bytes of
-scales that no row is written with."""
+scales that no row is written with, scales of scores and queries whose product
+leaves 32 bits."""
 import pytest
 import torch
 
@@ -55,3 +56,52 @@ def test_scales_past_the_largest_leave_rows_that_do_not_see_them(pkg, dev, d, by
             by = 2.0 ** -12 + 130 * 2.0 ** -24 * (qd.abs() @ ks.abs().t()).amax() * d ** -0.5 + 2.0 ** -20
             room = 2 * by * (w @ vs.abs()) + n * 2.0 ** -31 * vs.abs().amax() + 2.0 ** -25
             assert ((got[rows].cpu().double() - ref).abs() <= HALF[dtype] * ref.abs() + room * (1 + HALF[dtype])).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 130])  # tiles of 16 rows and of 128
+def test_scores_that_a_scale_makes_nothing(pkg, dev, rows, d):
+    """bf16 queries of 2^-60 to 2^-126 under a scale of 2^-40 and less: every
+    score is 0 beside a weight's bits, so a row is the mean of what it sees."""
+    heads, n = 32, 381
+    g = gen(91)
+    k, v = (torch.randn((n, 1, d), generator=g).half() for _ in range(2))
+    cache, table, (_, vs) = cache_of(pkg, dev, k, v)
+    vs = vs[:, 0]
+    for by, scale in ((-60, 2.0 ** -40), (-110, 2.0 ** -40), (-126, 2.0 ** -40), (-110, 2.0 ** -126), (-126, 1.0)):
+        q = (torch.randn((rows, heads, d), generator=g).clamp(-4, 4).double() * 2.0 ** by).to(torch.bfloat16).to(dev)
+        got = pkg.kv_attention(q, cache, table, ints(dev, n), cu=ints(dev, 0, rows), scale=scale).cpu().double()
+        for i in {0, rows // 2, rows - 1}:
+            seen = vs[:n - rows + i + 1]
+            want = seen.mean(0)
+            # weights are equal powers of two, sums of them exact, sums of values by 2^-24 of their magnitudes each
+            room = HALF[torch.bfloat16] * want.abs() + len(seen) * 2.0 ** -24 * seen.abs().mean(0)
+            assert ((got[i] - want).abs() <= room * (1 + 2.0 ** -8)).all(), (by, scale, i)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 130])  # tiles of 16 rows and of 128
+def test_scores_past_32_bits(pkg, dev, rows, dtype):
+    """Scores whose size is no 32-bit number: the key with the largest one is all
+    that remains, keys of zeros share where every score is 0."""
+    heads, n, d = 32, 381, 64
+    g = gen(93)
+    k, v = (torch.randn((n, 1, d), generator=g).half() for _ in range(2))
+    cache, table, (ks, vs) = cache_of(pkg, dev, k, v)
+    zeros, _, (_, vz) = cache_of(pkg, dev, torch.zeros_like(k), v)
+    q = torch.randn((rows, heads, d), generator=g).to(dtype)
+    for by, scale in ((0, 2.0 ** 100), (0, 2.0 ** 127), *(((100, 2.0 ** 60), (120, 2.0 ** 127)) if dtype == torch.bfloat16 else ())):
+        qs = (q.double() * 2.0 ** by).to(dtype)
+        got = pkg.kv_attention(qs.to(dev), cache, table, ints(dev, n), cu=ints(dev, 0, rows), scale=scale).cpu().double()
+        none = pkg.kv_attention(qs.to(dev), zeros, table, ints(dev, n), cu=ints(dev, 0, rows), scale=scale).cpu().double()
+        for i in {0, rows - 1}:
+            seen = n - rows + i + 1
+            s = q[i].double() @ ks[:seen, 0].t()
+            two = s.topk(2).values
+            # (the kernel's own scores are off by less than 2^-13: 64 roundings of sums below 2^7 in 2^-24)
+            clear = two[:, 0] - two[:, 1] > 2.0 ** -12
+            assert clear.sum() > heads // 2
+            assert torch.equal(got[i, clear], vs[s.argmax(-1), 0][clear]), (by, scale, i)
+            want = vz[:seen, 0].mean(0)
+            room = HALF[dtype] * want.abs() + seen * 2.0 ** -24 * vz[:seen, 0].abs().mean(0)
+            assert ((none[i] - want).abs() <= room * (1 + 2.0 ** -8)).all(), (by, scale, i)

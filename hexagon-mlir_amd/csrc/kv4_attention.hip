@@ -76,7 +76,8 @@ __device__ __forceinline__ half8v operand(uint32_t w, F&& scale) {
                d = numbers<3>(w) * scale(3);
   return half8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-// l + the sum of eight weights, as P.V takes them (two an instruction).
+// l + the sum of eight weights, as P.V takes them (two an instruction), those below
+// fp16's normal range with the bits that they keep there.
 __device__ __forceinline__ float sum_of(const half8v& p, float l) {
   const half2v one = {(_Float16)1.f, (_Float16)1.f};
 #pragma unroll

@@ -623,7 +623,9 @@ int hxmi_kv4_read(int is_bf16, const uint8_t* k_codes, const uint8_t* v_codes, c
  * hxmi_kv_attention over the 4-bit cache.  Keys and values go into the products
  * as they are held; a weight goes in with 11 bits, or as a multiple of 2^-31 of the
  * row's largest where that is coarser; the elements of a bf16 row of q are
- * multiples of 2^-38 of its largest.
+ * multiples of 2^-38 of its largest.  What a row is divided by is the sum of its
+ * weights: as they are in tiles of 16 rows, as they go into the product in tiles of
+ * 128 (which of them a call runs on depends on its average of rows a request).
  */
 int hxmi_kv4_attention(int is_bf16, const void* q, const uint8_t* k_codes, const uint8_t* v_codes,
                        const uint8_t* k_scale, const uint8_t* v_scale, const int32_t* block_table,

@@ -1,6 +1,8 @@
 """Attention over the 4-bit cache at the ends of what it can be given: bytes of
 scales that no row is written with, scales of scores and queries whose product
-leaves 32 bits."""
+leaves 32 bits, weights that fp16 holds without all of its bits."""
+import math
+
 import pytest
 import torch
 
@@ -105,3 +107,28 @@ def test_scores_past_32_bits(pkg, dev, rows, dtype):
             want = vz[:seen, 0].mean(0)
             room = HALF[dtype] * want.abs() + seen * 2.0 ** -24 * vz[:seen, 0].abs().mean(0)
             assert ((none[i] - want).abs() <= room * (1 + 2.0 ** -8)).all(), (by, scale, i)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows, kv_heads", [(1, 1), (130, 1), (130, 16)])  # 16 rows; 128, keys shared out; 128, most tiles whole
+def test_thousands_of_weights_below_fp16s_normal_range(pkg, dev, rows, kv_heads, d, dtype):
+    """A key 21.5 or 22 bits above 32000 others, whose weights together are about
+    one percent: they count in the sum as they do in the values."""
+    heads, n = 32 * kv_heads, 32011
+    k = torch.zeros((n, kv_heads, d), dtype=torch.float16)
+    v = torch.full((n, kv_heads, d), 0.75, dtype=torch.float16)  # (held as it is: 6 * 2^-3)
+    k[5], v[5] = 0.75, 0.0
+    v[5, :, 1] = 0.75  # of every key: what comes out there is the weights' sum over itself
+    cache, table, (ks, vs) = cache_of(pkg, dev, k, v, 64)
+    assert torch.equal(ks, k.double()) and torch.equal(vs, v.double())
+    q = torch.full((rows, heads, d), 0.5, dtype=dtype, device=dev)
+    for bits in (21.5, 22.0):
+        scale = bits * math.log(2) / (0.375 * d)
+        got = pkg.kv_attention(q, cache, table, ints(dev, n), cu=ints(dev, 0, rows), scale=scale).cpu().double()
+        rest = (n - rows + torch.arange(rows)[:, None].double()) * 2.0 ** -bits
+        want = 0.75 * rest / (1 + rest)
+        # a weight of 2^-22 is off by 2^-32 of the largest at most, 2^-10 of itself, by its score's 2^-24 of 2^5
+        # less, and the sum of the weights (other than the largest, which is a power of two) by as much
+        assert ((got[..., 0] - want).abs() <= (HALF[dtype] + 2.0 ** -9 + 2.0 ** -14) * want).all(), bits
+        assert ((got[..., 1] - 0.75).abs() <= 0.75 * (HALF[dtype] + 2.0 ** -11)).all(), bits

@@ -1118,10 +1118,11 @@ def qk_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                     o.copy_(v)
             return oq, ok
     strides = lambda t: (0, 0) if t is None else (t.stride(0), t.stride(1))  # noqa: E731
+    freq = inv_freq.contiguous()  # (held until the launch: memory of a dropped copy may be another thread's by then)
     with _on(x):
         _check(load_library().hxmi_qk_rope(
             int(x.dtype == torch.bfloat16), x.data_ptr(), _ptr(z), results[0].data_ptr(), _ptr(results[1]),
-            pos.data_ptr(), int(pos.dtype == torch.int64), inv_freq.contiguous().data_ptr(), _ptr(axis), _ptr(weights[0]),
+            pos.data_ptr(), int(pos.dtype == torch.int64), freq.data_ptr(), _ptr(axis), _ptr(weights[0]),
             _ptr(weights[1]), int(any(w is not None and w.dtype == torch.float32 for w in weights)), T, H,
             0 if z is None else z.shape[1], d, 2 * n, pos.shape[0] if pos.dim() == 2 else 1,
             pos.stride(0) if pos.dim() == 2 and pos.shape[0] > 1 else T, *strides(x), *strides(z), *strides(results[0]),

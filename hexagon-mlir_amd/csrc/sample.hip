@@ -71,12 +71,13 @@ struct SArgs {
 // Verification of drafted tokens: rows of requests, `u` a row's number for its
 // draft, `draw` a request's for the token after the accepted ones.
 struct RowState {
+  uint32_t state;
+  int owner;      // the request that the row was judged for, -1: none
   int64_t token;  // drawn (state kDrawn)
   uint64_t whole, least;
-  uint32_t state, tau, top, from;
+  uint32_t tau, top, from;
   int ties_end;  // equals of tau before this token are kept
   float t;
-  int owner;  // the request that the row was judged for, -1: none
 };
 enum : uint32_t { kDrawn, kAccepted, kToDraw };
 struct VArgs : SArgs {
@@ -362,11 +363,9 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
     }
     int64_t first, end;
     rows_of(a, lo, first, end);
+    if (threadIdx.x == 0) a.token[row] = -1;  // (verify_rows: accepted and drawn ones)
     if (row < first || row >= end) {  // of no request (or, where bounds do not ascend, one that the search passes by)
-      if (threadIdx.x == 0) {
-        a.token[row] = -1;
-        a.state[row] = RowState{.token = -1, .state = kDrawn, .owner = -1};
-      }
+      if (threadIdx.x == 0) a.state[row] = RowState{.state = kDrawn, .owner = -1, .token = -1};
       return;
     }
     owner = lo;
@@ -504,7 +503,7 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
   extremes();
   if (top > kInf || low + 1 < kMinusInf || top == kMinusInf) {
     if (threadIdx.x == 0) {
-      if constexpr (VERIFY) a.state[row] = RowState{.token = -1, .state = kDrawn, .owner = (int)owner};
+      if constexpr (VERIFY) a.state[row] = RowState{.state = kDrawn, .owner = (int)owner, .token = -1};
       else a.token[row] = -1;
     }
     return;
@@ -1025,7 +1024,7 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
         }
       }
       if (lane == 0)
-        a.state[row] = RowState{-1, whole, least, accepted ? kAccepted : kToDraw, tau, top, from, ties_end, t, (int)owner};
+        a.state[row] = RowState{accepted ? kAccepted : kToDraw, (int)owner, -1, whole, least, tau, top, from, ties_end, t};
       return;
     }
     if (in && !a.q && !final) {
@@ -1088,7 +1087,7 @@ __global__ __launch_bounds__(NT) void sample_rows(A a) {
       if (so_far > goal) break;
     }
     const int64_t token = (int64_t)(at * 64 + lane) * 8 + e;
-    if constexpr (VERIFY) a.state[row] = RowState{.token = token, .state = kDrawn, .owner = (int)owner};
+    if constexpr (VERIFY) a.state[row] = RowState{.state = kDrawn, .owner = (int)owner, .token = token};
     else a.token[row] = token;
   }
 }
@@ -1135,8 +1134,7 @@ __global__ __launch_bounds__(64 * VW) void verify_rows(VArgs a) {
     if (m) stop = i0 + __ffsll((unsigned long long)m) - 1;
   }
   if (share == 0) {
-    for (int64_t i = first + threadIdx.x; i < end; i += 64 * VW)
-      if (i != stop && a.state[i].owner == r) a.token[i] = i < stop ? a.drafts[i] : -1;
+    for (int64_t i = first + threadIdx.x; i < stop; i += 64 * VW) a.token[i] = a.drafts[i];
     if (threadIdx.x == 0) a.counts[r] = stop < end ? (int)(stop - first + 1) : 0;
   }
   if (stop >= end) return;  // (without rows)

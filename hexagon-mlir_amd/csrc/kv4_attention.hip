@@ -769,7 +769,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_attention_tiles(KArg
 // 8-bit one is planned for two): 64 requests of 8192 tokens over 4 heads 35.0 us in
 // two shares a tile, 31.5 in four.  Fewer tiles have their keys shared out as far
 // as it pays either way (64 tiles of 4000 keys: 10.0 us in eight, 11.4 in sixteen; 170
-// of drafts over 1500 keys: 11.0 in three, 11.4 in six).
+// of drafts over 1500 keys: 11.0 in three, 11.4 in six).  The line between them, 128
+// tiles, lies between those two, which are all that was measured around it; from there a
+// share has at least 512 keys (plan_of), below it 256.
 KvPlan plan4_of(const KvAttnSizes& p) {
   const int64_t group = p.heads / p.kv_heads;
   const int64_t tiles = p.cu ? p.tokens * group / 16 + p.requests : p.requests * ((group + 15) / 16);

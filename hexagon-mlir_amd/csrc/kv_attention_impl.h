@@ -145,8 +145,9 @@ inline KvPlan plan_of(const KvAttnSizes& p, int64_t slots = 512) {  // slots: wo
   r.tiles = p.cu ? p.tokens * group / rt + p.requests : p.requests * ((group + rt - 1) / rt);
   // The card takes 512 workgroups at a time, two a CU.  Whole rounds of them
   // run unshared; the tiles that are left share their keys out until they make
-  // one more round, at least one group of 64 keys a wave (eight stages of a
-  // 128-row tile) to a share.  575 tiles of 128 rows x 8000 keys, before later
+  // one more round, at least 256 keys to a share (a group of 64 for each wave), or
+  // 512 in 128-row tiles (eight stages) and where the card takes more than 512
+  // workgroups.  575 tiles of 128 rows x 8000 keys, before later
   // steps: 391 us unshared, 292 with all of them in two shares, 281 with the last
   // 63 in eight.  The table's width stands for the lengths, which only the GPU
   // knows: shares past a request's keys are joined for nothing (one user of 1900

@@ -8,8 +8,9 @@
 //
 // A pair's angle goes round once in 2 pi / inv_freq tokens, so positions in the
 // hundred thousands leave fp32 nothing of the fraction that counts: position *
-// (inv_freq / 2 pi) is taken in 64 bits and its whole turns dropped; cosine and
-// sine are polynomials in 32 bits over an eighth of a turn either way.
+// (inv_freq / 2 pi) is taken in 64 bits and its whole turns dropped (at inv_freq 1 off
+// by 2^-32 radians at position 2^20, 2^-21 at 2^31); cosine and sine are polynomials
+// in 32 bits over an eighth of a turn either way.
 //
 // A workgroup takes a few tokens: a thread computes each pair's cosine and
 // sine into LDS, once for all heads, then groups of lanes take heads, a lane the
